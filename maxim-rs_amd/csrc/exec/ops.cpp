@@ -1,0 +1,653 @@
+// The training and serving operators' host side (include/maxim_ops.h):
+// argument checks, the choice of kernel and split, and the launches. The
+// kernels are a code object of their own (csrc/ops), loaded per device by the
+// first call.
+
+#include "maxim_ops.h"
+
+#include <algorithm>
+#include <cstring>
+#include <limits>
+#include <map>
+#include <mutex>
+#include <string>
+
+#include "../ops/ops_args.h"
+#include "hip_api.hpp"
+#include "host.hpp"
+
+extern "C" const unsigned char mx_ops_hsaco[];
+
+namespace {
+
+using mx::Error;
+using mxh::check;
+using mxh::hip;
+
+constexpr int kMaxDevices = 64;
+constexpr int64_t kMaxExtent = std::numeric_limits<int32_t>::max() - 1024;
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------ the kernels
+
+struct Code {
+    mxh::hipModule_t mod = nullptr;
+    std::map<std::string, mxh::hipFunction_t> fns;
+};
+
+std::mutex g_mu;
+Code g_code[kMaxDevices];
+
+// The calling thread's current device, put back on the way out.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int dev) {
+        if (dev < 0 || dev >= kMaxDevices) throw Error("device ordinal out of range");
+        int now = -1;
+        check(hip().hipGetDevice(&now), "hipGetDevice");
+        if (now != dev) {
+            check(hip().hipSetDevice(dev), "hipSetDevice");
+            before = now;
+        }
+    }
+    ~OnDevice() {
+        if (before >= 0) hip().hipSetDevice(before);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+
+mxh::hipFunction_t function(int dev, const std::string &name) {
+    auto &H = hip();
+    std::lock_guard<std::mutex> lock(g_mu);
+    Code &c = g_code[dev];
+    if (!c.mod) check(H.hipModuleLoadData(&c.mod, mx_ops_hsaco), "hipModuleLoadData (operators' gfx950 code object)");
+    auto it = c.fns.find(name);
+    if (it != c.fns.end()) return it->second;
+    mxh::hipFunction_t f = nullptr;
+    check(H.hipModuleGetFunction(&f, c.mod, name.c_str()), ("hipModuleGetFunction " + name).c_str());
+    c.fns[name] = f;
+    return f;
+}
+
+template <typename A>
+void launch(int dev, void *stream, const std::string &name, int64_t gx, int64_t gy, unsigned block, const A &args) {
+    A copy = args;
+    void *params[] = {&copy};
+    check(hip().hipModuleLaunchKernel(function(dev, name), (unsigned)gx, (unsigned)gy, 1, block, 1, 1, 0,
+                                      (mxh::hipStream_t)stream, params, nullptr),
+          name.c_str());
+}
+
+// ------------------------------------------------------------- operands
+
+const char *kTypeName[] = {"f32", "f16", "bf16"};
+size_t type_size(int t) { return t == MXH_F32 ? 4 : 2; }
+
+std::string shape(const mxh_mat &m) { return "[" + std::to_string(m.rows) + "][" + std::to_string(m.cols) + "]"; }
+
+bool empty(const mxh_mat &m) { return m.rows == 0 || m.cols == 0; }
+// Contiguous along columns (features), or along rows (positions).
+bool along_cols(const mxh_mat &m) { return m.col_stride == 1 || m.cols <= 1; }
+bool along_rows(const mxh_mat &m) { return m.row_stride == 1 || m.rows <= 1; }
+
+const mxh_mat &need(const mxh_mat *m, const char *what) {
+    if (!m) throw Error(std::string(what) + ": missing");
+    return *m;
+}
+
+void check_mat(const mxh_mat &m, const char *what, int dtype, int64_t rows, int64_t cols) {
+    const std::string w = what;
+    if (m.dtype < MXH_F32 || m.dtype > MXH_BF16) throw Error(w + ": unknown type " + std::to_string(m.dtype));
+    if (m.dtype != dtype) throw Error(w + ": " + kTypeName[m.dtype] + " where x is " + kTypeName[dtype]);
+    if (m.rows != rows || m.cols != cols)
+        throw Error(w + ": " + shape(m) + ", expected [" + std::to_string(rows) + "][" + std::to_string(cols) + "]");
+    if (m.rows < 0 || m.cols < 0 || m.rows > kMaxExtent || m.cols > kMaxExtent)
+        throw Error(w + ": " + shape(m) + " is out of range");
+    if (m.row_stride < 0 || m.col_stride < 0) throw Error(w + ": a negative stride");
+    if (empty(m)) return;
+    if (!m.data) throw Error(w + ": no data");
+    if (!along_cols(m) && !along_rows(m))
+        throw Error(w + ": neither rows nor columns are contiguous (strides " + std::to_string(m.row_stride) + ", " +
+                    std::to_string(m.col_stride) + ")");
+    if ((uintptr_t)m.data % type_size(m.dtype)) throw Error(w + ": not aligned to its element");
+    // the farthest element's offset in bytes has to be a number
+    const __int128 far = ((__int128)(m.rows - 1) * m.row_stride + (__int128)(m.cols - 1) * m.col_stride) * 4;
+    if (far > std::numeric_limits<int64_t>::max() / 2) throw Error(w + ": strides out of range");
+}
+
+void check_first(const mxh_mat &x, const char *what) { check_mat(x, what, x.dtype, x.rows, x.cols); }
+
+void check_vec(const mxh_vec &v, const char *what, int64_t n, int dtype) {
+    const std::string w = what;
+    if (v.n != n) throw Error(w + ": " + std::to_string(v.n) + " elements, expected " + std::to_string(n));
+    if (v.dtype != MXH_F32 && v.dtype != dtype) throw Error(w + ": its type is neither fp32 nor x's");
+    if (n && !v.data) throw Error(w + ": no data");
+    if ((uintptr_t)v.data % type_size(v.dtype)) throw Error(w + ": not aligned to its element");
+}
+
+// The memory order that all of a call's matrices have: true, features
+// contiguous; false, positions. (One of a single row or column has both.)
+bool out_by_cols(const mxh_mat &m) { return along_cols(m) && (m.rows <= 1 || m.row_stride >= m.cols); }
+bool out_by_rows(const mxh_mat &m) { return along_rows(m) && (m.cols <= 1 || m.col_stride >= m.rows); }
+bool common_order(std::initializer_list<const mxh_mat *> ins, std::initializer_list<const mxh_mat *> outs) {
+    bool cols = true, rows = true;
+    for (const mxh_mat *m : ins)
+        if (m && !empty(*m)) cols = cols && along_cols(*m), rows = rows && along_rows(*m);
+    for (const mxh_mat *m : outs)
+        if (m && !empty(*m)) cols = cols && out_by_cols(*m), rows = rows && out_by_rows(*m);
+    if (!cols && !rows) throw Error("the matrices differ in memory order");
+    return cols;
+}
+
+// Elements of an output may not share storage.
+void check_out(const mxh_mat &m, const char *what) {
+    if (empty(m)) return;
+    if (!out_by_cols(m) && !out_by_rows(m)) throw Error(std::string(what) + ": elements of an output share storage");
+}
+
+struct Range {
+    uintptr_t lo, hi;
+};
+Range range(const mxh_mat &m) {
+    const uintptr_t p = (uintptr_t)m.data;
+    const uint64_t far = (uint64_t)(m.rows - 1) * m.row_stride + (uint64_t)(m.cols - 1) * m.col_stride + 1;
+    return {p, p + far * type_size(m.dtype)};
+}
+bool apart(Range a, Range b) { return a.hi <= b.lo || b.hi <= a.lo; }
+
+// Whether two views share an element: by their ranges, and where these cross
+// and the strides agree (slices of one buffer), by their offset in it.
+bool overlap(const mxh_mat &a, const mxh_mat &b) {
+    if (empty(a) || empty(b) || apart(range(a), range(b))) return false;
+    if (a.dtype != b.dtype) return true;
+    int64_t ld, inner_a, inner_b, outer_a, outer_b;
+    if (along_cols(a) && along_cols(b) && a.row_stride == b.row_stride) {
+        ld = a.row_stride, inner_a = a.cols, inner_b = b.cols, outer_a = a.rows, outer_b = b.rows;
+    } else if (along_rows(a) && along_rows(b) && a.col_stride == b.col_stride) {
+        ld = a.col_stride, inner_a = a.rows, inner_b = b.rows, outer_a = a.cols, outer_b = b.cols;
+    } else {
+        return true;
+    }
+    const int64_t size = (int64_t)type_size(a.dtype);
+    const int64_t bytes = (int64_t)((uintptr_t)b.data - (uintptr_t)a.data);
+    if (bytes % size) return true;
+    if (ld < std::max(inner_a, inner_b)) return true;
+    // b begins q whole lines and r elements past a, 0 <= r < ld: its lines
+    // begin on a's q lines on, or (r + inner_b > ld) run into the next ones
+    int64_t d = bytes / size, q = d / ld, r = d % ld;
+    if (r < 0) r += ld, --q;
+    auto lines = [&](int64_t off) { return off < outer_a && -off < outer_b; };
+    return (r < inner_a && lines(q)) || (r + inner_b > ld && lines(q + 1));
+}
+
+bool same(const mxh_mat &a, const mxh_mat &b) {
+    return a.data == b.data && (a.rows <= 1 || a.row_stride == b.row_stride) &&
+           (a.cols <= 1 || a.col_stride == b.col_stride) && a.rows == b.rows && a.cols == b.cols && a.dtype == b.dtype;
+}
+
+mxh_mat line(const void *p, int64_t n, int dtype) {
+    return mxh_mat{const_cast<void *>(p), 1, n, n, 1, dtype, 0};
+}
+mxh_mat line(const mxh_vec &v) { return line(v.data, v.n, v.dtype); }
+
+void refuse_overlap(const mxh_mat &out, const char *a, const mxh_mat &in, const char *b) {
+    if (overlap(out, in)) throw Error(std::string(a) + " overlaps " + b);
+}
+
+void check_workspace(const void *ws, uint64_t have, uint64_t want) {
+    if (!want) return;
+    if (!ws) throw Error("the call needs " + std::to_string(want) + " bytes of workspace");
+    if (have < want)
+        throw Error("the call needs " + std::to_string(want) + " bytes of workspace, not " + std::to_string(have));
+    if ((uintptr_t)ws % 16) throw Error("workspace: not aligned to 16 bytes");
+}
+
+void check_act(int act) {
+    if (act < MXH_NONE || act > MXH_SIGMOID) throw Error("unknown activation " + std::to_string(act));
+}
+
+// ------------------------------------------------------------- LayerNorm
+
+int64_t ln_parts(int64_t rows) { return std::min<int64_t>(256, cdiv(rows, 64)); }
+
+uint64_t ln_bwd_bytes(const mxh_mat &x) { return (uint64_t)ln_parts(x.rows) * 2 * x.cols * 4; }
+
+void join(int dev, void *stream, const float *part, int64_t nparts, int64_t n, void *out0, void *out1, int dtype) {
+    if (!n) return;
+    OpsJoinArgs j{};
+    j.part = part;
+    j.out0 = out0;
+    j.out1 = out1;
+    j.n = n;
+    j.nparts = (int32_t)nparts;
+    j.nout = out1 ? 2 : 1;
+    j.dtype = dtype;
+    launch(dev, stream, "mxo_join_parts", cdiv(n, 64), j.nout, 1024, j);
+}
+
+// ------------------------------------------------------------- products
+
+// One operand of a product: elements apart along its own axis and along the
+// summed one.
+struct Operand {
+    const void *data;
+    int64_t own, sum;
+};
+
+struct Product {
+    int dtype = 0;
+    int64_t m = 0, n = 0, k = 0;
+    Operand a{}, b{};
+    void *c = nullptr;
+    int64_t ldc = 0;
+    const mxh_vec *bias = nullptr;
+    bool bias_rows = false;
+    const void *res = nullptr;
+    int64_t ldr = 0;
+    void *z = nullptr;
+    int64_t ldz = 0;
+    int act = MXH_NONE;
+    float slope = 0.0f;
+};
+
+struct Plan {
+    int bm = 0, bn = 0;
+    int64_t splits = 1, kchunk = 0;
+    uint64_t bytes = 0;
+};
+
+// 128 x 128 tiles where there are enough of them for the 256 CUs, else
+// 64 x 64; and where these are few too, k in up to 64 runs, each at least
+// four LDS tiles long.
+Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k) {
+    Plan p;
+    p.bm = p.bn = cdiv(m, 128) * cdiv(n, 128) >= 256 ? 128 : 64;
+    const int64_t tiles = cdiv(m, p.bm) * cdiv(n, p.bn), bk = 128 / (int64_t)type_size(dtype);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, tiles), cdiv(k, 4 * bk), 64}));
+    p.kchunk = std::max<int64_t>(bk, cdiv(cdiv(k, splits), bk) * bk);
+    p.splits = std::max<int64_t>(1, cdiv(k, p.kchunk));
+    p.bytes = p.splits > 1 ? (uint64_t)p.splits * m * n * 4 : 0;
+    return p;
+}
+
+void product(int dev, void *stream, const Product &p, void *ws) {
+    if (!p.m || !p.n) return;
+    const Plan pl = plan_product(p.dtype, p.m, p.n, p.k);
+    OpsGemmArgs g{};
+    g.a = p.a.data;
+    g.b = p.b.data;
+    g.c = p.c;
+    g.z = p.z;
+    g.res = p.res;
+    g.part = static_cast<float *>(ws);
+    // contiguous along k (also where there is only one row to stride over),
+    // or along the operand's own axis
+    const bool ak = p.a.sum == 1, bk = p.b.sum == 1;
+    g.lda = ak ? p.a.own : p.a.sum;
+    g.ldb = bk ? p.b.own : p.b.sum;
+    g.ldc = p.ldc;
+    g.ldr = p.ldr;
+    g.ldz = p.ldz;
+    g.m = (int32_t)p.m;
+    g.n = (int32_t)p.n;
+    g.k = (int32_t)p.k;
+    g.splits = (int32_t)pl.splits;
+    g.kchunk = (int32_t)pl.kchunk;
+    const int64_t tm = cdiv(p.m, pl.bm), tn = cdiv(p.n, pl.bn);
+    g.tiles_m = (int32_t)tm;
+    g.tiles_n = (int32_t)tn;
+    g.act = p.act;
+    g.slope = p.slope;
+    if (p.bias) {
+        g.bias = p.bias->data;
+        g.bias_f32 = p.bias->dtype == MXH_F32 && p.dtype != MXH_F32;
+        g.bias_rows = p.bias_rows;
+    }
+    g.vec = p.n % 4 == 0;
+    if (tm * tn > std::numeric_limits<int32_t>::max() / pl.splits) throw Error("the product has too many tiles");
+    const std::string t = kTypeName[p.dtype];
+    launch(dev, stream,
+           "mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
+               (bk ? "k" : "m"),
+           tm * tn * pl.splits, 1, 256, g);
+    if (pl.splits > 1)
+        launch(dev, stream, "mxo_join_" + t, std::min<int64_t>(2048, cdiv(p.m * cdiv(p.n, 4), 256)), 1, 256, g);
+}
+
+// An operand of a product as (own axis, summed axis): rows summed over or not.
+Operand operand(const mxh_mat &m, bool sum_rows) {
+    Operand o{m.data, sum_rows ? m.col_stride : m.row_stride, sum_rows ? m.row_stride : m.col_stride};
+    const int64_t own_n = sum_rows ? m.cols : m.rows, sum_n = sum_rows ? m.rows : m.cols;
+    // an axis of one element has no stride of its own: the other one's order
+    // holds, and where both are single the element is contiguous
+    if (o.sum != 1 && sum_n <= 1 && o.own != 1) o.sum = 1;
+    if (o.sum != 1 && o.own != 1 && own_n <= 1) o.own = 1;
+    return o;
+}
+
+// out = p^T q or p q^T in out's order: rows of `out` run over a's own axis.
+Product oriented(const mxh_mat &out, const Operand &rows, const Operand &cols, int64_t k, bool by_cols) {
+    Product p;
+    p.dtype = out.dtype;
+    p.k = k;
+    p.c = out.data;
+    if (by_cols) {
+        p.m = out.rows, p.n = out.cols, p.a = rows, p.b = cols, p.ldc = out.row_stride;
+    } else {
+        p.m = out.cols, p.n = out.rows, p.a = cols, p.b = rows, p.ldc = out.col_stride;
+    }
+    return p;
+}
+
+uint64_t product_bytes(const mxh_mat &out, int64_t k, bool by_cols) {
+    if (empty(out)) return 0;
+    return by_cols ? plan_product(out.dtype, out.rows, out.cols, k).bytes
+                   : plan_product(out.dtype, out.cols, out.rows, k).bytes;
+}
+
+uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
+
+// mxh_dense_backward's workspace: dz where there is an activation, the bias's
+// partial sums, and one product's partial sums at a time.
+struct BwdLayout {
+    mxh_mat dz{};
+    int64_t parts = 0;
+    uint64_t dz_bytes = 0, part_bytes = 0, product_bytes = 0;
+    uint64_t total() const { return dz_bytes + part_bytes + product_bytes; }
+};
+
+BwdLayout bwd_layout(const mxh_mat &dy, const mxh_mat &x, const mxh_mat *dx, const mxh_mat *dw, const mxh_vec *db,
+                     int act) {
+    BwdLayout l;
+    l.dz = dy;
+    const bool products = dx || dw;
+    if (act != MXH_NONE && products) {
+        // rows (or planes) padded to 16 bytes, so that the products' loads are
+        const int64_t pad = 16 / (int64_t)type_size(dy.dtype);
+        if (along_cols(dy)) {
+            l.dz.row_stride = cdiv(dy.cols, pad) * pad, l.dz.col_stride = 1;
+            l.dz_bytes = up((uint64_t)dy.rows * l.dz.row_stride * type_size(dy.dtype));
+        } else {
+            l.dz.col_stride = cdiv(dy.rows, pad) * pad, l.dz.row_stride = 1;
+            l.dz_bytes = up((uint64_t)dy.cols * l.dz.col_stride * type_size(dy.dtype));
+        }
+    }
+    if (db) {
+        l.parts = std::min<int64_t>(256, cdiv(dy.rows, 64));
+        l.part_bytes = up((uint64_t)l.parts * dy.cols * 4);
+    }
+    if (dx) l.product_bytes = std::max(l.product_bytes, product_bytes(*dx, dy.cols, out_by_cols(*dx)));
+    if (dw) l.product_bytes = std::max(l.product_bytes, product_bytes(*dw, x.rows, out_by_cols(*dw)));
+    return l;
+}
+
+template <typename F>
+int guard(F &&f) {
+    try {
+        f();
+        return 0;
+    } catch (const std::exception &e) {
+        mx::set_error(e.what());
+    } catch (...) {
+        mx::set_error("unknown error");
+    }
+    return -1;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mxh_ops_ready(int device) {
+    return guard([&] {
+        OnDevice on(device);
+        function(device, "mxo_join_parts");
+    });
+}
+
+int mxh_layernorm(int device, void *stream, const mxh_mat *x, const mxh_vec *scale, const mxh_vec *bias, float eps,
+                  const mxh_mat *y, float *mean, float *rstd) {
+    return guard([&] {
+        const mxh_mat &X = need(x, "x"), &Y = need(y, "y");
+        check_first(X, "x");
+        check_mat(Y, "y", X.dtype, X.rows, X.cols);
+        check_out(Y, "y");
+        if (X.cols == 0) throw Error("x: no columns to normalise over");
+        if (!scale) throw Error("scale: missing");
+        check_vec(*scale, "scale", X.cols, X.dtype);
+        if (bias) {
+            check_vec(*bias, "bias", X.cols, X.dtype);
+            if (bias->dtype != scale->dtype) throw Error("bias and scale differ in type");
+        }
+        if (!(eps >= 0.0f)) throw Error("eps: not a number of at least 0");
+        const bool by_cols = common_order({x}, {y});
+        if (!same(X, Y)) refuse_overlap(Y, "y", X, "x");
+        const mxh_mat stats[2] = {line(mean, mean ? X.rows : 0, MXH_F32), line(rstd, rstd ? X.rows : 0, MXH_F32)};
+        refuse_overlap(stats[0], "mean", stats[1], "rstd");
+        for (const mxh_mat *o : {&Y, &stats[0], &stats[1]}) {
+            refuse_overlap(*o, "an output", line(*scale), "scale");
+            if (bias) refuse_overlap(*o, "an output", line(*bias), "bias");
+            if (o == &Y) continue;
+            refuse_overlap(*o, "a statistic", X, "x");
+            refuse_overlap(*o, "a statistic", Y, "y");
+        }
+        if (!X.rows) return;
+        OnDevice on(device);
+        OpsLnArgs a{};
+        a.x = X.data;
+        a.y = Y.data;
+        a.scale = scale->data;
+        a.bias = bias ? bias->data : nullptr;
+        a.mean = mean;
+        a.rstd = rstd;
+        a.rows = X.rows;
+        a.cols = X.cols;
+        a.xrs = X.row_stride, a.xcs = X.col_stride;
+        a.yrs = Y.row_stride, a.ycs = Y.col_stride;
+        a.eps = eps;
+        a.param_f32 = scale->dtype == MXH_F32;
+        (void)by_cols;
+        launch(device, stream, std::string("mxo_ln_any_") + kTypeName[X.dtype], std::min<int64_t>(X.rows, 65536), 1,
+               1024, a);
+    });
+}
+
+int mxh_layernorm_backward_workspace(const mxh_mat *x, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) throw Error("bytes: missing");
+        check_first(need(x, "x"), "x");
+        *bytes = ln_bwd_bytes(*x);
+    });
+}
+
+int mxh_layernorm_backward(int device, void *stream, const mxh_mat *dy, const mxh_mat *x, const mxh_vec *scale,
+                           const float *mean, const float *rstd, const mxh_mat *add, const mxh_mat *dx,
+                           const mxh_vec *dscale, const mxh_vec *dbias, void *workspace, uint64_t workspace_bytes) {
+    return guard([&] {
+        const mxh_mat &X = need(x, "x"), &DY = need(dy, "dy");
+        check_first(X, "x");
+        check_mat(DY, "dy", X.dtype, X.rows, X.cols);
+        if (X.cols == 0) throw Error("x: no columns to normalise over");
+        if (!scale) throw Error("scale: missing");
+        check_vec(*scale, "scale", X.cols, X.dtype);
+        if (X.rows && (!mean || !rstd)) throw Error("mean, rstd: missing");
+        if (add) {
+            if (!dx) throw Error("add without dx");
+            check_mat(*add, "add", X.dtype, X.rows, X.cols);
+        }
+        if (dx) {
+            check_mat(*dx, "dx", X.dtype, X.rows, X.cols);
+            check_out(*dx, "dx");
+        }
+        if (!dscale != !dbias) throw Error("dscale and dbias come together");
+        if (dscale) {
+            check_vec(*dscale, "dscale", X.cols, X.dtype);
+            check_vec(*dbias, "dbias", X.cols, X.dtype);
+            if (dscale->dtype != scale->dtype || dbias->dtype != scale->dtype)
+                throw Error("dscale and dbias have scale's type");
+        }
+        const bool by_cols = common_order({x, dy, add}, {dx});
+        const mxh_mat stats[2] = {line(mean, X.rows, MXH_F32), line(rstd, X.rows, MXH_F32)};
+        if (dx) {
+            if (!same(DY, *dx)) refuse_overlap(*dx, "dx", DY, "dy");
+            if (add && !same(*add, *dx)) refuse_overlap(*dx, "dx", *add, "add");
+            refuse_overlap(*dx, "dx", X, "x");
+            refuse_overlap(*dx, "dx", line(*scale), "scale");
+            for (const mxh_mat &s : stats) refuse_overlap(*dx, "dx", s, "the statistics");
+        }
+        if (dscale) {
+            const mxh_mat g[2] = {line(*dscale), line(*dbias)};
+            refuse_overlap(g[0], "dscale", g[1], "dbias");
+            for (const mxh_mat &o : g) {
+                for (const mxh_mat *in : {&X, &DY, dx, add, &stats[0], &stats[1]})
+                    if (in) refuse_overlap(o, "a parameter's gradient", *in, "another operand");
+                refuse_overlap(o, "a parameter's gradient", line(*scale), "scale");
+            }
+            check_workspace(workspace, workspace_bytes, ln_bwd_bytes(X));
+        }
+        OnDevice on(device);
+        const std::string t = kTypeName[X.dtype];
+        OpsLnBwdArgs a{};
+        a.dy = DY.data;
+        a.x = X.data;
+        a.scale = scale->data;
+        a.mean = mean;
+        a.rstd = rstd;
+        a.part = static_cast<float *>(workspace);
+        a.rows = X.rows;
+        a.cols = X.cols;
+        a.dyrs = DY.row_stride, a.dycs = DY.col_stride;
+        a.xrs = X.row_stride, a.xcs = X.col_stride;
+        if (add) a.add = add->data, a.ars = add->row_stride, a.acs = add->col_stride;
+        if (dx) a.dx = dx->data, a.dxrs = dx->row_stride, a.dxcs = dx->col_stride;
+        a.nparts = (int32_t)ln_parts(X.rows);
+        a.param_f32 = scale->dtype == MXH_F32;
+        (void)by_cols;
+        // the parameters' gradients first: dx may take dy's place
+        if (dscale) {
+            if (X.rows) launch(device, stream, "mxo_ln_param_any_" + t, cdiv(X.cols, 64), a.nparts, 256, a);
+            join(device, stream, a.part, a.nparts, X.cols, dscale->data, dbias->data, dscale->dtype);
+        }
+        if (dx && X.rows) launch(device, stream, "mxo_ln_bwd_any_" + t, std::min<int64_t>(X.rows, 65536), 1, 1024, a);
+    });
+}
+
+int mxh_dense_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) throw Error("bytes: missing");
+        check_first(need(x, "x"), "x");
+        check_mat(need(y, "y"), "y", x->dtype, x->rows, need(w, "w").rows);
+        *bytes = std::max(product_bytes(*y, x->cols, true), product_bytes(*y, x->cols, false));
+    });
+}
+
+int mxh_dense(int device, void *stream, const mxh_mat *x, const mxh_mat *w, const mxh_vec *bias, int act, float slope,
+              const mxh_mat *residual, const mxh_mat *y, const mxh_mat *z, void *workspace, uint64_t workspace_bytes) {
+    return guard([&] {
+        const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &Y = need(y, "y");
+        check_first(X, "x");
+        check_mat(W, "w", X.dtype, W.rows, X.cols);
+        check_mat(Y, "y", X.dtype, X.rows, W.rows);
+        check_out(Y, "y");
+        check_act(act);
+        if (bias) check_vec(*bias, "bias", W.rows, X.dtype);
+        if (residual) check_mat(*residual, "residual", X.dtype, X.rows, W.rows);
+        if (z) {
+            check_mat(*z, "z", X.dtype, X.rows, W.rows);
+            check_out(*z, "z");
+        }
+        const bool by_cols = common_order({residual}, {y, z});
+        for (const mxh_mat *o : {y, z}) {
+            if (!o) continue;
+            refuse_overlap(*o, "an output", X, "x");
+            refuse_overlap(*o, "an output", W, "w");
+            if (bias) refuse_overlap(*o, "an output", line(*bias), "bias");
+            if (residual && !(o == y && same(*residual, Y))) refuse_overlap(*o, "an output", *residual, "the residual");
+        }
+        if (z) refuse_overlap(Y, "y", *z, "z");
+        check_workspace(workspace, workspace_bytes, product_bytes(Y, X.cols, by_cols));
+        if (empty(Y)) return;
+        OnDevice on(device);
+        Product p = oriented(Y, operand(X, false), operand(W, false), X.cols, by_cols);
+        p.bias = bias;
+        p.bias_rows = !by_cols;
+        p.act = act;
+        p.slope = slope;
+        if (residual) p.res = residual->data, p.ldr = by_cols ? residual->row_stride : residual->col_stride;
+        if (z) p.z = z->data, p.ldz = by_cols ? z->row_stride : z->col_stride;
+        product(device, stream, p, workspace);
+    });
+}
+
+int mxh_dense_backward_workspace(const mxh_mat *dy, const mxh_mat *x, const mxh_mat *w, int act, const mxh_mat *dx,
+                                 const mxh_mat *dw, const mxh_vec *db, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) throw Error("bytes: missing");
+        check_first(need(x, "x"), "x");
+        check_mat(need(dy, "dy"), "dy", x->dtype, x->rows, need(w, "w").rows);
+        check_act(act);
+        *bytes = bwd_layout(*dy, *x, dx, dw, db, act).total();
+    });
+}
+
+int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_mat *x, const mxh_mat *w,
+                       const mxh_mat *z, int act, float slope, const mxh_mat *dx, const mxh_mat *dw,
+                       const mxh_vec *db, void *workspace, uint64_t workspace_bytes) {
+    return guard([&] {
+        const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &DY = need(dy, "dy");
+        check_first(X, "x");
+        check_mat(W, "w", X.dtype, W.rows, X.cols);
+        check_mat(DY, "dy", X.dtype, X.rows, W.rows);
+        check_act(act);
+        if (act != MXH_NONE && !z) throw Error("z: missing (the activation's derivative needs it)");
+        if (act == MXH_NONE) z = nullptr;
+        if (z) check_mat(*z, "z", X.dtype, X.rows, W.rows);
+        if (dx) {
+            check_mat(*dx, "dx", X.dtype, X.rows, X.cols);
+            check_out(*dx, "dx");
+        }
+        if (dw) {
+            check_mat(*dw, "dw", X.dtype, W.rows, W.cols);
+            check_out(*dw, "dw");
+        }
+        if (db) check_vec(*db, "db", W.rows, X.dtype);
+        if (z) common_order({dy, z}, {});
+        const mxh_mat dbl = db ? line(*db) : mxh_mat{};
+        const mxh_mat *outs[] = {dx, dw, db ? &dbl : nullptr}, *ins[] = {dy, x, w, z};
+        const char *on_[] = {"dx", "dw", "db"}, *in_[] = {"dy", "x", "w", "z"};
+        for (int i = 0; i < 3; ++i) {
+            if (!outs[i]) continue;
+            for (int j = 0; j < 4; ++j)
+                if (ins[j]) refuse_overlap(*outs[i], on_[i], *ins[j], in_[j]);
+            for (int j = 0; j < i; ++j)
+                if (outs[j]) refuse_overlap(*outs[i], on_[i], *outs[j], on_[j]);
+        }
+        BwdLayout l = bwd_layout(DY, X, dx, dw, db, act);
+        check_workspace(workspace, workspace_bytes, l.total());
+        OnDevice on(device);
+        char *ws = static_cast<char *>(workspace);
+        const std::string t = kTypeName[X.dtype];
+        OpsDzArgs a{};
+        a.dy = DY.data;
+        a.rows = DY.rows;
+        a.cols = DY.cols;
+        a.dyrs = DY.row_stride, a.dycs = DY.col_stride;
+        if (z) a.z = z->data, a.zrs = z->row_stride, a.zcs = z->col_stride;
+        if (l.dz_bytes) l.dz.data = a.dz = ws, a.drs = l.dz.row_stride, a.dcs = l.dz.col_stride;
+        if (db) a.part = reinterpret_cast<float *>(ws + l.dz_bytes);
+        a.nparts = (int32_t)(db ? l.parts : std::max<int64_t>(1, std::min<int64_t>(256, cdiv(DY.rows, 64))));
+        a.act = act;
+        a.slope = slope;
+        if ((a.dz || a.part) && !empty(DY)) launch(device, stream, "mxo_dz_any_" + t, cdiv(DY.cols, 64), a.nparts, 256, a);
+        if (db) join(device, stream, a.part, l.parts, DY.cols, db->data, nullptr, db->dtype);
+        void *pw = ws + l.dz_bytes + l.part_bytes;
+        if (dx && !empty(*dx))
+            product(device, stream, oriented(*dx, operand(l.dz, false), operand(W, true), W.rows, out_by_cols(*dx)), pw);
+        if (dw && !empty(*dw))
+            product(device, stream, oriented(*dw, operand(l.dz, true), operand(X, true), X.rows, out_by_cols(*dw)), pw);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,147 @@
+// Device helpers of the training and serving operators.
+#pragma once
+
+#include "../hip/common.h"
+#include "ops_args.h"
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v) {
+    return (float)v;
+}
+// Rounds to nearest even, as every store of a result does.
+template <typename T>
+__device__ __forceinline__ T from_f(float v) {
+    return (T)v;
+}
+
+// N consecutive elements at any alignment of the element: the memory system
+// takes unaligned vector accesses, so one load serves every row stride.
+template <typename T, int N>
+struct Vec {
+    T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_n(const T *p) {
+    Vec<T, N> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T *p, const Vec<T, N> &v) {
+    __builtin_memcpy(p, &v, sizeof(v));
+}
+// The first `have` of them (any number), the others zero.
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load_upto(const T *p, int64_t have) {
+    if (have >= N) return load_n<T, N>(p);
+    Vec<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = i < have ? p[i] : (T)0.0f;
+    return r;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_upto(T *p, const Vec<T, N> &v, int64_t have) {
+    if (have >= N) {
+        store_n<T, N>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < have) p[i] = v.v[i];
+}
+
+// A parameter vector's element, of the activations' type or fp32.
+template <typename T>
+__device__ __forceinline__ float param(const void *p, int64_t i, int f32) {
+    return f32 ? static_cast<const float *>(p)[i] : to_f<T>(static_cast<const T *>(p)[i]);
+}
+
+// e^-|z|'s form of the logistic function: s = 1 / (1 + e^-z) and its
+// derivative e / (1 + e)^2, e = e^-|z|, which never subtracts near numbers.
+// One exp2 and one reciprocal, 1 ulp each.
+__device__ __forceinline__ void logistic(float z, float &s, float &d) {
+    const float e = __builtin_amdgcn_exp2f(-fabsf(z) * 1.4426950408889634f);
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    s = z >= 0.0f ? r : e * r;
+    d = e * r * r;
+}
+
+constexpr float kTanhA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kTanhB = 0.044715f;
+
+// Phi(-ax), ax = |x|: 2^q(t), q the degree-7 polynomial fitted to log2 Phi(-t)
+// over [0, 6] for the least largest error of Phi, and 0 past 6 (Phi(-6) is
+// 1e-9). Within 1.4e-7 of Phi everywhere (the fit 3.6e-8, Horner in fp32 and
+// the exp2 the rest). common.h's gelu() has a fit of its own, weighted for
+// x Phi alone: at x = 0 its Phi is 2.7e-6 off, which a derivative would show,
+// and it keeps Phi(-6) past 6, which a product with a far x would.
+__device__ __forceinline__ float phi_tail(float ax) {
+    const float t = fminf(ax, 6.0f);
+    float q = __builtin_fmaf(8.47016599e-06f, t, -5.39037901e-05f);
+    q = __builtin_fmaf(q, t, -4.212356e-04f);
+    q = __builtin_fmaf(q, t, 7.38927163e-03f);
+    q = __builtin_fmaf(q, t, -5.26911095e-02f);
+    q = __builtin_fmaf(q, t, -4.59153146e-01f);
+    q = __builtin_fmaf(q, t, -1.15111089e+00f);
+    q = __builtin_fmaf(q, t, -9.99999881e-01f);
+    const float r = __builtin_amdgcn_exp2f(q);
+    return ax > 6.0f ? 0.0f : r;
+}
+
+// The activation. gelu, gelu_tanh and silu of minus infinity are their limit
+// 0 (the clamp keeps an infinity out of a product with 0); NaN stays NaN.
+__device__ __forceinline__ float act_fwd(int act, float slope, float z) {
+    if (act == MXO_NONE) return z;
+    if (act == MXO_LRELU) return z >= 0.0f ? z : slope * z;
+    float v, d;
+    if (act == MXO_GELU) {
+        v = fmaxf(z, 0.0f) - fminf(fabsf(z), 6.0f) * phi_tail(fabsf(z));
+    } else if (act == MXO_SIGMOID) {
+        logistic(z, v, d);
+    } else {
+        const float c = fmaxf(z, -1e4f);
+        const float u = act == MXO_SILU ? c : kTanhA * c * __builtin_fmaf(kTanhB * c, c, 1.0f);
+        float s;
+        logistic(u, s, d);
+        v = c * s;
+    }
+    return z != z ? z : v;
+}
+
+// Its derivative; at an infinity its limit, at NaN NaN (LeakyReLU: of a NaN
+// the slope, as its comparison gives).
+__device__ __forceinline__ float act_bwd(int act, float slope, float z) {
+    if (act == MXO_NONE) return 1.0f;
+    if (act == MXO_LRELU) return z >= 0.0f ? 1.0f : slope;
+    float v, s, d;
+    if (act == MXO_GELU) {
+        // Phi(z) + z phi(z); past |z| = 13 the density's term is below 3e-36
+        const float ax = fabsf(z), t = fminf(ax, 13.0f);
+        const float p = phi_tail(ax), g = 0.3989422804014327f * __builtin_amdgcn_exp2f(t * t * -0.7213475204444817f);
+        v = (z >= 0.0f ? 1.0f - p : p) + copysignf(t, z) * g;
+    } else if (act == MXO_SIGMOID) {
+        logistic(z, s, v);
+    } else if (act == MXO_SILU) {
+        const float c = fminf(fmaxf(z, -1e4f), 1e4f);
+        logistic(c, s, d);
+        v = __builtin_fmaf(c, d, s);
+    } else {
+        const float c = fminf(fmaxf(z, -1e4f), 1e4f);
+        logistic(kTanhA * c * __builtin_fmaf(kTanhB * c, c, 1.0f), s, d);
+        v = __builtin_fmaf(c * d, kTanhA * __builtin_fmaf(3.0f * kTanhB * c, c, 1.0f), s);
+    }
+    return z != z ? z : v;
+}
+
+// Sum over the 64 lanes, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}

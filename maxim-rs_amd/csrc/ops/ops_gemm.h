@@ -1,0 +1,275 @@
+// Matrix products of the Dense operators on the matrix cores.
+//
+// One block computes a BM x BN tile of C over a range of k. Both operands'
+// tiles go through LDS, 128 bytes of k at a time (64 16-bit elements or 32
+// floats), in two buffers: the next tile's loads are in flight while the
+// present one is multiplied. Either operand may be contiguous along k or
+// along its other axis, so no product of a forward or backward pass needs a
+// transposed copy: a 16-bit operand that is not contiguous along k is
+// transposed by ds_read_b64_tr_b16 on its way out of LDS, and an fp32 one is
+// read element by element, which its 16 times slower MFMA hides.
+//
+// The MFMA takes B's rows as its own A operand, so that a lane ends up with
+// four consecutive n of one m and C is written four elements at a time.
+#pragma once
+
+#include "ops_common.h"
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<f16> {
+    typedef f16x8 Frag;
+    static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<float> {
+    typedef f32x4 Frag;  // four k's of the lane's group, one MFMA each
+    static __device__ __forceinline__ f32x4 go(Frag a, Frag b, f32x4 c) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = mfma16(a[e], b[e], c);
+        return c;
+    }
+};
+
+// One operand's tile: ROWS of m (or n) by 128 bytes of k, in 16-byte chunks
+// at LDS positions p * 16. Contiguous along k: position p holds row p / 8, a
+// chunk of its 8 picked by exclusive or with the row, so the 16 rows a
+// fragment takes at one k fall into different banks. Contiguous along rows:
+// position p holds one k's chunk, 16-element segments exchanged likewise.
+template <typename T, bool KMAJ, int ROWS, int NT>
+struct Tile {
+    static constexpr int E = 16 / sizeof(T);    // elements a chunk
+    static constexpr int BK = 128 / sizeof(T);  // k's a tile
+    static constexpr int CHUNKS = ROWS * 8;
+    static constexpr int PER = CHUNKS / NT;     // chunks a thread brings
+    static constexpr int CPR = ROWS / E;        // chunks a k, contiguous along rows
+    static constexpr int G = sizeof(T);         // chunks a 16-element segment
+    static_assert(CHUNKS % NT == 0, "");
+    typedef Vec<T, E> Chunk;
+
+    static __device__ __forceinline__ int kswz(int k) {
+        return sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
+    }
+    // what position p holds: (row, k) of its chunk's first element
+    static __device__ __forceinline__ void where(int p, int &row, int &k) {
+        if (KMAJ) {
+            row = p >> 3;
+            k = ((p & 7) ^ ((row >> 1) & 7)) * E;
+        } else {
+            k = p / CPR;
+            const int c = p % CPR;
+            row = ((((c / G) ^ (kswz(k) & (ROWS / 16 - 1))) * G) + c % G) * E;
+        }
+    }
+    // the chunk of position p from global memory: zeros past the operand's
+    // `rows` rows and `kn` k's (g points at the tile's first element)
+    static __device__ __forceinline__ Chunk load(const T *g, int64_t ld, int p, int rows, int kn) {
+        int row, k;
+        where(p, row, k);
+        const int have = KMAJ ? (row < rows ? kn - k : 0) : (k < kn ? rows - row : 0);
+        return load_upto<T, E>(g + (KMAJ ? row * ld + k : k * ld + row), have);
+    }
+    // Lane l's part of rows [base, base + 16) at k's step kk (half a tile):
+    // row l % 16; k's 8 (l / 16) + 0..7 of the step's 32 (16-bit), or
+    // 4 (l / 16) + 0..3 of its 16 (fp32)
+    static __device__ __forceinline__ typename Mma<T>::Frag frag(const char *lds, int base, int kk, int l) {
+        const int r = l & 15, g = l >> 4;
+        if constexpr (KMAJ) {
+            const int row = base + r;
+            return *reinterpret_cast<const typename Mma<T>::Frag *>(
+                lds + row * 128 + (((kk * 4 + g) ^ ((row >> 1) & 7)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            // each group of 16 lanes reads a 4 x 16 block of (k, row) and
+            // gets it back with lane i holding row i's four k's
+            const int k = kk * 32 + g * 8 + (r >> 2);
+            const int seg = (base >> 4) ^ (((r >> 2) | (g & 1) << 2) & (ROWS / 16 - 1));
+            typedef __attribute__((address_space(3))) i16x4 *LP;
+            const char *p = lds + k * (ROWS * 2) + seg * 32 + (r & 3) * 8;
+            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)p);
+            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(p + 4 * ROWS * 2));
+            const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            return __builtin_bit_cast(typename Mma<T>::Frag, v);
+        } else {
+            typename Mma<T>::Frag v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = kk * 16 + g * 4 + e;
+                const int seg = (base >> 4) ^ (g & (ROWS / 16 - 1));
+                v[e] = *reinterpret_cast<const float *>(lds + k * (ROWS * 4) + seg * 64 + r * 4);
+            }
+            return v;
+        }
+    }
+};
+
+// Bias, z, activation and residual for four consecutive n of row m, rounding
+// once to T at each store. The sum and all of this are fp32.
+template <typename T>
+__device__ __forceinline__ void gemm_finish(const OpsGemmArgs &g, int64_t m, int64_t n, f32x4 v) {
+    const int64_t left = g.n - n;
+    if (m >= g.m || left <= 0) return;
+    const int64_t have = g.vec ? 4 : left;  // vec: n is a multiple of 4
+    if (g.bias) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < have) v[i] += param<T>(g.bias, g.bias_rows ? m : n + i, g.bias_f32);
+    }
+    Vec<T, 4> o;
+    if (g.z) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.v[i] = from_f<T>(v[i]);
+        store_upto<T, 4>(static_cast<T *>(g.z) + m * g.ldz + n, o, have);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = act_fwd(g.act, g.slope, v[i]);
+    if (g.res) {
+        const Vec<T, 4> r = load_upto<T, 4>(static_cast<const T *>(g.res) + m * g.ldr + n, have);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += to_f<T>(r.v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.v[i] = from_f<T>(v[i]);
+    store_upto<T, 4>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
+}
+
+// Which tile and split a block takes. Consecutive blocks go to the 8 XCDs in
+// turn, each with an L2 of its own: ids are dealt so that an XCD walks one
+// contiguous run, and the run goes up 8 tiles of m before it moves along n,
+// so the tiles under one L2 share operands.
+__device__ __forceinline__ void gemm_place(const OpsGemmArgs &g, int &tm, int &tn, int &s) {
+    const int n = gridDim.x, id = blockIdx.x, x = id & 7, q = n >> 3, r = n & 7;
+    int nid = x * q + min(x, r) + (id >> 3);
+    const int tiles = g.tiles_m * g.tiles_n;
+    s = nid / tiles;
+    nid -= s * tiles;
+    const int band = nid / (8 * g.tiles_n), m0 = band * 8, h = min(8, g.tiles_m - m0);
+    nid -= band * 8 * g.tiles_n;
+    tn = nid / h;
+    tm = m0 + nid - tn * h;
+}
+
+// WM x WN waves of 64 lanes, each (BM / WM) x (BN / WN) of the tile.
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_>
+__device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
+    constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+    typedef Tile<T, AK, BM, NT> TA;
+    typedef Tile<T, BK_, BN, NT> TB;
+    constexpr int BK = TA::BK, ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+    int tm, tn, s;
+    gemm_place(g, tm, tn, s);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int kbeg = s * g.kchunk, kend = min(g.k, kbeg + g.kchunk);
+    const int t = threadIdx.x, l = t & 63, w = t >> 6, wm = w / WN * (BM / WM), wn = w % WN * (BN / WN);
+    const int rows_a = min((int64_t)BM, g.m - m0), rows_b = min((int64_t)BN, g.n - n0);
+    const T *ga = static_cast<const T *>(g.a) + (AK ? m0 * g.lda + kbeg : kbeg * g.lda + m0);
+    const T *gb = static_cast<const T *>(g.b) + (BK_ ? n0 * g.ldb + kbeg : kbeg * g.ldb + n0);
+    typename TA::Chunk ra[TA::PER];
+    typename TB::Chunk rb[TB::PER];
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < TA::PER; ++i)
+            ra[i] = TA::load(ga + (AK ? k0 : k0 * g.lda), g.lda, i * NT + t, rows_a, kend - kbeg - k0);
+#pragma unroll
+        for (int i = 0; i < TB::PER; ++i)
+            rb[i] = TB::load(gb + (BK_ ? k0 : k0 * g.ldb), g.ldb, i * NT + t, rows_b, kend - kbeg - k0);
+    };
+    auto put = [&](char *at) {
+#pragma unroll
+        for (int i = 0; i < TA::PER; ++i) *reinterpret_cast<u32x4 *>(at + (i * NT + t) * 16) = __builtin_bit_cast(u32x4, ra[i]);
+#pragma unroll
+        for (int i = 0; i < TB::PER; ++i)
+            *reinterpret_cast<u32x4 *>(at + ABYTES + (i * NT + t) * 16) = __builtin_bit_cast(u32x4, rb[i]);
+    };
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    const int nk = (kend - kbeg + BK - 1) / BK;
+    if (nk > 0) {
+        fetch(0);
+        put(lds);
+    }
+    __syncthreads();
+    for (int kt = 0; kt < nk; ++kt) {
+        const char *at = lds + (kt & 1) * STAGE;
+        if (kt + 1 < nk) fetch((kt + 1) * BK);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            typename Mma<T>::Frag fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = TA::frag(at, wm + i * 16, kk, l);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = TB::frag(at + ABYTES, wn + j * 16, kk, l);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::go(fb[j], fa[i], acc[i][j]);
+        }
+        if (kt + 1 < nk) put(lds + ((kt + 1) & 1) * STAGE);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t m = m0 + wm + i * 16 + (l & 15);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int64_t n = n0 + wn + j * 16 + (l >> 4) * 4;
+            if (g.splits == 1) {
+                gemm_finish<T>(g, m, n, acc[i][j]);
+            } else if (m < g.m) {
+                Vec<float, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.v[e] = acc[i][j][e];
+                store_upto<float, 4>(g.part + ((int64_t)s * g.m + m) * g.n + n, o, g.n - n);
+            }
+        }
+    }
+}
+
+// The splits' sums added in their order, then the epilogue.
+template <typename T>
+__device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
+    const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / quads, n = (i - m * quads) * 4;
+        f32x4 v = {0, 0, 0, 0};
+        for (int s = 0; s < g.splits; ++s) {
+            const Vec<float, 4> p = load_upto<float, 4>(g.part + ((int64_t)s * g.m + m) * g.n + n, g.n - n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += p.v[e];
+        }
+        gemm_finish<T>(g, m, n, v);
+    }
+}
+
+#define OPS_GEMM1(name, T, BM, BN, WM, WN, tag, AK, BK)                                                    \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxo_gemm_##name##_##BM##x##BN##_##tag(      \
+        OpsGemmArgs g) {                                                                                   \
+        __shared__ __align__(128) char lds[2 * (BM + BN) * 128];                                           \
+        gemm_tile<T, BM, BN, WM, WN, AK, BK>(g, lds);                                                      \
+    }
+#define OPS_GEMM(name, T, BM, BN, WM, WN)                    \
+    OPS_GEMM1(name, T, BM, BN, WM, WN, kk, true, true)       \
+    OPS_GEMM1(name, T, BM, BN, WM, WN, km, true, false)      \
+    OPS_GEMM1(name, T, BM, BN, WM, WN, mk, false, true)      \
+    OPS_GEMM1(name, T, BM, BN, WM, WN, mm, false, false)
+
+#define OPS_GEMM_TYPE(name, T)                                                              \
+    OPS_GEMM(name, T, 128, 128, 2, 2)                                                       \
+    OPS_GEMM(name, T, 64, 64, 2, 2)                                                         \
+    extern "C" __global__ __launch_bounds__(256) void mxo_join_##name(OpsGemmArgs g) { gemm_join<T>(g); }
+
+OPS_GEMM_TYPE(bf16, bf16)
+OPS_GEMM_TYPE(f16, f16)
+OPS_GEMM_TYPE(f32, float)
