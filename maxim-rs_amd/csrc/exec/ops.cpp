@@ -210,9 +210,61 @@ void check_act(int act) {
 
 // ------------------------------------------------------------- LayerNorm
 
-int64_t ln_parts(int64_t rows) { return std::min<int64_t>(256, cdiv(rows, 64)); }
+// The kernel of a LayerNorm pass: by rows, `lpr` threads a row with `nv`
+// vectors of 16 bytes each, or in planar order `block` threads with `ch`
+// channels each; `whole` when the row fits the largest of them, else the
+// forms that read it three times. `grid` blocks walk over the rows; in the
+// backward pass each leaves one partial sum of the parameters' gradients.
+struct LnPlan {
+    std::string form;
+    unsigned block = 256;
+    int64_t grid = 1;
+    bool whole = true;
+    int64_t parts = 1;
+};
 
-uint64_t ln_bwd_bytes(const mxh_mat &x) { return (uint64_t)ln_parts(x.rows) * 2 * x.cols * 4; }
+LnPlan ln_plan(int dtype, int64_t rows, int64_t cols, bool by_cols, bool backward) {
+    LnPlan p;
+    const int64_t e = 16 / (int64_t)type_size(dtype), vecs = cdiv(cols, e);
+    if (by_cols) {
+        // the fewest threads that hold the row: sums stay inside a wave up to
+        // 128 vectors
+        static const int kForms[][2] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {1024, 2}};
+        for (const auto &f : kForms) {
+            if (vecs > f[0] * f[1]) continue;
+            p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]);
+            p.block = f[0] == 1024 || (backward && f[0] == 256) ? 1024 : 256;
+            const int64_t steps = cdiv(rows, p.block / f[0]);
+            const int64_t most = p.block == 1024 ? 512 : 2048;
+            // a partial sum costs as much as a row: at least eight rows each,
+            // once every CU has a block
+            p.grid = backward ? std::min(steps, std::max<int64_t>(256, std::min(most / 2, steps / 8))) : std::min(steps, most);
+            break;
+        }
+        if (p.form.empty()) p.form = "long", p.block = 1024, p.grid = std::min<int64_t>(rows, 65536), p.whole = false;
+    } else {
+        const int64_t tiles = cdiv(rows, 64);
+        static const int kForms[][2] = {{256, 1}, {256, 2}, {256, 4}, {256, 8}, {1024, 4}, {1024, 8}};
+        for (const auto &f : kForms) {
+            if (cols > f[0] / (64 / e) * f[1]) continue;
+            p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]);
+            p.block = f[0];
+            p.grid = std::min<int64_t>(tiles, backward ? (f[0] == 256 ? 1024 : 512) : 4096);
+            break;
+        }
+        if (p.form.empty()) p.form = "loop", p.block = 1024, p.grid = std::min<int64_t>(tiles, 65536), p.whole = false;
+    }
+    p.grid = std::max<int64_t>(1, p.grid);
+    p.parts = p.whole ? p.grid : std::min<int64_t>(256, std::max<int64_t>(1, cdiv(rows, 64)));
+    return p;
+}
+
+uint64_t ln_bwd_bytes(const mxh_mat &x) {
+    if (!x.rows) return 0;
+    const int64_t parts = std::max(ln_plan(x.dtype, x.rows, x.cols, true, true).parts,
+                                   ln_plan(x.dtype, x.rows, x.cols, false, true).parts);
+    return (uint64_t)parts * 2 * x.cols * 4;
+}
 
 void join(int dev, void *stream, const float *part, int64_t nparts, int64_t n, void *out0, void *out1, int dtype) {
     if (!n) return;
@@ -358,15 +410,24 @@ struct BwdLayout {
     uint64_t total() const { return dz_bytes + part_bytes + product_bytes; }
 };
 
-BwdLayout bwd_layout(const mxh_mat &dy, const mxh_mat &x, const mxh_mat *dx, const mxh_mat *dw, const mxh_vec *db,
-                     int act) {
+// Blocks enough for the card, 16 rows (or 256 vectors of positions) each at
+// least.
+int64_t dz_parts(const mxh_mat &dy, bool by_cols) {
+    const int64_t e = 16 / (int64_t)type_size(dy.dtype);
+    const int64_t across = by_cols ? cdiv(dy.cols, 64 * e) : dy.cols;
+    const int64_t most = by_cols ? cdiv(dy.rows, 16) : cdiv(dy.rows, 256 * e);
+    return std::max<int64_t>(1, std::min(cdiv(2048, std::max<int64_t>(1, across)), most));
+}
+
+BwdLayout bwd_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mxh_mat *dx, const mxh_mat *dw,
+                     const mxh_vec *db, int act) {
     BwdLayout l;
     l.dz = dy;
     const bool products = dx || dw;
     if (act != MXH_NONE && products) {
         // rows (or planes) padded to 16 bytes, so that the products' loads are
         const int64_t pad = 16 / (int64_t)type_size(dy.dtype);
-        if (along_cols(dy)) {
+        if (by_cols) {
             l.dz.row_stride = cdiv(dy.cols, pad) * pad, l.dz.col_stride = 1;
             l.dz_bytes = up((uint64_t)dy.rows * l.dz.row_stride * type_size(dy.dtype));
         } else {
@@ -375,7 +436,7 @@ BwdLayout bwd_layout(const mxh_mat &dy, const mxh_mat &x, const mxh_mat *dx, con
         }
     }
     if (db) {
-        l.parts = std::min<int64_t>(256, cdiv(dy.rows, 64));
+        l.parts = dz_parts(dy, by_cols);
         l.part_bytes = up((uint64_t)l.parts * dy.cols * 4);
     }
     if (dx) l.product_bytes = std::max(l.product_bytes, product_bytes(*dx, dy.cols, out_by_cols(*dx)));
@@ -448,9 +509,10 @@ int mxh_layernorm(int device, void *stream, const mxh_mat *x, const mxh_vec *sca
         a.yrs = Y.row_stride, a.ycs = Y.col_stride;
         a.eps = eps;
         a.param_f32 = scale->dtype == MXH_F32;
-        (void)by_cols;
-        launch(device, stream, std::string("mxo_ln_any_") + kTypeName[X.dtype], std::min<int64_t>(X.rows, 65536), 1,
-               1024, a);
+        const LnPlan p = ln_plan(X.dtype, X.rows, X.cols, by_cols, false);
+        launch(device, stream,
+               std::string(by_cols ? "mxo_ln_rows_" : "mxo_ln_planar_") + kTypeName[X.dtype] + "_" + p.form, p.grid, 1,
+               p.block, a);
     });
 }
 
@@ -522,15 +584,19 @@ int mxh_layernorm_backward(int device, void *stream, const mxh_mat *dy, const mx
         a.xrs = X.row_stride, a.xcs = X.col_stride;
         if (add) a.add = add->data, a.ars = add->row_stride, a.acs = add->col_stride;
         if (dx) a.dx = dx->data, a.dxrs = dx->row_stride, a.dxcs = dx->col_stride;
-        a.nparts = (int32_t)ln_parts(X.rows);
         a.param_f32 = scale->dtype == MXH_F32;
-        (void)by_cols;
-        // the parameters' gradients first: dx may take dy's place
-        if (dscale) {
-            if (X.rows) launch(device, stream, "mxo_ln_param_any_" + t, cdiv(X.cols, 64), a.nparts, 256, a);
-            join(device, stream, a.part, a.nparts, X.cols, dscale->data, dbias->data, dscale->dtype);
+        const LnPlan p = ln_plan(X.dtype, X.rows, X.cols, by_cols, true);
+        a.nparts = (int32_t)p.parts;
+        const std::string order = by_cols ? "rows_" : "planar_";
+        if (X.rows && dscale && !p.whole) {
+            // before dx, which may take dy's place
+            const int64_t e = by_cols ? 64 * 16 / (int64_t)type_size(X.dtype) : 1;
+            launch(device, stream, "mxo_ln_param_" + order + t, cdiv(X.cols, e), a.nparts, 256, a);
         }
-        if (dx && X.rows) launch(device, stream, "mxo_ln_bwd_any_" + t, std::min<int64_t>(X.rows, 65536), 1, 1024, a);
+        if (!dscale) a.part = nullptr;
+        if (X.rows && (dx || p.whole)) launch(device, stream, "mxo_ln_bwd_" + order + t + "_" + p.form, p.grid, 1, p.block, a);
+        if (dscale)
+            join(device, stream, a.part, X.rows ? p.parts : 0, X.cols, dscale->data, dbias->data, dscale->dtype);
     });
 }
 
@@ -588,7 +654,7 @@ int mxh_dense_backward_workspace(const mxh_mat *dy, const mxh_mat *x, const mxh_
         check_first(need(x, "x"), "x");
         check_mat(need(dy, "dy"), "dy", x->dtype, x->rows, need(w, "w").rows);
         check_act(act);
-        *bytes = bwd_layout(*dy, *x, dx, dw, db, act).total();
+        *bytes = std::max(bwd_layout(*dy, true, *x, dx, dw, db, act).total(), bwd_layout(*dy, false, *x, dx, dw, db, act).total());
     });
 }
 
@@ -613,7 +679,8 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
             check_out(*dw, "dw");
         }
         if (db) check_vec(*db, "db", W.rows, X.dtype);
-        if (z) common_order({dy, z}, {});
+        // z may settle the order of a dy of one row or column
+        const bool dz_cols = common_order({dy, z}, {});
         const mxh_mat dbl = db ? line(*db) : mxh_mat{};
         const mxh_mat *outs[] = {dx, dw, db ? &dbl : nullptr}, *ins[] = {dy, x, w, z};
         const char *on_[] = {"dx", "dw", "db"}, *in_[] = {"dy", "x", "w", "z"};
@@ -624,7 +691,7 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
             for (int j = 0; j < i; ++j)
                 if (outs[j]) refuse_overlap(*outs[i], on_[i], *outs[j], on_[j]);
         }
-        BwdLayout l = bwd_layout(DY, X, dx, dw, db, act);
+        BwdLayout l = bwd_layout(DY, dz_cols, X, dx, dw, db, act);
         check_workspace(workspace, workspace_bytes, l.total());
         OnDevice on(device);
         char *ws = static_cast<char *>(workspace);
@@ -637,11 +704,13 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         if (z) a.z = z->data, a.zrs = z->row_stride, a.zcs = z->col_stride;
         if (l.dz_bytes) l.dz.data = a.dz = ws, a.drs = l.dz.row_stride, a.dcs = l.dz.col_stride;
         if (db) a.part = reinterpret_cast<float *>(ws + l.dz_bytes);
-        a.nparts = (int32_t)(db ? l.parts : std::max<int64_t>(1, std::min<int64_t>(256, cdiv(DY.rows, 64))));
+        a.nparts = (int32_t)dz_parts(DY, dz_cols);
         a.act = act;
         a.slope = slope;
-        if ((a.dz || a.part) && !empty(DY)) launch(device, stream, "mxo_dz_any_" + t, cdiv(DY.cols, 64), a.nparts, 256, a);
-        if (db) join(device, stream, a.part, l.parts, DY.cols, db->data, nullptr, db->dtype);
+        if ((a.dz || a.part) && !empty(DY))
+            launch(device, stream, (dz_cols ? "mxo_dz_rows_" : "mxo_dz_planar_") + t,
+                   dz_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, a);
+        if (db) join(device, stream, a.part, DY.rows ? l.parts : 0, DY.cols, db->data, nullptr, db->dtype);
         void *pw = ws + l.dz_bytes + l.part_bytes;
         if (dx && !empty(*dx))
             product(device, stream, oriented(*dx, operand(l.dz, false), operand(W, true), W.rows, out_by_cols(*dx)), pw);
