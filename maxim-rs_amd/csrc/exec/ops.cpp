@@ -227,15 +227,16 @@ LnPlan ln_plan(int dtype, int64_t rows, int64_t cols, bool by_cols, bool backwar
     LnPlan p;
     const int64_t e = 16 / (int64_t)type_size(dtype), vecs = cdiv(cols, e);
     if (by_cols) {
-        // the fewest threads that hold the row: sums stay inside a wave up to
-        // 128 vectors
-        static const int kForms[][2] = {{8, 1}, {16, 1}, {32, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {1024, 2}};
+        // the fewest threads that hold the row, a vector each: sums stay
+        // inside a wave up to 64 vectors
+        static const int kForms[][2] = {{8, 1},   {16, 1},  {32, 1},  {64, 1},  {128, 1},
+                                        {256, 1}, {512, 1}, {1024, 1}, {1024, 2}};
         for (const auto &f : kForms) {
             if (vecs > f[0] * f[1]) continue;
             p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]);
-            p.block = f[0] == 1024 || (backward && f[0] == 256) ? 1024 : 256;
+            p.block = f[0] <= 64 ? 256 : backward ? 1024 : std::max(256, f[0]);
             const int64_t steps = cdiv(rows, p.block / f[0]);
-            const int64_t most = p.block == 1024 ? 512 : 2048;
+            const int64_t most = 524288 / p.block;
             // a partial sum costs as much as a row: at least eight rows each,
             // once every CU has a block
             p.grid = backward ? std::min(steps, std::max<int64_t>(256, std::min(most / 2, steps / 8))) : std::min(steps, most);
@@ -244,15 +245,15 @@ LnPlan ln_plan(int dtype, int64_t rows, int64_t cols, bool by_cols, bool backwar
         if (p.form.empty()) p.form = "long", p.block = 1024, p.grid = std::min<int64_t>(rows, 65536), p.whole = false;
     } else {
         const int64_t tiles = cdiv(rows, 64);
-        static const int kForms[][2] = {{256, 1}, {256, 2}, {256, 4}, {256, 8}, {1024, 4}, {1024, 8}};
+        static const int kForms[][2] = {{256, 1}, {256, 2}, {256, 4}, {512, 4}, {512, 8}};
         for (const auto &f : kForms) {
             if (cols > f[0] / (64 / e) * f[1]) continue;
             p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]);
             p.block = f[0];
-            p.grid = std::min<int64_t>(tiles, backward ? (f[0] == 256 ? 1024 : 512) : 4096);
+            p.grid = std::min<int64_t>(tiles, backward ? 262144 / f[0] : 4096);
             break;
         }
-        if (p.form.empty()) p.form = "loop", p.block = 1024, p.grid = std::min<int64_t>(tiles, 65536), p.whole = false;
+        if (p.form.empty()) p.form = "loop", p.block = 512, p.grid = std::min<int64_t>(tiles, 65536), p.whole = false;
     }
     p.grid = std::max<int64_t>(1, p.grid);
     p.parts = p.whole ? p.grid : std::min<int64_t>(256, std::max<int64_t>(1, cdiv(rows, 64)));
@@ -276,7 +277,7 @@ void join(int dev, void *stream, const float *part, int64_t nparts, int64_t n, v
     j.nparts = (int32_t)nparts;
     j.nout = out1 ? 2 : 1;
     j.dtype = dtype;
-    launch(dev, stream, "mxo_join_parts", cdiv(n, 64), j.nout, 1024, j);
+    launch(dev, stream, "mxo_join_parts", cdiv(n, 16), j.nout, 1024, j);
 }
 
 // ------------------------------------------------------------- products
@@ -306,27 +307,46 @@ struct Product {
 
 struct Plan {
     int bm = 0, bn = 0;
+    unsigned block = 256;
+    bool direct = false;
     int64_t splits = 1, kchunk = 0;
     uint64_t bytes = 0;
 };
 
-// 128 x 128 tiles where there are enough of them for the 256 CUs, else
-// 64 x 64; and where these are few too, k in up to 64 runs, each at least
-// four LDS tiles long.
-Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k) {
+// Tiles: 256 x 256 straight to LDS where the operands allow it and there are
+// tiles for most of the 256 CUs, else 128 x 128, else 64 x 64; and where these
+// are few too, k in up to 64 runs, each at least four LDS tiles long.
+Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct) {
     Plan p;
-    p.bm = p.bn = cdiv(m, 128) * cdiv(n, 128) >= 256 ? 128 : 64;
-    const int64_t tiles = cdiv(m, p.bm) * cdiv(n, p.bn), bk = 128 / (int64_t)type_size(dtype);
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, tiles), cdiv(k, 4 * bk), 64}));
+    auto tiles = [&](int b) { return cdiv(m, b) * cdiv(n, b); };
+    p.direct = direct;
+    const int b = direct && tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+    if (b == 64) p.direct = false;
+    p.bm = p.bn = b;
+    p.block = b == 256 ? 512 : 256;
+    const int64_t bk = 128 / (int64_t)type_size(dtype);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, tiles(b)), cdiv(k, 4 * bk), 64}));
     p.kchunk = std::max<int64_t>(bk, cdiv(cdiv(k, splits), bk) * bk);
     p.splits = std::max<int64_t>(1, cdiv(k, p.kchunk));
     p.bytes = p.splits > 1 ? (uint64_t)p.splits * m * n * 4 : 0;
     return p;
 }
 
+// Whether an operand's tiles can go straight to LDS: 16-byte loads of whole
+// chunks, at 32-bit offsets inside a tile of `tile` rows (or 64 k's).
+bool loads_direct(const Operand &o, bool by_k, int64_t own_n, int64_t sum_n, size_t size) {
+    const int64_t ld = by_k ? o.own : o.sum, extent = by_k ? sum_n : own_n;
+    return size == 2 && (uintptr_t)o.data % 16 == 0 && ld % 8 == 0 && extent % 8 == 0 && ld < (int64_t(1) << 21);
+}
+
 void product(int dev, void *stream, const Product &p, void *ws) {
     if (!p.m || !p.n) return;
-    const Plan pl = plan_product(p.dtype, p.m, p.n, p.k);
+    // contiguous along k (also where there is only one row to stride over),
+    // or along the operand's own axis
+    const bool ak = p.a.sum == 1, bk = p.b.sum == 1;
+    const size_t size = type_size(p.dtype);
+    const Plan pl = plan_product(p.dtype, p.m, p.n, p.k,
+                                 loads_direct(p.a, ak, p.m, p.k, size) && loads_direct(p.b, bk, p.n, p.k, size));
     OpsGemmArgs g{};
     g.a = p.a.data;
     g.b = p.b.data;
@@ -334,9 +354,6 @@ void product(int dev, void *stream, const Product &p, void *ws) {
     g.z = p.z;
     g.res = p.res;
     g.part = static_cast<float *>(ws);
-    // contiguous along k (also where there is only one row to stride over),
-    // or along the operand's own axis
-    const bool ak = p.a.sum == 1, bk = p.b.sum == 1;
     g.lda = ak ? p.a.own : p.a.sum;
     g.ldb = bk ? p.b.own : p.b.sum;
     g.ldc = p.ldc;
@@ -362,10 +379,15 @@ void product(int dev, void *stream, const Product &p, void *ws) {
     const std::string t = kTypeName[p.dtype];
     launch(dev, stream,
            "mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
-               (bk ? "k" : "m"),
-           tm * tn * pl.splits, 1, 256, g);
+               (bk ? "k" : "m") + (pl.direct ? "_d" : ""),
+           tm * tn * pl.splits, 1, pl.block, g);
     if (pl.splits > 1)
-        launch(dev, stream, "mxo_join_" + t, std::min<int64_t>(2048, cdiv(p.m * cdiv(p.n, 4), 256)), 1, 256, g);
+        {
+        // few sums of many splits: eight threads to each
+        const bool deep = pl.splits >= 16;
+        launch(dev, stream, (deep ? "mxo_join8_" : "mxo_join_") + t,
+               std::min<int64_t>(4096, cdiv(p.m * cdiv(p.n, 4), deep ? 32 : 256)), 1, 256, g);
+    }
 }
 
 // An operand of a product as (own axis, summed axis): rows summed over or not.
@@ -393,10 +415,11 @@ Product oriented(const mxh_mat &out, const Operand &rows, const Operand &cols, i
     return p;
 }
 
+// What a product may need, whichever way its operands load.
 uint64_t product_bytes(const mxh_mat &out, int64_t k, bool by_cols) {
     if (empty(out)) return 0;
-    return by_cols ? plan_product(out.dtype, out.rows, out.cols, k).bytes
-                   : plan_product(out.dtype, out.cols, out.rows, k).bytes;
+    const int64_t m = by_cols ? out.rows : out.cols, n = by_cols ? out.cols : out.rows;
+    return std::max(plan_product(out.dtype, m, n, k, false).bytes, plan_product(out.dtype, m, n, k, true).bytes);
 }
 
 uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }

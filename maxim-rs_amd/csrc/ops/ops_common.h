@@ -56,6 +56,39 @@ __device__ __forceinline__ void store_upto(T *p, const Vec<T, N> &v, int64_t hav
         if (i < have) p[i] = v.v[i];
 }
 
+// E elements at p, of which the first `have` are the operand's, the others
+// zeros. WHOLE: all of them or none (the extent is a multiple of E), which
+// takes no branch: where there are none, E elements at `any`, which are the
+// operand's too, are loaded and dropped.
+template <typename T, int E, bool WHOLE>
+__device__ __forceinline__ Vec<T, E> load_in(const T *p, const T *any, int64_t have) {
+    if constexpr (!WHOLE) return load_upto<T, E>(p, have);
+    Vec<T, E> r = load_n<T, E>(have > 0 ? p : any);
+#pragma unroll
+    for (int i = 0; i < E; ++i) r.v[i] = have > 0 ? r.v[i] : (T)0.0f;
+    return r;
+}
+template <typename T, int E, bool WHOLE>
+__device__ __forceinline__ void store_in(T *p, const Vec<T, E> &v, int64_t have) {
+    if constexpr (WHOLE) {
+        if (have > 0) store_n<T, E>(p, v);
+    } else {
+        store_upto<T, E>(p, v, have);
+    }
+}
+
+// The same value, of which the compiler keeps nothing it worked out before:
+// 16-bit elements are converted again from here on, instead of held as fp32
+// in twice the registers.
+template <typename T, int E>
+__device__ __forceinline__ void reread(Vec<T, E> &v) {
+    static_assert(sizeof(v) == 16, "");
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+    asm volatile("" : "+v"(w));
+    typedef Vec<T, E> V;
+    v = __builtin_bit_cast(V, w);
+}
+
 // A parameter vector's element, of the activations' type or fp32.
 template <typename T>
 __device__ __forceinline__ float param(const void *p, int64_t i, int f32) {

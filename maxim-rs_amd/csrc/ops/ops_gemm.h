@@ -41,6 +41,8 @@ struct Mma<float> {
     }
 };
 
+typedef __attribute__((address_space(3))) char LdsChar;
+
 // One operand's tile: ROWS of m (or n) by 128 bytes of k, in 16-byte chunks
 // at LDS positions p * 16. Contiguous along k: position p holds row p / 8, a
 // chunk of its 8 picked by exclusive or with the row, so the 16 rows a
@@ -82,21 +84,21 @@ struct Tile {
     // Lane l's part of rows [base, base + 16) at k's step kk (half a tile):
     // row l % 16; k's 8 (l / 16) + 0..7 of the step's 32 (16-bit), or
     // 4 (l / 16) + 0..3 of its 16 (fp32)
-    static __device__ __forceinline__ typename Mma<T>::Frag frag(const char *lds, int base, int kk, int l) {
+    static __device__ __forceinline__ typename Mma<T>::Frag frag(const LdsChar *lds, int base, int kk, int l) {
+        typedef const __attribute__((address_space(3))) typename Mma<T>::Frag *FP;
         const int r = l & 15, g = l >> 4;
         if constexpr (KMAJ) {
             const int row = base + r;
-            return *reinterpret_cast<const typename Mma<T>::Frag *>(
-                lds + row * 128 + (((kk * 4 + g) ^ ((row >> 1) & 7)) << 4));
+            return *(FP)(lds + (row * 128 + (((kk * 4 + g) ^ ((row >> 1) & 7)) << 4)));
         } else if constexpr (sizeof(T) == 2) {
             // each group of 16 lanes reads a 4 x 16 block of (k, row) and
             // gets it back with lane i holding row i's four k's
             const int k = kk * 32 + g * 8 + (r >> 2);
             const int seg = (base >> 4) ^ (((r >> 2) | (g & 1) << 2) & (ROWS / 16 - 1));
             typedef __attribute__((address_space(3))) i16x4 *LP;
-            const char *p = lds + k * (ROWS * 2) + seg * 32 + (r & 3) * 8;
-            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)p);
-            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(p + 4 * ROWS * 2));
+            const int at = k * (ROWS * 2) + seg * 32 + (r & 3) * 8;
+            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(lds + at));
+            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(lds + (at + 4 * ROWS * 2)));
             const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             return __builtin_bit_cast(typename Mma<T>::Frag, v);
         } else {
@@ -105,7 +107,7 @@ struct Tile {
             for (int e = 0; e < 4; ++e) {
                 const int k = kk * 16 + g * 4 + e;
                 const int seg = (base >> 4) ^ (g & (ROWS / 16 - 1));
-                v[e] = *reinterpret_cast<const float *>(lds + k * (ROWS * 4) + seg * 64 + r * 4);
+                v[e] = *(const __attribute__((address_space(3))) float *)(lds + (k * (ROWS * 4) + seg * 64 + r * 4));
             }
             return v;
         }
@@ -158,6 +160,29 @@ __device__ __forceinline__ void gemm_place(const OpsGemmArgs &g, int &tm, int &t
     tm = m0 + nid - tn * h;
 }
 
+// A wave's FM x FN blocks of 16 x 16 from (m0, n0) on: finished, or as split
+// s's partial sums.
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l,
+                                           const f32x4 (&acc)[FM][FN]) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t m = m0 + i * 16 + (l & 15);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int64_t n = n0 + j * 16 + (l >> 4) * 4;
+            if (g.splits == 1) {
+                gemm_finish<T>(g, m, n, acc[i][j]);
+            } else if (m < g.m) {
+                Vec<float, 4> o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o.v[e] = acc[i][j][e];
+                store_upto<float, 4>(g.part + ((int64_t)s * g.m + m) * g.n + n, o, g.n - n);
+            }
+        }
+    }
+}
+
 // WM x WN waves of 64 lanes, each (BM / WM) x (BN / WN) of the tile.
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_>
 __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
@@ -202,7 +227,7 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
     }
     __syncthreads();
     for (int kt = 0; kt < nk; ++kt) {
-        const char *at = lds + (kt & 1) * STAGE;
+        const LdsChar *at = (LdsChar *)lds + (kt & 1) * STAGE;
         if (kt + 1 < nk) fetch((kt + 1) * BK);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -219,37 +244,38 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
         if (kt + 1 < nk) put(lds + ((kt + 1) & 1) * STAGE);
         __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t m = m0 + wm + i * 16 + (l & 15);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t n = n0 + wn + j * 16 + (l >> 4) * 4;
-            if (g.splits == 1) {
-                gemm_finish<T>(g, m, n, acc[i][j]);
-            } else if (m < g.m) {
-                Vec<float, 4> o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = acc[i][j][e];
-                store_upto<float, 4>(g.part + ((int64_t)s * g.m + m) * g.n + n, o, g.n - n);
-            }
-        }
-    }
+    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, acc);
 }
 
-// The splits' sums added in their order, then the epilogue.
-template <typename T>
+// The splits' sums added in a fixed order, then the epilogue: WAYS threads to
+// four results, each every WAYS-th split, joined through LDS.
+template <typename T, int WAYS>
 __device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
-    const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / quads, n = (i - m * quads) * 4;
+    constexpr int Q = 256 / WAYS;
+    __shared__ f32x4 sh[WAYS > 1 ? 256 : 1];
+    const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m, plane = (int64_t)g.m * g.n;
+    const int q = threadIdx.x % Q, way = threadIdx.x / Q;
+    for (int64_t i0 = (int64_t)blockIdx.x * Q; i0 < total; i0 += (int64_t)gridDim.x * Q) {
+        const int64_t i = i0 + q, m = i / quads, n = (i - m * quads) * 4;
         f32x4 v = {0, 0, 0, 0};
-        for (int s = 0; s < g.splits; ++s) {
-            const Vec<float, 4> p = load_upto<float, 4>(g.part + ((int64_t)s * g.m + m) * g.n + n, g.n - n);
+        if (i < total) {
+            const float *p = g.part + m * g.n + n;
+#pragma unroll 4
+            for (int s = way; s < g.splits; s += WAYS) {
+                const Vec<float, 4> o = load_upto<float, 4>(p + s * plane, g.n - n);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += p.v[e];
+                for (int e = 0; e < 4; ++e) v[e] += o.v[e];
+            }
         }
-        gemm_finish<T>(g, m, n, v);
+        if constexpr (WAYS > 1) {
+            __syncthreads();
+            sh[threadIdx.x] = v;
+            __syncthreads();
+            if (way) continue;
+#pragma unroll
+            for (int k = 1; k < WAYS; ++k) v += sh[k * Q + q];
+        }
+        if (i < total) gemm_finish<T>(g, m, n, v);
     }
 }
 
@@ -268,7 +294,8 @@ __device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
 #define OPS_GEMM_TYPE(name, T)                                                              \
     OPS_GEMM(name, T, 128, 128, 2, 2)                                                       \
     OPS_GEMM(name, T, 64, 64, 2, 2)                                                         \
-    extern "C" __global__ __launch_bounds__(256) void mxo_join_##name(OpsGemmArgs g) { gemm_join<T>(g); }
+    extern "C" __global__ __launch_bounds__(256) void mxo_join_##name(OpsGemmArgs g) { gemm_join<T, 1>(g); }                \
+    extern "C" __global__ __launch_bounds__(256) void mxo_join8_##name(OpsGemmArgs g) { gemm_join<T, 8>(g); }
 
 OPS_GEMM_TYPE(bf16, bf16)
 OPS_GEMM_TYPE(f16, f16)

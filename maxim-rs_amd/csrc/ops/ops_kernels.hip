@@ -3,3 +3,4 @@
 // plans never loads it.
 #include "ops_rows.h"
 #include "ops_gemm.h"
+#include "ops_gemm_big.h"

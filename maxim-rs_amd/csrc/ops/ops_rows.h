@@ -42,34 +42,34 @@ __device__ __forceinline__ void row_sum2(float &a, float &b, float *at, int turn
 // LayerNorm of rows with contiguous columns: LPR threads a row, NV vectors of
 // 16 bytes a thread, so a row of up to LPR * NV * 16 bytes stays in
 // registers between the mean, the variance about it and the result. The
-// parameters are read once a block, which walks over rows.
-template <typename T, int LPR, int NV, int BT>
-__device__ __forceinline__ void ln_rows(const OpsLnArgs &a) {
+// parameters are read once a block, which walks over rows. WHOLE: rows are
+// whole vectors.
+template <typename T, int LPR, int NV, int BT, bool WHOLE>
+__device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
     constexpr int E = 16 / sizeof(T), RPB = BT / LPR;
-    __shared__ float at[4 * (BT / 64)];
     const int li = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    const int cols = (int)a.cols;
     const float n = (float)a.cols;
     float sc[NV][E], bi[NV][E];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int64_t c = (int64_t)(j * LPR + li) * E;
+        const int c = (j * LPR + li) * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            sc[j][e] = c + e < a.cols ? param<T>(a.scale, c + e, a.param_f32) : 0.0f;
-            bi[j][e] = a.bias && c + e < a.cols ? param<T>(a.bias, c + e, a.param_f32) : 0.0f;
+            sc[j][e] = c + e < cols ? param<T>(a.scale, c + e, a.param_f32) : 0.0f;
+            bi[j][e] = a.bias && c + e < cols ? param<T>(a.bias, c + e, a.param_f32) : 0.0f;
         }
     }
     int turn = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t r = r0 + grp;
-        const bool on = r < a.rows;
-        const T *x = static_cast<const T *>(a.x) + (on ? r : 0) * a.xrs;
+        const int64_t r = min(r0 + grp, a.rows - 1);  // past the end: the last row again, not stored
+        const T *x = static_cast<const T *>(a.x) + r * a.xrs;
         Vec<T, E> v[NV];
         float s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(j * LPR + li) * E;
-            v[j] = load_upto<T, E>(x + c, on ? a.cols - c : 0);
+            const int c = (j * LPR + li) * E;
+            v[j] = load_in<T, E, WHOLE>(x + c, x, cols - c);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -77,27 +77,26 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a) {
             for (int e = 0; e < E; ++e) s += to_f<T>(v[j].v[e]);
         float zero = 0.0f;
         row_sum2<LPR, BT>(s, zero, at, turn++);
-        // a division: the mean of equal values is that value
-        const float mean = s / n;
+        const float mean = s / n;  // a division: the mean of equal values is that value
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float d = to_f<T>(v[j].v[e]) - mean;
-                q += (int64_t)(j * LPR + li) * E + e < a.cols ? d * d : 0.0f;
+                q += (j * LPR + li) * E + e < cols ? d * d : 0.0f;
             }
         zero = 0.0f;
         row_sum2<LPR, BT>(q, zero, at, turn++);
         const float rstd = 1.0f / sqrtf(q / n + a.eps);
-        if (!on) continue;  // a whole group, behind its last barrier of the round
+        if (r0 + grp >= a.rows) continue;  // behind the round's last barrier
         T *y = static_cast<T *>(a.y) + r * a.yrs;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(j * LPR + li) * E;
+            const int c = (j * LPR + li) * E;
             Vec<T, E> o;
 #pragma unroll
             for (int e = 0; e < E; ++e) o.v[e] = from_f<T>((to_f<T>(v[j].v[e]) - mean) * rstd * sc[j][e] + bi[j][e]);
-            store_upto<T, E>(y + c, o, a.cols - c);
+            store_in<T, E, WHOLE>(y + c, o, cols - c);
         }
         if (li == 0) {
             if (a.mean) a.mean[r] = mean;
@@ -108,73 +107,91 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a) {
 
 // The backward pass in the same arrangement: dx from registers, the
 // parameters' gradients summed in registers over the block's rows, then over
-// its row groups in LDS.
-template <typename T, int LPR, int NV, int BT>
-__device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a) {
+// its row groups in LDS. With one vector a thread the next row's are loaded
+// before the present row's sums, whose barrier a large block's waves share;
+// two vectors leave no registers for that.
+template <typename T, int LPR, int NV, int BT, bool WHOLE>
+__device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, float *sums) {
     constexpr int E = 16 / sizeof(T), RPB = BT / LPR;
-    __shared__ float at[4 * (BT / 64)];
-    __shared__ float sums[RPB > 1 ? BT * NV * E : 1];
+    constexpr bool KEEP = NV == 1;  // the scale in registers; two vectors' would not leave room
     const int li = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+    const int cols = (int)a.cols;
     const float n = (float)a.cols;
-    float sc[NV][E], ds[NV][E], db[NV][E];
+    float sc[KEEP ? E : 1], ds[NV][E], db[NV][E];
+    if constexpr (KEEP)
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int64_t c = (int64_t)(j * LPR + li) * E;
+        for (int e = 0; e < E; ++e) sc[e] = li * E + e < cols ? param<T>(a.scale, li * E + e, a.param_f32) : 0.0f;
+    auto scale = [&](int j, int e) {
+        if constexpr (KEEP) return sc[e];
+        const int c = (j * LPR + li) * E + e;
+        return c < cols ? param<T>(a.scale, c, a.param_f32) : 0.0f;
+    };
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            sc[j][e] = c + e < a.cols ? param<T>(a.scale, c + e, a.param_f32) : 0.0f;
-            ds[j][e] = db[j][e] = 0.0f;
-        }
-    }
-    int turn = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t r = r0 + grp;
-        const bool on = r < a.rows;
-        const int64_t rr = on ? r : 0;
-        const float mean = a.mean[rr], rstd = on ? a.rstd[rr] : 0.0f;
-        Vec<T, E> vx[NV], vd[NV], va[NV];
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) ds[j][e] = db[j][e] = 0.0f;
+    Vec<T, E> vx[NV], vd[NV], va[NV];
+    float mean = 0.0f, rstd = 0.0f;
+    auto fetch = [&](int64_t r0) {
+        const int64_t r = min(r0 + grp, a.rows - 1);  // past the end: the last row again, not stored
+        const T *x = static_cast<const T *>(a.x) + r * a.xrs, *dy = static_cast<const T *>(a.dy) + r * a.dyrs;
+        const T *add = static_cast<const T *>(a.add) + r * a.ars;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int64_t c = (int64_t)(j * LPR + li) * E, have = on ? a.cols - c : 0;
-            vx[j] = load_upto<T, E>(static_cast<const T *>(a.x) + rr * a.xrs + c, have);
-            vd[j] = load_upto<T, E>(static_cast<const T *>(a.dy) + rr * a.dyrs + c, have);
-            if (a.add) va[j] = load_upto<T, E>(static_cast<const T *>(a.add) + rr * a.ars + c, have);
+            const int c = (j * LPR + li) * E;
+            vx[j] = load_in<T, E, WHOLE>(x + c, x, cols - c);
+            vd[j] = load_in<T, E, WHOLE>(dy + c, dy, cols - c);
+            if (a.add) va[j] = load_in<T, E, WHOLE>(add + c, add, cols - c);
         }
+        mean = a.mean[r];
+        rstd = a.rstd[r];
+    };
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int turn = 0;
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    if (KEEP && r0 < a.rows) fetch(r0);
+    for (; r0 < a.rows; r0 += step) {
+        const bool on = r0 + grp < a.rows;
+        if (!KEEP) fetch(r0);
+        Vec<T, E> cx[NV], cd[NV], ca[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) cx[j] = vx[j], cd[j] = vd[j], ca[j] = va[j];
+        const float m = mean, rs = rstd;
+        if (KEEP && r0 + step < a.rows) fetch(r0 + step);
         float s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                // past the row's end dy is 0, and so is what it adds (x's 0
-                // makes a finite xh there: mean and rstd are the row's own)
-                const float dy = to_f<T>(vd[j].v[e]);
-                const bool in = (int64_t)(j * LPR + li) * E + e < a.cols;
-                const float xh = in && on ? (to_f<T>(vx[j].v[e]) - mean) * rstd : 0.0f;
-                const float g = dy * sc[j][e];
+                const bool in = on && (j * LPR + li) * E + e < cols;
+                const float dy = in ? to_f<T>(cd[j].v[e]) : 0.0f;
+                const float xh = in ? (to_f<T>(cx[j].v[e]) - m) * rs : 0.0f;
+                const float g = dy * scale(j, e);
                 s += g;
                 q += g * xh;
                 ds[j][e] += dy * xh;
                 db[j][e] += dy;
             }
-        if (a.dx) {
-            row_sum2<LPR, BT>(s, q, at, turn++);
-            s /= n;
-            q /= n;
-            if (on) {
+        if (!a.dx) continue;
+        row_sum2<LPR, BT>(s, q, at, turn++);
+        s /= n;
+        q /= n;
+        if (!on) continue;
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int64_t c = (int64_t)(j * LPR + li) * E;
-                    Vec<T, E> o;
+        for (int j = 0; j < NV; ++j) reread(cx[j]), reread(cd[j]);
+        T *dx = static_cast<T *>(a.dx) + (r0 + grp) * a.dxrs;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float xh = (to_f<T>(vx[j].v[e]) - mean) * rstd;
-                        float v = rstd * (to_f<T>(vd[j].v[e]) * sc[j][e] - s - xh * q);
-                        if (a.add) v += to_f<T>(va[j].v[e]);
-                        o.v[e] = from_f<T>(v);
-                    }
-                    store_upto<T, E>(static_cast<T *>(a.dx) + r * a.dxrs + c, o, a.cols - c);
-                }
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * LPR + li) * E;
+            Vec<T, E> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float xh = (to_f<T>(cx[j].v[e]) - m) * rs;
+                float v = rs * (to_f<T>(cd[j].v[e]) * scale(j, e) - s - xh * q);
+                if (a.add) v += to_f<T>(ca[j].v[e]);
+                o.v[e] = from_f<T>(v);
             }
+            store_in<T, E, WHOLE>(dx + c, o, cols - c);
         }
     }
     if (!a.part) return;
@@ -188,7 +205,7 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) sums[grp * (LPR * NV * E) + (j * LPR + li) * E + e] = which ? db[j][e] : ds[j][e];
             __syncthreads();
-            for (int i = threadIdx.x; i < LPR * NV * E && i < a.cols; i += BT) {
+            for (int i = threadIdx.x; i < LPR * NV * E && i < cols; i += BT) {
                 float s = 0.0f;
 #pragma unroll 4
                 for (int g = 0; g < RPB; ++g) s += sums[g * (LPR * NV * E) + i];
@@ -197,11 +214,11 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a) {
         } else {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int64_t c = (int64_t)(j * LPR + li) * E;
+                const int c = (j * LPR + li) * E;
                 Vec<float, E> o;
 #pragma unroll
                 for (int e = 0; e < E; ++e) o.v[e] = which ? db[j][e] : ds[j][e];
-                store_upto<float, E>(part + which * a.cols + c, o, a.cols - c);
+                store_upto<float, E>(part + which * a.cols + c, o, cols - c);
             }
         }
     }
@@ -230,7 +247,7 @@ struct PlanarTile {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             float s = 0.0f;
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < W; ++i) s += at[i * 64 + p + e];
             v[e] = s;
         }
@@ -238,14 +255,15 @@ struct PlanarTile {
 };
 
 // LOOP: any number of channels, read again for each of the three passes.
-template <typename T, int BT, int CH, bool LOOP>
-__device__ __forceinline__ void ln_planar(const OpsLnArgs &a) {
+// WHOLE: the positions are whole vectors.
+template <typename T, int BT, int CH, bool LOOP, bool WHOLE>
+__device__ __forceinline__ void ln_planar(const OpsLnArgs &a, float *at) {
     typedef PlanarTile<T, BT> P;
     constexpr int E = P::E, LP = P::LP, S = P::S;
-    __shared__ float at[P::W * 64];
     const int pl = threadIdx.x % LP, sl = threadIdx.x / LP;
     const float n = (float)a.cols;
     const int rounds = LOOP ? (int)((a.cols + S * CH - 1) / (S * CH)) : 1;
+    const T *x = static_cast<const T *>(a.x);
     for (int64_t p0 = (int64_t)blockIdx.x * 64; p0 < a.rows; p0 += (int64_t)gridDim.x * 64) {
         const int64_t p = p0 + pl * E, have = a.rows - p;
         Vec<T, E> v[CH];
@@ -253,7 +271,7 @@ __device__ __forceinline__ void ln_planar(const OpsLnArgs &a) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int64_t c = ((int64_t)round * CH + j) * S + sl;
-                v[j] = load_upto<T, E>(static_cast<const T *>(a.x) + c * a.xcs + p, c < a.cols ? have : 0);
+                v[j] = load_in<T, E, WHOLE>(x + c * a.xcs + p, x, c < a.cols ? have : 0);
             }
         };
         float s[E], q[E];
@@ -294,7 +312,7 @@ __device__ __forceinline__ void ln_planar(const OpsLnArgs &a) {
                 Vec<T, E> o;
 #pragma unroll
                 for (int e = 0; e < E; ++e) o.v[e] = from_f<T>((to_f<T>(v[j].v[e]) - s[e]) * q[e] * sc + bi);
-                store_upto<T, E>(static_cast<T *>(a.y) + c * a.ycs + p, o, have);
+                store_in<T, E, WHOLE>(static_cast<T *>(a.y) + c * a.ycs + p, o, have);
             }
         }
         if (sl == 0) {
@@ -307,14 +325,14 @@ __device__ __forceinline__ void ln_planar(const OpsLnArgs &a) {
     }
 }
 
-template <typename T, int BT, int CH, bool LOOP>
-__device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a) {
+template <typename T, int BT, int CH, bool LOOP, bool WHOLE>
+__device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a, float *at) {
     typedef PlanarTile<T, BT> P;
     constexpr int E = P::E, LP = P::LP, S = P::S;
-    __shared__ float at[P::W * 64];
     const int pl = threadIdx.x % LP, sl = threadIdx.x / LP;
     const float n = (float)a.cols;
     const int rounds = LOOP ? (int)((a.cols + S * CH - 1) / (S * CH)) : 1;
+    const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy), *add = static_cast<const T *>(a.add);
     float ds[CH], db[CH];
 #pragma unroll
     for (int j = 0; j < CH; ++j) ds[j] = db[j] = 0.0f;
@@ -325,8 +343,8 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int64_t c = ((int64_t)round * CH + j) * S + sl, left = c < a.cols ? have : 0;
-                vx[j] = load_upto<T, E>(static_cast<const T *>(a.x) + c * a.xcs + p, left);
-                vd[j] = load_upto<T, E>(static_cast<const T *>(a.dy) + c * a.dycs + p, left);
+                vx[j] = load_in<T, E, WHOLE>(x + c * a.xcs + p, x, left);
+                vd[j] = load_in<T, E, WHOLE>(dy + c * a.dycs + p, dy, left);
             }
         };
         fetch(0);
@@ -344,11 +362,11 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a) {
                 const float sc = in ? param<T>(a.scale, c, a.param_f32) : 0.0f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float dy = to_f<T>(vd[j].v[e]);
+                    const float d = to_f<T>(vd[j].v[e]);
                     const float xh = in ? (to_f<T>(vx[j].v[e]) - m.v[e]) * r.v[e] : 0.0f;
-                    s[e] += dy * sc;
-                    q[e] += dy * sc * xh;
-                    if (!LOOP) ds[j] += dy * xh, db[j] += dy;
+                    s[e] += d * sc;
+                    q[e] += d * sc * xh;
+                    if (!LOOP) ds[j] += d * xh, db[j] += d;
                 }
             }
         }
@@ -357,6 +375,8 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a) {
         P::sum(q, at);
 #pragma unroll
         for (int e = 0; e < E; ++e) s[e] /= n, q[e] /= n;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) reread(vx[j]), reread(vd[j]);
         for (int round = 0; round < rounds; ++round) {
             if (LOOP) fetch(round);
 #pragma unroll
@@ -365,7 +385,7 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a) {
                 if (c >= a.cols) continue;
                 const float sc = param<T>(a.scale, c, a.param_f32);
                 Vec<T, E> o, va;
-                if (a.add) va = load_upto<T, E>(static_cast<const T *>(a.add) + c * a.acs + p, have);
+                if (a.add) va = load_in<T, E, WHOLE>(add + c * a.acs + p, add, have);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float xh = (to_f<T>(vx[j].v[e]) - m.v[e]) * r.v[e];
@@ -373,7 +393,7 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a) {
                     if (a.add) v += to_f<T>(va.v[e]);
                     o.v[e] = from_f<T>(v);
                 }
-                store_upto<T, E>(static_cast<T *>(a.dx) + c * a.dxcs + p, o, have);
+                store_in<T, E, WHOLE>(static_cast<T *>(a.dx) + c * a.dxcs + p, o, have);
             }
         }
     }
@@ -516,10 +536,9 @@ __device__ __forceinline__ void ln_param_planar(const OpsLnBwdArgs &a) {
 
 // dz = dy act'(z) and the bias's partial sums. Rows with contiguous columns:
 // 64 x E columns by a run of rows a block, a wave a row at a time.
-template <typename T>
-__device__ __forceinline__ void dz_rows(const OpsDzArgs &a) {
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void dz_rows(const OpsDzArgs &a, float (*sh)[64 * 16 / sizeof(T)]) {
     constexpr int E = 16 / sizeof(T);
-    __shared__ float sh[4][64 * E];
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + l) * E, p = blockIdx.y, have = a.cols - c;
     const int64_t chunk = (a.rows + a.nparts - 1) / a.nparts, end = min(a.rows, (p + 1) * chunk);
@@ -528,9 +547,9 @@ __device__ __forceinline__ void dz_rows(const OpsDzArgs &a) {
     for (int e = 0; e < E; ++e) s[e] = 0.0f;
     if (have > 0)
         for (int64_t r = p * chunk + w; r < end; r += 4) {
-            Vec<T, E> vd = load_upto<T, E>(static_cast<const T *>(a.dy) + r * a.dyrs + c, have);
-            Vec<T, E> vz;
-            if (a.z) vz = load_upto<T, E>(static_cast<const T *>(a.z) + r * a.zrs + c, have);
+            const T *dy = static_cast<const T *>(a.dy) + r * a.dyrs + c, *z = static_cast<const T *>(a.z) + r * a.zrs + c;
+            Vec<T, E> vd = load_in<T, E, WHOLE>(dy, dy, have), vz;
+            if (a.z) vz = load_in<T, E, WHOLE>(z, z, have);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 float v = to_f<T>(vd.v[e]);
@@ -538,7 +557,7 @@ __device__ __forceinline__ void dz_rows(const OpsDzArgs &a) {
                 s[e] += v;
                 vd.v[e] = from_f<T>(v);
             }
-            if (a.dz) store_upto<T, E>(static_cast<T *>(a.dz) + r * a.drs + c, vd, have);
+            if (a.dz) store_in<T, E, WHOLE>(static_cast<T *>(a.dz) + r * a.drs + c, vd, have);
         }
     if (!a.part) return;
 #pragma unroll
@@ -577,74 +596,85 @@ __device__ __forceinline__ void dz_planar(const OpsDzArgs &a) {
     if (threadIdx.x == 0) a.part[p * a.cols + c] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// Partial sums added in a fixed order: 16 rows of 64 columns a block, each
-// wave a sixteenth of the parts, then the waves' sums.
 __device__ __forceinline__ void join_store(void *out, int dtype, int64_t i, float v) {
     if (dtype == MXO_F32) static_cast<float *>(out)[i] = v;
     else if (dtype == MXO_F16) static_cast<f16 *>(out)[i] = from_f<f16>(v);
     else static_cast<bf16 *>(out)[i] = from_f<bf16>(v);
 }
+// Partial sums added in a fixed order: 16 columns a block, 64 threads down
+// the parts, eight loads in flight each, then a tree over the 64 in LDS. (64
+// columns a block walked 1024 parts of 32 columns in 17 us, this in 4.)
 extern "C" __global__ __launch_bounds__(1024) void mxo_join_parts(OpsJoinArgs a) {
-    __shared__ float sh[16][64];
-    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, which = blockIdx.y;
-    const int64_t c = (int64_t)blockIdx.x * 64 + l;
+    __shared__ float sh[64][17];
+    const int l = threadIdx.x & 15, w = threadIdx.x >> 4, which = blockIdx.y;
+    const int64_t c = (int64_t)blockIdx.x * 16 + l;
     float s = 0.0f;
-    if (c < a.n)
-        for (int p = w; p < a.nparts; p += 16) s += a.part[((int64_t)p * a.nout + which) * a.n + c];
+    if (c < a.n) {
+        const float *p = a.part + which * a.n + c;
+        const int64_t step = (int64_t)a.nout * a.n;
+#pragma unroll 8
+        for (int i = w; i < a.nparts; i += 64) s += p[i * step];
+    }
     sh[w][l] = s;
-    __syncthreads();
-    if (w || c >= a.n) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += sh[i][l];
-    join_store(which ? a.out1 : a.out0, a.dtype, c, s);
+    for (int half = 32; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (w < half) sh[w][l] += sh[w + half][l];
+    }
+    if (w == 0 && c < a.n) join_store(which ? a.out1 : a.out0, a.dtype, c, sh[0][l]);
 }
 
-#define OPS_LN_ROWS(name, T, LPR, NV, BT)                                                                       \
-    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_rows_##name##_##LPR##x##NV(OpsLnArgs a) {            \
-        ln_rows<T, LPR, NV, BT>(a);                                                                              \
+// Each kernel has both forms, of whole vectors and of any number of elements.
+#define OPS_BOTH(extent, E, call_whole, call_any) \
+    if ((extent) % (E) == 0) call_whole;          \
+    else call_any;
+
+#define OPS_LN_ROWS(name, T, LPR, NV, BT)                                                                             \
+    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_rows_##name##_##LPR##x##NV(OpsLnArgs a) {                 \
+        __shared__ float at[4 * (BT / 64)];                                                                           \
+        OPS_BOTH(a.cols, 16 / sizeof(T), (ln_rows<T, LPR, NV, BT, true>(a, at)), (ln_rows<T, LPR, NV, BT, false>(a, at))) \
     }
-#define OPS_LN_BWD_ROWS(name, T, LPR, NV, BT)                                                                   \
-    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_rows_##name##_##LPR##x##NV(OpsLnBwdArgs a) {     \
-        ln_bwd_rows<T, LPR, NV, BT>(a);                                                                          \
+#define OPS_LN_BWD_ROWS(name, T, LPR, NV, BT)                                                                         \
+    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_rows_##name##_##LPR##x##NV(OpsLnBwdArgs a) {          \
+        __shared__ float at[4 * (BT / 64)];                                                                           \
+        __shared__ float sums[BT > LPR ? BT * NV * 16 / sizeof(T) : 1];                                               \
+        OPS_BOTH(a.cols, 16 / sizeof(T), (ln_bwd_rows<T, LPR, NV, BT, true>(a, at, sums)),                            \
+                 (ln_bwd_rows<T, LPR, NV, BT, false>(a, at, sums)))                                                   \
     }
-#define OPS_LN_PLANAR(name, T, BT, CH)                                                                          \
-    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_planar_##name##_##BT##x##CH(OpsLnArgs a) {           \
-        ln_planar<T, BT, CH, false>(a);                                                                          \
-    }                                                                                                            \
-    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_planar_##name##_##BT##x##CH(OpsLnBwdArgs a) {    \
-        ln_bwd_planar<T, BT, CH, false>(a);                                                                      \
+#define OPS_LN_PLANAR1(name, T, tag, BT, CH, LOOP)                                                                    \
+    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_planar_##name##_##tag(OpsLnArgs a) {                      \
+        __shared__ float at[BT];                                                                                      \
+        OPS_BOTH(a.rows, 16 / sizeof(T), (ln_planar<T, BT, CH, LOOP, true>(a, at)),                                   \
+                 (ln_planar<T, BT, CH, LOOP, false>(a, at)))                                                          \
+    }                                                                                                                 \
+    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_planar_##name##_##tag(OpsLnBwdArgs a) {               \
+        __shared__ float at[BT];                                                                                      \
+        OPS_BOTH(a.rows, 16 / sizeof(T), (ln_bwd_planar<T, BT, CH, LOOP, true>(a, at)),                               \
+                 (ln_bwd_planar<T, BT, CH, LOOP, false>(a, at)))                                                      \
     }
+#define OPS_LN_PLANAR(name, T, BT, CH) OPS_LN_PLANAR1(name, T, BT##x##CH, BT, CH, false)
+#define OPS_LN_BOTH(name, T, LPR, NV, BT) \
+    OPS_LN_ROWS(name, T, LPR, NV, BT)     \
+    OPS_LN_BWD_ROWS(name, T, LPR, NV, BT)
 #define OPS_ROWS_TYPE(name, T)                                                                                        \
-    OPS_LN_ROWS(name, T, 8, 1, 256)                                                                                   \
-    OPS_LN_ROWS(name, T, 16, 1, 256)                                                                                  \
-    OPS_LN_ROWS(name, T, 32, 1, 256)                                                                                  \
-    OPS_LN_ROWS(name, T, 64, 1, 256)                                                                                  \
-    OPS_LN_ROWS(name, T, 64, 2, 256)                                                                                  \
+    OPS_LN_BOTH(name, T, 8, 1, 256)                                                                                   \
+    OPS_LN_BOTH(name, T, 16, 1, 256)                                                                                  \
+    OPS_LN_BOTH(name, T, 32, 1, 256)                                                                                  \
+    OPS_LN_BOTH(name, T, 64, 1, 256)                                                                                  \
+    OPS_LN_ROWS(name, T, 128, 1, 256)                                                                                 \
     OPS_LN_ROWS(name, T, 256, 1, 256)                                                                                 \
-    OPS_LN_ROWS(name, T, 256, 2, 256)                                                                                 \
-    OPS_LN_ROWS(name, T, 1024, 1, 1024)                                                                               \
-    OPS_LN_ROWS(name, T, 1024, 2, 1024)                                                                               \
-    OPS_LN_BWD_ROWS(name, T, 8, 1, 256)                                                                               \
-    OPS_LN_BWD_ROWS(name, T, 16, 1, 256)                                                                              \
-    OPS_LN_BWD_ROWS(name, T, 32, 1, 256)                                                                              \
-    OPS_LN_BWD_ROWS(name, T, 64, 1, 256)                                                                              \
-    OPS_LN_BWD_ROWS(name, T, 64, 2, 256)                                                                              \
+    OPS_LN_ROWS(name, T, 512, 1, 512)                                                                                 \
+    OPS_LN_BWD_ROWS(name, T, 128, 1, 1024)                                                                            \
     OPS_LN_BWD_ROWS(name, T, 256, 1, 1024)                                                                            \
-    OPS_LN_BWD_ROWS(name, T, 256, 2, 1024)                                                                            \
-    OPS_LN_BWD_ROWS(name, T, 1024, 1, 1024)                                                                           \
-    OPS_LN_BWD_ROWS(name, T, 1024, 2, 1024)                                                                           \
+    OPS_LN_BWD_ROWS(name, T, 512, 1, 1024)                                                                            \
+    OPS_LN_BOTH(name, T, 1024, 1, 1024)                                                                               \
+    OPS_LN_BOTH(name, T, 1024, 2, 1024)                                                                               \
     OPS_LN_PLANAR(name, T, 256, 1)                                                                                    \
     OPS_LN_PLANAR(name, T, 256, 2)                                                                                    \
     OPS_LN_PLANAR(name, T, 256, 4)                                                                                    \
-    OPS_LN_PLANAR(name, T, 256, 8)                                                                                    \
-    OPS_LN_PLANAR(name, T, 1024, 4)                                                                                   \
-    OPS_LN_PLANAR(name, T, 1024, 8)                                                                                   \
-    extern "C" __global__ __launch_bounds__(1024) void mxo_ln_planar_##name##_loop(OpsLnArgs a) {                     \
-        ln_planar<T, 1024, 4, true>(a);                                                                               \
-    }                                                                                                                 \
-    extern "C" __global__ __launch_bounds__(1024) void mxo_ln_bwd_planar_##name##_loop(OpsLnBwdArgs a) {              \
-        ln_bwd_planar<T, 1024, 4, true>(a);                                                                           \
-    }                                                                                                                 \
+    OPS_LN_PLANAR(name, T, 512, 4)                                                                                    \
+    OPS_LN_PLANAR(name, T, 512, 8)                                                                                    \
+    OPS_LN_PLANAR1(name, T, loop, 512, 4, true)                                                                      \
     extern "C" __global__ __launch_bounds__(1024) void mxo_ln_rows_##name##_long(OpsLnArgs a) { ln_long<T>(a); }      \
     extern "C" __global__ __launch_bounds__(1024) void mxo_ln_bwd_rows_##name##_long(OpsLnBwdArgs a) {                \
         ln_bwd_long<T>(a);                                                                                            \
@@ -653,7 +683,10 @@ extern "C" __global__ __launch_bounds__(1024) void mxo_join_parts(OpsJoinArgs a)
     extern "C" __global__ __launch_bounds__(256) void mxo_ln_param_planar_##name(OpsLnBwdArgs a) {                    \
         ln_param_planar<T>(a);                                                                                        \
     }                                                                                                                 \
-    extern "C" __global__ __launch_bounds__(256) void mxo_dz_rows_##name(OpsDzArgs a) { dz_rows<T>(a); }              \
+    extern "C" __global__ __launch_bounds__(256) void mxo_dz_rows_##name(OpsDzArgs a) {                               \
+        __shared__ float sh[4][64 * 16 / sizeof(T)];                                                                  \
+        OPS_BOTH(a.cols, 16 / sizeof(T), (dz_rows<T, true>(a, sh)), (dz_rows<T, false>(a, sh)))                       \
+    }                                                                                                                 \
     extern "C" __global__ __launch_bounds__(256) void mxo_dz_planar_##name(OpsDzArgs a) { dz_planar<T>(a); }
 
 OPS_ROWS_TYPE(bf16, bf16)
