@@ -333,10 +333,12 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct) {
 }
 
 // Whether an operand's tiles can go straight to LDS: 16-byte loads of whole
-// chunks, at 32-bit offsets inside a tile of `tile` rows (or 64 k's).
+// chunks, at 31-bit offsets inside a tile (of 256 rows or 64 k's), and lines
+// that do not overlap, so that an offset tells what is past the end.
 bool loads_direct(const Operand &o, bool by_k, int64_t own_n, int64_t sum_n, size_t size) {
     const int64_t ld = by_k ? o.own : o.sum, extent = by_k ? sum_n : own_n;
-    return size == 2 && (uintptr_t)o.data % 16 == 0 && ld % 8 == 0 && extent % 8 == 0 && ld < (int64_t(1) << 21);
+    return size == 2 && (uintptr_t)o.data % 16 == 0 && ld % 8 == 0 && extent % 8 == 0 && ld >= extent &&
+           ld < (int64_t(1) << 21);
 }
 
 void product(int dev, void *stream, const Product &p, void *ws) {

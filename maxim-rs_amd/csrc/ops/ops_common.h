@@ -147,6 +147,23 @@ __device__ __forceinline__ float act_fwd(int act, float slope, float z) {
     return z != z ? z : v;
 }
 
+template <int E>
+__device__ __forceinline__ void act_fwd_n(int act, float slope, float *v) {
+    // the choice once for all of them
+#define OPS_ACT(which)                                                 \
+    case which:                                                        \
+        _Pragma("unroll") for (int e = 0; e < E; ++e) v[e] = act_fwd(which, slope, v[e]); \
+        break;
+    switch (act) {
+        OPS_ACT(MXO_GELU)
+        OPS_ACT(MXO_GELU_TANH)
+        OPS_ACT(MXO_SILU)
+        OPS_ACT(MXO_LRELU)
+        OPS_ACT(MXO_SIGMOID)
+        default: break;
+    }
+}
+
 // Its derivative; at an infinity its limit, at NaN NaN (LeakyReLU: of a NaN
 // the slope, as its comparison gives).
 __device__ __forceinline__ float act_bwd(int act, float slope, float z) {
@@ -170,6 +187,25 @@ __device__ __forceinline__ float act_bwd(int act, float slope, float z) {
         v = __builtin_fmaf(c * d, kTanhA * __builtin_fmaf(3.0f * kTanhB * c, c, 1.0f), s);
     }
     return z != z ? z : v;
+}
+
+// v[e] *= act'(z[e])
+template <int E, typename Z>
+__device__ __forceinline__ void act_bwd_n(int act, float slope, float *v, Z z) {
+    switch (act) {
+#undef OPS_ACT
+#define OPS_ACT(which)                                                                     \
+    case which:                                                                            \
+        _Pragma("unroll") for (int e = 0; e < E; ++e) v[e] *= act_bwd(which, slope, z(e)); \
+        break;
+        OPS_ACT(MXO_GELU)
+        OPS_ACT(MXO_GELU_TANH)
+        OPS_ACT(MXO_SILU)
+        OPS_ACT(MXO_LRELU)
+        OPS_ACT(MXO_SIGMOID)
+        default: break;
+    }
+#undef OPS_ACT
 }
 
 // Sum over the 64 lanes, in every lane.

@@ -114,34 +114,50 @@ struct Tile {
     }
 };
 
-// Bias, z, activation and residual for four consecutive n of row m, rounding
-// once to T at each store. The sum and all of this are fp32.
-template <typename T>
-__device__ __forceinline__ void gemm_finish(const OpsGemmArgs &g, int64_t m, int64_t n, f32x4 v) {
-    const int64_t left = g.n - n;
-    if (m >= g.m || left <= 0) return;
-    const int64_t have = g.vec ? 4 : left;  // vec: n is a multiple of 4
+// What a run of E results of row m adds or needs from memory: fetched ahead of
+// the sums.
+template <typename T, int E>
+struct Extra {
+    Vec<T, E> res;
+    float bias_row;
+};
+template <typename T, int E>
+__device__ __forceinline__ void extra_fetch(const OpsGemmArgs &g, int64_t m, int64_t n, Extra<T, E> &x) {
+    if (m >= g.m || n >= g.n) return;
+    if (g.res) x.res = load_upto<T, E>(static_cast<const T *>(g.res) + m * g.ldr + n, g.n - n);
+    if (g.bias && g.bias_rows) x.bias_row = param<T>(g.bias, m, g.bias_f32);
+}
+// The bias of columns n on, zeros where it runs along the rows.
+template <typename T, int E>
+__device__ __forceinline__ void bias_fetch(const OpsGemmArgs &g, int64_t n, float *bias) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) bias[e] = g.bias && !g.bias_rows && n + e < g.n ? param<T>(g.bias, n + e, g.bias_f32) : 0.0f;
+}
+// Bias, z, activation and residual for E consecutive n of row m, rounding once
+// to T at each store. The sum and all of this are fp32.
+template <typename T, int E>
+__device__ __forceinline__ void gemm_finish(const OpsGemmArgs &g, int64_t m, int64_t n, float *v, const float *bias,
+                                            const Extra<T, E> &x) {
+    if (m >= g.m || n >= g.n) return;
+    const int64_t have = g.n - n;
     if (g.bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < have) v[i] += param<T>(g.bias, g.bias_rows ? m : n + i, g.bias_f32);
+        for (int e = 0; e < E; ++e) v[e] += g.bias_rows ? x.bias_row : bias[e];
     }
-    Vec<T, 4> o;
+    Vec<T, E> o;
     if (g.z) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o.v[i] = from_f<T>(v[i]);
-        store_upto<T, 4>(static_cast<T *>(g.z) + m * g.ldz + n, o, have);
+        for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(v[e]);
+        store_upto<T, E>(static_cast<T *>(g.z) + m * g.ldz + n, o, have);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = act_fwd(g.act, g.slope, v[i]);
+    act_fwd_n<E>(g.act, g.slope, v);
     if (g.res) {
-        const Vec<T, 4> r = load_upto<T, 4>(static_cast<const T *>(g.res) + m * g.ldr + n, have);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += to_f<T>(r.v[i]);
+        for (int e = 0; e < E; ++e) v[e] += to_f<T>(x.res.v[e]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = from_f<T>(v[i]);
-    store_upto<T, 4>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
+    for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(v[e]);
+    store_upto<T, E>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
 }
 
 // Which tile and split a block takes. Consecutive blocks go to the 8 XCDs in
@@ -161,25 +177,61 @@ __device__ __forceinline__ void gemm_place(const OpsGemmArgs &g, int &tm, int &t
 }
 
 // A wave's FM x FN blocks of 16 x 16 from (m0, n0) on: finished, or as split
-// s's partial sums.
+// s's partial sums. 32 rows at a time go through the wave's own part of LDS
+// (`at`, gemm_write_bytes<FN>() of it), rows four floats longer than they are
+// so that 16 rows' writes fall into different banks; what comes back is 16
+// bytes of results a lane, whole lines of C a wave, with the bias of a lane's
+// columns held in registers and the residual on its way before the sums.
+// (Written from the accumulators, with a bias load each, a 256 x 256 tile's
+// 32 quads a lane took 49 us.)
+template <int FN>
+constexpr int gemm_write_bytes() {
+    return 32 * (FN * 16 + 4) * 4;
+}
 template <typename T, int FM, int FN>
-__device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l,
+__device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
                                            const f32x4 (&acc)[FM][FN]) {
+    constexpr int E = 16 / sizeof(T), LD = FN * 16 + 4, LANES = FN * 16 / E, ROWS = 64 / LANES, STEPS = 32 / ROWS;
+    static_assert(FM % 2 == 0 && LANES <= 64, "");
+    float *own = reinterpret_cast<float *>(at);
+    const int lr = l / LANES, lc = l % LANES * E;
+    const int64_t n = n0 + lc;
+    float bias[E];
+    if (g.splits == 1) bias_fetch<T, E>(g, n, bias);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t m = m0 + i * 16 + (l & 15);
+    for (int i = 0; i < FM; i += 2) {
+        const int64_t m = m0 + i * 16 + lr;
+        Extra<T, E> x[STEPS];
+        if (g.splits == 1 && (g.res || g.bias_rows)) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t n = n0 + j * 16 + (l >> 4) * 4;
+            for (int k = 0; k < STEPS; ++k) extra_fetch<T, E>(g, m + k * ROWS, n, x[k]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                *reinterpret_cast<f32x4 *>(own + (h * 16 + (l & 15)) * LD + j * 16 + (l >> 4) * 4) = acc[i + h][j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            float v[E];
+            const float *p = own + (k * ROWS + lr) * LD + lc;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) *reinterpret_cast<f32x4 *>(v + e) = *reinterpret_cast<const f32x4 *>(p + e);
             if (g.splits == 1) {
-                gemm_finish<T>(g, m, n, acc[i][j]);
-            } else if (m < g.m) {
-                Vec<float, 4> o;
+                gemm_finish<T, E>(g, m + k * ROWS, n, v, bias, x[k]);
+            } else if (m + k * ROWS < g.m && n < g.n) {
+                Vec<float, E> o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o.v[e] = acc[i][j][e];
-                store_upto<float, 4>(g.part + ((int64_t)s * g.m + m) * g.n + n, o, g.n - n);
+                for (int e = 0; e < E; ++e) o.v[e] = v[e];
+                store_upto<float, E>(g.part + ((int64_t)s * g.m + m + k * ROWS) * g.n + n, o, g.n - n);
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
 
@@ -244,7 +296,8 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
         if (kt + 1 < nk) put(lds + ((kt + 1) & 1) * STAGE);
         __syncthreads();
     }
-    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, acc);
+    // behind the loop's last barrier: no wave reads the tiles any more
+    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, lds + w * gemm_write_bytes<FN>(), acc);
 }
 
 // The splits' sums added in a fixed order, then the epilogue: WAYS threads to
@@ -275,7 +328,12 @@ __device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
 #pragma unroll
             for (int k = 1; k < WAYS; ++k) v += sh[k * Q + q];
         }
-        if (i < total) gemm_finish<T>(g, m, n, v);
+        if (i >= total) continue;
+        float r[4] = {v[0], v[1], v[2], v[3]}, bias[4];
+        Extra<T, 4> x;
+        bias_fetch<T, 4>(g, n, bias);
+        extra_fetch<T, 4>(g, m, n, x);
+        gemm_finish<T, 4>(g, m, n, r, bias, x);
     }
 }
 

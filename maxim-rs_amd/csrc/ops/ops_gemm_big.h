@@ -11,8 +11,31 @@ __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, char *at, u
 }
 constexpr uint32_t kNowhere = 0x80000000u;
 
+// Waits for this wave's loads into LDS and its reads from it, then for the
+// other waves: a barrier alone does not wait for loads.
+__device__ __forceinline__ void tiles_landed() {
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): its reads are done too
+    __syncthreads();
+}
+
+// The order of a phase: its LDS reads, which the next phase multiplies, spread
+// over its own products. (Left alone the compiler puts each read right before
+// its use.)
+template <int READS, int PRODUCTS>
+__device__ __forceinline__ void spread() {
+    constexpr int EACH = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, DONE = EACH * READS;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+        if (i * EACH < PRODUCTS) __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+    if (DONE < PRODUCTS) __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - DONE, 0);
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_>
 __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char *b0, char *a1, char *b1) {
+    // the epilogue takes a quarter of the waves in each of the four arrays
+    static_assert((WM * WN + 3) / 4 * gemm_write_bytes<BN / WN / 16>() <= BM * 128 && BM == BN, "");
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef Tile<T, AK, BM, NT> TA;
     typedef Tile<T, BK_, BN, NT> TB;
@@ -26,74 +49,111 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
     const int rows_a = min((int64_t)BM, g.m - m0), rows_b = min((int64_t)BN, g.n - n0);
     const T *ga = static_cast<const T *>(g.a) + (AK ? m0 * g.lda + kbeg : kbeg * g.lda + m0);
     const T *gb = static_cast<const T *>(g.b) + (BK_ ? n0 * g.ldb + kbeg : kbeg * g.ldb + n0);
-    uint32_t oa[TA::PER], ob[TB::PER];
-    int ka[TA::PER], kb[TB::PER];
-#pragma unroll
-    for (int i = 0; i < TA::PER; ++i) {
-        int row, k;
-        TA::where(i * NT + t, row, k);
-        ka[i] = k;
-        oa[i] = row < rows_a ? (uint32_t)(AK ? row * g.lda + k : k * g.lda + row) * sizeof(T) : kNowhere;
-    }
-#pragma unroll
-    for (int i = 0; i < TB::PER; ++i) {
-        int row, k;
-        TB::where(i * NT + t, row, k);
-        kb[i] = k;
-        ob[i] = row < rows_b ? (uint32_t)(BK_ ? row * g.ldb + k : k * g.ldb + row) * sizeof(T) : kNowhere;
-    }
+    // A thread's chunks of a tile lie a fixed number of rows (along k: of k's)
+    // apart, one offset and a step. What lies past the operand's end along the
+    // strided axis is past the buffer's, past its end along the other one the
+    // offset is sent there.
+    int ra, ka, rb, kb;
+    TA::where(t, ra, ka);
+    TB::where(t, rb, kb);
+    const uint32_t step_a = (uint32_t)((AK ? NT / 8 : NT / TA::CPR) * g.lda * sizeof(T));
+    const uint32_t step_b = (uint32_t)((BK_ ? NT / 8 : NT / TB::CPR) * g.ldb * sizeof(T));
+    const uint32_t oa = AK || ra < rows_a ? (uint32_t)((AK ? ra * g.lda + ka : ka * g.lda + ra) * sizeof(T)) : kNowhere;
+    const uint32_t ob = BK_ || rb < rows_b ? (uint32_t)((BK_ ? rb * g.ldb + kb : kb * g.ldb + rb) * sizeof(T)) : kNowhere;
     auto stage = [&](int kt, char *at, char *bt) {
-        const int k0 = kt * BK, left = kend - kbeg - k0;
+        const int k0 = kt * BK, left = max(0, min(kend - kbeg - k0, BK));
         const __amdgpu_buffer_rsrc_t bufa =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(ga + (AK ? (int64_t)k0 : k0 * g.lda)), 0, 0x7fffffff, 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc((void *)(ga + (AK ? (int64_t)k0 : k0 * g.lda)), 0,
+                                              (int)((AK ? rows_a : left) * g.lda * sizeof(T)), 0x00020000);
         const __amdgpu_buffer_rsrc_t bufb =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(gb + (BK_ ? (int64_t)k0 : k0 * g.ldb)), 0, 0x7fffffff, 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc((void *)(gb + (BK_ ? (int64_t)k0 : k0 * g.ldb)), 0,
+                                              (int)((BK_ ? rows_b : left) * g.ldb * sizeof(T)), 0x00020000);
+        const uint32_t fa = !AK || ka < left ? oa : kNowhere, fb = !BK_ || kb < left ? ob : kNowhere;
 #pragma unroll
-        for (int i = 0; i < TA::PER; ++i) lds_load16(bufa, at + (i * NT + w * 64) * 16, ka[i] < left ? oa[i] : kNowhere);
+        for (int i = 0; i < TA::PER; ++i) lds_load16(bufa, at + (i * NT + w * 64) * 16, fa + i * step_a);
 #pragma unroll
-        for (int i = 0; i < TB::PER; ++i)
-            lds_load16(bufb, bt + (i * NT + w * 64) * 16, kb[i] < left ? ob[i] : kNowhere);
+        for (int i = 0; i < TB::PER; ++i) lds_load16(bufb, bt + (i * NT + w * 64) * 16, fb + i * step_b);
     };
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    auto compute = [&](const LdsChar *at, const LdsChar *bt) {
+    // A tile is four phases, two halves of k by two halves of the wave's rows,
+    // each multiplying fragments that the phase before it read from LDS.
+    constexpr int HM = FM / 2;
+    typedef typename Mma<T>::Frag Frag;
+    Frag fa[2][HM], fb[2][FN];
+    // A fragment's address is worked out when it is read: held through the
+    // loop, those of operands that are not contiguous along k (one register
+    // each, their swizzle depends on lane and row) do not fit beside the sums.
+    auto here = [&] {
+        int lane = l;
+        if (!AK || !BK_) asm volatile("" : "+v"(lane));
+        return lane;
+    };
+    auto take_a = [&](const LdsChar *at, int kk, int h) {
+        const int lane = here();
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            typename Mma<T>::Frag fa[FM], fb[FN];
+        for (int i = 0; i < HM; ++i) fa[h][i] = TA::frag(at, wm + (h * HM + i) * 16, kk, lane);
+    };
+    auto take_b = [&](const LdsChar *bt, int kk) {
+        const int lane = here();
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = TA::frag(at, wm + i * 16, kk, l);
+        for (int j = 0; j < FN; ++j) fb[kk][j] = TB::frag(bt, wn + j * 16, kk, lane);
+    };
+    auto multiply = [&](int kk, int h) {
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = TB::frag(bt, wn + j * 16, kk, l);
+        for (int i = 0; i < HM; ++i)
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::go(fb[j], fa[i], acc[i][j]);
-        }
+            for (int j = 0; j < FN; ++j) acc[h * HM + i][j] = Mma<T>::go(fb[kk][j], fa[h][i], acc[h * HM + i][j]);
+    };
+    // The last phase's fragments are in registers when it begins: then, with
+    // the next tile landed, the one after that is sent for into this one's
+    // place, a whole tile's time ahead of its use. Past the last tile the
+    // loads bring zeros without touching memory.
+    auto tile = [&](int kt, char *ac, char *bc, char *an, char *bn) {
+        constexpr int RA = HM * (AK ? 1 : 2), RB = FN * (BK_ ? 1 : 2);
+        take_a((LdsChar *)ac, 0, 1);
+        multiply(0, 0);
+        spread<RA, HM * FN>();
+        take_b((LdsChar *)bc, 1);
+        take_a((LdsChar *)ac, 1, 0);
+        multiply(0, 1);
+        spread<RA + RB, HM * FN>();
+        take_a((LdsChar *)ac, 1, 1);
+        multiply(1, 0);
+        spread<RA, HM * FN>();
+        tiles_landed();
+        stage(kt + 2, ac, bc);
+        __builtin_amdgcn_sched_barrier(0);  // sent for here, not where the scheduler finds room
+        take_b((LdsChar *)bn, 0);
+        take_a((LdsChar *)an, 0, 0);
+        multiply(1, 1);
+        spread<RA + RB, HM * FN>();
     };
     const int nk = (kend - kbeg + BK - 1) / BK;
-    if (nk > 0) stage(0, a0, b0);
+    stage(0, a0, b0);
+    stage(1, a1, b1);
+    tiles_landed();
+    take_b((LdsChar *)b0, 0);
+    take_a((LdsChar *)a0, 0, 0);
+    // two tiles a round, where nk is odd the last one of zeros: an exit between
+    // them would cost the registers that the fragments need
     for (int kt = 0; kt < nk; kt += 2) {
-        __syncthreads();
-        if (kt + 1 < nk) stage(kt + 1, a1, b1);
-        compute((LdsChar *)a0, (LdsChar *)b0);
-        __syncthreads();
-        if (kt + 1 < nk) {
-            if (kt + 2 < nk) stage(kt + 2, a0, b0);
-            compute((LdsChar *)a1, (LdsChar *)b1);
-        }
+        tile(kt, a0, b0, a1, b1);
+        tile(kt + 1, a1, b1, a0, b0);
     }
-    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, acc);
+    tiles_landed();  // the last loads too, zeros: the tiles' LDS is free
+    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, (w & 1 ? w & 2 ? b1 : a1 : w & 2 ? b0 : a0) + (w >> 2) * gemm_write_bytes<FN>(), acc);
 }
 
 #define OPS_DIRECT1(name, T, BM, BN, WM, WN, tag, AK, BK)                                                  \
     extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxo_gemm_##name##_##BM##x##BN##_##tag##_d(  \
         OpsGemmArgs g) {                                                                                   \
         __shared__ __align__(1024) char a0[BM * 128];                                                      \
-        __shared__ __align__(1024) char b0[BN * 128];                                                      \
         __shared__ __align__(1024) char a1[BM * 128];                                                      \
+        __shared__ __align__(1024) char b0[BN * 128];                                                      \
         __shared__ __align__(1024) char b1[BN * 128];                                                      \
         gemm_direct<T, BM, BN, WM, WN, AK, BK>(g, a0, b0, a1, b1);                                         \
     }

@@ -550,12 +550,14 @@ __device__ __forceinline__ void dz_rows(const OpsDzArgs &a, float (*sh)[64 * 16 
             const T *dy = static_cast<const T *>(a.dy) + r * a.dyrs + c, *z = static_cast<const T *>(a.z) + r * a.zrs + c;
             Vec<T, E> vd = load_in<T, E, WHOLE>(dy, dy, have), vz;
             if (a.z) vz = load_in<T, E, WHOLE>(z, z, have);
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = to_f<T>(vd.v[e]);
+            if (a.z) act_bwd_n<E>(a.act, a.slope, v, [&](int e) { return to_f<T>(vz.v[e]); });
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                float v = to_f<T>(vd.v[e]);
-                if (a.z) v *= act_bwd(a.act, a.slope, to_f<T>(vz.v[e]));
-                s[e] += v;
-                vd.v[e] = from_f<T>(v);
+                s[e] += v[e];
+                vd.v[e] = from_f<T>(v[e]);
             }
             if (a.dz) store_in<T, E, WHOLE>(static_cast<T *>(a.dz) + r * a.drs + c, vd, have);
         }
@@ -580,12 +582,14 @@ __device__ __forceinline__ void dz_planar(const OpsDzArgs &a) {
         Vec<T, E> vd = load_upto<T, E>(static_cast<const T *>(a.dy) + c * a.dycs + r, end - r);
         Vec<T, E> vz;
         if (a.z) vz = load_upto<T, E>(static_cast<const T *>(a.z) + c * a.zcs + r, end - r);
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = to_f<T>(vd.v[e]);
+        if (a.z) act_bwd_n<E>(a.act, a.slope, v, [&](int e) { return to_f<T>(vz.v[e]); });
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float v = to_f<T>(vd.v[e]);
-            if (a.z) v *= act_bwd(a.act, a.slope, to_f<T>(vz.v[e]));
-            if (r + e < end) s += v;
-            vd.v[e] = from_f<T>(v);
+            if (r + e < end) s += v[e];
+            vd.v[e] = from_f<T>(v[e]);
         }
         if (a.dz) store_upto<T, E>(static_cast<T *>(a.dz) + c * a.dcs + r, vd, end - r);
     }
