@@ -313,23 +313,54 @@ struct Plan {
     uint64_t bytes = 0;
 };
 
-// Tiles: 256 x 256 straight to LDS where the operands allow it and there are
-// tiles for most of the 256 CUs, else 128 x 128, else 64 x 64; and where these
-// are few too, k in up to 64 runs, each at least four LDS tiles long.
+// What a tile costs, measured in us on square products of 1024 to 8192: a step
+// of 128 bytes of k with one tile on a CU (`one`), with as many as its LDS
+// holds (`all`, for `fit` of them), and what a tile takes besides.
+struct TileCost {
+    int b, fit;
+    bool direct;
+    double one, all, rest;
+};
+const TileCost kTiles16[] = {{256, 1, true, 1.6, 1.6, 10.0},
+                             {128, 2, true, 0.65, 0.93, 7.0},
+                             {128, 2, false, 1.25, 1.8, 8.0},
+                             {64, 5, false, 0.62, 1.7, 4.0}};
+const TileCost kTiles32[] = {{128, 2, false, 2.45, 4.3, 8.0}, {64, 5, false, 0.85, 3.0, 5.0}};
+
+// The tile and the number of runs k is cut into that take the least time by
+// those costs: rounds of tiles over the 256 CUs, and for a cut k a second
+// launch and its partial sums written and read (at 5 TB/s). 4096 x 1024
+// results of 4096 products each: 128 x 128 uncut 47 us, cut in two 53 us, 256
+// x 256 cut in four 65 us; 1024 x 1024: cut in four 28 us, uncut 44 us.
 Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct) {
-    Plan p;
-    auto tiles = [&](int b) { return cdiv(m, b) * cdiv(n, b); };
-    p.direct = direct;
-    const int b = direct && tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
-    if (b == 64) p.direct = false;
-    p.bm = p.bn = b;
-    p.block = b == 256 ? 512 : 256;
-    const int64_t bk = 128 / (int64_t)type_size(dtype);
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, tiles(b)), cdiv(k, 4 * bk), 64}));
-    p.kchunk = std::max<int64_t>(bk, cdiv(cdiv(k, splits), bk) * bk);
-    p.splits = std::max<int64_t>(1, cdiv(k, p.kchunk));
-    p.bytes = p.splits > 1 ? (uint64_t)p.splits * m * n * 4 : 0;
-    return p;
+    Plan best;
+    double least = std::numeric_limits<double>::infinity();
+    const int64_t bk = 128 / (int64_t)type_size(dtype), steps = std::max<int64_t>(1, cdiv(k, bk));
+    auto consider = [&](const TileCost &t) {
+        if (t.direct && !direct) return;
+        const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b);
+        for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+            const int64_t each = cdiv(steps, cut), splits = cdiv(steps, each);
+            if (cut > 1 && (each < 2 || splits != cut)) continue;
+            const int64_t total = tiles * splits, full = total / (256 * t.fit), left = cdiv(total % (256 * t.fit), 256);
+            double us = full * (each * t.all + t.rest);
+            if (left) us += each * std::max(t.one, t.all * left / t.fit) + t.rest;
+            if (splits > 1) us += 5.0 + (double)splits * m * n * 8 / 5e6;
+            if (us >= least) continue;
+            least = us;
+            best.bm = best.bn = t.b;
+            best.block = t.b == 256 ? 512 : 256;
+            best.direct = t.direct;
+            best.splits = splits;
+            best.kchunk = each * bk;
+        }
+    };
+    if (type_size(dtype) == 2)
+        for (const TileCost &t : kTiles16) consider(t);
+    else
+        for (const TileCost &t : kTiles32) consider(t);
+    best.bytes = best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0;
+    return best;
 }
 
 // Whether an operand's tiles can go straight to LDS: 16-byte loads of whole

@@ -81,34 +81,39 @@ struct Tile {
         const int have = KMAJ ? (row < rows ? kn - k : 0) : (k < kn ? rows - row : 0);
         return load_upto<T, E>(g + (KMAJ ? row * ld + k : k * ld + row), have);
     }
-    // Lane l's part of rows [base, base + 16) at k's step kk (half a tile):
-    // row l % 16; k's 8 (l / 16) + 0..7 of the step's 32 (16-bit), or
-    // 4 (l / 16) + 0..3 of its 16 (fp32)
-    static __device__ __forceinline__ typename Mma<T>::Frag frag(const LdsChar *lds, int base, int kk, int l) {
-        typedef const __attribute__((address_space(3))) typename Mma<T>::Frag *FP;
+    // Where lane l's part of a fragment lies, but for the fragment's own
+    // constants: rows [base, base + 16) at k's step kk (half a tile), row l % 16
+    // of them; k's 8 (l / 16) + 0..7 of the step's 32 (16-bit), or 4 (l / 16) +
+    // 0..3 of its 16 (fp32). The swizzles are exclusive ors of address bits
+    // that nothing else of the lane's part uses, so a fragment is one more.
+    static __device__ __forceinline__ int lane_part(int l) {
         const int r = l & 15, g = l >> 4;
-        if constexpr (KMAJ) {
-            const int row = base + r;
-            return *(FP)(lds + (row * 128 + (((kk * 4 + g) ^ ((row >> 1) & 7)) << 4)));
-        } else if constexpr (sizeof(T) == 2) {
+        if constexpr (KMAJ) return r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
+        else if constexpr (sizeof(T) == 2) {
             // each group of 16 lanes reads a 4 x 16 block of (k, row) and
             // gets it back with lane i holding row i's four k's
-            const int k = kk * 32 + g * 8 + (r >> 2);
-            const int seg = (base >> 4) ^ (((r >> 2) | (g & 1) << 2) & (ROWS / 16 - 1));
+            const int k = g * 8 + (r >> 2);
+            return k * (ROWS * 2) + ((kswz(k) & (ROWS / 16 - 1)) << 5) + (r & 3) * 8;
+        } else {
+            return g * 4 * (ROWS * 4) + ((g & (ROWS / 16 - 1)) << 6) + r * 4;
+        }
+    }
+    static __device__ __forceinline__ typename Mma<T>::Frag frag(const LdsChar *lds, int base, int kk, int part) {
+        typedef const __attribute__((address_space(3))) typename Mma<T>::Frag *FP;
+        if constexpr (KMAJ) {
+            return *(FP)(lds + ((part ^ (kk << 6)) + base * 128));
+        } else if constexpr (sizeof(T) == 2) {
             typedef __attribute__((address_space(3))) i16x4 *LP;
-            const int at = k * (ROWS * 2) + seg * 32 + (r & 3) * 8;
+            const int at = (part ^ (base << 1)) + kk * 32 * (ROWS * 2);
             const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(lds + at));
             const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(lds + (at + 4 * ROWS * 2)));
             const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             return __builtin_bit_cast(typename Mma<T>::Frag, v);
         } else {
             typename Mma<T>::Frag v;
+            const int at = (part ^ (base << 2)) + kk * 16 * (ROWS * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int k = kk * 16 + g * 4 + e;
-                const int seg = (base >> 4) ^ (g & (ROWS / 16 - 1));
-                v[e] = *(const __attribute__((address_space(3))) float *)(lds + (k * (ROWS * 4) + seg * 64 + r * 4));
-            }
+            for (int e = 0; e < 4; ++e) v[e] = *(const __attribute__((address_space(3))) float *)(lds + (at + e * ROWS * 4));
             return v;
         }
     }
@@ -278,6 +283,7 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
         put(lds);
     }
     __syncthreads();
+    const int pa = TA::lane_part(l), pb = TB::lane_part(l);
     for (int kt = 0; kt < nk; ++kt) {
         const LdsChar *at = (LdsChar *)lds + (kt & 1) * STAGE;
         if (kt + 1 < nk) fetch((kt + 1) * BK);
@@ -285,9 +291,9 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
         for (int kk = 0; kk < 2; ++kk) {
             typename Mma<T>::Frag fa[FM], fb[FN];
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = TA::frag(at, wm + i * 16, kk, l);
+            for (int i = 0; i < FM; ++i) fa[i] = TA::frag(at, wm + i * 16, kk, pa);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = TB::frag(at + ABYTES, wn + j * 16, kk, l);
+            for (int j = 0; j < FN; ++j) fb[j] = TB::frag(at + ABYTES, wn + j * 16, kk, pb);
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll

@@ -56,23 +56,29 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
     int ra, ka, rb, kb;
     TA::where(t, ra, ka);
     TB::where(t, rb, kb);
-    const uint32_t step_a = (uint32_t)((AK ? NT / 8 : NT / TA::CPR) * g.lda * sizeof(T));
-    const uint32_t step_b = (uint32_t)((BK_ ? NT / 8 : NT / TB::CPR) * g.ldb * sizeof(T));
-    const uint32_t oa = AK || ra < rows_a ? (uint32_t)((AK ? ra * g.lda + ka : ka * g.lda + ra) * sizeof(T)) : kNowhere;
-    const uint32_t ob = BK_ || rb < rows_b ? (uint32_t)((BK_ ? rb * g.ldb + kb : kb * g.ldb + rb) * sizeof(T)) : kNowhere;
-    auto stage = [&](int kt, char *at, char *bt) {
-        const int k0 = kt * BK, left = max(0, min(kend - kbeg - k0, BK));
+    const int lda = (int)(g.lda * sizeof(T)), ldb = (int)(g.ldb * sizeof(T));
+    const uint32_t step_a = (AK ? NT / 8 : NT / TA::CPR) * lda, step_b = (BK_ ? NT / 8 : NT / TB::CPR) * ldb;
+    const uint32_t oa = AK || ra < rows_a ? (AK ? ra * lda + ka * (int)sizeof(T) : ka * lda + ra * (int)sizeof(T)) : kNowhere;
+    const uint32_t ob = BK_ || rb < rows_b ? (BK_ ? rb * ldb + kb * (int)sizeof(T) : kb * ldb + rb * (int)sizeof(T)) : kNowhere;
+    const char *next_a = reinterpret_cast<const char *>(ga), *next_b = reinterpret_cast<const char *>(gb);
+    int left = kend - kbeg;
+    // the next tile, in turn
+    auto stage = [&](char *at, char *bt) {
+        // (the compiler clamps in the vector unit; a buffer in vector registers
+        // would be loaded from lane by lane)
+        const int k = __builtin_amdgcn_readfirstlane(max(0, min(left, BK)));
         const __amdgpu_buffer_rsrc_t bufa =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(ga + (AK ? (int64_t)k0 : k0 * g.lda)), 0,
-                                              (int)((AK ? rows_a : left) * g.lda * sizeof(T)), 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc((void *)next_a, 0, (AK ? rows_a : k) * lda, 0x00020000);
         const __amdgpu_buffer_rsrc_t bufb =
-            __builtin_amdgcn_make_buffer_rsrc((void *)(gb + (BK_ ? (int64_t)k0 : k0 * g.ldb)), 0,
-                                              (int)((BK_ ? rows_b : left) * g.ldb * sizeof(T)), 0x00020000);
-        const uint32_t fa = !AK || ka < left ? oa : kNowhere, fb = !BK_ || kb < left ? ob : kNowhere;
+            __builtin_amdgcn_make_buffer_rsrc((void *)next_b, 0, (BK_ ? rows_b : k) * ldb, 0x00020000);
+        const uint32_t fa = !AK || ka < k ? oa : kNowhere, fb = !BK_ || kb < k ? ob : kNowhere;
 #pragma unroll
         for (int i = 0; i < TA::PER; ++i) lds_load16(bufa, at + (i * NT + w * 64) * 16, fa + i * step_a);
 #pragma unroll
         for (int i = 0; i < TB::PER; ++i) lds_load16(bufb, bt + (i * NT + w * 64) * 16, fb + i * step_b);
+        next_a += AK ? 128 : BK * lda;
+        next_b += BK_ ? 128 : BK * ldb;
+        left -= BK;
     };
     f32x4 acc[FM][FN];
 #pragma unroll
@@ -84,23 +90,23 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
     constexpr int HM = FM / 2;
     typedef typename Mma<T>::Frag Frag;
     Frag fa[2][HM], fb[2][FN];
-    // A fragment's address is worked out when it is read: held through the
-    // loop, those of operands that are not contiguous along k (one register
-    // each, their swizzle depends on lane and row) do not fit beside the sums.
-    auto here = [&] {
-        int lane = l;
-        if (!AK || !BK_) asm volatile("" : "+v"(lane));
-        return lane;
+    // In the largest tiles a fragment's address (its own register where the
+    // operand is not contiguous along k) is worked out when it is read: held
+    // through the loop they do not fit beside the sums.
+    const int pa = TA::lane_part(l), pb = TB::lane_part(l);
+    auto here = [&](int part) {
+        if (FM * FN >= 32 && (!AK || !BK_)) asm volatile("" : "+v"(part));
+        return part;
     };
     auto take_a = [&](const LdsChar *at, int kk, int h) {
-        const int lane = here();
+        const int part = here(pa);
 #pragma unroll
-        for (int i = 0; i < HM; ++i) fa[h][i] = TA::frag(at, wm + (h * HM + i) * 16, kk, lane);
+        for (int i = 0; i < HM; ++i) fa[h][i] = TA::frag(at, wm + (h * HM + i) * 16, kk, part);
     };
     auto take_b = [&](const LdsChar *bt, int kk) {
-        const int lane = here();
+        const int part = here(pb);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[kk][j] = TB::frag(bt, wn + j * 16, kk, lane);
+        for (int j = 0; j < FN; ++j) fb[kk][j] = TB::frag(bt, wn + j * 16, kk, part);
     };
     auto multiply = [&](int kk, int h) {
 #pragma unroll
@@ -112,7 +118,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
     // the next tile landed, the one after that is sent for into this one's
     // place, a whole tile's time ahead of its use. Past the last tile the
     // loads bring zeros without touching memory.
-    auto tile = [&](int kt, char *ac, char *bc, char *an, char *bn) {
+    auto tile = [&](char *ac, char *bc, char *an, char *bn) {
         constexpr int RA = HM * (AK ? 1 : 2), RB = FN * (BK_ ? 1 : 2);
         take_a((LdsChar *)ac, 0, 1);
         multiply(0, 0);
@@ -125,7 +131,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
         multiply(1, 0);
         spread<RA, HM * FN>();
         tiles_landed();
-        stage(kt + 2, ac, bc);
+        stage(ac, bc);
         __builtin_amdgcn_sched_barrier(0);  // sent for here, not where the scheduler finds room
         take_b((LdsChar *)bn, 0);
         take_a((LdsChar *)an, 0, 0);
@@ -133,16 +139,16 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
         spread<RA + RB, HM * FN>();
     };
     const int nk = (kend - kbeg + BK - 1) / BK;
-    stage(0, a0, b0);
-    stage(1, a1, b1);
+    stage(a0, b0);
+    stage(a1, b1);
     tiles_landed();
     take_b((LdsChar *)b0, 0);
     take_a((LdsChar *)a0, 0, 0);
     // two tiles a round, where nk is odd the last one of zeros: an exit between
     // them would cost the registers that the fragments need
     for (int kt = 0; kt < nk; kt += 2) {
-        tile(kt, a0, b0, a1, b1);
-        tile(kt + 1, a1, b1, a0, b0);
+        tile(a0, b0, a1, b1);
+        tile(a1, b1, a0, b0);
     }
     tiles_landed();  // the last loads too, zeros: the tiles' LDS is free
     gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, (w & 1 ? w & 2 ? b1 : a1 : w & 2 ? b0 : a0) + (w >> 2) * gemm_write_bytes<FN>(), acc);
