@@ -306,9 +306,10 @@ struct Product {
 };
 
 struct Plan {
+    bool skinny = false;  // the kernel of few rows
     int bm = 0, bn = 0;
     unsigned block = 256;
-    bool direct = false;
+    int stages = 0;  // straight to LDS with so many tiles there; 0: through registers
     int64_t splits = 1, kchunk = 0;
     uint64_t bytes = 0;
 };
@@ -317,27 +318,34 @@ struct Plan {
 // of 128 bytes of k with one tile on a CU (`one`), with as many as its LDS
 // holds (`all`, for `fit` of them), and what a tile takes besides.
 struct TileCost {
-    int b, fit;
-    bool direct;
+    int b, stages, fit;
     double one, all, rest;
 };
-const TileCost kTiles16[] = {{256, 1, true, 1.6, 1.6, 10.0},
-                             {128, 2, true, 0.65, 0.93, 7.0},
-                             {128, 2, false, 1.25, 1.8, 8.0},
-                             {64, 5, false, 0.62, 1.7, 4.0}};
-const TileCost kTiles32[] = {{128, 2, false, 2.45, 4.3, 8.0}, {64, 5, false, 0.85, 3.0, 5.0}};
+const TileCost kTiles16[] = {{256, 2, 1, 1.6, 1.6, 10.0}, {128, 4, 1, 0.54, 0.54, 6.0}, {128, 2, 2, 0.65, 0.93, 7.0},
+                             {64, 4, 2, 0.2, 0.39, 4.0},  {128, 0, 2, 1.25, 1.8, 8.0},  {64, 0, 5, 0.62, 1.7, 4.0}};
+const TileCost kTiles32[] = {{128, 4, 1, 2.0, 2.0, 6.0},  {128, 2, 2, 2.2, 3.8, 7.0},  {64, 4, 2, 0.6, 1.1, 4.0},
+                             {128, 0, 2, 2.45, 4.3, 8.0}, {64, 0, 5, 0.85, 3.0, 5.0}};
 
 // The tile and the number of runs k is cut into that take the least time by
 // those costs: rounds of tiles over the 256 CUs, and for a cut k a second
 // launch and its partial sums written and read (at 5 TB/s). 4096 x 1024
-// results of 4096 products each: 128 x 128 uncut 47 us, cut in two 53 us, 256
-// x 256 cut in four 65 us; 1024 x 1024: cut in four 28 us, uncut 44 us.
-Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct) {
+// results of 4096 products each: 128 x 128 uncut 41 us, cut in two 53 us, 256
+// x 256 cut in four 65 us; 1024 x 1024: 64 x 64 uncut 18 us, cut in four 28
+// us, 128 x 128 cut in four 26 us.
+//
+// Up to 16 rows against weights that are contiguous along k go to the kernel
+// that reads those once, without LDS tiles or a second launch.
+Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct, bool by_k) {
     Plan best;
+    if (by_k && m <= 16) {
+        best.skinny = true;
+        best.block = 512;
+        return best;
+    }
     double least = std::numeric_limits<double>::infinity();
     const int64_t bk = 128 / (int64_t)type_size(dtype), steps = std::max<int64_t>(1, cdiv(k, bk));
     auto consider = [&](const TileCost &t) {
-        if (t.direct && !direct) return;
+        if (t.stages && !direct) return;
         const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b);
         for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
             const int64_t each = cdiv(steps, cut), splits = cdiv(steps, each);
@@ -350,7 +358,7 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct) {
             least = us;
             best.bm = best.bn = t.b;
             best.block = t.b == 256 ? 512 : 256;
-            best.direct = t.direct;
+            best.stages = t.stages;
             best.splits = splits;
             best.kchunk = each * bk;
         }
@@ -368,8 +376,8 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct) {
 // that do not overlap, so that an offset tells what is past the end.
 bool loads_direct(const Operand &o, bool by_k, int64_t own_n, int64_t sum_n, size_t size) {
     const int64_t ld = by_k ? o.own : o.sum, extent = by_k ? sum_n : own_n;
-    return size == 2 && (uintptr_t)o.data % 16 == 0 && ld % 8 == 0 && extent % 8 == 0 && ld >= extent &&
-           ld < (int64_t(1) << 21);
+    const int64_t e = 16 / (int64_t)size;
+    return (uintptr_t)o.data % 16 == 0 && ld % e == 0 && extent % e == 0 && ld >= extent && ld < (int64_t(1) << 20);
 }
 
 void product(int dev, void *stream, const Product &p, void *ws) {
@@ -379,7 +387,7 @@ void product(int dev, void *stream, const Product &p, void *ws) {
     const bool ak = p.a.sum == 1, bk = p.b.sum == 1;
     const size_t size = type_size(p.dtype);
     const Plan pl = plan_product(p.dtype, p.m, p.n, p.k,
-                                 loads_direct(p.a, ak, p.m, p.k, size) && loads_direct(p.b, bk, p.n, p.k, size));
+                                 loads_direct(p.a, ak, p.m, p.k, size) && loads_direct(p.b, bk, p.n, p.k, size), ak && bk);
     OpsGemmArgs g{};
     g.a = p.a.data;
     g.b = p.b.data;
@@ -397,9 +405,7 @@ void product(int dev, void *stream, const Product &p, void *ws) {
     g.k = (int32_t)p.k;
     g.splits = (int32_t)pl.splits;
     g.kchunk = (int32_t)pl.kchunk;
-    const int64_t tm = cdiv(p.m, pl.bm), tn = cdiv(p.n, pl.bn);
-    g.tiles_m = (int32_t)tm;
-    g.tiles_n = (int32_t)tn;
+    const std::string t = kTypeName[p.dtype];
     g.act = p.act;
     g.slope = p.slope;
     if (p.bias) {
@@ -407,12 +413,17 @@ void product(int dev, void *stream, const Product &p, void *ws) {
         g.bias_f32 = p.bias->dtype == MXH_F32 && p.dtype != MXH_F32;
         g.bias_rows = p.bias_rows;
     }
-    g.vec = p.n % 4 == 0;
+    if (pl.skinny) {
+        launch(dev, stream, "mxo_skinny_" + t, cdiv(p.n, 16), 1, pl.block, g);
+        return;
+    }
+    const int64_t tm = cdiv(p.m, pl.bm), tn = cdiv(p.n, pl.bn);
+    g.tiles_m = (int32_t)tm;
+    g.tiles_n = (int32_t)tn;
     if (tm * tn > std::numeric_limits<int32_t>::max() / pl.splits) throw Error("the product has too many tiles");
-    const std::string t = kTypeName[p.dtype];
     launch(dev, stream,
            "mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
-               (bk ? "k" : "m") + (pl.direct ? "_d" : ""),
+               (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
            tm * tn * pl.splits, 1, pl.block, g);
     if (pl.splits > 1)
         {
@@ -452,7 +463,7 @@ Product oriented(const mxh_mat &out, const Operand &rows, const Operand &cols, i
 uint64_t product_bytes(const mxh_mat &out, int64_t k, bool by_cols) {
     if (empty(out)) return 0;
     const int64_t m = by_cols ? out.rows : out.cols, n = by_cols ? out.cols : out.rows;
-    return std::max(plan_product(out.dtype, m, n, k, false).bytes, plan_product(out.dtype, m, n, k, true).bytes);
+    return std::max(plan_product(out.dtype, m, n, k, false, false).bytes, plan_product(out.dtype, m, n, k, true, false).bytes);
 }
 
 uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }

@@ -26,8 +26,7 @@ struct OpsGemmArgs {
     int32_t act;
     float slope;
     int32_t bias_f32;   // the bias is fp32, else of the operands' type
-    int32_t bias_rows;  // one bias value per m instead of per n
-    int32_t vec;        // C, residual and z take four elements at once
+    int32_t bias_rows, pad;  // one bias value per m instead of per n
 };
 
 // x, y and the gradients [rows][cols] at rs and cs elements between rows and

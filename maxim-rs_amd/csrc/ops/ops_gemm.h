@@ -74,12 +74,28 @@ struct Tile {
         }
     }
     // the chunk of position p from global memory: zeros past the operand's
-    // `rows` rows and `kn` k's (g points at the tile's first element)
+    // `rows` rows and `kn` k's (g points at the tile's first element). INSIDE:
+    // the tile's k's and, contiguous along rows, its rows are all there; rows
+    // past the last may then be any row's (what they give is not stored).
+    template <bool INSIDE>
     static __device__ __forceinline__ Chunk load(const T *g, int64_t ld, int p, int rows, int kn) {
         int row, k;
         where(p, row, k);
+        if constexpr (INSIDE) return load_n<T, E>(g + (KMAJ ? min(row, rows - 1) * ld + k : k * ld + row));
         const int have = KMAJ ? (row < rows ? kn - k : 0) : (k < kn ? rows - row : 0);
         return load_upto<T, E>(g + (KMAJ ? row * ld + k : k * ld + row), have);
+    }
+    static __device__ __forceinline__ bool inside(int rows, int kn) { return kn >= BK && (KMAJ || rows == ROWS); }
+    // All of a thread's chunks. (One branch for the tile: with one a chunk each
+    // load was waited for before the next.)
+    static __device__ __forceinline__ void fetch(Chunk (&c)[PER], const T *g, int64_t ld, int t, int rows, int kn) {
+        if (inside(rows, kn)) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) c[i] = load<true>(g, ld, i * NT + t, rows, kn);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) c[i] = load<false>(g, ld, i * NT + t, rows, kn);
+        }
     }
     // Where lane l's part of a fragment lies, but for the fragment's own
     // constants: rows [base, base + 16) at k's step kk (half a tile), row l % 16
@@ -258,12 +274,8 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
     typename TA::Chunk ra[TA::PER];
     typename TB::Chunk rb[TB::PER];
     auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < TA::PER; ++i)
-            ra[i] = TA::load(ga + (AK ? k0 : k0 * g.lda), g.lda, i * NT + t, rows_a, kend - kbeg - k0);
-#pragma unroll
-        for (int i = 0; i < TB::PER; ++i)
-            rb[i] = TB::load(gb + (BK_ ? k0 : k0 * g.ldb), g.ldb, i * NT + t, rows_b, kend - kbeg - k0);
+        TA::fetch(ra, ga + (AK ? k0 : k0 * g.lda), g.lda, t, rows_a, kend - kbeg - k0);
+        TB::fetch(rb, gb + (BK_ ? k0 : k0 * g.ldb), g.ldb, t, rows_b, kend - kbeg - k0);
     };
     auto put = [&](char *at) {
 #pragma unroll

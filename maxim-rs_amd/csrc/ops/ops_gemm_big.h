@@ -1,5 +1,5 @@
-// Products of aligned 16-bit operands: both tiles go from memory straight to
-// LDS.
+// Products of operands aligned to 16 bytes: both tiles go from memory straight
+// to LDS.
 #pragma once
 
 #include "ops_gemm.h"
@@ -11,11 +11,16 @@ __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, char *at, u
 }
 constexpr uint32_t kNowhere = 0x80000000u;
 
-// Waits for this wave's loads into LDS and its reads from it, then for the
-// other waves: a barrier alone does not wait for loads.
+// Waits for this wave's loads into LDS, all but the last `AHEAD` of them, and
+// its reads from it, then for the other waves: a barrier alone waits for
+// neither.
+template <int AHEAD>
 __device__ __forceinline__ void tiles_landed() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): its reads are done too
-    __syncthreads();
+    static_assert(AHEAD < 64, "");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (AHEAD & 15) | (AHEAD >> 4) << 14);  // vmcnt(AHEAD), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // The order of a phase: its LDS reads, which the next phase multiplies, spread
@@ -32,9 +37,16 @@ __device__ __forceinline__ void spread() {
     if (DONE < PRODUCTS) __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - DONE, 0);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_>
-__device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char *b0, char *a1, char *b1) {
-    // the epilogue takes a quarter of the waves in each of the four arrays
+// LDS for one stage of both operands: arrays of their own, so that the compiler
+// can tell a read of one stage from the loads into the others (and does not
+// wait for those).
+struct Stage {
+    char *a, *b;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_, int ST>
+__device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&st)[ST]) {
+    // the epilogue takes a quarter of the waves in each of four arrays
     static_assert((WM * WN + 3) / 4 * gemm_write_bytes<BN / WN / 16>() <= BM * 128 && BM == BN, "");
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     typedef Tile<T, AK, BM, NT> TA;
@@ -115,61 +127,92 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, char *a0, char
             for (int j = 0; j < FN; ++j) acc[h * HM + i][j] = Mma<T>::go(fb[kk][j], fa[h][i], acc[h * HM + i][j]);
     };
     // The last phase's fragments are in registers when it begins: then, with
-    // the next tile landed, the one after that is sent for into this one's
-    // place, a whole tile's time ahead of its use. Past the last tile the
-    // loads bring zeros without touching memory.
-    auto tile = [&](char *ac, char *bc, char *an, char *bn) {
-        constexpr int RA = HM * (AK ? 1 : 2), RB = FN * (BK_ ? 1 : 2);
-        take_a((LdsChar *)ac, 0, 1);
+    // the next tile landed, the tile ST on is sent for into this one's place,
+    // ST - 1 tiles' time ahead of its use. Past the last tile the loads bring
+    // zeros without touching memory.
+    constexpr int LOADS = TA::PER + TB::PER, AHEAD = (ST - 2) * LOADS;
+    auto tile = [&](const Stage &c, const Stage &n) {
+        constexpr int READS = sizeof(T) == 4 ? 4 : 2;  // of a fragment not contiguous along k
+        constexpr int RA = HM * (AK ? 1 : READS), RB = FN * (BK_ ? 1 : READS), MP = HM * FN * (sizeof(T) == 4 ? 4 : 1);
+        take_a((LdsChar *)c.a, 0, 1);
         multiply(0, 0);
-        spread<RA, HM * FN>();
-        take_b((LdsChar *)bc, 1);
-        take_a((LdsChar *)ac, 1, 0);
+        spread<RA, MP>();
+        take_b((LdsChar *)c.b, 1);
+        take_a((LdsChar *)c.a, 1, 0);
         multiply(0, 1);
-        spread<RA + RB, HM * FN>();
-        take_a((LdsChar *)ac, 1, 1);
+        spread<RA + RB, MP>();
+        take_a((LdsChar *)c.a, 1, 1);
         multiply(1, 0);
-        spread<RA, HM * FN>();
-        tiles_landed();
-        stage(ac, bc);
+        spread<RA, MP>();
+        tiles_landed<AHEAD>();
+        stage(c.a, c.b);
         __builtin_amdgcn_sched_barrier(0);  // sent for here, not where the scheduler finds room
-        take_b((LdsChar *)bn, 0);
-        take_a((LdsChar *)an, 0, 0);
+        take_b((LdsChar *)n.b, 0);
+        take_a((LdsChar *)n.a, 0, 0);
         multiply(1, 1);
-        spread<RA + RB, HM * FN>();
+        spread<RA + RB, MP>();
     };
     const int nk = (kend - kbeg + BK - 1) / BK;
-    stage(a0, b0);
-    stage(a1, b1);
-    tiles_landed();
-    take_b((LdsChar *)b0, 0);
-    take_a((LdsChar *)a0, 0, 0);
-    // two tiles a round, where nk is odd the last one of zeros: an exit between
-    // them would cost the registers that the fragments need
-    for (int kt = 0; kt < nk; kt += 2) {
-        tile(a0, b0, a1, b1);
-        tile(a1, b1, a0, b0);
+#pragma unroll
+    for (int i = 0; i < ST; ++i) stage(st[i].a, st[i].b);
+    tiles_landed<AHEAD + LOADS>();
+    take_b((LdsChar *)st[0].b, 0);
+    take_a((LdsChar *)st[0].a, 0, 0);
+    // ST tiles a round and the rest one by one. (In the largest tiles, whose
+    // fragments leave no registers for a second exit, the last round is filled
+    // with a tile of zeros instead.)
+    constexpr bool FILL = FM * FN >= 32;
+    int kt = 0;
+    for (; FILL ? kt < nk : kt + ST <= nk; kt += ST) {
+#pragma unroll
+        for (int i = 0; i < ST; ++i) tile(st[i], st[(i + 1) % ST]);
     }
-    tiles_landed();  // the last loads too, zeros: the tiles' LDS is free
-    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, (w & 1 ? w & 2 ? b1 : a1 : w & 2 ? b0 : a0) + (w >> 2) * gemm_write_bytes<FN>(), acc);
+    if constexpr (!FILL) {
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) {
+            if (kt + i >= nk) break;
+            tile(st[i], st[i + 1]);
+        }
+    }
+    tiles_landed<0>();  // the last loads too, zeros: the tiles' LDS is free
+    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN>(), acc);
 }
 
-#define OPS_DIRECT1(name, T, BM, BN, WM, WN, tag, AK, BK)                                                  \
-    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxo_gemm_##name##_##BM##x##BN##_##tag##_d(  \
+#define OPS_STAGE(i, BM, BN)                              \
+    __shared__ __align__(1024) char a##i[BM * 128];       \
+    __shared__ __align__(1024) char b##i[BN * 128];
+#define OPS_DIRECT2(name, T, BM, BN, WM, WN, tag, AK, BK)                                                  \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxo_gemm_##name##_##BM##x##BN##_##tag##_d2( \
         OpsGemmArgs g) {                                                                                   \
-        __shared__ __align__(1024) char a0[BM * 128];                                                      \
-        __shared__ __align__(1024) char a1[BM * 128];                                                      \
-        __shared__ __align__(1024) char b0[BN * 128];                                                      \
-        __shared__ __align__(1024) char b1[BN * 128];                                                      \
-        gemm_direct<T, BM, BN, WM, WN, AK, BK>(g, a0, b0, a1, b1);                                         \
+        OPS_STAGE(0, BM, BN)                                                                               \
+        OPS_STAGE(1, BM, BN)                                                                               \
+        const Stage st[2] = {{a0, b0}, {a1, b1}};                                                          \
+        gemm_direct<T, BM, BN, WM, WN, AK, BK, 2>(g, st);                                                  \
     }
-#define OPS_DIRECT(name, T, BM, BN, WM, WN)                    \
-    OPS_DIRECT1(name, T, BM, BN, WM, WN, kk, true, true)       \
-    OPS_DIRECT1(name, T, BM, BN, WM, WN, km, true, false)      \
-    OPS_DIRECT1(name, T, BM, BN, WM, WN, mk, false, true)      \
-    OPS_DIRECT1(name, T, BM, BN, WM, WN, mm, false, false)
+#define OPS_DIRECT4(name, T, BM, BN, WM, WN, tag, AK, BK)                                                  \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxo_gemm_##name##_##BM##x##BN##_##tag##_d4( \
+        OpsGemmArgs g) {                                                                                   \
+        OPS_STAGE(0, BM, BN)                                                                               \
+        OPS_STAGE(1, BM, BN)                                                                               \
+        OPS_STAGE(2, BM, BN)                                                                               \
+        OPS_STAGE(3, BM, BN)                                                                               \
+        const Stage st[4] = {{a0, b0}, {a1, b1}, {a2, b2}, {a3, b3}};                                      \
+        gemm_direct<T, BM, BN, WM, WN, AK, BK, 4>(g, st);                                                  \
+    }
+#define OPS_DIRECT(ST, name, T, BM, BN, WM, WN)                     \
+    OPS_DIRECT##ST(name, T, BM, BN, WM, WN, kk, true, true)         \
+    OPS_DIRECT##ST(name, T, BM, BN, WM, WN, km, true, false)        \
+    OPS_DIRECT##ST(name, T, BM, BN, WM, WN, mk, false, true)        \
+    OPS_DIRECT##ST(name, T, BM, BN, WM, WN, mm, false, false)
 
-OPS_DIRECT(bf16, bf16, 256, 256, 2, 4)
-OPS_DIRECT(f16, f16, 256, 256, 2, 4)
-OPS_DIRECT(bf16, bf16, 128, 128, 2, 2)
-OPS_DIRECT(f16, f16, 128, 128, 2, 2)
+#define OPS_DIRECT_TYPE(name, T)              \
+    OPS_DIRECT(2, name, T, 256, 256, 2, 4)    \
+    OPS_DIRECT(2, name, T, 128, 128, 2, 2)    \
+    OPS_DIRECT(4, name, T, 128, 128, 2, 2)    \
+    OPS_DIRECT(4, name, T, 64, 64, 2, 2)
+
+OPS_DIRECT_TYPE(bf16, bf16)
+OPS_DIRECT_TYPE(f16, f16)
+OPS_DIRECT(2, f32, float, 128, 128, 2, 2)
+OPS_DIRECT(4, f32, float, 128, 128, 2, 2)
+OPS_DIRECT(4, f32, float, 64, 64, 2, 2)

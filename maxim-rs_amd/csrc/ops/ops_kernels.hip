@@ -4,3 +4,4 @@
 #include "ops_rows.h"
 #include "ops_gemm.h"
 #include "ops_gemm_big.h"
+#include "ops_skinny.h"

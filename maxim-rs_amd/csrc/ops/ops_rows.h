@@ -42,7 +42,8 @@ __device__ __forceinline__ void row_sum2(float &a, float &b, float *at, int turn
 // LayerNorm of rows with contiguous columns: LPR threads a row, NV vectors of
 // 16 bytes a thread, so a row of up to LPR * NV * 16 bytes stays in
 // registers between the mean, the variance about it and the result. The
-// parameters are read once a block, which walks over rows. WHOLE: rows are
+// parameters are read once a block, which walks over rows with the next one on
+// its way. WHOLE: rows are
 // whole vectors.
 template <typename T, int LPR, int NV, int BT, bool WHOLE>
 __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
@@ -61,16 +62,26 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
         }
     }
     int turn = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t r = min(r0 + grp, a.rows - 1);  // past the end: the last row again, not stored
-        const T *x = static_cast<const T *>(a.x) + r * a.xrs;
-        Vec<T, E> v[NV];
-        float s = 0.0f, q = 0.0f;
+    Vec<T, E> ahead[NV];
+    auto fetch = [&](int64_t r0) {
+        // past the end: the last row again, not stored
+        const T *x = static_cast<const T *>(a.x) + min(r0 + grp, a.rows - 1) * a.xrs;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * LPR + li) * E;
-            v[j] = load_in<T, E, WHOLE>(x + c, x, cols - c);
+            ahead[j] = load_in<T, E, WHOLE>(x + c, x, cols - c);
         }
+    };
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    int64_t r0 = (int64_t)blockIdx.x * RPB;
+    if (r0 < a.rows) fetch(r0);
+    for (; r0 < a.rows; r0 += step) {
+        const int64_t r = r0 + grp;
+        Vec<T, E> v[NV];
+        float s = 0.0f, q = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = ahead[j];
+        if (r0 + step < a.rows) fetch(r0 + step);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -88,7 +99,7 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
         zero = 0.0f;
         row_sum2<LPR, BT>(q, zero, at, turn++);
         const float rstd = 1.0f / sqrtf(q / n + a.eps);
-        if (r0 + grp >= a.rows) continue;  // behind the round's last barrier
+        if (r >= a.rows) continue;  // behind the round's last barrier
         T *y = static_cast<T *>(a.y) + r * a.yrs;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
