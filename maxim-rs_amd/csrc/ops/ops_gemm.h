@@ -60,7 +60,7 @@ struct Tile {
     typedef Vec<T, E> Chunk;
 
     static __device__ __forceinline__ int kswz(int k) {
-        return sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 2) & 3;
+        return sizeof(T) == 2 ? (k & 3) | ((k >> 3) & 1) << 2 : (k >> 3) & 3;
     }
     // what position p holds: (row, k) of its chunk's first element
     static __device__ __forceinline__ void where(int p, int &row, int &k) {
@@ -98,42 +98,144 @@ struct Tile {
         }
     }
     // Where lane l's part of a fragment lies, but for the fragment's own
-    // constants: rows [base, base + 16) at k's step kk (half a tile), row l % 16
-    // of them; k's 8 (l / 16) + 0..7 of the step's 32 (16-bit), or 4 (l / 16) +
-    // 0..3 of its 16 (fp32). The swizzles are exclusive ors of address bits
-    // that nothing else of the lane's part uses, so a fragment is one more.
+    // constants: rows [base, base + 16), row l % 16 of them; k's 8 (l / 16) +
+    // 0..7 of 32, which are half a tile (16-bit) or all of it (fp32). The
+    // swizzles are exclusive ors of address bits that nothing else of the
+    // lane's part uses, so a fragment is one more.
     static __device__ __forceinline__ int lane_part(int l) {
         const int r = l & 15, g = l >> 4;
-        if constexpr (KMAJ) return r * 128 + ((g ^ ((r >> 1) & 7)) << 4);
-        else if constexpr (sizeof(T) == 2) {
+        if constexpr (KMAJ) {
+            return r * 128 + (((sizeof(T) == 2 ? g : 2 * g) ^ ((r >> 1) & 7)) << 4);
+        } else if constexpr (sizeof(T) == 2) {
             // each group of 16 lanes reads a 4 x 16 block of (k, row) and
             // gets it back with lane i holding row i's four k's
             const int k = g * 8 + (r >> 2);
             return k * (ROWS * 2) + ((kswz(k) & (ROWS / 16 - 1)) << 5) + (r & 3) * 8;
         } else {
-            return g * 4 * (ROWS * 4) + ((g & (ROWS / 16 - 1)) << 6) + r * 4;
+            return g * 8 * (ROWS * 4) + ((g & (ROWS / 16 - 1)) << 6) + r * 4;
         }
     }
+    // kk: which half of a 16-bit tile
     static __device__ __forceinline__ typename Mma<T>::Frag frag(const LdsChar *lds, int base, int kk, int part) {
-        typedef const __attribute__((address_space(3))) typename Mma<T>::Frag *FP;
+        static_assert(sizeof(T) == 2, "");
         if constexpr (KMAJ) {
+            typedef const __attribute__((address_space(3))) typename Mma<T>::Frag *FP;
             return *(FP)(lds + ((part ^ (kk << 6)) + base * 128));
-        } else if constexpr (sizeof(T) == 2) {
+        } else {
             typedef __attribute__((address_space(3))) i16x4 *LP;
             const int at = (part ^ (base << 1)) + kk * 32 * (ROWS * 2);
             const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(lds + at));
             const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(lds + (at + 4 * ROWS * 2)));
             const i16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             return __builtin_bit_cast(typename Mma<T>::Frag, v);
-        } else {
-            typename Mma<T>::Frag v;
-            const int at = (part ^ (base << 2)) + kk * 16 * (ROWS * 4);
+        }
+    }
+    static __device__ __forceinline__ void floats(const LdsChar *lds, int base, int part, float (&v)[8]) {
+        static_assert(sizeof(T) == 4, "");
+        if constexpr (KMAJ) {
+            typedef const __attribute__((address_space(3))) f32x4 *FP;
+            const f32x4 lo = *(FP)(lds + (part + base * 128)), hi = *(FP)(lds + ((part ^ 16) + base * 128));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = *(const __attribute__((address_space(3))) float *)(lds + (at + e * ROWS * 4));
-            return v;
+            for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+        } else {
+            const int at = part ^ (base << 2);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = *(const __attribute__((address_space(3))) float *)(lds + (at + e * ROWS * 4));
         }
     }
 };
+
+// One tile of fp32 operands: three bf16 parts a float and six products of them
+// (common.h has the method, its precision and its range), or, exactly as fp32
+// products go, fp32 MFMAs. The six take 96 cycles of a SIMD where the fp32
+// ones take 256; the splitting, 4.5 vector operations an element, goes on
+// beside them.
+struct Split {
+    u32x4 h, m, l;
+};
+__device__ __forceinline__ Split split8(const float (&v)[8]) {
+    Split s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t h, m, l;
+        split2(v[2 * i] * kSplitScale, v[2 * i + 1] * kSplitScale, h, m, l);
+        s.h[i] = h, s.m[i] = m, s.l[i] = l;
+    }
+    return s;
+}
+template <typename TA, typename TB, int FM, int FN>
+__device__ __forceinline__ void split_tile(const LdsChar *at, const LdsChar *bt, int wm, int wn, int pa, int pb,
+                                           f32x4 (&acc)[FM][FN]) {
+    float v[8];
+    Split b[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        TB::floats(bt, wn + j * 16, pb, v);
+        b[j] = split8(v);
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        TA::floats(at, wm + i * 16, pa, v);
+        const Split a = split8(v);
+        // the smallest products first; FN sums apart, so none waits for the last
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j].h, a.l, acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j].l, a.h, acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j].m, a.m, acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j].h, a.m, acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j].m, a.h, acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j].h, a.h, acc[i][j]);
+    }
+}
+// The same tile's products of 16 rows from wm on, in fp32.
+template <typename TA, typename TB, int FN>
+__device__ __forceinline__ void fp32_tile(const LdsChar *at, const LdsChar *bt, int wm, int wn, int pa, int pb,
+                                          f32x4 (&acc)[FN]) {
+    float v[8], b[8];
+    TA::floats(at, wm, pa, v);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        TB::floats(bt, wn + j * 16, pb, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[j] = mfma16(b[e], v[e], acc[j]);
+    }
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
+// Scales a wave's sums back and tells whether all are finite.
+template <int FM, int FN>
+__device__ __forceinline__ bool unscale(f32x4 (&acc)[FM][FN]) {
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                fine = fine && finite(acc[i][j][e]);
+                acc[i][j][e] *= kUnsplit;
+            }
+    return fine;
+}
+// Of 16 rows' sums, those that are not finite, from fp32's.
+template <int FN>
+__device__ __forceinline__ void mend(f32x4 (&acc)[FN], const f32x4 (&fp32)[FN]) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = finite(acc[j][e]) ? acc[j][e] : fp32[j][e];
+}
+template <int FM, int FN>
+__device__ __forceinline__ void clear(f32x4 (&acc)[FM][FN]) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+}
 
 // What a run of E results of row m adds or needs from memory: fetched ahead of
 // the sums.
@@ -285,34 +387,55 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
             *reinterpret_cast<u32x4 *>(at + ABYTES + (i * NT + t) * 16) = __builtin_bit_cast(u32x4, rb[i]);
     };
     f32x4 acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    const int nk = (kend - kbeg + BK - 1) / BK;
-    if (nk > 0) {
-        fetch(0);
-        put(lds);
-    }
-    __syncthreads();
-    const int pa = TA::lane_part(l), pb = TB::lane_part(l);
-    for (int kt = 0; kt < nk; ++kt) {
-        const LdsChar *at = (LdsChar *)lds + (kt & 1) * STAGE;
-        if (kt + 1 < nk) fetch((kt + 1) * BK);
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            typename Mma<T>::Frag fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = TA::frag(at, wm + i * 16, kk, pa);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = TB::frag(at + ABYTES, wn + j * 16, kk, pb);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::go(fb[j], fa[i], acc[i][j]);
+    const int nk = (kend - kbeg + BK - 1) / BK, pa = TA::lane_part(l), pb = TB::lane_part(l);
+    auto run = [&](auto compute) {
+        if (nk > 0) {
+            fetch(0);
+            put(lds);
         }
-        if (kt + 1 < nk) put(lds + ((kt + 1) & 1) * STAGE);
         __syncthreads();
+        for (int kt = 0; kt < nk; ++kt) {
+            if (kt + 1 < nk) fetch((kt + 1) * BK);
+            const LdsChar *at = (LdsChar *)lds + (kt & 1) * STAGE;
+            compute(at, at + ABYTES);
+            if (kt + 1 < nk) put(lds + ((kt + 1) & 1) * STAGE);
+            __syncthreads();
+        }
+    };
+    clear(acc);
+    run([&](const LdsChar *at, const LdsChar *bt) {
+        if constexpr (sizeof(T) == 4) {
+            split_tile<TA, TB, FM, FN>(at, bt, wm, wn, pa, pb, acc);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                typename Mma<T>::Frag fa[FM], fb[FN];
+#pragma unroll
+                for (int i = 0; i < FM; ++i) fa[i] = TA::frag(at, wm + i * 16, kk, pa);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) fb[j] = TB::frag(bt, wn + j * 16, kk, pb);
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = Mma<T>::go(fb[j], fa[i], acc[i][j]);
+            }
+        }
+    });
+    if constexpr (sizeof(T) == 4) {
+        // sums that are not finite, of operands too large or not finite
+        // themselves, are formed again in fp32: 16 of a wave's rows at a time,
+        // the others keep their bits
+        if (__syncthreads_or(!unscale(acc)))
+            for (int h = 0; h < FM; ++h) {
+                f32x4 again[1][FN];
+                clear(again);
+                run([&](const LdsChar *at, const LdsChar *bt) {
+                    fp32_tile<TA, TB, FN>(at, bt, wm + h * 16, wn, pa, pb, again[0]);
+                });
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    if (i == h) mend(acc[i], again[0]);
+            }
     }
     // behind the loop's last barrier: no wave reads the tiles any more
     gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, lds + w * gemm_write_bytes<FN>(), acc);

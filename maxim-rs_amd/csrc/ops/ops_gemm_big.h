@@ -65,13 +65,25 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     // apart, one offset and a step. What lies past the operand's end along the
     // strided axis is past the buffer's, past its end along the other one the
     // offset is sent there.
-    int ra, ka, rb, kb;
-    TA::where(t, ra, ka);
-    TB::where(t, rb, kb);
+    // (In fp32 tiles that are contiguous along rows the swizzle differs from
+    // chunk to chunk: an offset each.)
+    constexpr int OA = AK || sizeof(T) == 2 ? 1 : TA::PER, OB = BK_ || sizeof(T) == 2 ? 1 : TB::PER;
     const int lda = (int)(g.lda * sizeof(T)), ldb = (int)(g.ldb * sizeof(T));
     const uint32_t step_a = (AK ? NT / 8 : NT / TA::CPR) * lda, step_b = (BK_ ? NT / 8 : NT / TB::CPR) * ldb;
-    const uint32_t oa = AK || ra < rows_a ? (AK ? ra * lda + ka * (int)sizeof(T) : ka * lda + ra * (int)sizeof(T)) : kNowhere;
-    const uint32_t ob = BK_ || rb < rows_b ? (BK_ ? rb * ldb + kb * (int)sizeof(T) : kb * ldb + rb * (int)sizeof(T)) : kNowhere;
+    uint32_t oa[OA], ob[OB];
+    int ka, kb;  // along k: the chunks' first k, the same in all of them
+#pragma unroll
+    for (int i = OA - 1; i >= 0; --i) {
+        int r;
+        TA::where(i * NT + t, r, ka);
+        oa[i] = AK || r < rows_a ? (AK ? r * lda + ka * (int)sizeof(T) : ka * lda + r * (int)sizeof(T)) : kNowhere;
+    }
+#pragma unroll
+    for (int i = OB - 1; i >= 0; --i) {
+        int r;
+        TB::where(i * NT + t, r, kb);
+        ob[i] = BK_ || r < rows_b ? (BK_ ? r * ldb + kb * (int)sizeof(T) : kb * ldb + r * (int)sizeof(T)) : kNowhere;
+    }
     const char *next_a = reinterpret_cast<const char *>(ga), *next_b = reinterpret_cast<const char *>(gb);
     int left = kend - kbeg;
     // the next tile, in turn
@@ -83,20 +95,64 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
             __builtin_amdgcn_make_buffer_rsrc((void *)next_a, 0, (AK ? rows_a : k) * lda, 0x00020000);
         const __amdgpu_buffer_rsrc_t bufb =
             __builtin_amdgcn_make_buffer_rsrc((void *)next_b, 0, (BK_ ? rows_b : k) * ldb, 0x00020000);
-        const uint32_t fa = !AK || ka < k ? oa : kNowhere, fb = !BK_ || kb < k ? ob : kNowhere;
+        const uint32_t fa = !AK || ka < k ? oa[0] : kNowhere, fb = !BK_ || kb < k ? ob[0] : kNowhere;
 #pragma unroll
-        for (int i = 0; i < TA::PER; ++i) lds_load16(bufa, at + (i * NT + w * 64) * 16, fa + i * step_a);
+        for (int i = 0; i < TA::PER; ++i)
+            lds_load16(bufa, at + (i * NT + w * 64) * 16, OA > 1 ? oa[OA > 1 ? i : 0] : fa + i * step_a);
 #pragma unroll
-        for (int i = 0; i < TB::PER; ++i) lds_load16(bufb, bt + (i * NT + w * 64) * 16, fb + i * step_b);
+        for (int i = 0; i < TB::PER; ++i)
+            lds_load16(bufb, bt + (i * NT + w * 64) * 16, OB > 1 ? ob[OB > 1 ? i : 0] : fb + i * step_b);
         next_a += AK ? 128 : BK * lda;
         next_b += BK_ ? 128 : BK * ldb;
         left -= BK;
     };
     f32x4 acc[FM][FN];
+    clear(acc);
+    const int nk = (kend - kbeg + BK - 1) / BK;
+    constexpr int LOADS = TA::PER + TB::PER, AHEAD = (ST - 2) * LOADS;
+    const int pa = TA::lane_part(l), pb = TB::lane_part(l);
+    if constexpr (sizeof(T) == 4) {
+        // A tile at a time: the one after the ST - 1 in LDS is sent for when
+        // all waves are done with the place it takes.
+        auto run = [&](auto compute) {
+            next_a = reinterpret_cast<const char *>(ga), next_b = reinterpret_cast<const char *>(gb);
+            left = kend - kbeg;
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+            for (int i = 0; i < ST - 1; ++i) stage(st[i].a, st[i].b);
+            auto tile = [&](const Stage &c, const Stage &last) {
+                tiles_landed<AHEAD>();
+                stage(last.a, last.b);
+                __builtin_amdgcn_sched_barrier(0);
+                compute((LdsChar *)c.a, (LdsChar *)c.b);
+            };
+            int kt = 0;
+            for (; kt + ST <= nk; kt += ST) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+                for (int i = 0; i < ST; ++i) tile(st[i], st[(i + ST - 1) % ST]);
+            }
+#pragma unroll
+            for (int i = 0; i < ST - 1; ++i) {
+                if (kt + i >= nk) break;
+                tile(st[i], st[(i + ST - 1) % ST]);
+            }
+            tiles_landed<0>();
+        };
+        run([&](const LdsChar *at, const LdsChar *bt) { split_tile<TA, TB, FM, FN>(at, bt, wm, wn, pa, pb, acc); });
+        // sums that are not finite, of operands too large or not finite
+        // themselves, are formed again in fp32: 16 of a wave's rows at a time,
+        // the others keep their bits
+        if (__syncthreads_or(!unscale(acc)))
+            for (int h = 0; h < FM; ++h) {
+                f32x4 again[1][FN];
+                clear(again);
+                run([&](const LdsChar *at, const LdsChar *bt) {
+                    fp32_tile<TA, TB, FN>(at, bt, wm + h * 16, wn, pa, pb, again[0]);
+                });
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+                    if (i == h) mend(acc[i], again[0]);
+            }
+    } else {
     // A tile is four phases, two halves of k by two halves of the wave's rows,
     // each multiplying fragments that the phase before it read from LDS.
     constexpr int HM = FM / 2;
@@ -105,7 +161,6 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     // In the largest tiles a fragment's address (its own register where the
     // operand is not contiguous along k) is worked out when it is read: held
     // through the loop they do not fit beside the sums.
-    const int pa = TA::lane_part(l), pb = TB::lane_part(l);
     auto here = [&](int part) {
         if (FM * FN >= 32 && (!AK || !BK_)) asm volatile("" : "+v"(part));
         return part;
@@ -130,10 +185,8 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     // the next tile landed, the tile ST on is sent for into this one's place,
     // ST - 1 tiles' time ahead of its use. Past the last tile the loads bring
     // zeros without touching memory.
-    constexpr int LOADS = TA::PER + TB::PER, AHEAD = (ST - 2) * LOADS;
     auto tile = [&](const Stage &c, const Stage &n) {
-        constexpr int READS = sizeof(T) == 4 ? 4 : 2;  // of a fragment not contiguous along k
-        constexpr int RA = HM * (AK ? 1 : READS), RB = FN * (BK_ ? 1 : READS), MP = HM * FN * (sizeof(T) == 4 ? 4 : 1);
+        constexpr int RA = HM * (AK ? 1 : 2), RB = FN * (BK_ ? 1 : 2), MP = HM * FN;
         take_a((LdsChar *)c.a, 0, 1);
         multiply(0, 0);
         spread<RA, MP>();
@@ -152,7 +205,6 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
         multiply(1, 1);
         spread<RA + RB, MP>();
     };
-    const int nk = (kend - kbeg + BK - 1) / BK;
 #pragma unroll
     for (int i = 0; i < ST; ++i) stage(st[i].a, st[i].b);
     tiles_landed<AHEAD + LOADS>();
@@ -173,6 +225,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
             if (kt + i >= nk) break;
             tile(st[i], st[i + 1]);
         }
+    }
     }
     tiles_landed<0>();  // the last loads too, zeros: the tiles' LDS is free
     gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN>(), acc);

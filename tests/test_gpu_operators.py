@@ -442,6 +442,82 @@ def test_dense_gradient_against_differences(act):
         assert abs(got - want) <= 2e-5 * size + 1e-6, (act, planar, float(got), float(want))
 
 
+# sizes that reach every tile, with and without a cut sum, aligned and not:
+# rows, k, n
+BIG_SHAPES = [(4096, 256, 4096), (2048, 512, 2048), (2048, 512, 4096), (1024, 512, 1024), (256, 8192, 256),
+              (2048, 511, 2047), (1023, 511, 1025), (2048, 1028, 1028), (40000, 64, 96), (16, 4096, 512)]
+
+
+@pytest.mark.parametrize("planar", [False, True])
+@pytest.mark.parametrize("wt", [False, True])
+@pytest.mark.parametrize("dt", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("rows,k,n", BIG_SHAPES)
+def test_products_of_every_tile(rows, k, n, dt, wt, planar):
+    """The products alone, in both directions, with the 64-bit products on the
+    card. Each of a sum's `terms` roundings is half a step at most of a partial
+    sum of random signs, which reaches sqrt(terms) of a product's deviation d:
+    together a walk of about terms d u / 2, where S is 0.64 terms d. So 8 u S
+    holds for every element with room (and terms u S always)."""
+    g = torch.Generator(device="cuda").manual_seed(rows + k + n)
+
+    def rand(a, b, flip, std=1.0):
+        t = (torch.randn(b, a, generator=g, device="cuda") if flip else torch.randn(a, b, generator=g, device="cuda"))
+        t = (t * std).to(dt)
+        return (t, t.t().double()) if flip else (t, t.double())
+
+    x, xv = rand(rows, k, planar)
+    dy, dyv = rand(rows, n, planar)
+    w, wv = rand(n, k, wt, 1 / math.sqrt(k))
+    w = w.t() if wt else w
+    y = O.dense(x, w, planar=planar)
+    dx, dw, db = O.dense_backward(dy, x, w, planar=planar)
+    for got, want, size, terms in (((y.t() if planar else y), xv @ wv.t(), xv.abs() @ wv.abs().t(), k),
+                                   ((dx.t() if planar else dx), dyv @ wv, dyv.abs() @ wv.abs(), n),
+                                   (dw, dyv.t() @ xv, dyv.abs().t() @ xv.abs(), rows)):
+        tol = min(terms, 8) * U * size + half(dt) * want.abs() * 1.01 + tiny(dt)
+        off = (got.double() - want).abs() - tol
+        assert bool((off <= 0).all()), (terms, float(off.max()))
+    eb = rows * U * dyv.abs().sum(0)
+    wb = dyv.sum(0)
+    assert bool(((db.double() - wb).abs() <= eb + half(dt) * (wb.abs() + eb) + tiny(dt)).all())
+
+
+@pytest.mark.parametrize("planar", [False, True])
+@pytest.mark.parametrize("shape", [(64, 64, 64), (2048, 512, 2048), (1023, 511, 1025)])
+def test_fp32_products_of_far_values(shape, planar):
+    """fp32 products are formed from three bf16 parts: tiny and huge operands
+    keep their bits, and infinities and NaN are what fp32 sums give."""
+    rows, k, n = shape
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, k, generator=g, device="cuda")
+    w = torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k)
+    put = (lambda t: t.t().contiguous()) if planar else (lambda t: t)
+    take = (lambda t: t.t()) if planar else (lambda t: t)
+    bound = lambda a, b: 8 * U * (a.abs() @ b.abs().t())  # as above  # noqa: E731
+    for sx, sw in ((2.0 ** -100, 1.0), (2.0 ** -120, 2.0 ** 20), (2.0 ** 100, 1.0), (2.0 ** 110, 2.0 ** -110),
+                   (2.0 ** 60, 2.0 ** 50)):
+        a, b = x * sx, w * sw
+        av, bv = a.double(), b.double()
+        want = av @ bv.t()
+        got = take(O.dense(put(a), b, planar=planar)).double()
+        assert bool(((got - want).abs() <= bound(av, bv) + U * want.abs() + 1e-44).all()), (sx, sw)
+    x[3, 5], x[7, 9], x[11, 13] = float("inf"), float("nan"), 3e38
+    w[:, 13] = w[:, 13].abs() + 2.0  # 3e38 times this leaves the range: infinity
+    got, want = take(O.dense(put(x), w, planar=planar)), x.double() @ w.double().t()
+    assert torch.isnan(got[7]).all() and torch.isinf(got[3]).all() and torch.equal(got[3].sign(), w[:, 5].sign())
+    assert torch.isposinf(got[11]).all()
+    keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+    keep[3] = keep[7] = keep[11] = False
+    # column 13's one large term stays in every later partial sum P, so the
+    # roundings are of P and not of a walk's sums: 96 of them at k = 512, rms
+    # 0.58 u P each with P = 6 and S = 20, are 1.7 u S rms and 10 u S at six
+    # deviations, past the 8 of sums of like terms. k u S bounds any order.
+    slack = k * U * (x.double().abs() @ w.double().abs().t()) + U * want.abs()
+    assert bool(((got.double() - want).abs()[keep] <= slack[keep]).all())
+    x[3] = x[7] = x[11] = 0.0  # the other rows' bits do not depend on these
+    assert torch.equal(take(O.dense(put(x), w, planar=planar))[keep], got[keep])
+
+
 # ------------------------------------------------------ used together
 
 
