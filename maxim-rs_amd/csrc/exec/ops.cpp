@@ -323,8 +323,8 @@ struct TileCost {
 };
 const TileCost kTiles16[] = {{256, 2, 1, 1.6, 1.6, 10.0}, {128, 4, 1, 0.54, 0.54, 6.0}, {128, 2, 2, 0.65, 0.93, 7.0},
                              {64, 4, 2, 0.2, 0.39, 4.0},  {128, 0, 2, 1.25, 1.8, 8.0},  {64, 0, 5, 0.62, 1.7, 4.0}};
-const TileCost kTiles32[] = {{128, 4, 1, 2.0, 2.0, 6.0},  {128, 2, 2, 2.2, 3.8, 7.0},  {64, 4, 2, 0.6, 1.1, 4.0},
-                             {128, 0, 2, 2.45, 4.3, 8.0}, {64, 0, 5, 0.85, 3.0, 5.0}};
+const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1, 5.0}, {128, 0, 1, 1.95, 1.95, 9.0},
+                             {64, 0, 5, 0.85, 2.6, 6.0}};
 
 // The tile and the number of runs k is cut into that take the least time by
 // those costs: rounds of tiles over the 256 CUs, and for a cut k a second

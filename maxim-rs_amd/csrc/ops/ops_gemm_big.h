@@ -141,7 +141,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
         // sums that are not finite, of operands too large or not finite
         // themselves, are formed again in fp32: 16 of a wave's rows at a time,
         // the others keep their bits
-        if (__syncthreads_or(!unscale(acc)))
+        if (any_wave<WM * WN>(st[0].a, t, !unscale(acc)))
             for (int h = 0; h < FM; ++h) {
                 f32x4 again[1][FN];
                 clear(again);
@@ -267,5 +267,4 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
 OPS_DIRECT_TYPE(bf16, bf16)
 OPS_DIRECT_TYPE(f16, f16)
 OPS_DIRECT(2, f32, float, 128, 128, 2, 2)
-OPS_DIRECT(4, f32, float, 128, 128, 2, 2)
 OPS_DIRECT(4, f32, float, 64, 64, 2, 2)

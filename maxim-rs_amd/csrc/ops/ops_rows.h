@@ -645,7 +645,7 @@ extern "C" __global__ __launch_bounds__(1024) void mxo_join_parts(OpsJoinArgs a)
     else call_any;
 
 #define OPS_LN_ROWS(name, T, LPR, NV, BT)                                                                             \
-    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_rows_##name##_##LPR##x##NV(OpsLnArgs a) {                 \
+    extern "C" __global__ __launch_bounds__(BT, NV == 1 ? 8 : 4) void mxo_ln_rows_##name##_##LPR##x##NV(OpsLnArgs a) { \
         __shared__ float at[4 * (BT / 64)];                                                                           \
         OPS_BOTH(a.cols, 16 / sizeof(T), (ln_rows<T, LPR, NV, BT, true>(a, at)), (ln_rows<T, LPR, NV, BT, false>(a, at))) \
     }
