@@ -287,6 +287,7 @@ void join(int dev, void *stream, const float *part, int64_t nparts, int64_t n, v
 struct Operand {
     const void *data;
     int64_t own, sum;
+    bool padded;  // lines hold zeros up to whole 16 bytes
 };
 
 struct Product {
@@ -310,6 +311,8 @@ struct Plan {
     int bm = 0, bn = 0;
     unsigned block = 256;
     int stages = 0;  // straight to LDS with so many tiles there; 0: through registers
+    bool pack_a = false, pack_b = false;  // copied to aligned lines first
+    uint64_t pack_bytes = 0;
     int64_t splits = 1, kchunk = 0;
     uint64_t bytes = 0;
 };
@@ -322,7 +325,7 @@ struct TileCost {
     double one, all, rest;
 };
 const TileCost kTiles16[] = {{256, 2, 1, 1.6, 1.6, 10.0}, {128, 4, 1, 0.54, 0.54, 6.0}, {128, 2, 2, 0.65, 0.93, 7.0},
-                             {64, 4, 2, 0.2, 0.39, 4.0},  {128, 0, 2, 1.25, 1.8, 8.0},  {64, 0, 5, 0.62, 1.7, 4.0}};
+                             {64, 4, 2, 0.2, 0.39, 4.0},  {128, 0, 2, 1.3, 1.8, 8.0},   {64, 0, 5, 1.1, 1.7, 4.0}};
 const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1, 5.0}, {128, 0, 1, 1.95, 1.95, 9.0},
                              {64, 0, 5, 0.85, 2.6, 6.0}};
 
@@ -335,7 +338,11 @@ const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1,
 //
 // Up to 16 rows against weights that are contiguous along k go to the kernel
 // that reads those once, without LDS tiles or a second launch.
-Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct, bool by_k) {
+//
+// `pack_a`, `pack_b`: the bytes of an operand whose tiles cannot go straight to
+// LDS as it lies; copying it to aligned lines first (4 us and its bytes twice)
+// is one more choice. 1237 x 1001 x 777 in fp16: through registers 22 us.
+Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, uint64_t pack_a, uint64_t pack_b, bool by_k) {
     Plan best;
     if (by_k && m <= 16) {
         best.skinny = true;
@@ -345,7 +352,7 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct, bool 
     double least = std::numeric_limits<double>::infinity();
     const int64_t bk = 128 / (int64_t)type_size(dtype), steps = std::max<int64_t>(1, cdiv(k, bk));
     auto consider = [&](const TileCost &t) {
-        if (t.stages && !direct) return;
+        const uint64_t pack = t.stages ? pack_a + pack_b : 0;
         const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b);
         for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
             const int64_t each = cdiv(steps, cut), splits = cdiv(steps, each);
@@ -354,11 +361,15 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct, bool 
             double us = full * (each * t.all + t.rest);
             if (left) us += each * std::max(t.one, t.all * left / t.fit) + t.rest;
             if (splits > 1) us += 5.0 + (double)splits * m * n * 8 / 5e6;
+            if (pack) us += 4.0 + 2.0 * pack / 4e6;
             if (us >= least) continue;
             least = us;
             best.bm = best.bn = t.b;
             best.block = t.b == 256 ? 512 : 256;
             best.stages = t.stages;
+            best.pack_a = t.stages && pack_a;
+            best.pack_b = t.stages && pack_b;
+            best.pack_bytes = pack;
             best.splits = splits;
             best.kchunk = each * bk;
         }
@@ -367,7 +378,7 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct, bool 
         for (const TileCost &t : kTiles16) consider(t);
     else
         for (const TileCost &t : kTiles32) consider(t);
-    best.bytes = best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0;
+    best.bytes = best.pack_bytes + (best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0);
     return best;
 }
 
@@ -375,26 +386,79 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, bool direct, bool 
 // chunks, at 31-bit offsets inside a tile (of 256 rows or 64 k's), and lines
 // that do not overlap, so that an offset tells what is past the end.
 bool loads_direct(const Operand &o, bool by_k, int64_t own_n, int64_t sum_n, size_t size) {
-    const int64_t ld = by_k ? o.own : o.sum, extent = by_k ? sum_n : own_n;
-    const int64_t e = 16 / (int64_t)size;
-    return (uintptr_t)o.data % 16 == 0 && ld % e == 0 && extent % e == 0 && ld >= extent && ld < (int64_t(1) << 20);
+    const int64_t ld = by_k ? o.own : o.sum, extent = by_k ? sum_n : own_n, e = 16 / (int64_t)size;
+    return (uintptr_t)o.data % 16 == 0 && ld % e == 0 && (extent % e == 0 || o.padded) && ld >= extent &&
+           ld < int64_t(1) << (by_k ? 21 : 23);
 }
 
-void product(int dev, void *stream, const Product &p, void *ws) {
-    if (!p.m || !p.n) return;
-    // contiguous along k (also where there is only one row to stride over),
-    // or along the operand's own axis
-    const bool ak = p.a.sum == 1, bk = p.b.sum == 1;
+uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
+
+// Contiguous along k (also where there is only one row to stride over), or
+// along the operand's own axis.
+bool by_k(const Operand &o) { return o.sum == 1; }
+
+// The lines of an operand packed: contiguous extent in whole 16 bytes.
+struct Packed {
+    int64_t lines, extent, ld;
+    uint64_t bytes;
+};
+Packed packed(bool along_k, int64_t own_n, int64_t sum_n, size_t size) {
+    Packed p;
+    const int64_t e = 16 / (int64_t)size;
+    p.lines = along_k ? own_n : sum_n;
+    p.extent = along_k ? sum_n : own_n;
+    p.ld = cdiv(p.extent, e) * e;
+    p.bytes = up((uint64_t)p.lines * p.ld * size);
+    return p;
+}
+
+Plan plan_of(const Product &p) {
+    if (!p.m || !p.n) return {};
+    const bool ak = by_k(p.a), bk = by_k(p.b);
     const size_t size = type_size(p.dtype);
-    const Plan pl = plan_product(p.dtype, p.m, p.n, p.k,
-                                 loads_direct(p.a, ak, p.m, p.k, size) && loads_direct(p.b, bk, p.n, p.k, size), ak && bk);
+    const uint64_t pa = loads_direct(p.a, ak, p.m, p.k, size) ? 0 : packed(ak, p.m, p.k, size).bytes;
+    const uint64_t pb = loads_direct(p.b, bk, p.n, p.k, size) ? 0 : packed(bk, p.n, p.k, size).bytes;
+    return plan_product(p.dtype, p.m, p.n, p.k, pa, pb, ak && bk);
+}
+
+void product(int dev, void *stream, const Product &given, void *ws) {
+    if (!given.m || !given.n) return;
+    Product p = given;
+    const bool ak = by_k(p.a), bk = by_k(p.b);
+    const size_t size = type_size(p.dtype);
+    const Plan pl = plan_of(p);
+    char *at = static_cast<char *>(ws);
+    OpsPackArgs pack{};
+    int jobs = 0;
+    int64_t blocks = 0;
+    auto add = [&](Operand &o, bool along_k, int64_t own_n) {
+        const Packed k = packed(along_k, own_n, p.k, size);
+        OpsPackJob &j = pack.job[jobs++];
+        j.src = o.data;
+        j.dst = at;
+        j.lines = k.lines, j.extent = k.extent;
+        j.src_ld = along_k ? o.own : o.sum;
+        j.dst_ld = k.ld;
+        const int64_t vecs = k.ld / (16 / (int64_t)size);
+        for (j.shift = 3; j.shift < 8 && (int64_t)4 << j.shift < vecs;) ++j.shift;
+        j.segs = (int32_t)cdiv(vecs, (int64_t)4 << j.shift);
+        blocks = std::max(blocks, cdiv(k.lines, 256 >> j.shift) * j.segs);
+        o = along_k ? Operand{at, k.ld, 1, true} : Operand{at, 1, k.ld, true};
+        at += k.bytes;
+    };
+    if (pl.pack_a) add(p.a, ak, p.m);
+    if (pl.pack_b) add(p.b, bk, p.n);
+    if (jobs) {
+        if (blocks > std::numeric_limits<int32_t>::max()) throw Error("the product's operands are too large");
+        launch(dev, stream, size == 2 ? "mxo_pack_16" : "mxo_pack_32", blocks, jobs, 256, pack);
+    }
     OpsGemmArgs g{};
     g.a = p.a.data;
     g.b = p.b.data;
     g.c = p.c;
     g.z = p.z;
     g.res = p.res;
-    g.part = static_cast<float *>(ws);
+    g.part = reinterpret_cast<float *>(at);
     g.lda = ak ? p.a.own : p.a.sum;
     g.ldb = bk ? p.b.own : p.b.sum;
     g.ldc = p.ldc;
@@ -425,8 +489,7 @@ void product(int dev, void *stream, const Product &p, void *ws) {
            "mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
                (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
            tm * tn * pl.splits, 1, pl.block, g);
-    if (pl.splits > 1)
-        {
+    if (pl.splits > 1) {
         // few sums of many splits: eight threads to each
         const bool deep = pl.splits >= 16;
         launch(dev, stream, (deep ? "mxo_join8_" : "mxo_join_") + t,
@@ -436,7 +499,7 @@ void product(int dev, void *stream, const Product &p, void *ws) {
 
 // An operand of a product as (own axis, summed axis): rows summed over or not.
 Operand operand(const mxh_mat &m, bool sum_rows) {
-    Operand o{m.data, sum_rows ? m.col_stride : m.row_stride, sum_rows ? m.row_stride : m.col_stride};
+    Operand o{m.data, sum_rows ? m.col_stride : m.row_stride, sum_rows ? m.row_stride : m.col_stride, false};
     const int64_t own_n = sum_rows ? m.cols : m.rows, sum_n = sum_rows ? m.rows : m.cols;
     // an axis of one element has no stride of its own: the other one's order
     // holds, and where both are single the element is contiguous
@@ -459,14 +522,9 @@ Product oriented(const mxh_mat &out, const Operand &rows, const Operand &cols, i
     return p;
 }
 
-// What a product may need, whichever way its operands load.
-uint64_t product_bytes(const mxh_mat &out, int64_t k, bool by_cols) {
-    if (empty(out)) return 0;
-    const int64_t m = by_cols ? out.rows : out.cols, n = by_cols ? out.cols : out.rows;
-    return std::max(plan_product(out.dtype, m, n, k, false, false).bytes, plan_product(out.dtype, m, n, k, true, false).bytes);
+Product dense_product(const mxh_mat &x, const mxh_mat &w, const mxh_mat &y, bool by_cols) {
+    return oriented(y, operand(x, false), operand(w, false), x.cols, by_cols);
 }
-
-uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
 
 // mxh_dense_backward's workspace: dz where there is an activation, the bias's
 // partial sums, and one product's partial sums at a time.
@@ -486,8 +544,21 @@ int64_t dz_parts(const mxh_mat &dy, bool by_cols) {
     return std::max<int64_t>(1, std::min(cdiv(2048, std::max<int64_t>(1, across)), most));
 }
 
-BwdLayout bwd_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mxh_mat *dx, const mxh_mat *dw,
-                     const mxh_vec *db, int act) {
+// dz as an operand: the pass that writes it fills its lines' ends with zeros.
+Operand dz_operand(const BwdLayout &l, bool sum_rows) {
+    Operand o = operand(l.dz, sum_rows);
+    o.padded = l.dz_bytes != 0;
+    return o;
+}
+Product product_dx(const BwdLayout &l, const mxh_mat &w, const mxh_mat &dx) {
+    return oriented(dx, dz_operand(l, false), operand(w, true), w.rows, out_by_cols(dx));
+}
+Product product_dw(const BwdLayout &l, const mxh_mat &x, const mxh_mat &dw) {
+    return oriented(dw, dz_operand(l, true), operand(x, true), x.rows, out_by_cols(dw));
+}
+
+BwdLayout bwd_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mxh_mat &w, const mxh_mat *dx,
+                     const mxh_mat *dw, const mxh_vec *db, int act) {
     BwdLayout l;
     l.dz = dy;
     const bool products = dx || dw;
@@ -501,13 +572,14 @@ BwdLayout bwd_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mx
             l.dz.col_stride = cdiv(dy.rows, pad) * pad, l.dz.row_stride = 1;
             l.dz_bytes = up((uint64_t)dy.cols * l.dz.col_stride * type_size(dy.dtype));
         }
+        l.dz.data = nullptr;  // aligned wherever the workspace is
     }
     if (db) {
         l.parts = dz_parts(dy, by_cols);
         l.part_bytes = up((uint64_t)l.parts * dy.cols * 4);
     }
-    if (dx) l.product_bytes = std::max(l.product_bytes, product_bytes(*dx, dy.cols, out_by_cols(*dx)));
-    if (dw) l.product_bytes = std::max(l.product_bytes, product_bytes(*dw, x.rows, out_by_cols(*dw)));
+    if (dx && !empty(*dx)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dx(l, w, *dx)).bytes);
+    if (dw && !empty(*dw)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dw(l, x, *dw)).bytes);
     return l;
 }
 
@@ -672,7 +744,11 @@ int mxh_dense_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, ui
         if (!bytes) throw Error("bytes: missing");
         check_first(need(x, "x"), "x");
         check_mat(need(y, "y"), "y", x->dtype, x->rows, need(w, "w").rows);
-        *bytes = std::max(product_bytes(*y, x->cols, true), product_bytes(*y, x->cols, false));
+        // a y of one row or column has both orders, and z or a residual may settle it
+        *bytes = 0;
+        if (empty(*y)) return;
+        if (out_by_cols(*y)) *bytes = plan_of(dense_product(*x, *w, *y, true)).bytes;
+        if (out_by_rows(*y)) *bytes = std::max(*bytes, plan_of(dense_product(*x, *w, *y, false)).bytes);
     });
 }
 
@@ -700,10 +776,10 @@ int mxh_dense(int device, void *stream, const mxh_mat *x, const mxh_mat *w, cons
             if (residual && !(o == y && same(*residual, Y))) refuse_overlap(*o, "an output", *residual, "the residual");
         }
         if (z) refuse_overlap(Y, "y", *z, "z");
-        check_workspace(workspace, workspace_bytes, product_bytes(Y, X.cols, by_cols));
         if (empty(Y)) return;
+        Product p = dense_product(X, W, Y, by_cols);
+        check_workspace(workspace, workspace_bytes, plan_of(p).bytes);
         OnDevice on(device);
-        Product p = oriented(Y, operand(X, false), operand(W, false), X.cols, by_cols);
         p.bias = bias;
         p.bias_rows = !by_cols;
         p.act = act;
@@ -721,7 +797,7 @@ int mxh_dense_backward_workspace(const mxh_mat *dy, const mxh_mat *x, const mxh_
         check_first(need(x, "x"), "x");
         check_mat(need(dy, "dy"), "dy", x->dtype, x->rows, need(w, "w").rows);
         check_act(act);
-        *bytes = std::max(bwd_layout(*dy, true, *x, dx, dw, db, act).total(), bwd_layout(*dy, false, *x, dx, dw, db, act).total());
+        *bytes = std::max(bwd_layout(*dy, true, *x, *w, dx, dw, db, act).total(), bwd_layout(*dy, false, *x, *w, dx, dw, db, act).total());
     });
 }
 
@@ -758,7 +834,7 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
             for (int j = 0; j < i; ++j)
                 if (outs[j]) refuse_overlap(*outs[i], on_[i], *outs[j], on_[j]);
         }
-        BwdLayout l = bwd_layout(DY, dz_cols, X, dx, dw, db, act);
+        BwdLayout l = bwd_layout(DY, dz_cols, X, W, dx, dw, db, act);
         check_workspace(workspace, workspace_bytes, l.total());
         OnDevice on(device);
         char *ws = static_cast<char *>(workspace);
@@ -780,9 +856,9 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         if (db) join(device, stream, a.part, DY.rows ? l.parts : 0, DY.cols, db->data, nullptr, db->dtype);
         void *pw = ws + l.dz_bytes + l.part_bytes;
         if (dx && !empty(*dx))
-            product(device, stream, oriented(*dx, operand(l.dz, false), operand(W, true), W.rows, out_by_cols(*dx)), pw);
+            product(device, stream, product_dx(l, W, *dx), pw);
         if (dw && !empty(*dw))
-            product(device, stream, oriented(*dw, operand(l.dz, true), operand(X, true), X.rows, out_by_cols(*dw)), pw);
+            product(device, stream, product_dw(l, X, *dw), pw);
     });
 }
 

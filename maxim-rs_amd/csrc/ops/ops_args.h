@@ -29,6 +29,19 @@ struct OpsGemmArgs {
     int32_t bias_rows, pad;  // one bias value per m instead of per n
 };
 
+// Operands of a product copied to lines of whole 16 bytes, zeros at their
+// ends: job blockIdx.y, 2^shift threads a line, four vectors each, `segs` such
+// runs a line.
+struct OpsPackJob {
+    const void *src;
+    void *dst;
+    int64_t lines, extent, src_ld, dst_ld;
+    int32_t shift, segs;
+};
+struct OpsPackArgs {
+    OpsPackJob job[2];
+};
+
 // x, y and the gradients [rows][cols] at rs and cs elements between rows and
 // columns, one of them 1.
 struct OpsLnArgs {

@@ -493,6 +493,32 @@ __device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
     }
 }
 
+// Lines of any alignment to lines of whole 16 bytes, four vectors a thread.
+template <typename T>
+__device__ __forceinline__ void pack_lines(const OpsPackArgs &args) {
+    constexpr int E = 16 / sizeof(T);
+    const OpsPackJob &a = args.job[blockIdx.y];
+    const int group = blockIdx.x / a.segs, seg = blockIdx.x - group * a.segs, t = threadIdx.x;
+    const int64_t line = (int64_t)group * (256 >> a.shift) + (t >> a.shift);
+    if (line >= a.lines) return;
+    const T *src = static_cast<const T *>(a.src) + line * a.src_ld;
+    T *dst = static_cast<T *>(a.dst) + line * a.dst_ld;
+    const int64_t v0 = ((int64_t)seg << (a.shift + 2)) + (t & ((1 << a.shift) - 1));
+    Vec<T, E> v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t at = (v0 + ((int64_t)j << a.shift)) * E;
+        v[j] = load_upto<T, E>(src + at, a.extent - at);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t at = (v0 + ((int64_t)j << a.shift)) * E;
+        if (at < a.dst_ld) store_n<T, E>(dst + at, v[j]);
+    }
+}
+extern "C" __global__ __launch_bounds__(256) void mxo_pack_16(OpsPackArgs a) { pack_lines<f16>(a); }
+extern "C" __global__ __launch_bounds__(256) void mxo_pack_32(OpsPackArgs a) { pack_lines<float>(a); }
+
 #define OPS_GEMM1(name, T, BM, BN, WM, WN, tag, AK, BK)                                                    \
     extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxo_gemm_##name##_##BM##x##BN##_##tag(      \
         OpsGemmArgs g) {                                                                                   \

@@ -570,7 +570,8 @@ __device__ __forceinline__ void dz_rows(const OpsDzArgs &a, float (*sh)[64 * 16 
                 s[e] += v[e];
                 vd.v[e] = from_f<T>(v[e]);
             }
-            if (a.dz) store_in<T, E, WHOLE>(static_cast<T *>(a.dz) + r * a.drs + c, vd, have);
+            // lines of dz are whole vectors, their ends zeros
+            if (a.dz) store_n<T, E>(static_cast<T *>(a.dz) + r * a.drs + c, vd);
         }
     if (!a.part) return;
 #pragma unroll
@@ -602,7 +603,8 @@ __device__ __forceinline__ void dz_planar(const OpsDzArgs &a) {
             if (r + e < end) s += v[e];
             vd.v[e] = from_f<T>(v[e]);
         }
-        if (a.dz) store_upto<T, E>(static_cast<T *>(a.dz) + c * a.dcs + r, vd, end - r);
+        // lines of dz are whole vectors, their ends zeros (a run is whole vectors)
+        if (a.dz) store_n<T, E>(static_cast<T *>(a.dz) + c * a.dcs + r, vd);
     }
     if (!a.part) return;
     s = wave_sum(s);

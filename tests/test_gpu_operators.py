@@ -445,7 +445,7 @@ def test_dense_gradient_against_differences(act):
 # sizes that reach every tile, with and without a cut sum, aligned and not:
 # rows, k, n
 BIG_SHAPES = [(4096, 256, 4096), (2048, 512, 2048), (2048, 512, 4096), (1024, 512, 1024), (256, 8192, 256),
-              (2048, 511, 2047), (1023, 511, 1025), (2048, 1028, 1028), (40000, 64, 96), (16, 4096, 512)]
+              (2048, 511, 2047), (4095, 1023, 2049), (1023, 511, 1025), (2048, 1028, 1028), (40000, 64, 96), (16, 4096, 512)]
 
 
 @pytest.mark.parametrize("planar", [False, True])

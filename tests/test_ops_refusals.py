@@ -115,7 +115,7 @@ def test_dense_refusals():
     refused("an output overlaps the residual", dn(x, w, b, y, res=mat(16, 24, 3 << 20), z=mat(16, 24, 3 << 20)))
     refused("y overlaps z", dn(x, w, b, y, z=y))
     # few outputs and a long sum are split over the card, which takes scratch
-    x, w, y = mat(2, 65536), mat(8, 65536, 1 << 20), mat(2, 8, 1 << 24)
+    x, w, y = mat(64, 65536), mat(8, 65536, 1 << 24), mat(64, 8, 1 << 26)
     size = C.c_uint64()
     assert O._lib().mxh_dense_workspace(x, w, y, size) == 0 and size.value > 0
     refused("bytes of workspace", dn(x, w, vec(8), y))
