@@ -148,15 +148,18 @@ def _act(act):
 
 def _new(x, X, n, planar):
     """An uninitialised result of x's positions with n features, in x's memory
-    order (X: x as a matrix)."""
+    order (X: x as a matrix): the tensor, and it as a matrix."""
     if n == X.cols and x.is_contiguous():
-        return _torch.empty_like(x)
-    rest = tuple(x.shape[1:] if planar else x.shape[:-1])
-    by_rows = X.row_stride == 1 and X.rows > 1 and (X.col_stride != 1 or X.cols == 1)
-    if planar == by_rows or X.rows <= 1:
-        return x.new_empty((n,) + rest if planar else rest + (n,))
-    t = x.new_empty((n,) + rest if by_rows else rest + (n,))
-    return t.movedim(-1, 0) if planar else t.movedim(0, -1)
+        t, by_rows = _torch.empty_like(x), planar
+    else:
+        rest = tuple(x.shape[1:] if planar else x.shape[:-1])
+        by_rows = X.row_stride == 1 and X.rows > 1 and (X.col_stride != 1 or X.cols == 1)
+        if X.rows <= 1:
+            by_rows = planar
+        t = x.new_empty((n,) + rest if by_rows else rest + (n,))
+        if by_rows != planar:
+            t = t.movedim(-1, 0) if planar else t.movedim(0, -1)
+    return t, Mat(t.data_ptr(), X.rows, n, 1 if by_rows else n, X.rows if by_rows else 1, X.dtype, 0)
 
 
 def _workspace(n, x):
@@ -179,8 +182,7 @@ def layernorm(x, scale, bias=None, eps=1e-6, planar=False, stats=False, out=None
     X = _mat(x, "x", d, planar)
     S = _vec(scale, "scale", d)
     B = None if bias is None else _vec(bias, "bias", d)
-    y = _new(x, X, X.cols, planar) if out is None else out
-    Y = X if y is x else _mat(y, "out", d, planar)
+    y, Y = _new(x, X, X.cols, planar) if out is None else (out, X if out is x else _mat(out, "out", d, planar))
     mean = rstd = None
     if stats:
         shape = x.shape[1:] if planar else x.shape[:-1]
@@ -204,15 +206,17 @@ def layernorm_backward(dy, x, scale, mean, rstd, add=None, planar=False, dx=True
     A = None if add is None else _mat(add, "add", d, planar)
     gx = DX = ds = db = DS = DB = ws = None
     if dx:
-        gx = _new(x, X, X.cols, planar) if out is None else out
-        DX = DY if gx is dy else A if gx is add and add is not None else _mat(gx, "out", d, planar)
+        if out is None:
+            gx, DX = _new(x, X, X.cols, planar)
+        else:
+            gx, DX = out, DY if out is dy else A if out is add else _mat(out, "out", d, planar)
     elif out is not None:
         raise P.MaximError("out without dx")
     n = 0
     if params:
-        ds = scale.new_empty(X.cols)
+        ds = scale.new_empty(S.n)
         db = _torch.empty_like(ds)
-        DS, DB = _vec(ds, "dscale", d), _vec(db, "dbias", d)
+        DS, DB = Vec(ds.data_ptr(), S.n, S.dtype, 0), Vec(db.data_ptr(), S.n, S.dtype, 0)
         size = C.c_uint64()
         _check(_L.mxh_layernorm_backward_workspace(X, size))
         n = size.value
@@ -233,12 +237,8 @@ def dense(x, w, bias=None, act=None, slope=0.0, residual=None, planar=False, sav
     B = None if bias is None else _vec(bias, "bias", d)
     R = None if residual is None else _mat(residual, "residual", d, planar)
     like, Like = (x, X) if residual is None else (residual, R)
-    y = _new(like, Like, W.rows, planar) if out is None else out
-    Y = _mat(y, "out", d, planar)
-    z = Z = None
-    if save:
-        z = _new(y, Y, W.rows, planar)
-        Z = _mat(z, "z", d, planar)
+    y, Y = _new(like, Like, W.rows, planar) if out is None else (out, _mat(out, "out", d, planar))
+    z, Z = _new(y, Y, W.rows, planar) if save else (None, None)
     size = C.c_uint64()
     _check(_L.mxh_dense_workspace(X, W, Y, size))
     ws = _workspace(size.value, x)
@@ -258,12 +258,12 @@ def dense_backward(dy, x, w, z=None, act=None, slope=0.0, planar=False, dx=True,
     Z = None if z is None else _mat(z, "z", d, planar)
     gx = gw = gb = DX = DW = DB = None
     if dx:
-        gx = _new(x, X, X.cols, planar)
-        DX = _mat(gx, "dx", d, planar)
+        gx, DX = _new(x, X, X.cols, planar)
     if dw:
         # in w's own memory order
         gw = w.new_empty(w.shape) if W.col_stride == 1 else w.new_empty((W.cols, W.rows)).t()
-        DW = _mat(gw, "dw", d, False)
+        DW = (Mat(gw.data_ptr(), W.rows, W.cols, W.cols, 1, W.dtype, 0) if W.col_stride == 1 else
+              Mat(gw.data_ptr(), W.rows, W.cols, 1, W.rows, W.dtype, 0))
     if db:
         gb = w.new_empty(W.rows, dtype=db_dtype)
         DB = _vec(gb, "db", d)
