@@ -326,8 +326,8 @@ struct TileCost {
 };
 const TileCost kTiles16[] = {{256, 2, 1, 1.6, 1.6, 10.0}, {128, 4, 1, 0.54, 0.54, 6.0}, {128, 2, 2, 0.65, 0.93, 7.0},
                              {64, 4, 2, 0.2, 0.39, 4.0},  {128, 0, 2, 1.3, 1.8, 8.0},   {64, 0, 5, 1.1, 1.7, 4.0}};
-const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1, 5.0}, {128, 0, 1, 1.95, 1.95, 9.0},
-                             {64, 0, 5, 0.85, 2.6, 6.0}};
+const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1, 5.0}, {64, 2, 5, 0.75, 2.35, 5.0},
+                             {128, 0, 1, 1.95, 1.95, 9.0}, {64, 0, 5, 0.85, 2.6, 6.0}};
 
 // The tile and the number of runs k is cut into that take the least time by
 // those costs: rounds of tiles over the 256 CUs, and for a cut k a second
@@ -354,9 +354,9 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, uint64_t pack_a, u
     auto consider = [&](const TileCost &t) {
         const uint64_t pack = t.stages ? pack_a + pack_b : 0;
         const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b);
-        for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
             const int64_t each = cdiv(steps, cut), splits = cdiv(steps, each);
-            if (cut > 1 && (each < 2 || splits != cut)) continue;
+            if (cut > 1 && each < 2) continue;
             const int64_t total = tiles * splits, full = total / (256 * t.fit), left = cdiv(total % (256 * t.fit), 256);
             double us = full * (each * t.all + t.rest);
             if (left) us += each * std::max(t.one, t.all * left / t.fit) + t.rest;

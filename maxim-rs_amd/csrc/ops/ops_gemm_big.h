@@ -268,3 +268,4 @@ OPS_DIRECT_TYPE(bf16, bf16)
 OPS_DIRECT_TYPE(f16, f16)
 OPS_DIRECT(2, f32, float, 128, 128, 2, 2)
 OPS_DIRECT(4, f32, float, 64, 64, 2, 2)
+OPS_DIRECT(2, f32, float, 64, 64, 2, 2)
