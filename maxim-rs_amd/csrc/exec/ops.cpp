@@ -6,11 +6,13 @@
 #include "maxim_ops.h"
 
 #include <algorithm>
+#include <array>
 #include <cstring>
 #include <limits>
 #include <map>
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "../ops/ops_args.h"
 #include "hip_api.hpp"
@@ -211,9 +213,9 @@ void check_act(int act) {
 // ------------------------------------------------------------- LayerNorm
 
 // The kernel of a LayerNorm pass: by rows, `lpr` threads a row with `nv`
-// vectors of 16 bytes each, or in planar order `block` threads with `ch`
-// channels each; `whole` when the row fits the largest of them, else the
-// forms that read it three times. `grid` blocks walk over the rows; in the
+// vectors of 16 bytes each, or in planar order `block` threads, so many lanes
+// along the positions and channels a thread; `whole` when the backward kernel
+// sums the parameters' gradients too, else another does. `grid` blocks walk over the rows; in the
 // backward pass each leaves one partial sum of the parameters' gradients.
 struct LnPlan {
     std::string form;
@@ -234,6 +236,7 @@ LnPlan ln_plan(int dtype, int64_t rows, int64_t cols, bool by_cols, bool backwar
         for (const auto &f : kForms) {
             if (vecs > f[0] * f[1]) continue;
             p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]);
+            p.whole = !(backward && f[1] > 1 && type_size(dtype) == 2);
             p.block = f[0] <= 64 ? 256 : backward ? 1024 : std::max(256, f[0]);
             const int64_t steps = cdiv(rows, p.block / f[0]);
             const int64_t most = 524288 / p.block;
@@ -244,12 +247,26 @@ LnPlan ln_plan(int dtype, int64_t rows, int64_t cols, bool by_cols, bool backwar
         }
         if (p.form.empty()) p.form = "long", p.block = 1024, p.grid = std::min<int64_t>(rows, 65536), p.whole = false;
     } else {
-        const int64_t tiles = cdiv(rows, 64);
-        static const int kForms[][2] = {{256, 1}, {256, 2}, {256, 4}, {512, 4}, {512, 8}};
-        for (const auto &f : kForms) {
-            if (cols > f[0] / (64 / e) * f[1]) continue;
-            p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]);
+        // threads, lanes of 16 bytes along the positions, channels a thread:
+        // the most lanes that still leave two tiles a CU, else 16 or 8. The
+        // backward pass holds two matrices and the parameters' sums: at most
+        // eight channels of fp32, four of 16 bits, go into registers.
+        typedef std::vector<std::array<int, 3>> Forms;
+        static const Forms kForward16 = {{256, 64, 4}, {256, 64, 8}, {512, 64, 8},  {512, 64, 16}, {512, 32, 16}, {512, 16, 1},
+                                         {512, 16, 2}, {512, 16, 4}, {512, 16, 8}, {512, 16, 16}, {512, 8, 16}};
+        static const Forms kForward32 = {{256, 64, 4}, {256, 64, 8}, {512, 16, 2}, {512, 64, 16}, {512, 32, 16},
+                                         {512, 16, 4}, {512, 16, 8}, {512, 16, 16}, {512, 8, 16}};
+        static const Forms kBackward16 = {{256, 64, 4}, {512, 64, 4}, {512, 32, 4}, {512, 16, 1},
+                                          {512, 16, 2}, {512, 16, 4}, {512, 8, 4}};
+        static const Forms kBackward32 = {{256, 64, 4}, {512, 64, 4}, {512, 64, 8}, {512, 32, 8}, {512, 16, 1},
+                                          {512, 16, 2}, {512, 16, 4}, {512, 16, 8}, {512, 8, 8}};
+        int64_t tiles = cdiv(rows, 16 * e);
+        for (const auto &f : !backward ? e == 8 ? kForward16 : kForward32 : e == 8 ? kBackward16 : kBackward32) {
+            if (cols > f[0] / f[1] * f[2]) continue;
+            if (f[1] > 16 && cdiv(rows, f[1] * e) < 512) continue;
+            p.form = std::to_string(f[0]) + "x" + std::to_string(f[1]) + "x" + std::to_string(f[2]);
             p.block = f[0];
+            tiles = cdiv(rows, f[1] * e);
             p.grid = std::min<int64_t>(tiles, backward ? 262144 / f[0] : 4096);
             break;
         }

@@ -56,17 +56,36 @@ __device__ __forceinline__ void store_upto(T *p, const Vec<T, N> &v, int64_t hav
         if (i < have) p[i] = v.v[i];
 }
 
-// E elements at p, of which the first `have` are the operand's, the others
-// zeros. WHOLE: all of them or none (the extent is a multiple of E), which
-// takes no branch: where there are none, E elements at `any`, which are the
-// operand's too, are loaded and dropped.
+// E elements at p, of which the first `have` are the operand's and the others
+// anything, for the user to leave out (left out here, a load ahead of its use
+// would be waited for). WHOLE: all of them or none (the extent is a multiple of E). A lane
+// without any loads at `any`, which are the operand's too, and drops them. A
+// lane with some loads E all the same where that stays inside the operand, up
+// to its last E elements at `last`: at the ends of all rows but the last few.
+// So only a wave there takes a branch, and loads are not waited for one by one.
 template <typename T, int E, bool WHOLE>
-__device__ __forceinline__ Vec<T, E> load_in(const T *p, const T *any, int64_t have) {
-    if constexpr (!WHOLE) return load_upto<T, E>(p, have);
-    Vec<T, E> r = load_n<T, E>(have > 0 ? p : any);
+__device__ __forceinline__ u32x4 load_raw(const T *p, const T *any, const T *last, int64_t have) {
+    static_assert(E * sizeof(T) == 16, "");
+    u32x4 w;
+    if (!WHOLE && __builtin_amdgcn_ballot_w64((have > 0 ? p : any) > last) != 0)
+        w = __builtin_bit_cast(u32x4, load_upto<T, E>(p, have));
+    else
+        __builtin_memcpy(&w, have > 0 ? p : any, 16);
+    return w;
+}
+// The same with zeros past the first `have`. (Dropped by whole registers:
+// element by element a 16-bit vector would be held in eight of them.)
+template <typename T, int E, bool WHOLE>
+__device__ __forceinline__ u32x4 load_in(const T *p, const T *any, const T *last, int64_t have) {
+    u32x4 w = load_raw<T, E, WHOLE>(p, any, last, have);
+    const int h = (int)min(have, (int64_t)E);
 #pragma unroll
-    for (int i = 0; i < E; ++i) r.v[i] = have > 0 ? r.v[i] : (T)0.0f;
-    return r;
+    for (int i = 0; i < 4; ++i) {
+        if (WHOLE) w[i] = have > 0 ? w[i] : 0u;
+        else if (sizeof(T) == 2) w[i] = h > 2 * i + 1 ? w[i] : h == 2 * i + 1 ? w[i] & 0xffffu : 0u;
+        else w[i] = h > i ? w[i] : 0u;
+    }
+    return w;
 }
 template <typename T, int E, bool WHOLE>
 __device__ __forceinline__ void store_in(T *p, const Vec<T, E> &v, int64_t have) {
@@ -77,16 +96,27 @@ __device__ __forceinline__ void store_in(T *p, const Vec<T, E> &v, int64_t have)
     }
 }
 
-// The same value, of which the compiler keeps nothing it worked out before:
-// 16-bit elements are converted again from here on, instead of held as fp32
-// in twice the registers.
-template <typename T, int E>
-__device__ __forceinline__ void reread(Vec<T, E> &v) {
-    static_assert(sizeof(v) == 16, "");
-    u32x4 w = __builtin_bit_cast(u32x4, v);
-    asm volatile("" : "+v"(w));
-    typedef Vec<T, E> V;
-    v = __builtin_bit_cast(V, w);
+// 16 bytes of elements as they lie, converted where they are used: taken apart,
+// a 16-bit vector would be held in eight registers instead of four.
+template <typename T>
+__device__ __forceinline__ float elem(const u32x4 &w, int e) {
+    if constexpr (sizeof(T) == 4) {
+        const uint32_t u = w[e];  // (of the vector's element itself the cast takes the first one)
+        return __builtin_bit_cast(float, u);
+    } else if constexpr (__is_same(T, bf16)) {
+        return __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    } else {
+        return (float)__builtin_bit_cast(f16, (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu));
+    }
+}
+// The same value, of which the compiler keeps nothing that it worked out before:
+// elements are converted again from here on.
+__device__ __forceinline__ void reread(u32x4 &w) { asm volatile("" : "+v"(w)); }
+
+// The same number, of which nothing is worked out before this place.
+__device__ __forceinline__ int64_t here(int64_t v) {
+    asm volatile("" : "+s"(v));
+    return v;
 }
 
 // A parameter vector's element, of the activations' type or fp32.

@@ -62,14 +62,15 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
         }
     }
     int turn = 0;
-    Vec<T, E> ahead[NV];
+    u32x4 ahead[NV];
     auto fetch = [&](int64_t r0) {
         // past the end: the last row again, not stored
-        const T *x = static_cast<const T *>(a.x) + min(r0 + grp, a.rows - 1) * a.xrs;
+        const T *x0 = static_cast<const T *>(a.x), *x = x0 + min(r0 + grp, a.rows - 1) * a.xrs;
+        const T *last = x0 + (a.rows - 1) * a.xrs + cols - E;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * LPR + li) * E;
-            ahead[j] = load_in<T, E, WHOLE>(x + c, x, cols - c);
+            ahead[j] = load_raw<T, E, WHOLE>(x + c, x, last, cols - c);
         }
     };
     const int64_t step = (int64_t)gridDim.x * RPB;
@@ -77,7 +78,7 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
     if (r0 < a.rows) fetch(r0);
     for (; r0 < a.rows; r0 += step) {
         const int64_t r = r0 + grp;
-        Vec<T, E> v[NV];
+        u32x4 v[NV];
         float s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) v[j] = ahead[j];
@@ -85,7 +86,7 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += to_f<T>(v[j].v[e]);
+            for (int e = 0; e < E; ++e) s += (j * LPR + li) * E + e < cols ? elem<T>(v[j], e) : 0.0f;
         float zero = 0.0f;
         row_sum2<LPR, BT>(s, zero, at, turn++);
         const float mean = s / n;  // a division: the mean of equal values is that value
@@ -93,7 +94,7 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float d = to_f<T>(v[j].v[e]) - mean;
+                const float d = elem<T>(v[j], e) - mean;
                 q += (j * LPR + li) * E + e < cols ? d * d : 0.0f;
             }
         zero = 0.0f;
@@ -106,7 +107,7 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
             const int c = (j * LPR + li) * E;
             Vec<T, E> o;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o.v[e] = from_f<T>((to_f<T>(v[j].v[e]) - mean) * rstd * sc[j][e] + bi[j][e]);
+            for (int e = 0; e < E; ++e) o.v[e] = from_f<T>((elem<T>(v[j], e) - mean) * rstd * sc[j][e] + bi[j][e]);
             store_in<T, E, WHOLE>(y + c, o, cols - c);
         }
         if (li == 0) {
@@ -120,8 +121,10 @@ __device__ __forceinline__ void ln_rows(const OpsLnArgs &a, float *at) {
 // parameters' gradients summed in registers over the block's rows, then over
 // its row groups in LDS. With one vector a thread the next row's are loaded
 // before the present row's sums, whose barrier a large block's waves share;
-// two vectors leave no registers for that.
-template <typename T, int LPR, int NV, int BT, bool WHOLE>
+// two vectors leave no registers for that, nor, of 16-bit elements, for the
+// parameters' sums (PARAMS off: those are another launch's; with them 4096 rows
+// of 16384 bf16 spilled and took 422 us).
+template <typename T, int LPR, int NV, int BT, bool PARAMS, bool WHOLE>
 __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, float *sums) {
     constexpr int E = 16 / sizeof(T), RPB = BT / LPR;
     constexpr bool KEEP = NV == 1;  // the scale in registers; two vectors' would not leave room
@@ -141,18 +144,19 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, fl
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < E; ++e) ds[j][e] = db[j][e] = 0.0f;
-    Vec<T, E> vx[NV], vd[NV], va[NV];
+    u32x4 vx[NV], vd[NV], va[NV];
     float mean = 0.0f, rstd = 0.0f;
     auto fetch = [&](int64_t r0) {
         const int64_t r = min(r0 + grp, a.rows - 1);  // past the end: the last row again, not stored
         const T *x = static_cast<const T *>(a.x) + r * a.xrs, *dy = static_cast<const T *>(a.dy) + r * a.dyrs;
         const T *add = static_cast<const T *>(a.add) + r * a.ars;
+        const int64_t on = a.rows - 1 - r, end = cols - E;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * LPR + li) * E;
-            vx[j] = load_in<T, E, WHOLE>(x + c, x, cols - c);
-            vd[j] = load_in<T, E, WHOLE>(dy + c, dy, cols - c);
-            if (a.add) va[j] = load_in<T, E, WHOLE>(add + c, add, cols - c);
+            vx[j] = load_raw<T, E, WHOLE>(x + c, x, x + on * a.xrs + end, cols - c);
+            vd[j] = load_raw<T, E, WHOLE>(dy + c, dy, dy + on * a.dyrs + end, cols - c);
+            if (a.add) va[j] = load_raw<T, E, WHOLE>(add + c, add, add + on * a.ars + end, cols - c);
         }
         mean = a.mean[r];
         rstd = a.rstd[r];
@@ -164,7 +168,7 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, fl
     for (; r0 < a.rows; r0 += step) {
         const bool on = r0 + grp < a.rows;
         if (!KEEP) fetch(r0);
-        Vec<T, E> cx[NV], cd[NV], ca[NV];
+        u32x4 cx[NV], cd[NV], ca[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) cx[j] = vx[j], cd[j] = vd[j], ca[j] = va[j];
         const float m = mean, rs = rstd;
@@ -175,13 +179,12 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, fl
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const bool in = on && (j * LPR + li) * E + e < cols;
-                const float dy = in ? to_f<T>(cd[j].v[e]) : 0.0f;
-                const float xh = in ? (to_f<T>(cx[j].v[e]) - m) * rs : 0.0f;
+                const float dy = in ? elem<T>(cd[j], e) : 0.0f;
+                const float xh = in ? (elem<T>(cx[j], e) - m) * rs : 0.0f;
                 const float g = dy * scale(j, e);
                 s += g;
                 q += g * xh;
-                ds[j][e] += dy * xh;
-                db[j][e] += dy;
+                if (PARAMS) ds[j][e] += dy * xh, db[j][e] += dy;
             }
         if (!a.dx) continue;
         row_sum2<LPR, BT>(s, q, at, turn++);
@@ -189,7 +192,8 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, fl
         q /= n;
         if (!on) continue;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) reread(cx[j]), reread(cd[j]);
+        for (int j = 0; j < NV; ++j)
+            if (NV > 1) reread(cx[j]), reread(cd[j]);
         T *dx = static_cast<T *>(a.dx) + (r0 + grp) * a.dxrs;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -197,15 +201,15 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, fl
             Vec<T, E> o;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float xh = (to_f<T>(cx[j].v[e]) - m) * rs;
-                float v = rs * (to_f<T>(cd[j].v[e]) * scale(j, e) - s - xh * q);
-                if (a.add) v += to_f<T>(ca[j].v[e]);
+                const float xh = (elem<T>(cx[j], e) - m) * rs;
+                float v = rs * (elem<T>(cd[j], e) * scale(j, e) - s - xh * q);
+                if (a.add) v += elem<T>(ca[j], e);
                 o.v[e] = from_f<T>(v);
             }
             store_in<T, E, WHOLE>(dx + c, o, cols - c);
         }
     }
-    if (!a.part) return;
+    if (!PARAMS || !a.part) return;
     float *part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -235,135 +239,156 @@ __device__ __forceinline__ void ln_bwd_rows(const OpsLnBwdArgs &a, float *at, fl
     }
 }
 
-// Planar order: 64 positions a block (LP lanes of 16 bytes), S = BT / LP
-// threads down the channels, CH channels a thread, all in registers. Sums
-// over channels run over a thread's own, the wave's lanes and, through LDS,
-// the block's waves.
-template <typename T, int BT>
+// Planar order: LP lanes of 16 bytes along the positions, S = BT / LP threads
+// down the channels, CH channels a thread, all in registers. Sums over channels
+// run over a thread's own, the wave's lanes and, through LDS, the block's
+// waves. Many lanes along the positions leave little to add across threads:
+// 32 bf16 channels of 2^21 pixels took 151 us with 8 lanes.
+template <typename T, int BT, int LP>
 struct PlanarTile {
-    static constexpr int E = 16 / sizeof(T), LP = 64 / E, S = BT / LP, W = BT / 64;
-    // E sums a thread, one a position, over the block's channels
-    static __device__ __forceinline__ void sum(float *v, float *at) {
+    static constexpr int E = 16 / sizeof(T), S = BT / LP, W = BT / 64, POS = LP * E;
+    // N sums for each of a thread's E positions, over the block's channels;
+    // `at` holds N * W * POS floats
+    template <int N>
+    static __device__ __forceinline__ void sum(float (&v)[N][E], float *at) {
         const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int o = LP; o < 64; o <<= 1) v[e] += __shfl_xor(v[e], o);
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int o = LP; o < 64; o <<= 1) v[n][e] += __shfl_xor(v[n][e], o);
         __syncthreads();
         if (lane < LP)
 #pragma unroll
-            for (int e = 0; e < E; ++e) at[w * 64 + lane * E + e] = v[e];
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int e = 0; e < E; e += 4)
+                    *reinterpret_cast<f32x4 *>(at + (n * W + w) * POS + lane * E + e) =
+                        f32x4{v[n][e], v[n][e + 1], v[n][e + 2], v[n][e + 3]};
         __syncthreads();
         const int p = (lane % LP) * E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            float s = 0.0f;
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                f32x4 s = {0, 0, 0, 0};
 #pragma unroll 4
-            for (int i = 0; i < W; ++i) s += at[i * 64 + p + e];
-            v[e] = s;
-        }
+                for (int i = 0; i < W; ++i) s += *reinterpret_cast<const f32x4 *>(at + (n * W + i) * POS + p + e);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[n][e + k] = s[k];
+            }
     }
 };
 
+// (Addresses are the lane's own part plus the channel's, worked out in the
+// scalar unit for each tile, which here() sees to: kept over the tiles they
+// would take more registers than the data.)
 // LOOP: any number of channels, read again for each of the three passes.
 // WHOLE: the positions are whole vectors.
-template <typename T, int BT, int CH, bool LOOP, bool WHOLE>
+template <typename T, int BT, int LP, int CH, bool LOOP, bool WHOLE>
 __device__ __forceinline__ void ln_planar(const OpsLnArgs &a, float *at) {
-    typedef PlanarTile<T, BT> P;
-    constexpr int E = P::E, LP = P::LP, S = P::S;
+    typedef PlanarTile<T, BT, LP> P;
+    constexpr int E = P::E, S = P::S;
     const int pl = threadIdx.x % LP, sl = threadIdx.x / LP;
     const float n = (float)a.cols;
     const int rounds = LOOP ? (int)((a.cols + S * CH - 1) / (S * CH)) : 1;
     const T *x = static_cast<const T *>(a.x);
-    for (int64_t p0 = (int64_t)blockIdx.x * 64; p0 < a.rows; p0 += (int64_t)gridDim.x * 64) {
+    for (int64_t p0 = (int64_t)blockIdx.x * P::POS; p0 < a.rows; p0 += (int64_t)gridDim.x * P::POS) {
+        const int64_t sx = here(S * a.xcs), sy = here(S * a.ycs);
         const int64_t p = p0 + pl * E, have = a.rows - p;
-        Vec<T, E> v[CH];
+        u32x4 v[CH];
         auto fetch = [&](int round) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int64_t c = ((int64_t)round * CH + j) * S + sl;
-                v[j] = load_in<T, E, WHOLE>(x + c * a.xcs + p, x, c < a.cols ? have : 0);
+                v[j] = load_in<T, E, WHOLE>(x + (sl * a.xcs + p) + (round * CH + j) * sx, x, x + (a.cols - 1) * a.xcs + a.rows - E, c < a.cols ? have : 0);
             }
         };
-        float s[E], q[E];
+        float s[1][E], q[1][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] = q[e] = 0.0f;
+        for (int e = 0; e < E; ++e) s[0][e] = q[0][e] = 0.0f;
         for (int round = 0; round < rounds; ++round) {
             fetch(round);
 #pragma unroll
             for (int j = 0; j < CH; ++j)
 #pragma unroll
-                for (int e = 0; e < E; ++e) s[e] += to_f<T>(v[j].v[e]);
+                for (int e = 0; e < E; ++e) s[0][e] += elem<T>(v[j], e);
         }
         P::sum(s, at);
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] /= n;
+        for (int e = 0; e < E; ++e) s[0][e] /= n;
         for (int round = 0; round < rounds; ++round) {
             if (LOOP) fetch(round);
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
+                reread(v[j]);
                 const bool in = ((int64_t)round * CH + j) * S + sl < a.cols;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float d = to_f<T>(v[j].v[e]) - s[e];
-                    q[e] += in ? d * d : 0.0f;
+                    const float d = elem<T>(v[j], e) - s[0][e];
+                    q[0][e] += in ? d * d : 0.0f;
                 }
             }
         }
         P::sum(q, at);
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[e] = 1.0f / sqrtf(q[e] / n + a.eps);
+        for (int e = 0; e < E; ++e) q[0][e] = 1.0f / sqrtf(q[0][e] / n + a.eps);
         for (int round = 0; round < rounds; ++round) {
             if (LOOP) fetch(round);
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
+                reread(v[j]);
                 const int64_t c = ((int64_t)round * CH + j) * S + sl;
                 if (c >= a.cols) continue;
                 const float sc = param<T>(a.scale, c, a.param_f32), bi = a.bias ? param<T>(a.bias, c, a.param_f32) : 0.0f;
                 Vec<T, E> o;
 #pragma unroll
-                for (int e = 0; e < E; ++e) o.v[e] = from_f<T>((to_f<T>(v[j].v[e]) - s[e]) * q[e] * sc + bi);
-                store_in<T, E, WHOLE>(static_cast<T *>(a.y) + c * a.ycs + p, o, have);
+                for (int e = 0; e < E; ++e) o.v[e] = from_f<T>((elem<T>(v[j], e) - s[0][e]) * q[0][e] * sc + bi);
+                store_in<T, E, WHOLE>(static_cast<T *>(a.y) + (sl * a.ycs + p) + (round * CH + j) * sy, o, have);
             }
         }
         if (sl == 0) {
             Vec<float, E> m, r;
 #pragma unroll
-            for (int e = 0; e < E; ++e) m.v[e] = s[e], r.v[e] = q[e];
+            for (int e = 0; e < E; ++e) m.v[e] = s[0][e], r.v[e] = q[0][e];
             if (a.mean) store_upto<float, E>(a.mean + p, m, have);
             if (a.rstd) store_upto<float, E>(a.rstd + p, r, have);
         }
     }
 }
 
-template <typename T, int BT, int CH, bool LOOP, bool WHOLE>
+template <typename T, int BT, int LP, int CH, bool LOOP, bool WHOLE>
 __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a, float *at) {
-    typedef PlanarTile<T, BT> P;
-    constexpr int E = P::E, LP = P::LP, S = P::S;
+    typedef PlanarTile<T, BT, LP> P;
+    constexpr int E = P::E, S = P::S;
     const int pl = threadIdx.x % LP, sl = threadIdx.x / LP;
     const float n = (float)a.cols;
     const int rounds = LOOP ? (int)((a.cols + S * CH - 1) / (S * CH)) : 1;
     const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy), *add = static_cast<const T *>(a.add);
+    const T *xl = x + (a.cols - 1) * a.xcs + a.rows - E, *dyl = dy + (a.cols - 1) * a.dycs + a.rows - E;
+    const T *addl = add + (a.cols - 1) * a.acs + a.rows - E;
     float ds[CH], db[CH];
 #pragma unroll
     for (int j = 0; j < CH; ++j) ds[j] = db[j] = 0.0f;
-    for (int64_t p0 = (int64_t)blockIdx.x * 64; p0 < a.rows; p0 += (int64_t)gridDim.x * 64) {
+    for (int64_t p0 = (int64_t)blockIdx.x * P::POS; p0 < a.rows; p0 += (int64_t)gridDim.x * P::POS) {
+        const int64_t sx = here(S * a.xcs), sdy = here(S * a.dycs), sa = here(S * a.acs), sdx = here(S * a.dxcs);
         const int64_t p = p0 + pl * E, have = a.rows - p;
-        Vec<T, E> vx[CH], vd[CH];
+        u32x4 vx[CH], vd[CH];
         auto fetch = [&](int round) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int64_t c = ((int64_t)round * CH + j) * S + sl, left = c < a.cols ? have : 0;
-                vx[j] = load_in<T, E, WHOLE>(x + c * a.xcs + p, x, left);
-                vd[j] = load_in<T, E, WHOLE>(dy + c * a.dycs + p, dy, left);
+                vx[j] = load_in<T, E, WHOLE>(x + (sl * a.xcs + p) + (round * CH + j) * sx, x, xl, left);
+                vd[j] = load_in<T, E, WHOLE>(dy + (sl * a.dycs + p) + (round * CH + j) * sdy, dy, dyl, left);
             }
         };
         fetch(0);
         // past the last position rstd is 0, so what lies there adds nothing
         const Vec<float, E> m = load_upto<float, E>(a.mean + p, have), r = load_upto<float, E>(a.rstd + p, have);
-        float s[E], q[E];
+        float sum[2][E];  // of g and of g xh
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] = q[e] = 0.0f;
+        for (int e = 0; e < E; ++e) sum[0][e] = sum[1][e] = 0.0f;
         for (int round = 0; round < rounds; ++round) {
             if (round) fetch(round);
 #pragma unroll
@@ -373,19 +398,20 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a, float *at) 
                 const float sc = in ? param<T>(a.scale, c, a.param_f32) : 0.0f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float d = to_f<T>(vd[j].v[e]);
-                    const float xh = in ? (to_f<T>(vx[j].v[e]) - m.v[e]) * r.v[e] : 0.0f;
-                    s[e] += d * sc;
-                    q[e] += d * sc * xh;
+                    const float d = elem<T>(vd[j], e);
+                    const float xh = in ? (elem<T>(vx[j], e) - m.v[e]) * r.v[e] : 0.0f;
+                    sum[0][e] += d * sc;
+                    sum[1][e] += d * sc * xh;
                     if (!LOOP) ds[j] += d * xh, db[j] += d;
                 }
+                // one channel's elements as fp32 at a time
+                if (CH >= 8) __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (!a.dx) continue;
-        P::sum(s, at);
-        P::sum(q, at);
+        P::sum(sum, at);
 #pragma unroll
-        for (int e = 0; e < E; ++e) s[e] /= n, q[e] /= n;
+        for (int e = 0; e < E; ++e) sum[0][e] /= n, sum[1][e] /= n;
 #pragma unroll
         for (int j = 0; j < CH; ++j) reread(vx[j]), reread(vd[j]);
         for (int round = 0; round < rounds; ++round) {
@@ -395,16 +421,17 @@ __device__ __forceinline__ void ln_bwd_planar(const OpsLnBwdArgs &a, float *at) 
                 const int64_t c = ((int64_t)round * CH + j) * S + sl;
                 if (c >= a.cols) continue;
                 const float sc = param<T>(a.scale, c, a.param_f32);
-                Vec<T, E> o, va;
-                if (a.add) va = load_in<T, E, WHOLE>(add + c * a.acs + p, add, have);
+                Vec<T, E> o;
+                u32x4 va;
+                if (a.add) va = load_in<T, E, WHOLE>(add + (sl * a.acs + p) + (round * CH + j) * sa, add, addl, have);
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const float xh = (to_f<T>(vx[j].v[e]) - m.v[e]) * r.v[e];
-                    float v = r.v[e] * (to_f<T>(vd[j].v[e]) * sc - s[e] - xh * q[e]);
-                    if (a.add) v += to_f<T>(va.v[e]);
+                    const float xh = (elem<T>(vx[j], e) - m.v[e]) * r.v[e];
+                    float v = r.v[e] * (elem<T>(vd[j], e) * sc - sum[0][e] - xh * sum[1][e]);
+                    if (a.add) v += elem<T>(va, e);
                     o.v[e] = from_f<T>(v);
                 }
-                store_in<T, E, WHOLE>(static_cast<T *>(a.dx) + c * a.dxcs + p, o, have);
+                store_in<T, E, WHOLE>(static_cast<T *>(a.dx) + (sl * a.dxcs + p) + (round * CH + j) * sdx, o, have);
             }
         }
     }
@@ -436,23 +463,40 @@ __device__ __forceinline__ float block_sum(float v, float *at) {
 // over it, the later two from the caches.
 template <typename T>
 __device__ __forceinline__ void ln_long(const OpsLnArgs &a) {
+    constexpr int E = 16 / sizeof(T);
     __shared__ float at[16];
+    const float n = (float)a.cols;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + r * a.xrs;
+        const T *xl = x + (a.rows - 1 - r) * a.xrs + a.cols - E;
         T *y = static_cast<T *>(a.y) + r * a.yrs;
         float s = 0.0f;
-        for (int64_t c = threadIdx.x; c < a.cols; c += 1024) s += to_f<T>(x[c]);
-        const float mean = block_sum(s, at) / (float)a.cols;
-        s = 0.0f;
-        for (int64_t c = threadIdx.x; c < a.cols; c += 1024) {
-            const float d = to_f<T>(x[c]) - mean;
-            s += d * d;
+        for (int64_t c = threadIdx.x * E; c < a.cols; c += 1024 * E) {
+            const u32x4 v = load_in<T, E, false>(x + c, x, xl, a.cols - c);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s += elem<T>(v, e);
         }
-        const float rstd = 1.0f / sqrtf(block_sum(s, at) / (float)a.cols + a.eps);
-        for (int64_t c = threadIdx.x; c < a.cols; c += 1024) {
-            const float d = (to_f<T>(x[c]) - mean) * rstd;
-            const float b = a.bias ? param<T>(a.bias, c, a.param_f32) : 0.0f;
-            y[c] = from_f<T>(d * param<T>(a.scale, c, a.param_f32) + b);
+        const float mean = block_sum(s, at) / n;
+        s = 0.0f;
+        for (int64_t c = threadIdx.x * E; c < a.cols; c += 1024 * E) {
+            const u32x4 v = load_in<T, E, false>(x + c, x, xl, a.cols - c);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = elem<T>(v, e) - mean;
+                s += c + e < a.cols ? d * d : 0.0f;
+            }
+        }
+        const float rstd = 1.0f / sqrtf(block_sum(s, at) / n + a.eps);
+        for (int64_t c = threadIdx.x * E; c < a.cols; c += 1024 * E) {
+            const u32x4 v = load_in<T, E, false>(x + c, x, xl, a.cols - c);
+            Vec<T, E> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (c + e >= a.cols) continue;
+                const float b = a.bias ? param<T>(a.bias, c + e, a.param_f32) : 0.0f;
+                o.v[e] = from_f<T>((elem<T>(v, e) - mean) * rstd * param<T>(a.scale, c + e, a.param_f32) + b);
+            }
+            store_upto<T, E>(y + c, o, a.cols - c);
         }
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[r] = mean;
@@ -463,27 +507,45 @@ __device__ __forceinline__ void ln_long(const OpsLnArgs &a) {
 
 template <typename T>
 __device__ __forceinline__ void ln_bwd_long(const OpsLnBwdArgs &a) {
+    constexpr int E = 16 / sizeof(T);
     __shared__ float at[16];
+    const float n = (float)a.cols;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T *x = static_cast<const T *>(a.x) + r * a.xrs;
         const T *dy = static_cast<const T *>(a.dy) + r * a.dyrs;
         const T *add = a.add ? static_cast<const T *>(a.add) + r * a.ars : nullptr;
         T *dx = static_cast<T *>(a.dx) + r * a.dxrs;
+        const int64_t rest = a.rows - 1 - r, end = a.cols - E;
         const float mean = a.mean[r], rstd = a.rstd[r];
         float s = 0.0f, q = 0.0f;
-        for (int64_t c = threadIdx.x; c < a.cols; c += 1024) {
-            const float gr = to_f<T>(dy[c]) * param<T>(a.scale, c, a.param_f32);
-            s += gr;
-            q += gr * ((to_f<T>(x[c]) - mean) * rstd);
+        for (int64_t c = threadIdx.x * E; c < a.cols; c += 1024 * E) {
+            const u32x4 vx = load_in<T, E, false>(x + c, x, x + rest * a.xrs + end, a.cols - c);
+            const u32x4 vd = load_in<T, E, false>(dy + c, dy, dy + rest * a.dyrs + end, a.cols - c);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (c + e >= a.cols) continue;
+                const float gr = elem<T>(vd, e) * param<T>(a.scale, c + e, a.param_f32);
+                s += gr;
+                q += gr * ((elem<T>(vx, e) - mean) * rstd);
+            }
         }
-        s = block_sum(s, at) / (float)a.cols;
-        q = block_sum(q, at) / (float)a.cols;
-        for (int64_t c = threadIdx.x; c < a.cols; c += 1024) {
-            const float gr = to_f<T>(dy[c]) * param<T>(a.scale, c, a.param_f32);
-            const float xh = (to_f<T>(x[c]) - mean) * rstd;
-            float v = rstd * (gr - s - xh * q);
-            if (add) v += to_f<T>(add[c]);
-            dx[c] = from_f<T>(v);
+        s = block_sum(s, at) / n;
+        q = block_sum(q, at) / n;
+        for (int64_t c = threadIdx.x * E; c < a.cols; c += 1024 * E) {
+            const u32x4 vx = load_in<T, E, false>(x + c, x, x + rest * a.xrs + end, a.cols - c);
+            const u32x4 vd = load_in<T, E, false>(dy + c, dy, dy + rest * a.dyrs + end, a.cols - c);
+            u32x4 va;
+            Vec<T, E> o;
+            if (add) va = load_in<T, E, false>(add + c, add, add + rest * a.ars + end, a.cols - c);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (c + e >= a.cols) continue;
+                const float gr = elem<T>(vd, e) * param<T>(a.scale, c + e, a.param_f32);
+                float v = rstd * (gr - s - (elem<T>(vx, e) - mean) * rstd * q);
+                if (add) v += elem<T>(va, e);
+                o.v[e] = from_f<T>(v);
+            }
+            store_upto<T, E>(dx + c, o, a.cols - c);
         }
     }
 }
@@ -503,14 +565,16 @@ __device__ __forceinline__ void ln_param_rows(const OpsLnBwdArgs &a) {
     for (int e = 0; e < E; ++e) s[e] = b[e] = 0.0f;
     if (have > 0)
         for (int64_t r = p * chunk + w; r < end; r += 4) {
-            const Vec<T, E> vd = load_upto<T, E>(static_cast<const T *>(a.dy) + r * a.dyrs + c, have);
-            const Vec<T, E> vx = load_upto<T, E>(static_cast<const T *>(a.x) + r * a.xrs + c, have);
+            const T *dy = static_cast<const T *>(a.dy) + r * a.dyrs + c, *x = static_cast<const T *>(a.x) + r * a.xrs + c;
+            const int64_t rest = a.rows - 1 - r, end = a.cols - E - c;
+            const u32x4 vd = load_in<T, E, false>(dy, dy, dy + rest * a.dyrs + end, have);
+            const u32x4 vx = load_in<T, E, false>(x, x, x + rest * a.xrs + end, have);
             const float m = a.mean[r], rs = a.rstd[r];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float dy = to_f<T>(vd.v[e]);
-                s[e] += dy * ((to_f<T>(vx.v[e]) - m) * rs);
-                b[e] += dy;
+                const float d = elem<T>(vd, e);
+                s[e] += e < have ? d * ((elem<T>(vx, e) - m) * rs) : 0.0f;
+                b[e] += d;
             }
         }
 #pragma unroll
@@ -559,19 +623,23 @@ __device__ __forceinline__ void dz_rows(const OpsDzArgs &a, float (*sh)[64 * 16 
     if (have > 0)
         for (int64_t r = p * chunk + w; r < end; r += 4) {
             const T *dy = static_cast<const T *>(a.dy) + r * a.dyrs + c, *z = static_cast<const T *>(a.z) + r * a.zrs + c;
-            Vec<T, E> vd = load_in<T, E, WHOLE>(dy, dy, have), vz;
-            if (a.z) vz = load_in<T, E, WHOLE>(z, z, have);
+            // a lane without columns has left already
+            const int64_t rest = a.rows - 1 - r, end = a.cols - E - c;
+            const u32x4 vd = load_in<T, E, WHOLE>(dy, dy, dy + rest * a.dyrs + end, have);
+            u32x4 vz;
+            if (a.z) vz = load_in<T, E, WHOLE>(z, z, z + rest * a.zrs + end, have);
             float v[E];
+            Vec<T, E> o;
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = to_f<T>(vd.v[e]);
-            if (a.z) act_bwd_n<E>(a.act, a.slope, v, [&](int e) { return to_f<T>(vz.v[e]); });
+            for (int e = 0; e < E; ++e) v[e] = elem<T>(vd, e);
+            if (a.z) act_bwd_n<E>(a.act, a.slope, v, [&](int e) { return elem<T>(vz, e); });
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 s[e] += v[e];
-                vd.v[e] = from_f<T>(v[e]);
+                o.v[e] = from_f<T>(v[e]);
             }
             // lines of dz are whole vectors, their ends zeros
-            if (a.dz) store_n<T, E>(static_cast<T *>(a.dz) + r * a.drs + c, vd);
+            if (a.dz) store_n<T, E>(static_cast<T *>(a.dz) + r * a.drs + c, o);
         }
     if (!a.part) return;
 #pragma unroll
@@ -655,21 +723,24 @@ extern "C" __global__ __launch_bounds__(1024) void mxo_join_parts(OpsJoinArgs a)
     extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_rows_##name##_##LPR##x##NV(OpsLnBwdArgs a) {          \
         __shared__ float at[4 * (BT / 64)];                                                                           \
         __shared__ float sums[BT > LPR ? BT * NV * 16 / sizeof(T) : 1];                                               \
-        OPS_BOTH(a.cols, 16 / sizeof(T), (ln_bwd_rows<T, LPR, NV, BT, true>(a, at, sums)),                            \
-                 (ln_bwd_rows<T, LPR, NV, BT, false>(a, at, sums)))                                                   \
+        constexpr bool P = NV == 1 || sizeof(T) == 4;                                                                 \
+        OPS_BOTH(a.cols, 16 / sizeof(T), (ln_bwd_rows<T, LPR, NV, BT, P, true>(a, at, sums)),                         \
+                 (ln_bwd_rows<T, LPR, NV, BT, P, false>(a, at, sums)))                                                \
     }
-#define OPS_LN_PLANAR1(name, T, tag, BT, CH, LOOP)                                                                    \
+#define OPS_LN_FWD_PLANAR1(name, T, tag, BT, LP, CH, LOOP)                                                            \
     extern "C" __global__ __launch_bounds__(BT) void mxo_ln_planar_##name##_##tag(OpsLnArgs a) {                      \
-        __shared__ float at[BT];                                                                                      \
-        OPS_BOTH(a.rows, 16 / sizeof(T), (ln_planar<T, BT, CH, LOOP, true>(a, at)),                                   \
-                 (ln_planar<T, BT, CH, LOOP, false>(a, at)))                                                          \
-    }                                                                                                                 \
-    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_planar_##name##_##tag(OpsLnBwdArgs a) {               \
-        __shared__ float at[BT];                                                                                      \
-        OPS_BOTH(a.rows, 16 / sizeof(T), (ln_bwd_planar<T, BT, CH, LOOP, true>(a, at)),                               \
-                 (ln_bwd_planar<T, BT, CH, LOOP, false>(a, at)))                                                      \
+        __shared__ __align__(16) float at[BT / 64 * LP * 16 / sizeof(T)];                                             \
+        OPS_BOTH(a.rows, 16 / sizeof(T), (ln_planar<T, BT, LP, CH, LOOP, true>(a, at)),                               \
+                 (ln_planar<T, BT, LP, CH, LOOP, false>(a, at)))                                                      \
     }
-#define OPS_LN_PLANAR(name, T, BT, CH) OPS_LN_PLANAR1(name, T, BT##x##CH, BT, CH, false)
+#define OPS_LN_BWD_PLANAR1(name, T, tag, BT, LP, CH, LOOP)                                                            \
+    extern "C" __global__ __launch_bounds__(BT) void mxo_ln_bwd_planar_##name##_##tag(OpsLnBwdArgs a) {               \
+        __shared__ __align__(16) float at[2 * BT / 64 * LP * 16 / sizeof(T)];                                         \
+        OPS_BOTH(a.rows, 16 / sizeof(T), (ln_bwd_planar<T, BT, LP, CH, LOOP, true>(a, at)),                           \
+                 (ln_bwd_planar<T, BT, LP, CH, LOOP, false>(a, at)))                                                  \
+    }
+#define OPS_LN_FWD_PLANAR(name, T, BT, LP, CH) OPS_LN_FWD_PLANAR1(name, T, BT##x##LP##x##CH, BT, LP, CH, false)
+#define OPS_LN_BWD_PLANAR(name, T, BT, LP, CH) OPS_LN_BWD_PLANAR1(name, T, BT##x##LP##x##CH, BT, LP, CH, false)
 #define OPS_LN_BOTH(name, T, LPR, NV, BT) \
     OPS_LN_ROWS(name, T, LPR, NV, BT)     \
     OPS_LN_BWD_ROWS(name, T, LPR, NV, BT)
@@ -686,12 +757,22 @@ extern "C" __global__ __launch_bounds__(1024) void mxo_join_parts(OpsJoinArgs a)
     OPS_LN_BWD_ROWS(name, T, 512, 1, 1024)                                                                            \
     OPS_LN_BOTH(name, T, 1024, 1, 1024)                                                                               \
     OPS_LN_BOTH(name, T, 1024, 2, 1024)                                                                               \
-    OPS_LN_PLANAR(name, T, 256, 1)                                                                                    \
-    OPS_LN_PLANAR(name, T, 256, 2)                                                                                    \
-    OPS_LN_PLANAR(name, T, 256, 4)                                                                                    \
-    OPS_LN_PLANAR(name, T, 512, 4)                                                                                    \
-    OPS_LN_PLANAR(name, T, 512, 8)                                                                                    \
-    OPS_LN_PLANAR1(name, T, loop, 512, 4, true)                                                                      \
+    OPS_LN_FWD_PLANAR(name, T, 256, 64, 4)                                                                            \
+    OPS_LN_FWD_PLANAR(name, T, 256, 64, 8)                                                                            \
+    OPS_LN_FWD_PLANAR(name, T, 512, 64, 16)                                                                           \
+    OPS_LN_FWD_PLANAR(name, T, 512, 32, 16)                                                                           \
+    OPS_LN_FWD_PLANAR(name, T, 512, 16, 2)                                                                            \
+    OPS_LN_FWD_PLANAR(name, T, 512, 16, 4)                                                                            \
+    OPS_LN_FWD_PLANAR(name, T, 512, 16, 8)                                                                            \
+    OPS_LN_FWD_PLANAR(name, T, 512, 16, 16)                                                                           \
+    OPS_LN_FWD_PLANAR(name, T, 512, 8, 16)                                                                            \
+    OPS_LN_BWD_PLANAR(name, T, 256, 64, 4)                                                                            \
+    OPS_LN_BWD_PLANAR(name, T, 512, 64, 4)                                                                            \
+    OPS_LN_BWD_PLANAR(name, T, 512, 16, 1)                                                                            \
+    OPS_LN_BWD_PLANAR(name, T, 512, 16, 2)                                                                            \
+    OPS_LN_BWD_PLANAR(name, T, 512, 16, 4)                                                                            \
+    OPS_LN_FWD_PLANAR1(name, T, loop, 512, 16, 4, true)                                                               \
+    OPS_LN_BWD_PLANAR1(name, T, loop, 512, 16, 4, true)                                                               \
     extern "C" __global__ __launch_bounds__(1024) void mxo_ln_rows_##name##_long(OpsLnArgs a) { ln_long<T>(a); }      \
     extern "C" __global__ __launch_bounds__(1024) void mxo_ln_bwd_rows_##name##_long(OpsLnBwdArgs a) {                \
         ln_bwd_long<T>(a);                                                                                            \
@@ -709,3 +790,15 @@ extern "C" __global__ __launch_bounds__(1024) void mxo_join_parts(OpsJoinArgs a)
 OPS_ROWS_TYPE(bf16, bf16)
 OPS_ROWS_TYPE(f16, f16)
 OPS_ROWS_TYPE(f32, float)
+OPS_LN_BWD_PLANAR(f32, float, 512, 64, 8)
+OPS_LN_BWD_PLANAR(f32, float, 512, 32, 8)
+OPS_LN_BWD_PLANAR(f32, float, 512, 16, 8)
+OPS_LN_BWD_PLANAR(f32, float, 512, 8, 8)
+OPS_LN_FWD_PLANAR(bf16, bf16, 512, 64, 8)
+OPS_LN_FWD_PLANAR(f16, f16, 512, 64, 8)
+OPS_LN_FWD_PLANAR(bf16, bf16, 512, 16, 1)
+OPS_LN_FWD_PLANAR(f16, f16, 512, 16, 1)
+OPS_LN_BWD_PLANAR(bf16, bf16, 512, 32, 4)
+OPS_LN_BWD_PLANAR(f16, f16, 512, 32, 4)
+OPS_LN_BWD_PLANAR(bf16, bf16, 512, 8, 4)
+OPS_LN_BWD_PLANAR(f16, f16, 512, 8, 4)
