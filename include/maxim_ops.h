@@ -17,7 +17,11 @@
  * and an output must not overlap any other operand, but where a call says so.
  *
  * Sums, means and variances are fp32; a result is rounded once, to nearest
- * even, when it is stored. No atomics: the same call gives the same bits.
+ * even, when it is stored. fp32 products are formed on the bf16 matrix cores
+ * from three bf16 parts of each operand (every bit of a float, whatever its
+ * size; a product is off by 1.1e-7 of itself at most), and sums that are not
+ * finite again in fp32, so infinities and NaN are fp32's. No atomics: the same
+ * call gives the same bits.
  *
  * Every call is asynchronous, in stream order on `stream` (a hipStream_t of
  * `device`; NULL: the device's default stream). It allocates nothing and
@@ -27,7 +31,8 @@
  *
  * Where a call needs scratch, `workspace` is device memory of at least the
  * bytes that its _workspace function gives for the same operands, 16-byte
- * aligned; the call owns it until the stream has passed. Two calls may share
+ * aligned and apart from all of them; the call owns it until the stream has
+ * passed. Two calls may share
  * it in stream order; calls (or captured graphs) that can overlap need one
  * each.
  *

@@ -153,82 +153,83 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
                     if (i == h) mend(acc[i], again[0]);
             }
     } else {
-    // A tile is four phases, two halves of k by two halves of the wave's rows,
-    // each multiplying fragments that the phase before it read from LDS.
-    constexpr int HM = FM / 2;
-    typedef typename Mma<T>::Frag Frag;
-    Frag fa[2][HM], fb[2][FN];
-    // In the largest tiles a fragment's address (its own register where the
-    // operand is not contiguous along k) is worked out when it is read: held
-    // through the loop they do not fit beside the sums.
-    auto here = [&](int part) {
-        if (FM * FN >= 32 && (!AK || !BK_)) asm volatile("" : "+v"(part));
-        return part;
-    };
-    auto take_a = [&](const LdsChar *at, int kk, int h) {
-        const int part = here(pa);
+        // A tile is four phases, two halves of k by two halves of the wave's rows,
+        // each multiplying fragments that the phase before it read from LDS.
+        constexpr int HM = FM / 2;
+        typedef typename Mma<T>::Frag Frag;
+        Frag fa[2][HM], fb[2][FN];
+        // In the largest tiles a fragment's address (its own register where the
+        // operand is not contiguous along k) is worked out when it is read: held
+        // through the loop they do not fit beside the sums.
+        auto here = [&](int part) {
+            if (FM * FN >= 32 && (!AK || !BK_)) asm volatile("" : "+v"(part));
+            return part;
+        };
+        auto take_a = [&](const LdsChar *at, int kk, int h) {
+            const int part = here(pa);
 #pragma unroll
-        for (int i = 0; i < HM; ++i) fa[h][i] = TA::frag(at, wm + (h * HM + i) * 16, kk, part);
-    };
-    auto take_b = [&](const LdsChar *bt, int kk) {
-        const int part = here(pb);
+            for (int i = 0; i < HM; ++i) fa[h][i] = TA::frag(at, wm + (h * HM + i) * 16, kk, part);
+        };
+        auto take_b = [&](const LdsChar *bt, int kk) {
+            const int part = here(pb);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[kk][j] = TB::frag(bt, wn + j * 16, kk, part);
-    };
-    auto multiply = [&](int kk, int h) {
+            for (int j = 0; j < FN; ++j) fb[kk][j] = TB::frag(bt, wn + j * 16, kk, part);
+        };
+        auto multiply = [&](int kk, int h) {
 #pragma unroll
-        for (int i = 0; i < HM; ++i)
+            for (int i = 0; i < HM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[h * HM + i][j] = Mma<T>::go(fb[kk][j], fa[h][i], acc[h * HM + i][j]);
-    };
-    // The last phase's fragments are in registers when it begins: then, with
-    // the next tile landed, the tile ST on is sent for into this one's place,
-    // ST - 1 tiles' time ahead of its use. Past the last tile the loads bring
-    // zeros without touching memory.
-    auto tile = [&](const Stage &c, const Stage &n) {
-        constexpr int RA = HM * (AK ? 1 : 2), RB = FN * (BK_ ? 1 : 2), MP = HM * FN;
-        take_a((LdsChar *)c.a, 0, 1);
-        multiply(0, 0);
-        spread<RA, MP>();
-        take_b((LdsChar *)c.b, 1);
-        take_a((LdsChar *)c.a, 1, 0);
-        multiply(0, 1);
-        spread<RA + RB, MP>();
-        take_a((LdsChar *)c.a, 1, 1);
-        multiply(1, 0);
-        spread<RA, MP>();
-        tiles_landed<AHEAD>();
-        stage(c.a, c.b);
-        __builtin_amdgcn_sched_barrier(0);  // sent for here, not where the scheduler finds room
-        take_b((LdsChar *)n.b, 0);
-        take_a((LdsChar *)n.a, 0, 0);
-        multiply(1, 1);
-        spread<RA + RB, MP>();
-    };
+                for (int j = 0; j < FN; ++j) acc[h * HM + i][j] = Mma<T>::go(fb[kk][j], fa[h][i], acc[h * HM + i][j]);
+        };
+        // The last phase's fragments are in registers when it begins: then, with
+        // the next tile landed, the tile ST on is sent for into this one's place,
+        // ST - 1 tiles' time ahead of its use. Past the last tile the loads bring
+        // zeros without touching memory.
+        auto tile = [&](const Stage &c, const Stage &n) {
+            constexpr int RA = HM * (AK ? 1 : 2), RB = FN * (BK_ ? 1 : 2), MP = HM * FN;
+            take_a((LdsChar *)c.a, 0, 1);
+            multiply(0, 0);
+            spread<RA, MP>();
+            take_b((LdsChar *)c.b, 1);
+            take_a((LdsChar *)c.a, 1, 0);
+            multiply(0, 1);
+            spread<RA + RB, MP>();
+            take_a((LdsChar *)c.a, 1, 1);
+            multiply(1, 0);
+            spread<RA, MP>();
+            tiles_landed<AHEAD>();
+            stage(c.a, c.b);
+            __builtin_amdgcn_sched_barrier(0);  // sent for here, not where the scheduler finds room
+            take_b((LdsChar *)n.b, 0);
+            take_a((LdsChar *)n.a, 0, 0);
+            multiply(1, 1);
+            spread<RA + RB, MP>();
+        };
 #pragma unroll
-    for (int i = 0; i < ST; ++i) stage(st[i].a, st[i].b);
-    tiles_landed<AHEAD + LOADS>();
-    take_b((LdsChar *)st[0].b, 0);
-    take_a((LdsChar *)st[0].a, 0, 0);
-    // ST tiles a round and the rest one by one. (In the largest tiles, whose
-    // fragments leave no registers for a second exit, the last round is filled
-    // with a tile of zeros instead.)
-    constexpr bool FILL = FM * FN >= 32;
-    int kt = 0;
-    for (; FILL ? kt < nk : kt + ST <= nk; kt += ST) {
+        for (int i = 0; i < ST; ++i) stage(st[i].a, st[i].b);
+        tiles_landed<AHEAD + LOADS>();
+        take_b((LdsChar *)st[0].b, 0);
+        take_a((LdsChar *)st[0].a, 0, 0);
+        // ST tiles a round and the rest one by one. (In the largest tiles, whose
+        // fragments leave no registers for a second exit, the last round is filled
+        // with a tile of zeros instead.)
+        constexpr bool FILL = FM * FN >= 32;
+        int kt = 0;
+        for (; FILL ? kt < nk : kt + ST <= nk; kt += ST) {
 #pragma unroll
-        for (int i = 0; i < ST; ++i) tile(st[i], st[(i + 1) % ST]);
-    }
-    if constexpr (!FILL) {
+            for (int i = 0; i < ST; ++i) tile(st[i], st[(i + 1) % ST]);
+        }
+        if constexpr (!FILL) {
 #pragma unroll
-        for (int i = 0; i < ST - 1; ++i) {
-            if (kt + i >= nk) break;
-            tile(st[i], st[i + 1]);
+            for (int i = 0; i < ST - 1; ++i) {
+                if (kt + i >= nk) break;
+                tile(st[i], st[i + 1]);
+            }
         }
     }
-    }
     tiles_landed<0>();  // the last loads too, zeros: the tiles' LDS is free
-    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN>(), acc);
+    char *own = (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN>();
+    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, own, acc);
 }
 
 #define OPS_STAGE(i, BM, BN)                              \

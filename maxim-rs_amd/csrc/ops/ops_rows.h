@@ -293,7 +293,7 @@ __device__ __forceinline__ void ln_planar(const OpsLnArgs &a, float *at) {
     const int pl = threadIdx.x % LP, sl = threadIdx.x / LP;
     const float n = (float)a.cols;
     const int rounds = LOOP ? (int)((a.cols + S * CH - 1) / (S * CH)) : 1;
-    const T *x = static_cast<const T *>(a.x);
+    const T *x = static_cast<const T *>(a.x), *xl = x + (a.cols - 1) * a.xcs + a.rows - E;
     for (int64_t p0 = (int64_t)blockIdx.x * P::POS; p0 < a.rows; p0 += (int64_t)gridDim.x * P::POS) {
         const int64_t sx = here(S * a.xcs), sy = here(S * a.ycs);
         const int64_t p = p0 + pl * E, have = a.rows - p;
@@ -302,7 +302,7 @@ __device__ __forceinline__ void ln_planar(const OpsLnArgs &a, float *at) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int64_t c = ((int64_t)round * CH + j) * S + sl;
-                v[j] = load_in<T, E, WHOLE>(x + (sl * a.xcs + p) + (round * CH + j) * sx, x, x + (a.cols - 1) * a.xcs + a.rows - E, c < a.cols ? have : 0);
+                v[j] = load_in<T, E, WHOLE>(x + (sl * a.xcs + p) + (round * CH + j) * sx, x, xl, c < a.cols ? have : 0);
             }
         };
         float s[1][E], q[1][E];

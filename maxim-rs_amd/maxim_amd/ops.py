@@ -4,7 +4,9 @@ LayerNorm and Dense, forward and backward, in fp32, fp16 or bf16.
 Tensors are torch's, on the card; results and workspaces come from torch's
 allocator and the kernels go to torch's current stream of that device, so the
 calls mix with torch's own work and can be captured into its graphs (after
-`ready()`, which loads the kernels). There is no CPU fallback.
+`ready()`, which loads the kernels). There is no CPU fallback. torch has to be
+imported before the process first uses the executor, so that both share one
+HIP runtime; otherwise the calls are refused.
 
 Features are a tensor's last dimension, positions all the others (token
 order, the default), or, with planar=True, features the first dimension and
@@ -41,6 +43,12 @@ _raw_stream = None
 _types = {}
 
 
+def _runtimes():
+    """The HIP runtimes mapped into this process."""
+    with open("/proc/self/maps") as f:
+        return sorted({line.split()[-1] for line in f if "libamdhip64" in line})
+
+
 def _lib():
     """The library with the operators' entry points declared."""
     global _L, _torch, _raw_stream
@@ -49,6 +57,10 @@ def _lib():
             import torch  # before the library looks for a HIP runtime: torch's is the one to share
         except ImportError as e:
             raise P.MaximError("maxim_amd.ops works on torch tensors: %s" % e)
+        if len(_runtimes()) > 1:
+            # the executor has brought its own up; torch's tensors and streams are unknown to it
+            raise P.MaximError("two HIP runtimes in the process (%s): import torch before the executor's first use"
+                               % ", ".join(_runtimes()))
         L = _hip_lib()
         V, I, F, U = C.c_void_p, C.c_int, C.c_float, C.c_uint64
         M, N, B = C.POINTER(Mat), C.POINTER(Vec), C.POINTER(C.c_uint64)

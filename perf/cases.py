@@ -17,7 +17,7 @@ Kinds of case:
           convolutions, channel attention, residual) at `c` channels
   conv    one convolution: 3x3, 4x4 stride 2 or transposed 2x2 stride 2, of
           any height and width
-All data is fp32, the only type the framework has. There is no backward.
+All data is fp32, the only type the executor has.
 """
 
 import math

@@ -155,6 +155,26 @@ def test_python_refusals():
             call()
 
 
+def test_a_second_hip_runtime_is_refused():
+    """A runtime that the executor loaded before torch brought its own."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ("import ctypes, sys\n"
+            "sys.path.insert(0, %r)\n"
+            "try:\n    ctypes.CDLL('/opt/rocm/lib/libamdhip64.so')\n"
+            "except OSError:\n    sys.exit(7)\n"
+            "from maxim_amd import ops, plan\n"
+            "try:\n    ops._lib()\n"
+            "except plan.MaximError as e:\n    sys.exit(0 if 'two HIP runtimes' in str(e) else 1)\n"
+            "sys.exit(0 if len(ops._runtimes()) == 1 else 2)\n" % os.path.join(root, "maxim-rs_amd"))
+    rc = subprocess.run([sys.executable, "-c", code]).returncode
+    if rc == 7:
+        pytest.skip("no HIP runtime outside torch")
+    assert rc == 0
+
+
 def test_every_declared_operator_is_exported():
     import os
     import re
