@@ -248,17 +248,22 @@ LnPlan ln_plan(int dtype, int64_t rows, int64_t cols, bool by_cols, bool backwar
         if (p.form.empty()) p.form = "long", p.block = 1024, p.grid = std::min<int64_t>(rows, 65536), p.whole = false;
     } else {
         // threads, lanes of 16 bytes along the positions, channels a thread:
-        // the most lanes that still leave two tiles a CU, else 16 or 8. The
-        // backward pass holds two matrices and the parameters' sums: at most
-        // eight channels of fp32, four of 16 bits, go into registers.
+        // many lanes where the channels still fit and two tiles a CU are left,
+        // else 16 or 8. The backward pass holds two matrices and the
+        // parameters' sums: at most eight channels of fp32, four of 16 bits,
+        // go into registers. 2^26 bf16 elements: 32 channels with 64 lanes 78
+        // us, with 16 177; 64 channels 79 and 94; 128 channels 75 and 66, so
+        // 16; 256 channels with 32 lanes 78, with 16 88. Backward, 32 channels
+        // with 64 lanes 140 and 16 176; 2^25 floats, 128 channels with 32
+        // lanes 95, with 16 88.
         typedef std::vector<std::array<int, 3>> Forms;
-        static const Forms kForward16 = {{256, 64, 4}, {256, 64, 8}, {512, 64, 8},  {512, 64, 16}, {512, 32, 16}, {512, 16, 1},
-                                         {512, 16, 2}, {512, 16, 4}, {512, 16, 8}, {512, 16, 16}, {512, 8, 16}};
+        static const Forms kForward16 = {{256, 64, 4}, {256, 64, 8},  {256, 64, 16}, {512, 16, 1},  {512, 16, 2},
+                                         {512, 16, 4}, {512, 32, 16}, {512, 16, 8},  {512, 16, 16}, {512, 8, 16}};
         static const Forms kForward32 = {{256, 64, 4}, {256, 64, 8}, {512, 16, 2}, {512, 64, 16}, {512, 32, 16},
                                          {512, 16, 4}, {512, 16, 8}, {512, 16, 16}, {512, 8, 16}};
         static const Forms kBackward16 = {{256, 64, 4}, {512, 64, 4}, {512, 32, 4}, {512, 16, 1},
                                           {512, 16, 2}, {512, 16, 4}, {512, 8, 4}};
-        static const Forms kBackward32 = {{256, 64, 4}, {512, 64, 4}, {512, 64, 8}, {512, 32, 8}, {512, 16, 1},
+        static const Forms kBackward32 = {{256, 64, 4}, {512, 64, 4}, {512, 64, 8}, {512, 16, 1},
                                           {512, 16, 2}, {512, 16, 4}, {512, 16, 8}, {512, 8, 8}};
         int64_t tiles = cdiv(rows, 16 * e);
         for (const auto &f : !backward ? e == 8 ? kForward16 : kForward32 : e == 8 ? kBackward16 : kBackward32) {

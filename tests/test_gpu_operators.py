@@ -227,6 +227,62 @@ def test_layernorm_backward_of_nothing_and_of_parts():
     assert O.layernorm(e, s).shape == (0, 96)
 
 
+def at_ends(rows):
+    """Positions from both ends and from between, across several tiles' borders."""
+    g = torch.Generator().manual_seed(rows)
+    return torch.cat([torch.arange(1100), torch.randint(0, rows, (500,), generator=g), torch.arange(rows - 1100, rows)])
+
+
+# channels: one up to each of the widths that the kernels of many positions
+# hold, odd ones and those of an image's stages
+MANY = [(262144 + 520, 3), (262144 + 1, 16), (262144 + 24, 27), (262144 + 5, 32), (262144 + 8, 40), (300003, 64),
+        (140000, 72), (131072 + 9, 100), (131072 + 8, 128), (131072 + 3, 200), (66000, 256)]
+
+
+@pytest.mark.parametrize("dt", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("rows,cols", MANY)
+def test_layernorm_of_many_positions(rows, cols, dt):
+    """Planar order with positions enough for the kernels of many lanes. Each
+    position's bounds are those of check_layernorm and check_ln_backward. The
+    parameters' sums: a lane adds at most 64 terms (eight of a vector, eight
+    tiles at most here), lanes and waves 16 more, the joining of the blocks' 64
+    more: 144 roundings."""
+    x, xv = make(cols, rows, cols, dt, True, 0, 1.5, 0.3)
+    s, sv = vec(cols + 1, cols, dt, 0.1, 1.0)
+    b, bv = vec(cols + 2, cols, dt, 0.1)
+    y, m, r = O.layernorm(x, s, b, planar=True, stats=True)
+    at = at_ends(rows)
+    xs = xv[at]
+    want, mw, rw, xh = ln_reference(xs, sv, bv, 1e-6)
+    n = cols / 64 + 32
+    me = n * U * xs.abs().mean(1)
+    near(m.double().cpu()[at], mw, me + U * mw.abs(), "mean")
+    d = (xs - mw[:, None]).abs()
+    ve = me ** 2 + ((n + 4) * U * d * d + 2 * U * d * xs.abs()).mean(1)
+    rel = 0.5 * ve / ((d * d).mean(1) + 1e-6) * 1.01 + 6 * U
+    near(r.double().cpu()[at], rw, rw * rel, "rstd")
+    err = (rw[:, None] * (me[:, None] + U * xs.abs()) + xh.abs() * (rel[:, None] + 4 * U)) * sv.abs()
+    near(y.cpu()[:, at].t().double(), want, err + 2 * U * (want.abs() + bv.abs()) + half(dt) * (want.abs() + err) + tiny(dt), "y")
+
+    dy, dyv = make(cols + 3, rows, cols, dt, True)
+    dx, ds, db = O.layernorm_backward(dy, x, s, m, r, add=y, planar=True)
+    mv, rv, av = m.double().cpu()[at], r.double().cpu()[at], y.cpu()[:, at].t().double()
+    wx, _, _, xh, g = ln_backward_reference(dyv[at], xs, sv, mv, rv, av)
+    n = cols / 64 + 40
+    xe = 2 * U * (xh.abs() + rv[:, None] * xs.abs())
+    p, q = g.abs().mean(1, keepdim=True), (g * xh).abs().mean(1, keepdim=True)
+    qe = n * U * q + (g.abs() * xe).mean(1, keepdim=True)
+    err = rv[:, None] * (4 * U * g.abs() + n * U * p + xh.abs() * qe + xe * q + 4 * U * (xh.abs() * q + p))
+    near(dx.cpu()[:, at].t().double(), wx, err + 4 * U * (wx.abs() + av.abs()) + half(dt) * (wx.abs() + err) + tiny(dt), "dx")
+    x64, dy64 = x.double(), dy.double()
+    xh = (x64 - m.double()) * r.double()
+    es = (dy64.abs() * (144 * U * xh.abs() + 2 * U * (xh.abs() + r.double() * x64.abs()))).sum(1).cpu()
+    ws, wb = (dy64 * xh).sum(1).cpu(), dy64.sum(1).cpu()
+    near(ds.double().cpu(), ws, es + half(dt) * (ws.abs() + es) + tiny(dt), "dscale")
+    eb = 144 * U * dy64.abs().sum(1).cpu()
+    near(db.double().cpu(), wb, eb + half(dt) * (wb.abs() + eb) + tiny(dt), "dbias")
+
+
 def test_layernorm_gradient_against_differences():
     """<dx, v> is the derivative of <dy, y> along v, and so for the parameters:
     central differences of the formula in 64 bits, off by step^2 / 6 of the
