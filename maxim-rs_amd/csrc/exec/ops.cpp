@@ -215,8 +215,9 @@ void check_act(int act) {
 // The kernel of a LayerNorm pass: by rows, `lpr` threads a row with `nv`
 // vectors of 16 bytes each, or in planar order `block` threads, so many lanes
 // along the positions and channels a thread; `whole` when the backward kernel
-// sums the parameters' gradients too, else another does. `grid` blocks walk over the rows; in the
-// backward pass each leaves one partial sum of the parameters' gradients.
+// sums the parameters' gradients too, else another does. `grid` blocks walk
+// over the rows; in the backward pass each leaves one partial sum of the
+// parameters' gradients.
 struct LnPlan {
     std::string form;
     unsigned block = 256;

@@ -283,6 +283,18 @@ def test_layernorm_of_many_positions(rows, cols, dt):
     near(db.double().cpu(), wb, eb + half(dt) * (wb.abs() + eb) + tiny(dt), "dbias")
 
 
+# rows enough that each kernel's blocks take several in turn
+MANY_ROWS = [(65536 + 77, 20), (33000, 100), (17000, 256), (8200, 500), (4200, 777), (2100, 2048), (1100, 4096), (530, 8192),
+             (530, 16384)]
+
+
+@pytest.mark.parametrize("dt", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("rows,cols", MANY_ROWS)
+def test_layernorm_of_many_rows(rows, cols, dt):
+    check_layernorm(rows, cols, dt, False, 0, dt)
+    check_ln_backward(rows, cols, dt, False, 0, dt, True)
+
+
 def test_layernorm_gradient_against_differences():
     """<dx, v> is the derivative of <dy, y> along v, and so for the parameters:
     central differences of the formula in 64 bits, off by step^2 / 6 of the
