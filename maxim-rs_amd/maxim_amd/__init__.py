@@ -2,7 +2,8 @@
 
 `plan` wraps the plan contract (include/maxim_plan.h): the graph builder, the
 packed arena, checkpoints, padding. `hip` wraps the gfx950 executor
-(include/maxim_hip.h). Both are ctypes over lib/libmaxim_hip.so.
+(include/maxim_hip.h), `ops` LayerNorm and Dense on torch tensors, forward and
+backward (include/maxim_ops.h). All are ctypes over lib/libmaxim_hip.so.
 """
 
 from . import plan  # noqa: F401
