@@ -340,6 +340,22 @@ struct Plan {
     uint64_t bytes = 0;
 };
 
+// How an operand's lines reach the tiles that go straight to LDS: as they lie,
+// or copied (`pack` bytes); `ld` elements from line to line there.
+struct Side {
+    bool by_k;
+    uint64_t pack;
+    int64_t ld;
+};
+
+// Whether a tile of `b` rows (along k) or 128 bytes of k's (along the operand's
+// own axis) spans less than 2^31 bytes: its offsets, the size of the buffer
+// that bounds it, which has to stay below the offset of lanes without a chunk,
+// and the step to the next tile have 31 bits.
+bool spans(const Side &s, int64_t b, size_t size) {
+    return s.ld < (int64_t(1) << 31) / (s.by_k ? b * (int64_t)size : 128);
+}
+
 // What a tile costs, measured in us on square products of 1024 to 8192: a step
 // of 128 bytes of k with one tile on a CU (`one`), with as many as its LDS
 // holds (`all`, for `fit` of them), and what a tile takes besides.
@@ -362,12 +378,13 @@ const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1,
 // Up to 16 rows against weights that are contiguous along k go to the kernel
 // that reads those once, without LDS tiles or a second launch.
 //
-// `pack_a`, `pack_b`: the bytes of an operand whose tiles cannot go straight to
-// LDS as it lies; copying it to aligned lines first (4 us and its bytes twice)
-// is one more choice. 1237 x 1001 x 777 in fp16: through registers 22 us.
-Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, uint64_t pack_a, uint64_t pack_b, bool by_k) {
+// An operand whose tiles cannot go straight to LDS as it lies can be copied to
+// aligned lines first (4 us and its bytes twice), which is one more choice:
+// 1237 x 1001 x 777 in fp16 takes 22 us through registers. Lines too long for a
+// tile's offsets (spans()) go through registers, whose addresses have 64 bits.
+Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, const Side &b) {
     Plan best;
-    if (by_k && m <= 16) {
+    if (a.by_k && b.by_k && m <= 16) {
         best.skinny = true;
         best.block = 512;
         return best;
@@ -375,7 +392,8 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, uint64_t pack_a, u
     double least = std::numeric_limits<double>::infinity();
     const int64_t bk = 128 / (int64_t)type_size(dtype), steps = std::max<int64_t>(1, cdiv(k, bk));
     auto consider = [&](const TileCost &t) {
-        const uint64_t pack = t.stages ? pack_a + pack_b : 0;
+        if (t.stages && !(spans(a, t.b, type_size(dtype)) && spans(b, t.b, type_size(dtype)))) return;
+        const uint64_t pack = t.stages ? a.pack + b.pack : 0;
         const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b);
         for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
             const int64_t each = cdiv(steps, cut), splits = cdiv(steps, each);
@@ -390,8 +408,8 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, uint64_t pack_a, u
             best.bm = best.bn = t.b;
             best.block = t.b == 256 ? 512 : 256;
             best.stages = t.stages;
-            best.pack_a = t.stages && pack_a;
-            best.pack_b = t.stages && pack_b;
+            best.pack_a = t.stages && a.pack;
+            best.pack_b = t.stages && b.pack;
             best.pack_bytes = pack;
             best.splits = splits;
             best.kchunk = each * bk;
@@ -403,15 +421,6 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, uint64_t pack_a, u
         for (const TileCost &t : kTiles32) consider(t);
     best.bytes = best.pack_bytes + (best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0);
     return best;
-}
-
-// Whether an operand's tiles can go straight to LDS: 16-byte loads of whole
-// chunks, at 31-bit offsets inside a tile (of 256 rows or 64 k's), and lines
-// that do not overlap, so that an offset tells what is past the end.
-bool loads_direct(const Operand &o, bool by_k, int64_t own_n, int64_t sum_n, size_t size) {
-    const int64_t ld = by_k ? o.own : o.sum, extent = by_k ? sum_n : own_n, e = 16 / (int64_t)size;
-    return (uintptr_t)o.data % 16 == 0 && ld % e == 0 && (extent % e == 0 || o.padded) && ld >= extent &&
-           ld < int64_t(1) << (by_k ? 21 : 23);
 }
 
 uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
@@ -435,13 +444,24 @@ Packed packed(bool along_k, int64_t own_n, int64_t sum_n, size_t size) {
     return p;
 }
 
+// An operand's tiles go straight to LDS as it lies where 16-byte loads bring
+// whole chunks, where lines do not overlap, so that an offset tells what is past
+// the end, and where the smallest tile's offsets reach; else from a copy.
+Side side(const Operand &o, int64_t own_n, int64_t sum_n, size_t size) {
+    const bool k = by_k(o);
+    const int64_t e = 16 / (int64_t)size, extent = k ? sum_n : own_n;
+    const Side here{k, 0, k ? o.own : o.sum};
+    if ((uintptr_t)o.data % 16 == 0 && here.ld % e == 0 && (extent % e == 0 || o.padded) && here.ld >= extent &&
+        spans(here, 64, size))
+        return here;
+    const Packed p = packed(k, own_n, sum_n, size);
+    return {k, p.bytes, p.ld};
+}
+
 Plan plan_of(const Product &p) {
     if (!p.m || !p.n) return {};
-    const bool ak = by_k(p.a), bk = by_k(p.b);
     const size_t size = type_size(p.dtype);
-    const uint64_t pa = loads_direct(p.a, ak, p.m, p.k, size) ? 0 : packed(ak, p.m, p.k, size).bytes;
-    const uint64_t pb = loads_direct(p.b, bk, p.n, p.k, size) ? 0 : packed(bk, p.n, p.k, size).bytes;
-    return plan_product(p.dtype, p.m, p.n, p.k, pa, pb, ak && bk);
+    return plan_product(p.dtype, p.m, p.n, p.k, side(p.a, p.m, p.k, size), side(p.b, p.n, p.k, size));
 }
 
 void product(int dev, void *stream, const Product &given, void *ws) {

@@ -74,7 +74,8 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     // strided axis is past the buffer's, past its end along the other one the
     // offset is sent there.
     // (In fp32 tiles that are contiguous along rows the swizzle differs from
-    // chunk to chunk: an offset each.)
+    // chunk to chunk: an offset each.) All of it fits 31 bits, which the host
+    // sees to (spans() in exec/ops.cpp); from tile to tile the base moves.
     constexpr int OA = AK || sizeof(T) == 2 ? 1 : TA::PER, OB = BK_ || sizeof(T) == 2 ? 1 : TB::PER;
     const int lda = (int)(g.lda * sizeof(T)), ldb = (int)(g.ldb * sizeof(T));
     const uint32_t step_a = (AK ? NT / 8 : NT / TA::CPR) * lda, step_b = (BK_ ? NT / 8 : NT / TB::CPR) * ldb;

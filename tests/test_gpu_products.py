@@ -1,0 +1,73 @@
+"""Dense on device tensors where its kernels' addressing and the choice between
+them matter: long lines, operands of different memory orders, few features.
+References are 64-bit products on the card."""
+
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from maxim_amd import ops as O  # noqa: E402
+from test_gpu_operators import TYPES, U, half, tiny  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def named(request, gpu_ok):
+    print(request.node.name, flush=True)
+    O.ready()
+    yield
+    torch.cuda.empty_cache()
+
+
+def rand(gen, a, b, dt, std=1.0):
+    return (torch.randn(a, b, generator=gen, device="cuda") * std).to(dt)
+
+
+def close(got, want, size, terms, dt, what):
+    """Within a result's own rounding and `terms` roundings of its sum. Each of
+    those is half a step at most of a partial sum of random signs, which
+    reaches sqrt(terms) of a product's deviation d: together a walk of about
+    terms d u / 2 where S, the sum of the magnitudes, is 0.64 terms d: 8 u S
+    leaves ten deviations (and terms u S holds always)."""
+    tol = min(terms, 8) * U * size + half(dt) * want.abs() * 1.01 + tiny(dt)
+    off = (got.double() - want).abs() - tol
+    assert bool((off <= 0).all()), (what, float(off.max()))
+
+
+def long_sum(a, b, step=1 << 21):
+    """a b^T and |a| |b|^T over the last axis, in 64 bits and in pieces."""
+    want = torch.zeros(a.shape[0], b.shape[0], dtype=torch.float64, device="cuda")
+    size = want.clone()
+    for i in range(0, a.shape[1], step):
+        p, q = a[:, i:i + step].double(), b[:, i:i + step].double()
+        want += p @ q.t().contiguous()
+        size += p.abs() @ q.abs().t().contiguous()
+    return want, size
+
+
+@pytest.mark.parametrize("dt,k,n,more", [(torch.bfloat16, 128, 136, 8), (torch.float16, 72, 40, 3),
+                                         (torch.float32, 40, 72, 8)], ids=["bf16", "f16", "f32"])
+def test_planes_of_many_positions(dt, k, n, more):
+    """Planes past 2^24 positions, where a tile's lines are further apart than
+    31 bits reach: the results at both ends and in between, dw in full."""
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    rows = (1 << 24) + more
+    x, dy = rand(gen, k, rows, dt), rand(gen, n, rows, dt)
+    w = rand(gen, n, k, dt, 1 / math.sqrt(k))
+    b = rand(gen, 1, n, dt).view(n)
+    at = torch.cat([torch.arange(700), torch.arange((1 << 23) - 300, (1 << 23) + 300), torch.arange(rows - 700, rows),
+                    torch.randint(0, rows, (500,), generator=torch.Generator().manual_seed(1))]).cuda()
+    w64 = w.double()
+    y = O.dense(x, w, b, planar=True)
+    xs = x[:, at].double()
+    close(y[:, at], w64 @ xs + b.double()[:, None], w64.abs() @ xs.abs() + b.double().abs()[:, None], k + 1, dt, "y")
+    del y
+    dx, dw, db = O.dense_backward(dy, x, w, planar=True)
+    ds = dy[:, at].double()
+    close(dx[:, at], w64.t().contiguous() @ ds, w64.t().abs().contiguous() @ ds.abs(), n, dt, "dx")
+    want, size = long_sum(dy, x)
+    close(dw, want, size, rows, dt, "dw")
+    close(db, dy.double().sum(1), dy.double().abs().sum(1), rows, dt, "db")

@@ -1,0 +1,89 @@
+"""What the operators' host side launches, checked without a device: a HIP
+runtime that writes the launches down takes calls on made-up addresses
+(fake_card.py)."""
+
+import random
+import re
+
+import pytest
+
+pytest.importorskip("torch")
+
+import fake_card as F  # noqa: E402
+
+F32, F16, BF16 = 0, 1, 2
+
+
+@pytest.fixture(scope="module")
+def card(tmp_path_factory):
+    so = F.library(tmp_path_factory.mktemp("fake"))
+    if so is None:
+        pytest.skip("no g++")
+    return lambda calls: F.run(so, calls)
+
+
+def dense_calls(rows, k, n, dtype, planar=False, pad=0, wt=False, act=0, x_planar=None):
+    """A Dense and its backward pass over [rows][k] -> [rows][n]."""
+    xp = planar if x_planar is None else x_planar
+    at = [(i + 1) << 52 for i in range(8)]
+    x = F.mat(rows, k, at[0], not xp, pad, dtype)
+    w = F.mat(n, k, at[1], not wt, 0, dtype)
+    y, dy, z = (F.mat(rows, n, a, not planar, p, dtype) for a, p in ((at[2], 0), (at[3], pad), (at[4], pad)))
+    dx, dw = F.mat(rows, k, at[5], not planar, 0, dtype), F.mat(n, k, at[6], not wt, 0, dtype)
+    return [{"op": "dense", "x": x, "w": w, "y": y, "bias": F.vec(n, at[7], dtype), "act": act},
+            {"op": "dense_backward", "dy": dy, "x": x, "w": w, "z": z if act else None, "act": act, "dx": dx, "dw": dw,
+             "db": F.vec(n, at[7], dtype)}]
+
+
+def check_products(call, result):
+    """A product's operands as the kernels' addresses need them."""
+    assert result["rc"] == 0, (result["error"], call)
+    size = F.SIZE[call["x"][5]]
+    for l in result["launches"]:
+        for i in "01":
+            if "dst" + i in l:
+                assert F.WORKSPACE <= l["dst" + i] and l["end" + i] <= F.WORKSPACE + result["workspace"], (l, call)
+        f = re.match(r"mxo_gemm_\w+?_(\d+)x\d+_([km])([km])_d\d$", l["kernel"])
+        if not f:
+            continue
+        tile, bk = int(f[1]), 128 // size
+        for along, ld, p in ((f[2], l["lda"], l["a"]), (f[3], l["ldb"], l["b"])):
+            assert p % 16 == 0 and ld * size % 16 == 0, (l, call)
+            # a tile's lines, the buffer that bounds them and the step to the
+            # next tile are offsets of 31 bits
+            assert (tile if along == "k" else bk) * ld * size < 1 << 31, (l, call)
+
+
+# rows, k, n: planes of 2^24 positions and more, and sums as long
+LARGE = [((1 << 24) + d, k, n) for d in (0, 8, 3) for k, n in ((128, 256), (512, 512), (16, 2048), (64, 64))] + [
+    (1 << 25, 512, 512), (1 << 26, 64, 256), (1 << 23, 256, 256), (1 << 21, 128, 128), ((1 << 21) + 1, 640, 640),
+    (512, (1 << 21) + 3, 512), (512, 1 << 22, 256), (256, 640, (1 << 23) + 1), (300, 1 << 24, 300)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_long_lines_keep_to_31_bits(card, dtype):
+    calls = []
+    for rows, k, n in LARGE:
+        for i in range(16):
+            calls += dense_calls(rows, k, n, dtype, bool(i & 1), 3 if i & 2 else 0, bool(i & 4), x_planar=bool(i & 8),
+                                 act=int(i % 3 == 0))
+    for c, r in zip(calls, card(calls)):
+        check_products(c, r)
+
+
+def test_drawn_products_keep_to_31_bits(card):
+    rng = random.Random(5)
+
+    def size(most):
+        n = int(2 ** rng.uniform(0, most))
+        return n if rng.random() < 0.5 else (n + 63) // 64 * 64
+
+    calls = []
+    for _ in range(1500):
+        sizes = [size(26), size(11), size(11)]
+        rng.shuffle(sizes)
+        rows, k, n = sizes[0], min(sizes[1], 1 << 23), min(sizes[2], 1 << 23)
+        calls += dense_calls(rows, k, n, rng.choice([F32, F16, BF16]), rng.random() < 0.5, rng.choice([0, 0, 3, 8]),
+                             rng.random() < 0.5, rng.choice([0, 1]), rng.random() < 0.5)
+    for c, r in zip(calls, card(calls)):
+        check_products(c, r)
