@@ -375,8 +375,18 @@ const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1,
 // x 256 cut in four 65 us; 1024 x 1024: 64 x 64 uncut 18 us, cut in four 28
 // us, 128 x 128 cut in four 26 us.
 //
-// Up to 16 rows against weights that are contiguous along k go to the kernel
-// that reads those once, without LDS tiles or a second launch.
+// Up to 16 rows, both operands contiguous along k, can also go to the kernel
+// that reads the other operand once, without LDS tiles or a second launch: a
+// block for 16 columns and all of k, so it is quick where k is short or there
+// are columns enough (0.07 to 0.11 us a step of 128 bytes for every 256 blocks,
+// by the rows; the tiles then no faster than the operand comes from memory).
+// bf16, one row and 16: k = 4096 to 4096 columns 9.0 and 10.6 us, as tiles 11.6
+// and 11.4; k = 1024 to 64 columns 3.8 and 4.5, tiles 5.5 and 5.6; k = 16384 to
+// 1024 columns 23 and 31, tiles 12; k = 262144 to 64 columns 334 and 447,
+// tiles 14 and 18. fp32, 16 rows: k = 1024 to 4096 columns 7.6, tiles 13; k =
+// 4096 to 64 columns 17, tiles 8.4. (The gradient of a planar Dense's weights
+// sums over all positions: 32 to 16 features of 448 x 640, fp32, 985 us by few
+// rows, 35 by tiles.)
 //
 // An operand whose tiles cannot go straight to LDS as it lies can be copied to
 // aligned lines first (4 us and its bytes twice), which is one more choice:
@@ -384,11 +394,6 @@ const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1,
 // tile's offsets (spans()) go through registers, whose addresses have 64 bits.
 Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, const Side &b) {
     Plan best;
-    if (a.by_k && b.by_k && m <= 16) {
-        best.skinny = true;
-        best.block = 512;
-        return best;
-    }
     double least = std::numeric_limits<double>::infinity();
     const int64_t bk = 128 / (int64_t)type_size(dtype), steps = std::max<int64_t>(1, cdiv(k, bk));
     auto consider = [&](const TileCost &t) {
@@ -419,6 +424,15 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, con
         for (const TileCost &t : kTiles16) consider(t);
     else
         for (const TileCost &t : kTiles32) consider(t);
+    if (a.by_k && b.by_k && m <= 16) {
+        const double few = 4.0 + (0.065 + 0.0025 * m) * steps * std::max(1.0, cdiv(n, 16) / 256.0);
+        if (few <= std::max(least, (double)n * k * type_size(dtype) / 4.9e6)) {
+            best = Plan();
+            best.skinny = true;
+            best.block = 512;
+            return best;
+        }
+    }
     best.bytes = best.pack_bytes + (best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0);
     return best;
 }

@@ -87,3 +87,18 @@ def test_drawn_products_keep_to_31_bits(card):
                              rng.random() < 0.5, rng.choice([0, 1]), rng.random() < 0.5)
     for c, r in zip(calls, card(calls)):
         check_products(c, r)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_few_features_keep_the_card_busy(card, dtype):
+    """The gradient of a planar Dense's weights sums over every position: with
+    few features too it is spread over the card, 256 CUs. A short sum into few
+    columns takes one launch, and many columns need no cut."""
+    calls = [dense_calls(448 * 640, k, n, dtype, True)[1] for k in (3, 32, 64, 128) for n in (1, 3, 8, 16, 17)]
+    for c, r in zip(calls, card(calls)):
+        check_products(c, r)
+        dw = [l for l in r["launches"] if "k" in l and l["k"] == 448 * 640]
+        assert len(dw) == 1 and dw[0]["gx"] >= 240, (dw, c)
+    calls = [dense_calls(rows, k, n, dtype)[0] for rows in (1, 16) for k, n in ((64, 64), (1024, 64), (1024, 4096), (4096, 4096))]
+    for c, r in zip(calls, card(calls)):
+        assert [l["kernel"][:10] for l in r["launches"]] == ["mxo_skinny"], (r, c)
