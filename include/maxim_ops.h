@@ -19,7 +19,7 @@
  * Sums, means and variances are fp32; a result is rounded once, to nearest
  * even, when it is stored. fp32 products are formed on the bf16 matrix cores
  * from three bf16 parts of each operand (every bit of a float, whatever its
- * size; a product is off by 1.1e-7 of itself at most), and sums that are not
+ * size; one product is off by 1.82e-7 of itself at most), and sums that are not
  * finite again in fp32, so infinities and NaN are fp32's. No atomics: the same
  * call gives the same bits.
  *

@@ -19,11 +19,13 @@ __device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
 // Computations", ARITH 2019). A float splits exactly into three
 // bf16 parts, x = h + m + l (8 + 8 + 8 significand bits, each part the rounded
 // remainder of the last), and of the nine products of two split floats the six
-// of order 2^0, 2^-8 and 2^-16 are kept; what is dropped is below 2^-24 of the
-// product (a sum of one term is off by 1.1e-7 of it at most, an fp32 product by
-// 6.0e-8). Each v_mfma_f32_16x16x32_bf16 adds 32 exact products in fp32 with
-// one rounding, so a sum of K products is rounded 6 K / 32 times where the
-// fp32 MFMA chain rounds K times: against 64-bit sums of N(0, 1) products the
+// of order 2^0, 2^-8 and 2^-16 are kept; what is dropped is up to 2^-24 of the
+// product. Each v_mfma_f32_16x16x32_bf16 adds 32 exact products in fp32 to
+// within one step, 2^-23 (the hardware does not round to nearest here: 2^28
+// products of operands in [1, 2) came out up to 2.9 x 2^-24 off, 0.2 x 2^-24 low
+// in the mean, where nearest would give 2.0), so a sum of one term is off by
+// 1.82e-7 of it at most, an fp32 product by 6.0e-8. A sum of K products is
+// rounded 6 K / 32 times where the fp32 MFMA chain rounds K times: against 64-bit sums of N(0, 1) products the
 // relative error is 3.7e-8 / 9.2e-8 / 1.5e-7 / 2.3e-7 at K = 32 / 64 / 128 /
 // 256, the fp32 MFMA's 1.0e-7 / 1.4e-7 / 2.0e-7 / 2.9e-7. Six bf16 MFMAs take
 // 96 cycles of a SIMD for the 32 k's that eight fp32 ones take 256 for, and

@@ -95,3 +95,17 @@ def test_few_features_over_many_positions(n, dt):
             want, size = long_sum(dy, x)
             close(dw, want, size, rows, dt, "dw")
             close(db, d64.sum(1), d64.abs().sum(1), rows, dt, "db")
+
+
+def test_one_product_in_fp32():
+    """A product of three-part operands alone: within 3.04 u of itself, as
+    close() derives it; exact where the parts are."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for span in (1.0, 0.01):
+        x = 1 + span * torch.rand(1 << 18, 1, generator=gen, device="cuda")
+        w = 1 + span * torch.rand(256, 1, generator=gen, device="cuda")
+        want = x.double() @ w.double().t()
+        off = float((O.dense(x, w).double() / want - 1).abs().max())
+        assert off <= 3.04 * U * 1.0001 < 1.82e-7, off / U
+    x, w = x.bfloat16().float(), w.bfloat16().float()
+    assert torch.equal(O.dense(x, w), x @ w.t())
