@@ -165,9 +165,8 @@ def _new(x, X, n, planar):
         t, by_rows = _torch.empty_like(x), planar
     else:
         rest = tuple(x.shape[1:] if planar else x.shape[:-1])
-        by_rows = X.row_stride == 1 and X.rows > 1 and (X.col_stride != 1 or X.cols == 1)
-        if X.rows <= 1:
-            by_rows = planar
+        # both strides 1, or a single position: the call's own order
+        by_rows = planar if X.rows <= 1 or X.row_stride == X.col_stride == 1 else X.row_stride == 1
         t = x.new_empty((n,) + rest if by_rows else rest + (n,))
         if by_rows != planar:
             t = t.movedim(-1, 0) if planar else t.movedim(0, -1)

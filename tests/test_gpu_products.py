@@ -109,3 +109,32 @@ def test_one_product_in_fp32():
         assert off <= 3.04 * U * 1.0001 < 1.82e-7, off / U
     x, w = x.bfloat16().float(), w.bfloat16().float()
     assert torch.equal(O.dense(x, w), x @ w.t())
+
+
+@pytest.mark.parametrize("planar", [False, True])
+@pytest.mark.parametrize("k,n", [(1, 7), (1, 1), (7, 1)])
+def test_one_feature_forward_and_backward(k, n, planar):
+    """What the forward call gives, its backward call takes beside ordinary
+    gradients."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    rows, dt = 100, torch.float32
+    x, dy = (rand(gen, *((c, rows) if planar else (rows, c)), dt) for c in (k, n))
+    w = rand(gen, n, k, dt)
+    y, z = O.dense(x, w, act="gelu", planar=planar, save=True)
+    assert y.is_contiguous() and z.is_contiguous() and y.shape == dy.shape
+    dx, dw, db = O.dense_backward(dy, x, w, z=z, act="gelu", planar=planar)
+    x64 = (x.t() if planar else x).double().cpu().requires_grad_()
+    w64 = w.double().cpu().requires_grad_()
+    z64 = x64 @ w64.t()
+    y64 = z64 * 0.5 * torch.special.erfc(-z64 / math.sqrt(2))
+    y64.backward((dy.t() if planar else dy).double().cpu())
+    # sums of terms + 1 roundings, z's u |z| times a slope below 1.2, and the
+    # fits: gelu within 3e-7 (1 + |z|), its derivative within 6e-7 (1 + |z|)
+    xa, wa, za = x64.detach().abs(), w64.detach().abs(), z64.detach().abs()
+    da = (dy.t() if planar else dy).double().cpu().abs()
+    ze = (k + 4) * U * (xa @ wa.t())
+    dze = da * (6e-7 * (1 + za) + 0.8 * ze) + 2 * U * da
+    for got, want, tol in ((y.t() if planar else y, y64.detach(), 1.2 * ze + 3e-7 * (1 + za) + 2 * U * za),
+                           (dx.t() if planar else dx, x64.grad, dze @ wa + (n + 4) * U * 1.2 * (da @ wa)),
+                           (dw, w64.grad, dze.t() @ xa + (rows + 4) * U * 1.2 * (da.t() @ xa))):
+        assert ((got.double().cpu() - want).abs() <= tol).all()
