@@ -157,11 +157,15 @@ __device__ __forceinline__ float phi_tail(float ax) {
     return ax > 6.0f ? 0.0f : r;
 }
 
-// The activation. gelu, gelu_tanh and silu of minus infinity are their limit
-// 0 (the clamp keeps an infinity out of a product with 0); NaN stays NaN.
+// The activation. gelu, gelu_tanh, silu and lrelu of slope 0 of minus infinity
+// are their limit 0 (an infinity is kept out of a product with 0); NaN stays
+// NaN.
 __device__ __forceinline__ float act_fwd(int act, float slope, float z) {
     if (act == MXO_NONE) return z;
-    if (act == MXO_LRELU) return z >= 0.0f ? z : slope * z;
+    if (act == MXO_LRELU) {
+        const float c = slope == 0.0f && z == -__builtin_inff() ? -1.0f : z;
+        return z >= 0.0f ? z : slope * c;
+    }
     float v, d;
     if (act == MXO_GELU) {
         v = fmaxf(z, 0.0f) - fminf(fabsf(z), 6.0f) * phi_tail(fabsf(z));

@@ -138,3 +138,19 @@ def test_one_feature_forward_and_backward(k, n, planar):
                            (dx.t() if planar else dx, x64.grad, dze @ wa + (n + 4) * U * 1.2 * (da @ wa)),
                            (dw, w64.grad, dze.t() @ xa + (rows + 4) * U * 1.2 * (da.t() @ xa))):
         assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("rows", [1, 40])
+def test_relu_at_the_ends(rows, dt):
+    """LeakyReLU of slope 0 is ReLU: 0 at minus infinity too, NaN at NaN; any
+    other slope keeps the infinity."""
+    one = torch.ones(1, 1, dtype=dt, device="cuda")
+    z = torch.tensor([-float("inf"), -60000.0, -1.0, -0.0, 0.0, 2.0, float("inf"), float("nan")], dtype=dt, device="cuda")
+    x = z.view(-1, 1).repeat(rows, 1)
+    want = torch.nn.functional.relu(z.float()).to(dt)
+    got = O.dense(x, one, act="lrelu", slope=0.0).view(rows, -1)
+    assert torch.equal(got[:, :7], want[:7].expand(rows, 7)) and torch.isnan(got[:, 7]).all()
+    got = O.dense(x, one, act="lrelu", slope=0.5).view(rows, -1)
+    assert torch.equal(got[:, :7], torch.where(z < 0, 0.5 * z, z)[:7].expand(rows, 7)) and torch.isnan(got[:, 7]).all()
+    assert torch.equal(O.dense(x, one, act="lrelu", slope=-0.5).view(rows, -1)[:, 0], z[6].expand(rows))
