@@ -15,7 +15,8 @@ either the features or the positions contiguous; others are refused, not
 copied. Results have x's memory order (Dense's y and z the residual's, where
 there is one). The calls record no autograd graph: each forward call has a backward
 call beside it, and tensors that require a gradient are refused while torch
-records one (use torch.no_grad(), as an autograd.Function's methods do).
+records one (use torch.no_grad(), as an autograd.Function's methods do); so are
+tensors that carry a forward-mode tangent.
 """
 
 import ctypes as C
@@ -39,6 +40,7 @@ class Vec(C.Structure):
 
 _L = None
 _torch = None
+_forward_ad = None
 _raw_stream = None
 _types = {}
 
@@ -51,7 +53,7 @@ def _runtimes():
 
 def _lib():
     """The library with the operators' entry points declared."""
-    global _L, _torch, _raw_stream
+    global _L, _torch, _forward_ad, _raw_stream
     if _L is None:
         try:
             import torch  # before the library looks for a HIP runtime: torch's is the one to share
@@ -79,8 +81,9 @@ def _lib():
             f.restype = I
             f.argtypes = args
         _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-        _L, _torch = L, torch
+        _torch, _forward_ad = torch, torch.autograd.forward_ad
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _L = L  # last: another thread that sees it sees the rest
     return _L
 
 
@@ -94,7 +97,8 @@ def _tensor(t, what, device):
     try:
         code = _types.get(t.dtype)
         if code is not None and t.is_cuda and t.get_device() == device and not (
-                t.requires_grad and _torch.is_grad_enabled()):
+                t.requires_grad and _torch.is_grad_enabled()) and (
+                _forward_ad._current_level < 0 or _forward_ad.unpack_dual(t).tangent is None):
             return code
     except AttributeError:
         raise P.MaximError("%s: not a tensor" % what)
@@ -104,6 +108,8 @@ def _tensor(t, what, device):
         raise P.MaximError("%s: on another device than x" % what)
     if code is None:
         raise P.MaximError("%s: %s, not float32, float16 or bfloat16" % (what, t.dtype))
+    if not (t.requires_grad and _torch.is_grad_enabled()):
+        raise P.MaximError("%s carries a forward-mode tangent, which this call would drop" % what)
     raise P.MaximError("%s requires a gradient, which this call does not record: use torch.no_grad()" % what)
 
 

@@ -9,6 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from maxim_amd import ops as O  # noqa: E402
+from maxim_amd import plan as P  # noqa: E402
 from test_gpu_operators import TYPES, U, half, tiny  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -154,3 +155,13 @@ def test_relu_at_the_ends(rows, dt):
     got = O.dense(x, one, act="lrelu", slope=0.5).view(rows, -1)
     assert torch.equal(got[:, :7], torch.where(z < 0, 0.5 * z, z)[:7].expand(rows, 7)) and torch.isnan(got[:, 7]).all()
     assert torch.equal(O.dense(x, one, act="lrelu", slope=-0.5).view(rows, -1)[:, 0], z[6].expand(rows))
+
+
+def test_tangents_are_refused_on_the_card():
+    x, w = torch.ones(8, 16, device="cuda"), torch.ones(4, 16, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(x, x)
+        for call in (lambda: O.dense(d, w), lambda: O.dense(w, d), lambda: O.layernorm(d, w[0])):
+            with pytest.raises(P.MaximError, match="forward-mode tangent"):
+                call()
+        assert torch.equal(O.dense(x, w), torch.full((8, 4), 16.0, device="cuda"))

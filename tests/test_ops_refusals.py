@@ -184,3 +184,50 @@ def test_every_declared_operator_is_exported():
     assert len(names) == 8
     for n in names:
         assert hasattr(O._lib(), n), n
+
+
+def test_tangents_are_refused():
+    """A call would drop a forward-mode tangent: tensors that carry one are
+    refused, but inside an autograd.Function, which sees none."""
+    from torch.autograd import forward_ad
+
+    class Card:
+        """A CPU tensor that says that it is the card's."""
+        dtype, is_cuda, requires_grad = torch.float32, True, False
+
+        def __init__(self, t):
+            self.t = t
+
+        def get_device(self):
+            return 0
+
+    O._lib()
+    tell = forward_ad.unpack_dual
+    x = torch.zeros(3)
+    try:
+        forward_ad.unpack_dual = lambda t: tell(t.t)
+        assert O._tensor(Card(x), "x", 0) == 0
+        with forward_ad.dual_level():
+            d = forward_ad.make_dual(x, torch.ones(3))
+            assert O._tensor(Card(x), "x", 0) == 0
+            with pytest.raises(P.MaximError, match="x carries a forward-mode tangent"):
+                O._tensor(Card(d), "x", 0)
+
+            class Twice(torch.autograd.Function):
+                @staticmethod
+                def forward(v):
+                    assert O._tensor(Card(v), "x", 0) == 0
+                    return 2 * v
+
+                @staticmethod
+                def setup_context(ctx, inputs, output):
+                    pass
+
+                @staticmethod
+                def jvp(ctx, t):
+                    return 2 * t
+
+            assert torch.equal(tell(Twice.apply(d)).tangent, torch.full((3,), 2.0))
+        assert O._tensor(Card(x), "x", 0) == 0
+    finally:
+        forward_ad.unpack_dual = tell
