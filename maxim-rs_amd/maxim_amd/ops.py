@@ -183,6 +183,13 @@ def _workspace(n, x):
     return x.new_empty(n, dtype=_torch.uint8) if n else None
 
 
+def _written(out):
+    """Tells autograd that a caller's tensor has new values (a result of the
+    call's own has no history)."""
+    if out is not None:
+        _torch.autograd.graph.increment_version(out)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -206,6 +213,7 @@ def layernorm(x, scale, bias=None, eps=1e-6, planar=False, stats=False, out=None
         mean = x.new_empty(shape, dtype=_torch.float32)
         rstd = _torch.empty_like(mean)
     _check(_L.mxh_layernorm(d, _stream(d), X, S, B, eps, Y, _ptr(mean), _ptr(rstd)))
+    _written(out)
     return (y, mean, rstd) if stats else y
 
 
@@ -240,6 +248,7 @@ def layernorm_backward(dy, x, scale, mean, rstd, add=None, planar=False, dx=True
         ws = _workspace(n, x)
     _check(_L.mxh_layernorm_backward(d, _stream(d), DY, X, S, mean.data_ptr(), rstd.data_ptr(), A, DX, DS, DB,
                                      _ptr(ws), n))
+    _written(out)
     return gx, ds, db
 
 
@@ -260,6 +269,7 @@ def dense(x, w, bias=None, act=None, slope=0.0, residual=None, planar=False, sav
     _check(_L.mxh_dense_workspace(X, W, Y, size))
     ws = _workspace(size.value, x)
     _check(_L.mxh_dense(d, _stream(d), X, W, B, a, slope, R, Y, Z, _ptr(ws), size.value))
+    _written(out)
     return (y, z) if save else y
 
 

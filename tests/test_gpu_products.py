@@ -165,3 +165,31 @@ def test_tangents_are_refused_on_the_card():
             with pytest.raises(P.MaximError, match="forward-mode tangent"):
                 call()
         assert torch.equal(O.dense(x, w), torch.full((8, 4), 16.0, device="cuda"))
+
+
+def test_what_out_overwrites_is_known_to_autograd():
+    """A result written over a tensor that an earlier operation kept for its
+    backward pass: torch says so instead of using the new values."""
+    s, w = torch.ones(16, device="cuda"), torch.eye(16, device="cuda")
+
+    def layernorm(t):
+        O.layernorm(t, s, out=t)
+
+    def dense(t):
+        O.dense(torch.ones_like(t), w, residual=t, out=t)
+
+    def layernorm_backward(t):
+        _, m, r = O.layernorm(torch.ones_like(t), s, stats=True)
+        O.layernorm_backward(t, torch.ones_like(t), s, m, r, out=t)
+
+    for call in (layernorm, dense, layernorm_backward):
+        p = torch.randn(8, 16, device="cuda", requires_grad=True)
+        y = p.exp()  # keeps its result
+        with torch.no_grad():
+            before = y._version
+            call(y)
+            assert y._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        with torch.inference_mode():
+            call(torch.randn(8, 16, device="cuda"))
