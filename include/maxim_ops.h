@@ -12,9 +12,11 @@
  * `row_stride` and `col_stride` elements apart, one of the two 1. So the
  * executor's planar [c][h][w] order is (row_stride 1, col_stride h * w) and a
  * token-major [n][c] array (row_stride c, col_stride 1); slices of wider
- * buffers and broadcast inputs (a stride of 0) need no copy. Any sizes, any
- * alignment of the element. An output's own elements must not share storage,
- * and an output must not overlap any other operand, but where a call says so.
+ * buffers and broadcast inputs (a stride of 0) need no copy. Any alignment of
+ * the element, any sizes whose launches have fewer than 2^32 threads each
+ * (others, of 2^24 features and more, are refused). An output's own elements
+ * must not share storage, and an output must not overlap any other operand, but
+ * where a call says so.
  *
  * Sums, means and variances are fp32; a result is rounded once, to nearest
  * even, when it is stored. fp32 products are formed on the bf16 matrix cores

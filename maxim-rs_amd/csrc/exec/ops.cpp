@@ -73,14 +73,41 @@ mxh::hipFunction_t function(int dev, const std::string &name) {
     return f;
 }
 
-template <typename A>
-void launch(int dev, void *stream, const std::string &name, int64_t gx, int64_t gy, unsigned block, const A &args) {
-    A copy = args;
-    void *params[] = {&copy};
-    check(hip().hipModuleLaunchKernel(function(dev, name), (unsigned)gx, (unsigned)gy, 1, block, 1, 1, 0,
-                                      (mxh::hipStream_t)stream, params, nullptr),
-          name.c_str());
-}
+// A call's launches, of which none is made before all are known to fit: the
+// threads of a launch are counted in 32 bits.
+class Launches {
+    struct One {
+        std::string name;
+        unsigned gx, gy, block;
+        alignas(8) char args[192];
+    };
+    One at_[8];  // a Dense's backward pass: dz and its join, twice packing, product and join
+    int n_ = 0;
+
+public:
+    template <typename A>
+    void add(const std::string &name, int64_t gx, int64_t gy, unsigned block, const A &args) {
+        static_assert(sizeof(A) <= sizeof(One::args), "");
+        if (gx > (int64_t)UINT32_MAX / block || gy > 65535)
+            throw Error("the operands are too large: " + name + " would take more threads than one launch can have");
+        One &o = at_[n_++];
+        o.name = name;
+        o.gx = (unsigned)gx, o.gy = (unsigned)gy, o.block = block;
+        std::memcpy(o.args, &args, sizeof(A));
+    }
+    void run(int dev, void *stream) {
+        OnDevice on(dev);
+        mxh::hipFunction_t f[8];
+        for (int i = 0; i < n_; ++i) f[i] = function(dev, at_[i].name);
+        for (int i = 0; i < n_; ++i) {
+            One &o = at_[i];
+            void *params[] = {o.args};
+            check(hip().hipModuleLaunchKernel(f[i], o.gx, o.gy, 1, o.block, 1, 1, 0, (mxh::hipStream_t)stream, params,
+                                              nullptr),
+                  o.name.c_str());
+        }
+    }
+};
 
 // ------------------------------------------------------------- operands
 
@@ -290,7 +317,7 @@ uint64_t ln_bwd_bytes(const mxh_mat &x) {
     return (uint64_t)parts * 2 * x.cols * 4;
 }
 
-void join(int dev, void *stream, const float *part, int64_t nparts, int64_t n, void *out0, void *out1, int dtype) {
+void join(Launches &launches, const float *part, int64_t nparts, int64_t n, void *out0, void *out1, int dtype) {
     if (!n) return;
     OpsJoinArgs j{};
     j.part = part;
@@ -300,7 +327,7 @@ void join(int dev, void *stream, const float *part, int64_t nparts, int64_t n, v
     j.nparts = (int32_t)nparts;
     j.nout = out1 ? 2 : 1;
     j.dtype = dtype;
-    launch(dev, stream, "mxo_join_parts", cdiv(n, 16), j.nout, 1024, j);
+    launches.add("mxo_join_parts", cdiv(n, 16), j.nout, 1024, j);
 }
 
 // ------------------------------------------------------------- products
@@ -478,7 +505,7 @@ Plan plan_of(const Product &p) {
     return plan_product(p.dtype, p.m, p.n, p.k, side(p.a, p.m, p.k, size), side(p.b, p.n, p.k, size));
 }
 
-void product(int dev, void *stream, const Product &given, void *ws) {
+void product(Launches &launches, const Product &given, void *ws) {
     if (!given.m || !given.n) return;
     Product p = given;
     const bool ak = by_k(p.a), bk = by_k(p.b);
@@ -505,10 +532,7 @@ void product(int dev, void *stream, const Product &given, void *ws) {
     };
     if (pl.pack_a) add(p.a, ak, p.m);
     if (pl.pack_b) add(p.b, bk, p.n);
-    if (jobs) {
-        if (blocks > std::numeric_limits<int32_t>::max()) throw Error("the product's operands are too large");
-        launch(dev, stream, size == 2 ? "mxo_pack_16" : "mxo_pack_32", blocks, jobs, 256, pack);
-    }
+    if (jobs) launches.add(size == 2 ? "mxo_pack_16" : "mxo_pack_32", blocks, jobs, 256, pack);
     OpsGemmArgs g{};
     g.a = p.a.data;
     g.b = p.b.data;
@@ -535,22 +559,20 @@ void product(int dev, void *stream, const Product &given, void *ws) {
         g.bias_rows = p.bias_rows;
     }
     if (pl.skinny) {
-        launch(dev, stream, "mxo_skinny_" + t, cdiv(p.n, 16), 1, pl.block, g);
+        launches.add("mxo_skinny_" + t, cdiv(p.n, 16), 1, pl.block, g);
         return;
     }
     const int64_t tm = cdiv(p.m, pl.bm), tn = cdiv(p.n, pl.bn);
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
-    if (tm * tn > std::numeric_limits<int32_t>::max() / pl.splits) throw Error("the product has too many tiles");
-    launch(dev, stream,
-           "mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
-               (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
-           tm * tn * pl.splits, 1, pl.block, g);
+    launches.add("mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
+                     (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
+                 tm * tn * pl.splits, 1, pl.block, g);
     if (pl.splits > 1) {
         // few sums of many splits: eight threads to each
         const bool deep = pl.splits >= 16;
-        launch(dev, stream, (deep ? "mxo_join8_" : "mxo_join_") + t,
-               std::min<int64_t>(4096, cdiv(p.m * cdiv(p.n, 4), deep ? 32 : 256)), 1, 256, g);
+        launches.add((deep ? "mxo_join8_" : "mxo_join_") + t,
+                     std::min<int64_t>(4096, cdiv(p.m * cdiv(p.n, 4), deep ? 32 : 256)), 1, 256, g);
     }
 }
 
@@ -691,7 +713,6 @@ int mxh_layernorm(int device, void *stream, const mxh_mat *x, const mxh_vec *sca
             refuse_overlap(*o, "a statistic", Y, "y");
         }
         if (!X.rows) return;
-        OnDevice on(device);
         OpsLnArgs a{};
         a.x = X.data;
         a.y = Y.data;
@@ -706,9 +727,10 @@ int mxh_layernorm(int device, void *stream, const mxh_mat *x, const mxh_vec *sca
         a.eps = eps;
         a.param_f32 = scale->dtype == MXH_F32;
         const LnPlan p = ln_plan(X.dtype, X.rows, X.cols, by_cols, false);
-        launch(device, stream,
-               std::string(by_cols ? "mxo_ln_rows_" : "mxo_ln_planar_") + kTypeName[X.dtype] + "_" + p.form, p.grid, 1,
-               p.block, a);
+        Launches launches;
+        launches.add(std::string(by_cols ? "mxo_ln_rows_" : "mxo_ln_planar_") + kTypeName[X.dtype] + "_" + p.form, p.grid,
+                     1, p.block, a);
+        launches.run(device, stream);
     });
 }
 
@@ -765,7 +787,7 @@ int mxh_layernorm_backward(int device, void *stream, const mxh_mat *dy, const mx
             }
             check_workspace(workspace, workspace_bytes, ln_bwd_bytes(X));
         }
-        OnDevice on(device);
+        Launches launches;
         const std::string t = kTypeName[X.dtype];
         OpsLnBwdArgs a{};
         a.dy = DY.data;
@@ -787,12 +809,12 @@ int mxh_layernorm_backward(int device, void *stream, const mxh_mat *dy, const mx
         if (X.rows && dscale && !p.whole) {
             // before dx, which may take dy's place
             const int64_t e = by_cols ? 64 * 16 / (int64_t)type_size(X.dtype) : 1;
-            launch(device, stream, "mxo_ln_param_" + order + t, cdiv(X.cols, e), a.nparts, 256, a);
+            launches.add("mxo_ln_param_" + order + t, cdiv(X.cols, e), a.nparts, 256, a);
         }
         if (!dscale) a.part = nullptr;
-        if (X.rows && (dx || p.whole)) launch(device, stream, "mxo_ln_bwd_" + order + t + "_" + p.form, p.grid, 1, p.block, a);
-        if (dscale)
-            join(device, stream, a.part, X.rows ? p.parts : 0, X.cols, dscale->data, dbias->data, dscale->dtype);
+        if (X.rows && (dx || p.whole)) launches.add("mxo_ln_bwd_" + order + t + "_" + p.form, p.grid, 1, p.block, a);
+        if (dscale) join(launches, a.part, X.rows ? p.parts : 0, X.cols, dscale->data, dbias->data, dscale->dtype);
+        launches.run(device, stream);
     });
 }
 
@@ -836,14 +858,15 @@ int mxh_dense(int device, void *stream, const mxh_mat *x, const mxh_mat *w, cons
         if (empty(Y)) return;
         Product p = dense_product(X, W, Y, by_cols);
         check_workspace(workspace, workspace_bytes, plan_of(p).bytes);
-        OnDevice on(device);
         p.bias = bias;
         p.bias_rows = !by_cols;
         p.act = act;
         p.slope = slope;
         if (residual) p.res = residual->data, p.ldr = by_cols ? residual->row_stride : residual->col_stride;
         if (z) p.z = z->data, p.ldz = by_cols ? z->row_stride : z->col_stride;
-        product(device, stream, p, workspace);
+        Launches launches;
+        product(launches, p, workspace);
+        launches.run(device, stream);
     });
 }
 
@@ -893,7 +916,7 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         }
         BwdLayout l = bwd_layout(DY, dz_cols, X, W, dx, dw, db, act);
         check_workspace(workspace, workspace_bytes, l.total());
-        OnDevice on(device);
+        Launches launches;
         char *ws = static_cast<char *>(workspace);
         const std::string t = kTypeName[X.dtype];
         OpsDzArgs a{};
@@ -908,14 +931,13 @@ int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         a.act = act;
         a.slope = slope;
         if ((a.dz || a.part) && !empty(DY))
-            launch(device, stream, (dz_cols ? "mxo_dz_rows_" : "mxo_dz_planar_") + t,
-                   dz_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, a);
-        if (db) join(device, stream, a.part, DY.rows ? l.parts : 0, DY.cols, db->data, nullptr, db->dtype);
+            launches.add((dz_cols ? "mxo_dz_rows_" : "mxo_dz_planar_") + t,
+                         dz_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, a);
+        if (db) join(launches, a.part, DY.rows ? l.parts : 0, DY.cols, db->data, nullptr, db->dtype);
         void *pw = ws + l.dz_bytes + l.part_bytes;
-        if (dx && !empty(*dx))
-            product(device, stream, product_dx(l, W, *dx), pw);
-        if (dw && !empty(*dw))
-            product(device, stream, product_dw(l, X, *dw), pw);
+        if (dx && !empty(*dx)) product(launches, product_dx(l, W, *dx), pw);
+        if (dw && !empty(*dw)) product(launches, product_dw(l, X, *dw), pw);
+        launches.run(device, stream);
     });
 }
 

@@ -102,3 +102,30 @@ def test_few_features_keep_the_card_busy(card, dtype):
     calls = [dense_calls(rows, k, n, dtype)[0] for rows in (1, 16) for k, n in ((64, 64), (1024, 64), (1024, 4096), (4096, 4096))]
     for c, r in zip(calls, card(calls)):
         assert [l["kernel"][:10] for l in r["launches"]] == ["mxo_skinny"], (r, c)
+
+
+def test_a_call_too_large_launches_nothing(card):
+    """A launch has at most 2^32 threads; a call with one that would not fit is
+    refused before any of its launches."""
+    at = [(i + 1) << 52 for i in range(8)]
+    calls = []
+    for dtype in (F32, BF16):
+        for planar in (False, True):
+            for rows, cols in ((2, 1 << 26), (40, 1 << 24), (3, (1 << 30) + 8), (1, 1 << 27), (1 << 30, 2)):
+                x, dy, dx = (F.mat(rows, cols, a, not planar, 8, dtype) for a in at[:3])
+                p = [F.vec(cols, a, dtype) for a in at[3:6]]
+                calls.append({"op": "layernorm", "x": x, "y": dx, "scale": p[0]})
+                calls.append({"op": "layernorm_backward", "dy": dy, "x": x, "dx": dx, "scale": p[0], "dscale": p[1],
+                              "dbias": p[2], "mean": at[6], "rstd": at[7]})
+            for rows, k, n in ((40, 16, 1 << 24), (8, 16, (1 << 27) + 5), (3, 1 << 27, 8), ((1 << 31) - 2000, 64, 64),
+                               (1 << 30, 16, 16), (2, 5, 1 << 30), (1 << 28, 33, 7)):
+                for act in (0, 1):
+                    calls += dense_calls(rows, k, n, dtype, planar, 3, act=act)
+    said = set()
+    for c, r in zip(calls, card(calls)):
+        assert r["rc"] == 0 or not r["launches"], (r, c)
+        assert all(l["gx"] * l["block"] < 1 << 32 for l in r["launches"])
+        if r["rc"]:
+            assert "one launch" in r["error"], r["error"]
+            said.add(c["op"])
+    assert said == {"layernorm_backward", "dense", "dense_backward"}
