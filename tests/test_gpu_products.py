@@ -10,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 from maxim_amd import ops as O  # noqa: E402
 from maxim_amd import plan as P  # noqa: E402
-from test_gpu_operators import TYPES, U, half, tiny  # noqa: E402
+from test_gpu_operators import TYPES, U, check_layernorm, check_ln_backward, half, tiny  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +193,50 @@ def test_what_out_overwrites_is_known_to_autograd():
             y.sum().backward()
         with torch.inference_mode():
             call(torch.randn(8, 16, device="cuda"))
+
+
+# sizes that, with x in another memory order than y and dy, reach the tiles that
+# matrices of one order do not (test_ops_launches.py holds that every kernel is
+# reached); rows, k, n
+MIXED_SHAPES = [(100, 40, 72), (4095, 1023, 2049), (2048, 512, 2048), (2048, 512, 4096), (256, 8192, 256), (40000, 64, 96),
+                (4287, 6971, 194), (24450, 783, 1028), (612, 2826, 4389), (2284, 633, 7599), (31971, 707, 209)]
+
+
+@pytest.mark.parametrize("planar", [False, True])
+@pytest.mark.parametrize("wt", [False, True])
+@pytest.mark.parametrize("dt", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("rows,k,n", MIXED_SHAPES)
+def test_products_of_mixed_orders(rows, k, n, dt, wt, planar):
+    """x in one memory order, y and dy in the other, into and out of buffers
+    of their own width and wider."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    for pad in (0, 3):
+        # the call's order is y's; x is a view of the other
+        x = rand(gen, *((rows, k + pad) if planar else (k, rows + pad)), dt)[:, :k if planar else rows].t()
+        dy = rand(gen, *((n, rows + pad) if planar else (rows, n + pad)), dt)[:, :rows if planar else n]
+        w = rand(gen, k, n, dt, 1 / math.sqrt(k)).t() if wt else rand(gen, n, k, dt, 1 / math.sqrt(k))
+        y = O.dense(x, w, planar=planar, out=torch.empty_like(dy))
+        assert y.stride() == dy.stride() or y.is_contiguous()
+        dx, dw, db = O.dense_backward(dy, x, w, planar=planar)
+        assert dx.shape == x.shape and dx.t().is_contiguous()
+        x64, d64, w64 = ((t.t() if planar else t).double().contiguous() for t in (x, dy, w.t() if planar else w))
+        for got, a, b, terms, what in ((y.t() if planar else y, x64, w64.t(), k, "y"), (dx.t() if planar else dx, d64, w64, n, "dx"),
+                                       (dw, d64.t(), x64, rows, "dw")):
+            close(got, a @ b, a.abs() @ b.abs(), terms, dt, (what, pad))
+        close(db, d64.sum(0), d64.abs().sum(0), rows, dt, "db")
+
+
+# planar channels past those that registers hold, positions
+LOOP_SHAPES = [(1, 1025), (7, 1025), (100, 1500), (1000, 2049), (64, 3000), (129, 5000)]
+
+
+@pytest.mark.parametrize("dt", TYPES.values(), ids=TYPES)
+@pytest.mark.parametrize("rows,cols", LOOP_SHAPES)
+def test_layernorm_of_many_planes(rows, cols, dt):
+    for pad in (0, 8, 3):
+        check_layernorm(rows, cols, dt, True, pad, dt if pad else torch.float32, seed=pad)
+        check_ln_backward(rows, cols, dt, True, pad, dt if pad else torch.float32, pad == 8, seed=pad)
+    x = torch.randn(cols, rows + 3, device="cuda").to(dt)[:, :rows]
+    s = torch.randn(cols, device="cuda").to(dt)
+    want = O.layernorm(x, s, planar=True)
+    assert torch.equal(O.layernorm(x, s, planar=True, out=x), want)

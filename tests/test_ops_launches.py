@@ -23,13 +23,14 @@ def card(tmp_path_factory):
 
 
 def dense_calls(rows, k, n, dtype, planar=False, pad=0, wt=False, act=0, x_planar=None):
-    """A Dense and its backward pass over [rows][k] -> [rows][n]."""
+    """A Dense and its backward pass over [rows][k] -> [rows][n], as the Python
+    binding makes them: y in dy's order, dx in x's, dw in w's."""
     xp = planar if x_planar is None else x_planar
     at = [(i + 1) << 52 for i in range(8)]
     x = F.mat(rows, k, at[0], not xp, pad, dtype)
     w = F.mat(n, k, at[1], not wt, 0, dtype)
     y, dy, z = (F.mat(rows, n, a, not planar, p, dtype) for a, p in ((at[2], 0), (at[3], pad), (at[4], pad)))
-    dx, dw = F.mat(rows, k, at[5], not planar, 0, dtype), F.mat(n, k, at[6], not wt, 0, dtype)
+    dx, dw = F.mat(rows, k, at[5], not xp, 0, dtype), F.mat(n, k, at[6], not wt, 0, dtype)
     return [{"op": "dense", "x": x, "w": w, "y": y, "bias": F.vec(n, at[7], dtype), "act": act},
             {"op": "dense_backward", "dy": dy, "x": x, "w": w, "z": z if act else None, "act": act, "dx": dx, "dw": dw,
              "db": F.vec(n, at[7], dtype)}]
@@ -129,3 +130,46 @@ def test_a_call_too_large_launches_nothing(card):
             assert "one launch" in r["error"], r["error"]
             said.add(c["op"])
     assert said == {"layernorm_backward", "dense", "dense_backward"}
+
+
+def layernorm_calls(rows, cols, dtype, planar, pad, add=None):
+    at = [(i + 1) << 52 for i in range(9)]
+    x, dy, a = (F.mat(rows, cols, v, not planar, pad, dtype) for v in at[:3])
+    y, dx = (F.mat(rows, cols, v, not planar, 0, dtype) for v in at[3:5])
+    p = [F.vec(cols, v, dtype) for v in at[5:8]]
+    return [{"op": "layernorm", "x": x, "y": y, "scale": p[0]},
+            {"op": "layernorm_backward", "dy": dy, "x": x, "add": a if add else None, "dx": dx, "scale": p[0],
+             "dscale": p[1], "dbias": p[2], "mean": at[8], "rstd": at[8] + (1 << 40)}]
+
+
+def test_the_device_tests_reach_every_kernel(card):
+    """Each kernel that the host can choose is one that a test on the device
+    runs, by the shapes, orders and paddings that those tests take."""
+    import test_gpu_operators as G
+    import test_gpu_products as H
+    from test_ops_kernels import chosen
+    calls = []
+    for dtype in (F32, F16, BF16):
+        for planar in (False, True):
+            for s in G.DENSE_SHAPES:
+                for pad, wt in ((0, False), (8, True), (3, False), (0, True)):
+                    calls += dense_calls(*s, dtype, planar, pad, wt, act=1)
+            for s in G.BIG_SHAPES:
+                for wt in (False, True):
+                    calls += dense_calls(*s, dtype, planar, 0, wt)
+            for s in H.MIXED_SHAPES:
+                for wt in (False, True):
+                    for pad in (0, 3):
+                        calls += dense_calls(*s, dtype, planar, pad, wt, x_planar=not planar)
+            for s in G.LN_SHAPES:
+                for pad in (0, 8, 3):
+                    calls += layernorm_calls(*(s[::-1] if planar else s), dtype, planar, pad)
+            for s in G.MANY if planar else G.MANY_ROWS:
+                calls += layernorm_calls(*s, dtype, planar, 0)
+            for s in H.LOOP_SHAPES:
+                calls += layernorm_calls(*s, dtype, planar, 0)
+    reached = set()
+    for c, r in zip(calls, card(calls)):
+        assert r["rc"] == 0, (r["error"], c)
+        reached |= {l["kernel"] for l in r["launches"]}
+    assert reached == chosen(), sorted(chosen() - reached)
