@@ -62,9 +62,7 @@ struct OpsLnBwdArgs {
     int64_t rows, cols;
     int64_t dyrs, dycs, xrs, xcs, ars, acs, dxrs, dxcs;
     int32_t nparts, param_f32;
-    int32_t want, pad;  // MXO_WANT_*
 };
-enum { MXO_WANT_DX = 1, MXO_WANT_PARAMS = 2 };
 
 // dz = dy act'(z), and the partial sums of dz over the rows.
 struct OpsDzArgs {
