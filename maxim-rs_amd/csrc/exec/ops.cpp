@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <array>
 #include <cstring>
+#include <iterator>
 #include <limits>
 #include <map>
 #include <mutex>
@@ -447,19 +448,23 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, con
             best.kchunk = each * bk;
         }
     };
-    if (type_size(dtype) == 2)
-        for (const TileCost &t : kTiles16) consider(t);
-    else
-        for (const TileCost &t : kTiles32) consider(t);
+    const bool half = type_size(dtype) == 2;
+    const TileCost *const tiles = half ? kTiles16 : kTiles32, *const end = half ? std::end(kTiles16) : std::end(kTiles32);
+    Plan skinny;
+    skinny.skinny = true;
+    skinny.block = 512;
+    double few = std::numeric_limits<double>::infinity();
     if (a.by_k && b.by_k && m <= 16) {
-        const double few = 4.0 + (0.065 + 0.0025 * m) * steps * std::max(1.0, cdiv(n, 16) / 256.0);
-        if (few <= std::max(least, (double)n * k * type_size(dtype) / 4.9e6)) {
-            best = Plan();
-            best.skinny = true;
-            best.block = 512;
-            return best;
-        }
+        few = 4.0 + (0.065 + 0.0025 * m) * steps * std::max(1.0, cdiv(n, 16) / 256.0);
+        // what the tiles take at least, uncut or cut, without trying each cut:
+        // a token's call need not wait for that
+        double bound = least;
+        for (const TileCost *t = tiles; t != end; ++t) bound = std::min(bound, t->rest + std::min(steps * t->one, 2 * t->one + 5.0));
+        const double bytes = (double)n * k * type_size(dtype) / 4.9e6;
+        if (few <= std::max(bound, bytes)) return skinny;
     }
+    for (const TileCost *t = tiles; t != end; ++t) consider(*t);
+    if (few <= least) return skinny;
     best.bytes = best.pack_bytes + (best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0);
     return best;
 }
