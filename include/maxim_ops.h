@@ -3,20 +3,21 @@
  * and backward, as hand-written gfx950 kernels.
  *
  * The executor (maxim_hip.h) runs one inference plan over its own fp32 arena.
- * These calls are for the programs beside it: fine-tuning a MAXIM checkpoint
- * (whose blocks are LayerNorm, Dense, GELU, Dense, residual), or training and
- * serving token models, in fp32, fp16 or bf16. No counterpart in the
- * reference, which has no gradients and no 16-bit types.
+ * These calls are for the programs beside it: training and serving token models,
+ * or tuning the LayerNorm and Dense layers of a MAXIM checkpoint's blocks (the
+ * gradients of its convolutions, gates and resizing are the program's own), in
+ * fp32, fp16 or bf16. No counterpart in the reference, which has no gradients
+ * and no 16-bit types.
  *
  * Matrices are views: rows are positions (pixels or tokens), columns features,
  * `row_stride` and `col_stride` elements apart, one of the two 1. So the
  * executor's planar [c][h][w] order is (row_stride 1, col_stride h * w) and a
  * token-major [n][c] array (row_stride c, col_stride 1); slices of wider
  * buffers and broadcast inputs (a stride of 0) need no copy. Any alignment of
- * the element, any sizes whose launches have fewer than 2^32 threads each
- * (others, of 2^24 features and more, are refused). An output's own elements
- * must not share storage, and an output must not overlap any other operand, but
- * where a call says so.
+ * the element, any sizes whose launches have fewer than 2^32 threads each (a
+ * call with a larger one is refused: some of 2^24 features or 2^27 positions and
+ * more). An output's own elements must not share storage, and an output must
+ * not overlap any other operand, but where a call says so.
  *
  * Sums, means and variances are fp32; a result is rounded once, to nearest
  * even, when it is stored. fp32 products are formed on the bf16 matrix cores
@@ -114,8 +115,8 @@ int mxh_dense_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, ui
  * dz = dy * act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz (the
  * residual's gradient is dy itself). Any of dx, dw and db may be NULL. z is
  * the forward pass's, of dy's order; NULL when act is MXH_NONE. The products
- * take dz rounded to x's type, db sums it before the rounding. db is of x's
- * type or fp32.
+ * take dz rounded to x's type (in fp16 a dz past 65504 is infinite), db sums it
+ * before the rounding. db is of x's type or fp32.
  */
 int mxh_dense_backward(int device, void *stream, const mxh_mat *dy, const mxh_mat *x, const mxh_mat *w,
                        const mxh_mat *z, int act, float slope, const mxh_mat *dx, const mxh_mat *dw,

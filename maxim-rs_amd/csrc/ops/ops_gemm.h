@@ -7,7 +7,8 @@
 // along its other axis, so no product of a forward or backward pass needs a
 // transposed copy: a 16-bit operand that is not contiguous along k is
 // transposed by ds_read_b64_tr_b16 on its way out of LDS, and an fp32 one is
-// read element by element, which its 16 times slower MFMA hides.
+// read element by element, beside the splitting of what has been read and six
+// matrix instructions where 16 bits take one.
 //
 // The MFMA takes B's rows as its own A operand, so that a lane ends up with
 // four consecutive n of one m and C is written four elements at a time.
@@ -149,8 +150,8 @@ struct Tile {
 // (common.h has the method, its precision and its range), or, exactly as fp32
 // products go, fp32 MFMAs. The six take 96 cycles of a SIMD where the fp32
 // ones take 256. The splitting, 4.5 vector operations an element, runs beside
-// the products of another wave: 4096^3 takes 766 us (179 TFLOP/s; in fp32
-// 970), and putting each row's splitting between the row before's products
+// the products of another wave: 4096^3 takes 722-814 us (169-190 TFLOP/s, the
+// library's fp32 product 139-151; with fp32 MFMAs here 970), and putting each row's splitting between the row before's products
 // made it 785, shifts and subtractions for the dot products changed nothing.
 struct Split {
     u32x4 h, m, l;

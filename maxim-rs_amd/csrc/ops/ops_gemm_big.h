@@ -2,12 +2,12 @@
 // to LDS.
 //
 // Bound by the matrix cores where there are tiles enough, at the clock their
-// power leaves: bf16 8192^3 in 840-910 us (1.2-1.3 PFLOP/s; the library's
-// product 1.36), 4096^3 in 113 us. 8192 x 2048 x 8192 with 134 MB of results
-// 262 us, with gelu 269, with the 134 MB of z as well 290: a 256 x 256 tile
-// fills a CU's LDS, so its results are written before its CU's next tile is
-// begun. Two smaller tiles a CU hide that, and lose more in products an LDS
-// byte read.
+// power leaves: bf16 8192^3 in 820-910 us (1.2-1.3 PFLOP/s; the library's
+// product 680-810), 4096^3 in 108-125 us (89-100). 8192 x 2048 x 8192 with 134
+// MB of results 262 us, with gelu 269, with the 134 MB of z as well 290: a
+// 256 x 256 tile takes 128 KiB of a CU's 160 KiB of LDS, so no second one fits
+// beside it and its results are written before its CU's next tile is begun. Two
+// smaller tiles a CU hide that, and lose more in products an LDS byte read.
 #pragma once
 
 #include "ops_gemm.h"

@@ -6,9 +6,10 @@
 // memory into the matrix cores' operand registers, eight loads ahead of their
 // use, and the rows of A likewise from the caches. The waves' sums are added
 // in LDS, so no partial sums go through memory and there is one launch.
-// (4096 x 4096 bf16 weights: 8.7 us for one row, 3.9 TB/s, 10.5 us for 16; as
-// 64 x 64 tiles cut in eight and joined 12 + 4 us. With two blocks of rows a
-// wave 17 rows took 14.7 us, the tiles 12.1.)
+// (4096 x 4096 bf16 weights: 9.0 us for one row, 3.7 TB/s, 10.6 us for 16; as
+// 64 x 64 tiles, cut and joined, 11.6 and 11.4. With two blocks of rows a wave
+// 17 rows took 14.7 us, the tiles 12.1.) Where k is long and the columns few
+// the card stands idle: plan_product (exec/ops.cpp) has the rule, and both sides.
 #pragma once
 
 #include "ops_gemm.h"
