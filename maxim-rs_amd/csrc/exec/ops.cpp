@@ -454,7 +454,7 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, con
     skinny.skinny = true;
     skinny.block = 512;
     double few = std::numeric_limits<double>::infinity();
-    if (a.by_k && b.by_k && m <= 16) {
+    if (a.by_k && b.by_k && m <= 16 && cdiv(n, 16) <= UINT32_MAX / skinny.block) {
         few = 4.0 + (0.065 + 0.0025 * m) * steps * std::max(1.0, cdiv(n, 16) / 256.0);
         // what the tiles take at least, uncut or cut, without trying each cut:
         // a token's call need not wait for that

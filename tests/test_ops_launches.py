@@ -173,3 +173,13 @@ def test_the_device_tests_reach_every_kernel(card):
         assert r["rc"] == 0, (r["error"], c)
         reached |= {l["kernel"] for l in r["launches"]}
     assert reached == chosen(), sorted(chosen() - reached)
+
+
+def test_few_rows_and_very_many_columns(card):
+    """More columns than the few-rows kernel's grid holds are the tiles'."""
+    calls = []
+    for n in ((1 << 27) - 16, (1 << 27) - 15, (1 << 27) + 5, (1 << 29) + 1):
+        for dtype in (F32, BF16):
+            calls.append(dense_calls(8, 16, n, dtype)[0])
+    for c, r in zip(calls, card(calls)):
+        check_products(c, r)
