@@ -1,0 +1,185 @@
+// The gated Dense's host side (include/maxim_block_ops.h): argument checks and the
+// launches. Forward it is a product of ops.cpp with pairs of lines, backward a
+// pass that forms dz and a Dense's two products.
+
+#include "maxim_block_ops.h"
+#include "ops_host.hpp"
+
+namespace mxops {
+
+// x, y and z in the results' order, the weights either way. An axis of one
+// element has no stride of its own: the order that the call has is said.
+static Product gated_product(const mxh_mat &x, const mxh_mat &w, const mxh_mat &y, bool by_cols) {
+    Product p;
+    p.dtype = y.dtype;
+    p.k = x.cols;
+    p.c = y.data;
+    const Operand weights = along_cols(w) ? Operand{w.data, w.row_stride, 1, false, 'k'}
+                                          : Operand{w.data, 1, w.col_stride, false, 'm'};
+    if (by_cols) {
+        p.pair = Pair::kN;
+        p.m = y.rows, p.n = y.cols, p.ldc = y.row_stride;
+        p.a = Operand{x.data, x.row_stride, 1, false, 'k'};
+        p.b = weights;
+    } else {
+        p.pair = Pair::kM;
+        p.m = y.cols, p.n = y.rows, p.ldc = y.col_stride;
+        p.a = weights;
+        p.b = Operand{x.data, 1, x.col_stride, false, 'm'};
+    }
+    return p;
+}
+
+static int64_t halves(const mxh_mat &w) {
+    if (w.rows % 2) throw Error("w: " + std::to_string(w.rows) + " rows are no gate's and as many values'");
+    return w.rows / 2;
+}
+
+static mxh_mat like(const mxh_mat &m, int64_t cols) {
+    mxh_mat r = m;
+    r.cols = cols;
+    return r;
+}
+
+static BwdLayout gated_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mxh_mat &w, const mxh_mat *dx,
+                              const mxh_mat *dw, const mxh_vec *db) {
+    BwdLayout l;
+    l.dz = like(dy, 2 * dy.cols);
+    if (dx || dw) place_dz(l, dy, 2 * dy.cols, by_cols);
+    if (db) {
+        l.parts = dz_parts(dy, by_cols);
+        l.part_bytes = up((uint64_t)l.parts * 2 * dy.cols * 4);
+    }
+    if (dx && !empty(*dx)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dx(l, w, *dx)).bytes);
+    if (dw && !empty(*dw)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dw(l, x, *dw)).bytes);
+    return l;
+}
+
+}  // namespace mxops
+
+using namespace mxops;
+
+extern "C" {
+
+int mxh_gated_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) throw Error("bytes: missing");
+        check_first(need(x, "x"), "x");
+        check_mat(need(w, "w"), "w", x->dtype, w->rows, x->cols);
+        check_mat(need(y, "y"), "y", x->dtype, x->rows, halves(*w));
+        // operands of one row or column have both orders, and z may settle it
+        *bytes = 0;
+        if (empty(*y)) return;
+        if (along_cols(*x) && out_by_cols(*y)) *bytes = plan_of(gated_product(*x, *w, *y, true)).bytes;
+        if (along_rows(*x) && out_by_rows(*y)) *bytes = std::max(*bytes, plan_of(gated_product(*x, *w, *y, false)).bytes);
+    });
+}
+
+int mxh_gated(int device, void *stream, const mxh_mat *x, const mxh_mat *w, const mxh_vec *bias, int act, float slope,
+              const mxh_mat *y, const mxh_mat *z, void *workspace, uint64_t workspace_bytes) {
+    return guard([&] {
+        const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &Y = need(y, "y");
+        check_first(X, "x");
+        check_mat(W, "w", X.dtype, W.rows, X.cols);
+        check_mat(Y, "y", X.dtype, X.rows, halves(W));
+        check_out(Y, "y");
+        check_act(act);
+        if (bias) check_vec(*bias, "bias", W.rows, X.dtype);
+        if (z) {
+            check_mat(*z, "z", X.dtype, X.rows, W.rows);
+            check_out(*z, "z");
+        }
+        const bool by_cols = common_order({x}, {y, z});
+        for (const mxh_mat *o : {y, z}) {
+            if (!o) continue;
+            refuse_overlap(*o, "an output", X, "x");
+            refuse_overlap(*o, "an output", W, "w");
+            if (bias) refuse_overlap(*o, "an output", line(*bias), "bias");
+        }
+        if (z) refuse_overlap(Y, "y", *z, "z");
+        if (empty(Y)) return;
+        Product p = gated_product(X, W, Y, by_cols);
+        check_workspace(workspace, workspace_bytes, plan_of(p).bytes);
+        p.bias = bias;
+        p.bias_rows = !by_cols;
+        p.act = act;
+        p.slope = slope;
+        if (z) p.z = z->data, p.ldz = by_cols ? z->row_stride : z->col_stride;
+        Launches launches;
+        product(launches, p, workspace);
+        launches.run(device, stream);
+    });
+}
+
+int mxh_gated_backward_workspace(const mxh_mat *dy, const mxh_mat *x, const mxh_mat *w, const mxh_mat *dx,
+                                 const mxh_mat *dw, const mxh_vec *db, uint64_t *bytes) {
+    return guard([&] {
+        if (!bytes) throw Error("bytes: missing");
+        check_first(need(x, "x"), "x");
+        check_mat(need(w, "w"), "w", x->dtype, w->rows, x->cols);
+        check_mat(need(dy, "dy"), "dy", x->dtype, x->rows, halves(*w));
+        if (dx) check_mat(*dx, "dx", x->dtype, x->rows, x->cols);
+        if (dw) check_mat(*dw, "dw", x->dtype, w->rows, w->cols);
+        *bytes = std::max(gated_layout(*dy, true, *x, *w, dx, dw, db).total(),
+                          gated_layout(*dy, false, *x, *w, dx, dw, db).total());
+    });
+}
+
+int mxh_gated_backward(int device, void *stream, const mxh_mat *dy, const mxh_mat *x, const mxh_mat *w,
+                       const mxh_mat *z, int act, float slope, const mxh_mat *dx, const mxh_mat *dw,
+                       const mxh_vec *db, void *workspace, uint64_t workspace_bytes) {
+    return guard([&] {
+        const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &DY = need(dy, "dy"), &Z = need(z, "z");
+        check_first(X, "x");
+        check_mat(W, "w", X.dtype, W.rows, X.cols);
+        check_mat(DY, "dy", X.dtype, X.rows, halves(W));
+        check_mat(Z, "z", X.dtype, X.rows, W.rows);
+        check_act(act);
+        if (dx) {
+            check_mat(*dx, "dx", X.dtype, X.rows, X.cols);
+            check_out(*dx, "dx");
+        }
+        if (dw) {
+            check_mat(*dw, "dw", X.dtype, W.rows, W.cols);
+            check_out(*dw, "dw");
+        }
+        if (db) check_vec(*db, "db", W.rows, X.dtype);
+        const bool by_cols = common_order({dy, z}, {});
+        const mxh_mat dbl = db ? line(*db) : mxh_mat{};
+        const mxh_mat *outs[] = {dx, dw, db ? &dbl : nullptr}, *ins[] = {dy, x, w, z};
+        const char *on_[] = {"dx", "dw", "db"}, *in_[] = {"dy", "x", "w", "z"};
+        for (int i = 0; i < 3; ++i) {
+            if (!outs[i]) continue;
+            for (int j = 0; j < 4; ++j) refuse_overlap(*outs[i], on_[i], *ins[j], in_[j]);
+            for (int j = 0; j < i; ++j)
+                if (outs[j]) refuse_overlap(*outs[i], on_[i], *outs[j], on_[j]);
+        }
+        BwdLayout l = gated_layout(DY, by_cols, X, W, dx, dw, db);
+        check_workspace(workspace, workspace_bytes, l.total());
+        Launches launches;
+        char *ws = static_cast<char *>(workspace);
+        const std::string t = kTypeName[X.dtype];
+        OpsDzArgs a{};
+        a.dy = DY.data;
+        a.z = Z.data;
+        a.rows = DY.rows;
+        a.cols = DY.cols;
+        a.dyrs = DY.row_stride, a.dycs = DY.col_stride;
+        a.zrs = Z.row_stride, a.zcs = Z.col_stride;
+        if (l.dz_bytes) l.dz.data = a.dz = ws, a.drs = l.dz.row_stride, a.dcs = l.dz.col_stride;
+        if (db) a.part = reinterpret_cast<float *>(ws + l.dz_bytes);
+        a.nparts = (int32_t)dz_parts(DY, by_cols);
+        a.act = act;
+        a.slope = slope;
+        if ((a.dz || a.part) && !empty(DY))
+            launches.add((by_cols ? "mxg_dz_rows_" : "mxg_dz_planar_") + t,
+                         by_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, a);
+        if (db) join(launches, a.part, DY.rows ? l.parts : 0, W.rows, db->data, nullptr, db->dtype);
+        void *pw = ws + l.dz_bytes + l.part_bytes;
+        if (dx && !empty(*dx)) product(launches, product_dx(l, W, *dx), pw);
+        if (dw && !empty(*dw)) product(launches, product_dw(l, X, *dw), pw);
+        launches.run(device, stream);
+    });
+}
+
+}  // extern "C"

@@ -1,241 +1,58 @@
-// The training and serving operators' host side (include/maxim_ops.h):
-// argument checks, the choice of kernel and split, and the launches. The
-// kernels are a code object of their own (csrc/ops), loaded per device by the
-// first call.
+// The training and serving operators' host side (include/maxim_ops.h): the
+// kernels' loading, LayerNorm and Dense: argument checks, the choice of kernel
+// and split, and the launches. The kernels are code objects of their own
+// (csrc/ops), loaded per device by the first call.
 
-#include "maxim_ops.h"
+#include "ops_host.hpp"
 
-#include <algorithm>
-#include <array>
-#include <cstring>
-#include <iterator>
-#include <limits>
 #include <map>
 #include <mutex>
-#include <string>
 #include <vector>
 
-#include "../ops/ops_args.h"
-#include "hip_api.hpp"
-#include "host.hpp"
+extern "C" const unsigned char mx_ops_hsaco[], mx_gated_hsaco[];
 
-extern "C" const unsigned char mx_ops_hsaco[];
+namespace mxops {
 
-namespace {
-
-using mx::Error;
-using mxh::check;
-using mxh::hip;
-
-constexpr int kMaxDevices = 64;
-constexpr int64_t kMaxExtent = std::numeric_limits<int32_t>::max() - 1024;
-
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// ------------------------------------------------------------ the kernels
+// The code objects, by their kernels' prefix.
+struct Object {
+    char prefix[5];
+    const unsigned char *image;
+    const char *what;
+};
+const Object kObjects[] = {{"mxo_", mx_ops_hsaco, "hipModuleLoadData (operators' gfx950 code object)"},
+                           {"mxg_", mx_gated_hsaco, "hipModuleLoadData (gated operators' gfx950 code object)"}};
+constexpr int kNumObjects = sizeof(kObjects) / sizeof(kObjects[0]);
 
 struct Code {
-    mxh::hipModule_t mod = nullptr;
+    mxh::hipModule_t mod[kNumObjects] = {};
     std::map<std::string, mxh::hipFunction_t> fns;
 };
 
 std::mutex g_mu;
 Code g_code[kMaxDevices];
 
-// The calling thread's current device, put back on the way out.
-struct OnDevice {
-    int before = -1;
-    explicit OnDevice(int dev) {
-        if (dev < 0 || dev >= kMaxDevices) throw Error("device ordinal out of range");
-        int now = -1;
-        check(hip().hipGetDevice(&now), "hipGetDevice");
-        if (now != dev) {
-            check(hip().hipSetDevice(dev), "hipSetDevice");
-            before = now;
-        }
-    }
-    ~OnDevice() {
-        if (before >= 0) hip().hipSetDevice(before);
-    }
-    OnDevice(const OnDevice &) = delete;
-    OnDevice &operator=(const OnDevice &) = delete;
-};
+mxh::hipModule_t module(Code &c, int i) {
+    if (!c.mod[i]) check(hip().hipModuleLoadData(&c.mod[i], kObjects[i].image), kObjects[i].what);
+    return c.mod[i];
+}
 
 mxh::hipFunction_t function(int dev, const std::string &name) {
-    auto &H = hip();
     std::lock_guard<std::mutex> lock(g_mu);
     Code &c = g_code[dev];
-    if (!c.mod) check(H.hipModuleLoadData(&c.mod, mx_ops_hsaco), "hipModuleLoadData (operators' gfx950 code object)");
     auto it = c.fns.find(name);
     if (it != c.fns.end()) return it->second;
+    int i = 0;
+    while (i < kNumObjects && name.compare(0, 4, kObjects[i].prefix)) ++i;
+    if (i == kNumObjects) throw Error(name + ": in no code object");
     mxh::hipFunction_t f = nullptr;
-    check(H.hipModuleGetFunction(&f, c.mod, name.c_str()), ("hipModuleGetFunction " + name).c_str());
+    check(hip().hipModuleGetFunction(&f, module(c, i), name.c_str()), ("hipModuleGetFunction " + name).c_str());
     c.fns[name] = f;
     return f;
 }
 
-// A call's launches, of which none is made before all are known to fit: the
-// threads of a launch are counted in 32 bits.
-class Launches {
-    struct One {
-        std::string name;
-        unsigned gx, gy, block;
-        alignas(8) char args[192];
-    };
-    One at_[8];  // a Dense's backward pass: dz and its join, twice packing, product and join
-    int n_ = 0;
-
-public:
-    template <typename A>
-    void add(const std::string &name, int64_t gx, int64_t gy, unsigned block, const A &args) {
-        static_assert(sizeof(A) <= sizeof(One::args), "");
-        if (gx > (int64_t)UINT32_MAX / block || gy > 65535)
-            throw Error("the operands are too large: " + name + " would take more threads than one launch can have");
-        One &o = at_[n_++];
-        o.name = name;
-        o.gx = (unsigned)gx, o.gy = (unsigned)gy, o.block = block;
-        std::memcpy(o.args, &args, sizeof(A));
-    }
-    void run(int dev, void *stream) {
-        OnDevice on(dev);
-        mxh::hipFunction_t f[8];
-        for (int i = 0; i < n_; ++i) f[i] = function(dev, at_[i].name);
-        for (int i = 0; i < n_; ++i) {
-            One &o = at_[i];
-            void *params[] = {o.args};
-            check(hip().hipModuleLaunchKernel(f[i], o.gx, o.gy, 1, o.block, 1, 1, 0, (mxh::hipStream_t)stream, params,
-                                              nullptr),
-                  o.name.c_str());
-        }
-    }
-};
-
-// ------------------------------------------------------------- operands
-
-const char *kTypeName[] = {"f32", "f16", "bf16"};
-size_t type_size(int t) { return t == MXH_F32 ? 4 : 2; }
-
-std::string shape(const mxh_mat &m) { return "[" + std::to_string(m.rows) + "][" + std::to_string(m.cols) + "]"; }
-
-bool empty(const mxh_mat &m) { return m.rows == 0 || m.cols == 0; }
-// Contiguous along columns (features), or along rows (positions).
-bool along_cols(const mxh_mat &m) { return m.col_stride == 1 || m.cols <= 1; }
-bool along_rows(const mxh_mat &m) { return m.row_stride == 1 || m.rows <= 1; }
-
-const mxh_mat &need(const mxh_mat *m, const char *what) {
-    if (!m) throw Error(std::string(what) + ": missing");
-    return *m;
-}
-
-void check_mat(const mxh_mat &m, const char *what, int dtype, int64_t rows, int64_t cols) {
-    const std::string w = what;
-    if (m.dtype < MXH_F32 || m.dtype > MXH_BF16) throw Error(w + ": unknown type " + std::to_string(m.dtype));
-    if (m.dtype != dtype) throw Error(w + ": " + kTypeName[m.dtype] + " where x is " + kTypeName[dtype]);
-    if (m.rows != rows || m.cols != cols)
-        throw Error(w + ": " + shape(m) + ", expected [" + std::to_string(rows) + "][" + std::to_string(cols) + "]");
-    if (m.rows < 0 || m.cols < 0 || m.rows > kMaxExtent || m.cols > kMaxExtent)
-        throw Error(w + ": " + shape(m) + " is out of range");
-    if (m.row_stride < 0 || m.col_stride < 0) throw Error(w + ": a negative stride");
-    if (empty(m)) return;
-    if (!m.data) throw Error(w + ": no data");
-    if (!along_cols(m) && !along_rows(m))
-        throw Error(w + ": neither rows nor columns are contiguous (strides " + std::to_string(m.row_stride) + ", " +
-                    std::to_string(m.col_stride) + ")");
-    if ((uintptr_t)m.data % type_size(m.dtype)) throw Error(w + ": not aligned to its element");
-    // the farthest element's offset in bytes has to be a number
-    const __int128 far = ((__int128)(m.rows - 1) * m.row_stride + (__int128)(m.cols - 1) * m.col_stride) * 4;
-    if (far > std::numeric_limits<int64_t>::max() / 2) throw Error(w + ": strides out of range");
-}
-
-void check_first(const mxh_mat &x, const char *what) { check_mat(x, what, x.dtype, x.rows, x.cols); }
-
-void check_vec(const mxh_vec &v, const char *what, int64_t n, int dtype) {
-    const std::string w = what;
-    if (v.n != n) throw Error(w + ": " + std::to_string(v.n) + " elements, expected " + std::to_string(n));
-    if (v.dtype != MXH_F32 && v.dtype != dtype) throw Error(w + ": its type is neither fp32 nor x's");
-    if (n && !v.data) throw Error(w + ": no data");
-    if ((uintptr_t)v.data % type_size(v.dtype)) throw Error(w + ": not aligned to its element");
-}
-
-// The memory order that all of a call's matrices have: true, features
-// contiguous; false, positions. (One of a single row or column has both.)
-bool out_by_cols(const mxh_mat &m) { return along_cols(m) && (m.rows <= 1 || m.row_stride >= m.cols); }
-bool out_by_rows(const mxh_mat &m) { return along_rows(m) && (m.cols <= 1 || m.col_stride >= m.rows); }
-bool common_order(std::initializer_list<const mxh_mat *> ins, std::initializer_list<const mxh_mat *> outs) {
-    bool cols = true, rows = true;
-    for (const mxh_mat *m : ins)
-        if (m && !empty(*m)) cols = cols && along_cols(*m), rows = rows && along_rows(*m);
-    for (const mxh_mat *m : outs)
-        if (m && !empty(*m)) cols = cols && out_by_cols(*m), rows = rows && out_by_rows(*m);
-    if (!cols && !rows) throw Error("the matrices differ in memory order");
-    return cols;
-}
-
-// Elements of an output may not share storage.
-void check_out(const mxh_mat &m, const char *what) {
-    if (empty(m)) return;
-    if (!out_by_cols(m) && !out_by_rows(m)) throw Error(std::string(what) + ": elements of an output share storage");
-}
-
-struct Range {
-    uintptr_t lo, hi;
-};
-Range range(const mxh_mat &m) {
-    const uintptr_t p = (uintptr_t)m.data;
-    const uint64_t far = (uint64_t)(m.rows - 1) * m.row_stride + (uint64_t)(m.cols - 1) * m.col_stride + 1;
-    return {p, p + far * type_size(m.dtype)};
-}
-bool apart(Range a, Range b) { return a.hi <= b.lo || b.hi <= a.lo; }
-
-// Whether two views share an element: by their ranges, and where these cross
-// and the strides agree (slices of one buffer), by their offset in it.
-bool overlap(const mxh_mat &a, const mxh_mat &b) {
-    if (empty(a) || empty(b) || apart(range(a), range(b))) return false;
-    if (a.dtype != b.dtype) return true;
-    int64_t ld, inner_a, inner_b, outer_a, outer_b;
-    if (along_cols(a) && along_cols(b) && a.row_stride == b.row_stride) {
-        ld = a.row_stride, inner_a = a.cols, inner_b = b.cols, outer_a = a.rows, outer_b = b.rows;
-    } else if (along_rows(a) && along_rows(b) && a.col_stride == b.col_stride) {
-        ld = a.col_stride, inner_a = a.rows, inner_b = b.rows, outer_a = a.cols, outer_b = b.cols;
-    } else {
-        return true;
-    }
-    const int64_t size = (int64_t)type_size(a.dtype);
-    const int64_t bytes = (int64_t)((uintptr_t)b.data - (uintptr_t)a.data);
-    if (bytes % size) return true;
-    if (ld < std::max(inner_a, inner_b)) return true;
-    // b begins q whole lines and r elements past a, 0 <= r < ld: its lines
-    // begin on a's q lines on, or (r + inner_b > ld) run into the next ones
-    int64_t d = bytes / size, q = d / ld, r = d % ld;
-    if (r < 0) r += ld, --q;
-    auto lines = [&](int64_t off) { return off < outer_a && -off < outer_b; };
-    return (r < inner_a && lines(q)) || (r + inner_b > ld && lines(q + 1));
-}
-
-bool same(const mxh_mat &a, const mxh_mat &b) {
-    return a.data == b.data && (a.rows <= 1 || a.row_stride == b.row_stride) &&
-           (a.cols <= 1 || a.col_stride == b.col_stride) && a.rows == b.rows && a.cols == b.cols && a.dtype == b.dtype;
-}
-
-mxh_mat line(const void *p, int64_t n, int dtype) {
-    return mxh_mat{const_cast<void *>(p), 1, n, n, 1, dtype, 0};
-}
-mxh_mat line(const mxh_vec &v) { return line(v.data, v.n, v.dtype); }
-
-void refuse_overlap(const mxh_mat &out, const char *a, const mxh_mat &in, const char *b) {
-    if (overlap(out, in)) throw Error(std::string(a) + " overlaps " + b);
-}
-
-void check_workspace(const void *ws, uint64_t have, uint64_t want) {
-    if (!want) return;
-    if (!ws) throw Error("the call needs " + std::to_string(want) + " bytes of workspace");
-    if (have < want)
-        throw Error("the call needs " + std::to_string(want) + " bytes of workspace, not " + std::to_string(have));
-    if ((uintptr_t)ws % 16) throw Error("workspace: not aligned to 16 bytes");
-}
-
-void check_act(int act) {
-    if (act < MXH_NONE || act > MXH_SIGMOID) throw Error("unknown activation " + std::to_string(act));
+void load_all(int dev) {
+    std::lock_guard<std::mutex> lock(g_mu);
+    for (int i = 0; i < kNumObjects; ++i) module(g_code[dev], i);
 }
 
 // ------------------------------------------------------------- LayerNorm
@@ -333,41 +150,6 @@ void join(Launches &launches, const float *part, int64_t nparts, int64_t n, void
 
 // ------------------------------------------------------------- products
 
-// One operand of a product: elements apart along its own axis and along the
-// summed one.
-struct Operand {
-    const void *data;
-    int64_t own, sum;
-    bool padded;  // lines hold zeros up to whole 16 bytes
-};
-
-struct Product {
-    int dtype = 0;
-    int64_t m = 0, n = 0, k = 0;
-    Operand a{}, b{};
-    void *c = nullptr;
-    int64_t ldc = 0;
-    const mxh_vec *bias = nullptr;
-    bool bias_rows = false;
-    const void *res = nullptr;
-    int64_t ldr = 0;
-    void *z = nullptr;
-    int64_t ldz = 0;
-    int act = MXH_NONE;
-    float slope = 0.0f;
-};
-
-struct Plan {
-    bool skinny = false;  // the kernel of few rows
-    int bm = 0, bn = 0;
-    unsigned block = 256;
-    int stages = 0;  // straight to LDS with so many tiles there; 0: through registers
-    bool pack_a = false, pack_b = false;  // copied to aligned lines first
-    uint64_t pack_bytes = 0;
-    int64_t splits = 1, kchunk = 0;
-    uint64_t bytes = 0;
-};
-
 // How an operand's lines reach the tiles that go straight to LDS: as they lie,
 // or copied (`pack` bytes); `ld` elements from line to line there.
 struct Side {
@@ -420,25 +202,31 @@ const TileCost kTiles32[] = {{128, 2, 2, 1.65, 2.95, 8.0}, {64, 4, 2, 0.65, 1.1,
 // aligned lines first (4 us and its bytes twice), which is one more choice:
 // 1237 x 1001 x 777 in fp16 takes 22 us through registers. Lines too long for a
 // tile's offsets (spans()) go through registers, whose addresses have 64 bits.
-Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, const Side &b) {
+//
+// A gated product (`pair`) takes its tiles' rows of B (along n) or A (along m)
+// half from the gate's weights and half from the values': half as many results
+// a tile, twice as many sums.
+Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, const Side &b, Pair pair) {
     Plan best;
     double least = std::numeric_limits<double>::infinity();
     const int64_t bk = 128 / (int64_t)type_size(dtype), steps = std::max<int64_t>(1, cdiv(k, bk));
     auto consider = [&](const TileCost &t) {
+        if (pair != Pair::kNone && !t.stages && t.b != 64) return;
         if (t.stages && !(spans(a, t.b, type_size(dtype)) && spans(b, t.b, type_size(dtype)))) return;
         const uint64_t pack = t.stages ? a.pack + b.pack : 0;
-        const int64_t tiles = cdiv(m, t.b) * cdiv(n, t.b);
+        const int64_t bm = pair == Pair::kM ? t.b / 2 : t.b, bn = pair == Pair::kN ? t.b / 2 : t.b;
+        const int64_t tiles = cdiv(m, bm) * cdiv(n, bn), sums = m * n * (pair == Pair::kNone ? 1 : 2);
         for (int64_t cut : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256}) {
             const int64_t each = cdiv(steps, cut), splits = cdiv(steps, each);
             if (cut > 1 && each < 2) continue;
             const int64_t total = tiles * splits, full = total / (256 * t.fit), left = cdiv(total % (256 * t.fit), 256);
             double us = full * (each * t.all + t.rest);
             if (left) us += each * std::max(t.one, t.all * left / t.fit) + t.rest;
-            if (splits > 1) us += 5.0 + (double)splits * m * n * 8 / 5e6;
+            if (splits > 1) us += 5.0 + (double)splits * sums * 8 / 5e6;
             if (pack) us += 4.0 + 2.0 * pack / 4e6;
             if (us >= least) continue;
             least = us;
-            best.bm = best.bn = t.b;
+            best.bm = (int)bm, best.bn = (int)bn, best.tile = t.b;
             best.block = t.b == 256 ? 512 : 256;
             best.stages = t.stages;
             best.pack_a = t.stages && a.pack;
@@ -454,7 +242,7 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, con
     skinny.skinny = true;
     skinny.block = 512;
     double few = std::numeric_limits<double>::infinity();
-    if (a.by_k && b.by_k && m <= 16 && cdiv(n, 16) <= UINT32_MAX / skinny.block) {
+    if (a.by_k && b.by_k && m <= 16 && pair != Pair::kM && cdiv(n, 16) <= UINT32_MAX / skinny.block) {
         few = 4.0 + (0.065 + 0.0025 * m) * steps * std::max(1.0, cdiv(n, 16) / 256.0);
         // what the tiles take at least, uncut or cut, without trying each cut:
         // a token's call need not wait for that
@@ -465,15 +253,14 @@ Plan plan_product(int dtype, int64_t m, int64_t n, int64_t k, const Side &a, con
     }
     for (const TileCost *t = tiles; t != end; ++t) consider(*t);
     if (few <= least) return skinny;
-    best.bytes = best.pack_bytes + (best.splits > 1 ? (uint64_t)best.splits * m * n * 4 : 0);
+    const uint64_t sums = (uint64_t)m * n * (pair == Pair::kNone ? 1 : 2);
+    best.bytes = best.pack_bytes + (best.splits > 1 ? best.splits * sums * 4 : 0);
     return best;
 }
 
-uint64_t up(uint64_t n) { return (n + 255) / 256 * 256; }
-
 // Contiguous along k (also where there is only one row to stride over), or
 // along the operand's own axis.
-bool by_k(const Operand &o) { return o.sum == 1; }
+bool by_k(const Operand &o) { return o.form ? o.form == 'k' : o.sum == 1; }
 
 // The lines of an operand packed: contiguous extent in whole 16 bytes.
 struct Packed {
@@ -503,11 +290,24 @@ Side side(const Operand &o, int64_t own_n, int64_t sum_n, size_t size) {
     const Packed p = packed(k, own_n, sum_n, size);
     return {k, p.bytes, p.ld};
 }
+// A gated product's weights: where they are contiguous along their own axis, the
+// values' half too begins at whole chunks, or the tiles go through registers.
+Side gated_side(const Operand &o, int64_t half, int64_t sum_n, size_t size) {
+    Side s = side(o, 2 * half, sum_n, size);
+    if (!s.by_k && half % (16 / (int64_t)size)) s.ld = std::numeric_limits<int64_t>::max();
+    return s;
+}
+
+// The operands' lines along their own axes.
+int64_t own_a(const Product &p) { return p.pair == Pair::kM ? 2 * p.m : p.m; }
+int64_t own_b(const Product &p) { return p.pair == Pair::kN ? 2 * p.n : p.n; }
 
 Plan plan_of(const Product &p) {
     if (!p.m || !p.n) return {};
     const size_t size = type_size(p.dtype);
-    return plan_product(p.dtype, p.m, p.n, p.k, side(p.a, p.m, p.k, size), side(p.b, p.n, p.k, size));
+    const Side a = p.pair == Pair::kM ? gated_side(p.a, p.m, p.k, size) : side(p.a, p.m, p.k, size);
+    const Side b = p.pair == Pair::kN ? gated_side(p.b, p.n, p.k, size) : side(p.b, p.n, p.k, size);
+    return plan_product(p.dtype, p.m, p.n, p.k, a, b, p.pair);
 }
 
 void product(Launches &launches, const Product &given, void *ws) {
@@ -532,11 +332,11 @@ void product(Launches &launches, const Product &given, void *ws) {
         for (j.shift = 3; j.shift < 8 && (int64_t)4 << j.shift < vecs;) ++j.shift;
         j.segs = (int32_t)cdiv(vecs, (int64_t)4 << j.shift);
         blocks = std::max(blocks, cdiv(k.lines, 256 >> j.shift) * j.segs);
-        o = along_k ? Operand{at, k.ld, 1, true} : Operand{at, 1, k.ld, true};
+        o = along_k ? Operand{at, k.ld, 1, true, 'k'} : Operand{at, 1, k.ld, true, 'm'};
         at += k.bytes;
     };
-    if (pl.pack_a) add(p.a, ak, p.m);
-    if (pl.pack_b) add(p.b, bk, p.n);
+    if (pl.pack_a) add(p.a, ak, own_a(p));
+    if (pl.pack_b) add(p.b, bk, own_b(p));
     if (jobs) launches.add(size == 2 ? "mxo_pack_16" : "mxo_pack_32", blocks, jobs, 256, pack);
     OpsGemmArgs g{};
     g.a = p.a.data;
@@ -556,6 +356,8 @@ void product(Launches &launches, const Product &given, void *ws) {
     g.splits = (int32_t)pl.splits;
     g.kchunk = (int32_t)pl.kchunk;
     const std::string t = kTypeName[p.dtype];
+    // the gated products' kernels: pairs along n, along m
+    const std::string of = p.pair == Pair::kNone ? "mxo_" : "mxg_", along = p.pair == Pair::kNone ? "" : p.pair == Pair::kN ? "n_" : "m_";
     g.act = p.act;
     g.slope = p.slope;
     if (p.bias) {
@@ -564,19 +366,19 @@ void product(Launches &launches, const Product &given, void *ws) {
         g.bias_rows = p.bias_rows;
     }
     if (pl.skinny) {
-        launches.add("mxo_skinny_" + t, cdiv(p.n, 16), 1, pl.block, g);
+        launches.add(of + "skinny_" + t, cdiv(p.n, 16), 1, pl.block, g);
         return;
     }
     const int64_t tm = cdiv(p.m, pl.bm), tn = cdiv(p.n, pl.bn);
     g.tiles_m = (int32_t)tm;
     g.tiles_n = (int32_t)tn;
-    launches.add("mxo_gemm_" + t + "_" + std::to_string(pl.bm) + "x" + std::to_string(pl.bn) + "_" + (ak ? "k" : "m") +
-                     (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
+    const std::string b = std::to_string(pl.tile);
+    launches.add(of + "gemm_" + along + t + "_" + b + "x" + b + "_" + (ak ? "k" : "m") + (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
                  tm * tn * pl.splits, 1, pl.block, g);
     if (pl.splits > 1) {
         // few sums of many splits: eight threads to each
         const bool deep = pl.splits >= 16;
-        launches.add((deep ? "mxo_join8_" : "mxo_join_") + t,
+        launches.add(of + (deep ? "join8_" : "join_") + along + t,
                      std::min<int64_t>(4096, cdiv(p.m * cdiv(p.n, 4), deep ? 32 : 256)), 1, 256, g);
     }
 }
@@ -610,15 +412,6 @@ Product dense_product(const mxh_mat &x, const mxh_mat &w, const mxh_mat &y, bool
     return oriented(y, operand(x, false), operand(w, false), x.cols, by_cols);
 }
 
-// mxh_dense_backward's workspace: dz where there is an activation, the bias's
-// partial sums, and one product's partial sums at a time.
-struct BwdLayout {
-    mxh_mat dz{};
-    int64_t parts = 0;
-    uint64_t dz_bytes = 0, part_bytes = 0, product_bytes = 0;
-    uint64_t total() const { return dz_bytes + part_bytes + product_bytes; }
-};
-
 // Blocks enough for the card, 16 rows (or 256 vectors of positions) each at
 // least.
 int64_t dz_parts(const mxh_mat &dy, bool by_cols) {
@@ -641,23 +434,26 @@ Product product_dw(const BwdLayout &l, const mxh_mat &x, const mxh_mat &dw) {
     return oriented(dw, dz_operand(l, true), operand(x, true), x.rows, out_by_cols(dw));
 }
 
+void place_dz(BwdLayout &l, const mxh_mat &dy, int64_t cols, bool by_cols) {
+    l.dz = dy;
+    l.dz.cols = cols;
+    const int64_t pad = 16 / (int64_t)type_size(dy.dtype);
+    if (by_cols) {
+        l.dz.row_stride = cdiv(cols, pad) * pad, l.dz.col_stride = 1;
+        l.dz_bytes = up((uint64_t)dy.rows * l.dz.row_stride * type_size(dy.dtype));
+    } else {
+        l.dz.col_stride = cdiv(dy.rows, pad) * pad, l.dz.row_stride = 1;
+        l.dz_bytes = up((uint64_t)cols * l.dz.col_stride * type_size(dy.dtype));
+    }
+    l.dz.data = nullptr;  // aligned wherever the workspace is
+}
+
 BwdLayout bwd_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mxh_mat &w, const mxh_mat *dx,
                      const mxh_mat *dw, const mxh_vec *db, int act) {
     BwdLayout l;
     l.dz = dy;
     const bool products = dx || dw;
-    if (act != MXH_NONE && products) {
-        // rows (or planes) padded to 16 bytes, so that the products' loads are
-        const int64_t pad = 16 / (int64_t)type_size(dy.dtype);
-        if (by_cols) {
-            l.dz.row_stride = cdiv(dy.cols, pad) * pad, l.dz.col_stride = 1;
-            l.dz_bytes = up((uint64_t)dy.rows * l.dz.row_stride * type_size(dy.dtype));
-        } else {
-            l.dz.col_stride = cdiv(dy.rows, pad) * pad, l.dz.row_stride = 1;
-            l.dz_bytes = up((uint64_t)dy.cols * l.dz.col_stride * type_size(dy.dtype));
-        }
-        l.dz.data = nullptr;  // aligned wherever the workspace is
-    }
+    if (act != MXH_NONE && products) place_dz(l, dy, dy.cols, by_cols);
     if (db) {
         l.parts = dz_parts(dy, by_cols);
         l.part_bytes = up((uint64_t)l.parts * dy.cols * 4);
@@ -666,28 +462,16 @@ BwdLayout bwd_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mx
     if (dw && !empty(*dw)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dw(l, x, *dw)).bytes);
     return l;
 }
+}  // namespace mxops
 
-template <typename F>
-int guard(F &&f) {
-    try {
-        f();
-        return 0;
-    } catch (const std::exception &e) {
-        mx::set_error(e.what());
-    } catch (...) {
-        mx::set_error("unknown error");
-    }
-    return -1;
-}
-
-}  // namespace
+using namespace mxops;
 
 extern "C" {
 
 int mxh_ops_ready(int device) {
     return guard([&] {
         OnDevice on(device);
-        function(device, "mxo_join_parts");
+        load_all(device);
     });
 }
 

@@ -1,0 +1,389 @@
+// The gated Dense: z = x w^T + bias with w's rows (and z's features) in two
+// halves (a | c), y = act(a) c, and the backward pass's dz.
+//
+// Forward it is a product whose epilogue needs two sums for a result. The
+// tiles of ops_gemm.h take both: of a wave's rows of the weights' operand half
+// are the gate's and half the values' of the same features (Tile's HALF), so
+// its sums of a and of c lie in the same lanes, and neither z nor a second
+// product goes through memory unless z is kept. The weights are B where
+// features are contiguous in the results (PAIR_N), A in planar order (PAIR_M).
+#pragma once
+
+#include "ops_gemm_big.h"
+
+// What E results of row m need from memory: one bias of each half where it
+// runs along the rows.
+template <typename T>
+struct GatedBias {
+    float a, c;
+};
+template <typename T>
+__device__ __forceinline__ GatedBias<T> gated_bias_row(const OpsGemmArgs &g, int64_t m) {
+    if (!g.bias || !g.bias_rows || m >= g.m) return {0.0f, 0.0f};
+    return {param<T>(g.bias, m, g.bias_f32), param<T>(g.bias, m + g.m, g.bias_f32)};
+}
+// The biases of columns n on, zeros where they run along the rows.
+template <typename T, int E>
+__device__ __forceinline__ void gated_bias_cols(const OpsGemmArgs &g, int64_t n, float *a, float *c) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool in = g.bias && !g.bias_rows && n + e < g.n;
+        a[e] = in ? param<T>(g.bias, n + e, g.bias_f32) : 0.0f;
+        c[e] = in ? param<T>(g.bias, n + e + g.n, g.bias_f32) : 0.0f;
+    }
+}
+
+// y and z for E consecutive n of row m from the sums of both halves. The sums,
+// the activation and the product are fp32, each store rounds once.
+template <typename T, int E, int PAIR>
+__device__ __forceinline__ void gated_finish(const OpsGemmArgs &g, int64_t m, int64_t n, float *a, float *c) {
+    if (m >= g.m || n >= g.n) return;
+    const int64_t have = g.n - n;
+    Vec<T, E> o;
+    if (g.z) {
+        T *z = static_cast<T *>(g.z) + m * g.ldz + n;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(a[e]);
+        store_upto<T, E>(z, o, have);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(c[e]);
+        store_upto<T, E>(z + (PAIR == PAIR_N ? (int64_t)g.n : g.m * g.ldz), o, have);
+    }
+    act_fwd_n<E>(g.act, g.slope, a);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(a[e] * c[e]);
+    store_upto<T, E>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
+}
+
+// Where split s's partial sums of row m, column n of a half lie: [splits][m][2 n]
+// or [splits][2 m][n].
+template <int PAIR>
+__device__ __forceinline__ float *gated_part(const OpsGemmArgs &g, int s, int64_t m, int64_t n) {
+    return g.part + ((int64_t)s * g.m * (PAIR == PAIR_M ? 2 : 1) + m) * ((int64_t)g.n * (PAIR == PAIR_N ? 2 : 1)) + n;
+}
+template <int PAIR>
+__device__ __forceinline__ int64_t gated_part_half(const OpsGemmArgs &g) {
+    return PAIR == PAIR_N ? (int64_t)g.n : (int64_t)g.m * g.n;
+}
+
+// A wave's FM x FN blocks of 16 x 16 sums, which are half as many results from
+// (m0, n0) on: gemm_write's way through LDS, 32 rows at a time with both halves
+// in a row (PAIR_N), or 16 rows of each half (PAIR_M).
+template <typename T, int FM, int FN, int PAIR>
+__device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
+                                            const f32x4 (&acc)[FM][FN]) {
+    constexpr int E = 16 / sizeof(T), LD = FN * 16 + 4;
+    constexpr int COLS = PAIR == PAIR_N ? FN * 8 : FN * 16, TALL = PAIR == PAIR_N ? 32 : 16;
+    constexpr int LANES = COLS / E, ROWS = 64 / LANES < TALL ? 64 / LANES : TALL, STEPS = TALL / ROWS;
+    constexpr int OTHER = PAIR == PAIR_N ? COLS : 16 * LD;  // a value's sum from its gate's
+    static_assert(FM % 2 == 0 && FN % 2 == 0 && LANES * ROWS == 64, "");
+    float *own = reinterpret_cast<float *>(at);
+    const int lr = l / LANES, lc = l % LANES * E;
+    const int64_t n = n0 + lc;
+    float ba[E], bc[E];
+    if (g.splits == 1) gated_bias_cols<T, E>(g, n, ba, bc);
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i) {
+        const int64_t m = m0 + i * TALL + lr;
+        GatedBias<T> row[STEPS];
+        if (PAIR == PAIR_M && g.splits == 1) {
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) row[k] = gated_bias_row<T>(g, m + k * ROWS);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                *reinterpret_cast<f32x4 *>(own + (h * 16 + (l & 15)) * LD + j * 16 + (l >> 4) * 4) =
+                    acc[PAIR == PAIR_N ? 2 * i + h : i + h * (FM / 2)][j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            float a[E], c[E];
+            const float *p = own + (k * ROWS + lr) * LD + lc;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                *reinterpret_cast<f32x4 *>(a + e) = *reinterpret_cast<const f32x4 *>(p + e);
+                *reinterpret_cast<f32x4 *>(c + e) = *reinterpret_cast<const f32x4 *>(p + OTHER + e);
+            }
+            if (g.splits == 1) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    a[e] += PAIR == PAIR_M ? row[k].a : ba[e];
+                    c[e] += PAIR == PAIR_M ? row[k].c : bc[e];
+                }
+                gated_finish<T, E, PAIR>(g, m + k * ROWS, n, a, c);
+            } else if (m + k * ROWS < g.m && n < g.n) {
+                float *o = gated_part<PAIR>(g, s, m + k * ROWS, n);
+                store_upto<float, E>(o, __builtin_bit_cast(Vec<float, E>, a), g.n - n);
+                store_upto<float, E>(o + gated_part_half<PAIR>(g), __builtin_bit_cast(Vec<float, E>, c), g.n - n);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// The splits' sums of both halves added in a fixed order, then the epilogue:
+// WAYS threads to four results, each every WAYS-th split, joined through LDS.
+template <typename T, int WAYS, int PAIR>
+__device__ __forceinline__ void gated_join(const OpsGemmArgs &g) {
+    constexpr int Q = 256 / WAYS;
+    __shared__ f32x4 sh[2][WAYS > 1 ? 256 : 1];
+    const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m, half = gated_part_half<PAIR>(g);
+    const int64_t plane = 2 * (int64_t)g.m * g.n;
+    const int q = threadIdx.x % Q, way = threadIdx.x / Q;
+    for (int64_t i0 = (int64_t)blockIdx.x * Q; i0 < total; i0 += (int64_t)gridDim.x * Q) {
+        const int64_t i = i0 + q, m = i / quads, n = (i - m * quads) * 4;
+        f32x4 a = {0, 0, 0, 0}, c = a;
+        if (i < total) {
+            const float *p = gated_part<PAIR>(g, 0, m, n);
+#pragma unroll 4
+            for (int s = way; s < g.splits; s += WAYS) {
+                const Vec<float, 4> va = load_upto<float, 4>(p + s * plane, g.n - n);
+                const Vec<float, 4> vc = load_upto<float, 4>(p + s * plane + half, g.n - n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] += va.v[e], c[e] += vc.v[e];
+            }
+        }
+        if constexpr (WAYS > 1) {
+            __syncthreads();
+            sh[0][threadIdx.x] = a;
+            sh[1][threadIdx.x] = c;
+            __syncthreads();
+            if (way) continue;
+#pragma unroll
+            for (int k = 1; k < WAYS; ++k) a += sh[0][k * Q + q], c += sh[1][k * Q + q];
+        }
+        if (i >= total) continue;
+        float ra[4], rc[4], ba[4], bc[4];
+        gated_bias_cols<T, 4>(g, n, ba, bc);
+        const GatedBias<T> row = gated_bias_row<T>(g, m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ra[e] = a[e] + ba[e] + row.a, rc[e] = c[e] + bc[e] + row.c;
+        gated_finish<T, 4, PAIR>(g, m, n, ra, rc);
+    }
+}
+
+// Up to 16 rows: ops_skinny.h's way, the block's 16 features of both halves at
+// once, each weight read once.
+template <typename T>
+__device__ __forceinline__ void gated_skinny(const OpsGemmArgs &g) {
+    constexpr int E = 16 / sizeof(T), STEP = 4 * E, W = 8, AHEAD = 4;
+    typedef typename Mma<T>::Frag Frag;
+    __shared__ f32x4 sums[2][W][64];
+    const int t = threadIdx.x, l = t & 63, w = t >> 6, r = l & 15, q = l >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int each = (g.k + W * STEP - 1) / (W * STEP) * STEP, kbeg = w * each + q * E, kend = min(g.k, (w + 1) * each);
+    const T *b = static_cast<const T *>(g.b) + min(n0 + r, (int64_t)g.n - 1) * g.ldb;
+    const T *c = b + (int64_t)g.n * g.ldb;
+    const T *a = static_cast<const T *>(g.a) + (int64_t)min(r, g.m - 1) * g.lda;
+    f32x4 gate = {0, 0, 0, 0}, value = gate;
+    const int steps = each / STEP, whole = max(0, (kend - w * each)) / STEP;
+    auto go = [&](const Vec<T, E> &fb, const Vec<T, E> &fc, const Vec<T, E> &fa) {
+        gate = Mma<T>::go(__builtin_bit_cast(Frag, fb), __builtin_bit_cast(Frag, fa), gate);
+        value = Mma<T>::go(__builtin_bit_cast(Frag, fc), __builtin_bit_cast(Frag, fa), value);
+    };
+    int s = 0;
+    for (; s + AHEAD <= whole; s += AHEAD) {
+        Vec<T, E> fb[AHEAD], fc[AHEAD], fa[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int k = kbeg + (s + j) * STEP;
+            fb[j] = load_n<T, E>(b + k);
+            fc[j] = load_n<T, E>(c + k);
+            fa[j] = load_n<T, E>(a + k);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) go(fb[j], fc[j], fa[j]);
+    }
+    for (; s < steps; ++s) {
+        const int k = kbeg + s * STEP;
+        go(load_upto<T, E>(b + k, kend - k), load_upto<T, E>(c + k, kend - k), load_upto<T, E>(a + k, kend - k));
+    }
+    sums[0][w][l] = gate;
+    sums[1][w][l] = value;
+    __syncthreads();
+    if (t >= 64) return;
+    gate = sums[0][0][l], value = sums[1][0][l];
+#pragma unroll
+    for (int k = 1; k < W; ++k) gate += sums[0][k][l], value += sums[1][k][l];
+    // lane l: row l % 16, columns 4 (l / 16) + 0..3
+    const int64_t m = r, n = n0 + q * 4;
+    float ra[4], rc[4], ba[4], bc[4];
+    gated_bias_cols<T, 4>(g, n, ba, bc);
+    const GatedBias<T> row = gated_bias_row<T>(g, m);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ra[e] = gate[e] + ba[e] + row.a, rc[e] = value[e] + bc[e] + row.c;
+    gated_finish<T, 4, PAIR_N>(g, m, n, ra, rc);
+}
+
+// dz = (dy c act'(a) | dy act(a)) and the bias's partial sums, one pass over dy
+// and z. Stored rounded to the operands' type, as the products' matrix cores
+// take it (ops_rows.h has what that costs); the bias's sums take it before.
+//
+// v: dy in, da out; u: a in, dc out.
+template <int E>
+__device__ __forceinline__ void gated_dz_n(int act, float slope, float *v, float *u, const float *c) {
+    float s[E], d[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) d[e] = v[e] * c[e], s[e] = u[e];
+    act_bwd_n<E>(act, slope, d, [&](int e) { return u[e]; });
+    act_fwd_n<E>(act, slope, s);
+#pragma unroll
+    for (int e = 0; e < E; ++e) u[e] = v[e] * s[e], v[e] = d[e];
+}
+
+// Rows with contiguous features: 64 x E features by a run of rows a block, a
+// wave a row at a time.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void gated_dz_rows(const OpsDzArgs &a, float (*sh)[2][64 * 16 / sizeof(T)]) {
+    constexpr int E = 16 / sizeof(T);
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + l) * E, p = blockIdx.y, have = a.cols - c;
+    const int64_t chunk = (a.rows + a.nparts - 1) / a.nparts, end = min(a.rows, (p + 1) * chunk);
+    float sa[E], sc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sa[e] = sc[e] = 0.0f;
+    if (have > 0)
+        for (int64_t r = p * chunk + w; r < end; r += 4) {
+            const T *dy = static_cast<const T *>(a.dy) + r * a.dyrs + c, *z = static_cast<const T *>(a.z) + r * a.zrs + c;
+            // a lane without features has left already
+            const int64_t rest = a.rows - 1 - r, last = a.cols - E - c;
+            const u32x4 vd = load_in<T, E, WHOLE>(dy, dy, dy + rest * a.dyrs + last, have);
+            const u32x4 vz = load_in<T, E, WHOLE>(z, z, z + rest * a.zrs + last, have);
+            const u32x4 vc = load_in<T, E, WHOLE>(z + a.cols, z + a.cols, z + a.cols + rest * a.zrs + last, have);
+            float v[E], u[E], m[E];
+            Vec<T, E> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = elem<T>(vd, e), u[e] = elem<T>(vz, e), m[e] = elem<T>(vc, e);
+            gated_dz_n<E>(a.act, a.slope, v, u, m);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                // features past the last are not there to be summed or stored
+                sa[e] += v[e], sc[e] += u[e];
+                o.v[e] = from_f<T>(v[e]);
+            }
+            if (a.dz) {
+                T *dz = static_cast<T *>(a.dz) + r * a.drs + c;
+                store_in<T, E, WHOLE>(dz, o, have);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(u[e]);
+                store_in<T, E, WHOLE>(dz + a.cols, o, have);
+                // the products' loads take lines of whole vectors, zeros at their ends
+                if (!WHOLE && have <= E)
+                    for (int64_t k = 2 * a.cols - c; k < a.drs - c; ++k) dz[k] = (T)0.0f;
+            }
+        }
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sh[w][0][l * E + e] = sa[e], sh[w][1][l * E + e] = sc[e];
+    __syncthreads();
+    for (int k = threadIdx.x; k < 128 * E; k += 256) {
+        const int h = k >= 64 * E, i = k - h * 64 * E;
+        const int64_t col = (int64_t)blockIdx.x * 64 * E + i;
+        if (col < a.cols)
+            a.part[(2 * p + h) * a.cols + col] = (sh[0][h][i] + sh[1][h][i]) + (sh[2][h][i] + sh[3][h][i]);
+    }
+}
+// Planar order: one feature by a run of positions a block.
+template <typename T>
+__device__ __forceinline__ void gated_dz_planar(const OpsDzArgs &a) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ float sh[2][4];
+    const int64_t c = blockIdx.x, p = blockIdx.y;
+    const int64_t chunk = ((a.rows + a.nparts - 1) / a.nparts + E - 1) / E * E, end = min(a.rows, (p + 1) * chunk);
+    const T *dy = static_cast<const T *>(a.dy) + c * a.dycs, *z = static_cast<const T *>(a.z) + c * a.zcs;
+    T *dz = static_cast<T *>(a.dz) + c * a.dcs;
+    float sa = 0.0f, sc = 0.0f;
+    for (int64_t r = p * chunk + threadIdx.x * E; r < end; r += 256 * E) {
+        const Vec<T, E> vd = load_upto<T, E>(dy + r, end - r), vz = load_upto<T, E>(z + r, end - r);
+        const Vec<T, E> vc = load_upto<T, E>(z + a.cols * a.zcs + r, end - r);
+        float v[E], u[E], m[E];
+        Vec<T, E> oa, oc;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = to_f<T>(vd.v[e]), u[e] = to_f<T>(vz.v[e]), m[e] = to_f<T>(vc.v[e]);
+        gated_dz_n<E>(a.act, a.slope, v, u, m);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (r + e < end) sa += v[e], sc += u[e];
+            oa.v[e] = from_f<T>(v[e]), oc.v[e] = from_f<T>(u[e]);
+        }
+        // lines of dz are whole vectors, their ends zeros (a run is whole vectors)
+        if (a.dz) {
+            store_n<T, E>(dz + r, oa);
+            store_n<T, E>(dz + a.cols * a.dcs + r, oc);
+        }
+    }
+    if (!a.part) return;
+    sa = wave_sum(sa), sc = wave_sum(sc);
+    if ((threadIdx.x & 63) == 0) sh[0][threadIdx.x >> 6] = sa, sh[1][threadIdx.x >> 6] = sc;
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const float *s = sh[threadIdx.x];
+        a.part[(2 * p + threadIdx.x) * a.cols + c] = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+}
+
+#define OPS_GATED1(name, T, B, WM, WN, axis, PAIR, tag, AK, BK)                                                  \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxg_gemm_##axis##_##name##_##B##x##B##_##tag(     \
+        OpsGemmArgs g) {                                                                                         \
+        __shared__ __align__(128) char lds[4 * B * 128];                                                         \
+        gemm_tile<T, B, B, WM, WN, AK, BK, PAIR>(g, lds);                                                        \
+    }
+#define OPS_GATED_D2(name, T, B, WM, WN, axis, PAIR, tag, AK, BK)                                                \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxg_gemm_##axis##_##name##_##B##x##B##_##tag##_d2( \
+        OpsGemmArgs g) {                                                                                         \
+        OPS_STAGE(0, B, B)                                                                                       \
+        OPS_STAGE(1, B, B)                                                                                       \
+        const Stage st[2] = {{a0, b0}, {a1, b1}};                                                                \
+        gemm_direct<T, B, B, WM, WN, AK, BK, 2, PAIR>(g, st);                                                    \
+    }
+#define OPS_GATED_D4(name, T, B, WM, WN, axis, PAIR, tag, AK, BK)                                                \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxg_gemm_##axis##_##name##_##B##x##B##_##tag##_d4( \
+        OpsGemmArgs g) {                                                                                         \
+        OPS_STAGE(0, B, B)                                                                                       \
+        OPS_STAGE(1, B, B)                                                                                       \
+        OPS_STAGE(2, B, B)                                                                                       \
+        OPS_STAGE(3, B, B)                                                                                       \
+        const Stage st[4] = {{a0, b0}, {a1, b1}, {a2, b2}, {a3, b3}};                                            \
+        gemm_direct<T, B, B, WM, WN, AK, BK, 4, PAIR>(g, st);                                                    \
+    }
+// x has the results' order: rows along k with w either way (PAIR_N), or planes
+#define OPS_GATED_ALL(KIND, name, T, B, WM, WN)                        \
+    KIND(name, T, B, WM, WN, n, PAIR_N, kk, true, true)                \
+    KIND(name, T, B, WM, WN, n, PAIR_N, km, true, false)               \
+    KIND(name, T, B, WM, WN, m, PAIR_M, km, true, false)               \
+    KIND(name, T, B, WM, WN, m, PAIR_M, mm, false, false)
+#define OPS_GATED_JOIN(name, T, axis, PAIR)                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void mxg_join_##axis##_##name(OpsGemmArgs g) { gated_join<T, 1, PAIR>(g); } \
+    extern "C" __global__ __launch_bounds__(256) void mxg_join8_##axis##_##name(OpsGemmArgs g) { gated_join<T, 8, PAIR>(g); }
+#define OPS_GATED_TYPE(name, T)                                                                                          \
+    OPS_GATED_ALL(OPS_GATED1, name, T, 64, 2, 2)                                                                         \
+    OPS_GATED_JOIN(name, T, n, PAIR_N)                                                                                   \
+    OPS_GATED_JOIN(name, T, m, PAIR_M)                                                                                   \
+    extern "C" __global__ __launch_bounds__(512) void mxg_skinny_##name(OpsGemmArgs g) { gated_skinny<T>(g); }           \
+    extern "C" __global__ __launch_bounds__(256) void mxg_dz_rows_##name(OpsDzArgs a) {                                  \
+        __shared__ float sh[4][2][64 * 16 / sizeof(T)];                                                                  \
+        if (a.cols % (16 / sizeof(T)) == 0) gated_dz_rows<T, true>(a, sh);                                               \
+        else gated_dz_rows<T, false>(a, sh);                                                                             \
+    }                                                                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void mxg_dz_planar_##name(OpsDzArgs a) { gated_dz_planar<T>(a); }
+
+OPS_GATED_TYPE(bf16, bf16)
+OPS_GATED_TYPE(f16, f16)
+OPS_GATED_TYPE(f32, float)
+OPS_GATED_ALL(OPS_GATED_D2, bf16, bf16, 256, 2, 4)
+OPS_GATED_ALL(OPS_GATED_D2, f16, f16, 256, 2, 4)
+OPS_GATED_ALL(OPS_GATED_D2, bf16, bf16, 128, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D2, f16, f16, 128, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D4, bf16, bf16, 128, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D4, f16, f16, 128, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D4, bf16, bf16, 64, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D4, f16, f16, 64, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D2, f32, float, 128, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D4, f32, float, 64, 2, 2)
+OPS_GATED_ALL(OPS_GATED_D2, f32, float, 64, 2, 2)

@@ -44,12 +44,19 @@ struct Mma<float> {
 
 typedef __attribute__((address_space(3))) char LdsChar;
 
+// Whether a product is gated (ops_gated.h), and the axis with both halves.
+enum { PAIR_NONE = 0, PAIR_N, PAIR_M };
+
 // One operand's tile: ROWS of m (or n) by 128 bytes of k, in 16-byte chunks
 // at LDS positions p * 16. Contiguous along k: position p holds row p / 8, a
 // chunk of its 8 picked by exclusive or with the row, so the 16 rows a
 // fragment takes at one k fall into different banks. Contiguous along rows:
 // position p holds one k's chunk, 16-element segments exchanged likewise.
-template <typename T, bool KMAJ, int ROWS, int NT>
+//
+// HALF: the rows are a gated product's (ops_gated.h), HALF of the gate's and
+// HALF of the values' in turn, so that a wave has both halves of its results;
+// the values' begin `pair` elements past the gate's.
+template <typename T, bool KMAJ, int ROWS, int NT, int HALF = 0>
 struct Tile {
     static constexpr int E = 16 / sizeof(T);    // elements a chunk
     static constexpr int BK = 128 / sizeof(T);  // k's a tile
@@ -74,28 +81,38 @@ struct Tile {
             row = ((((c / G) ^ (kswz(k) & (ROWS / 16 - 1))) * G) + c % G) * E;
         }
     }
+    // the operand's row that a tile's row is, and whether it is a value's
+    static __device__ __forceinline__ int line(int row) { return HALF ? row / (2 * HALF) * HALF + row % HALF : row; }
+    static __device__ __forceinline__ bool second(int row) { return HALF != 0 && (row / HALF) & 1; }
     // the chunk of position p from global memory: zeros past the operand's
     // `rows` rows and `kn` k's (g points at the tile's first element). INSIDE:
     // the tile's k's and, contiguous along rows, its rows are all there; rows
     // past the last may then be any row's (what they give is not stored).
     template <bool INSIDE>
-    static __device__ __forceinline__ Chunk load(const T *g, int64_t ld, int p, int rows, int kn) {
+    static __device__ __forceinline__ Chunk load(const T *g, int64_t ld, int p, int rows, int kn, int64_t pair) {
         int row, k;
         where(p, row, k);
+        if constexpr (HALF != 0) {
+            g += second(row) ? pair : 0;
+            row = line(row);
+        }
         if constexpr (INSIDE) return load_n<T, E>(g + (KMAJ ? min(row, rows - 1) * ld + k : k * ld + row));
         const int have = KMAJ ? (row < rows ? kn - k : 0) : (k < kn ? rows - row : 0);
         return load_upto<T, E>(g + (KMAJ ? row * ld + k : k * ld + row), have);
     }
-    static __device__ __forceinline__ bool inside(int rows, int kn) { return kn >= BK && (KMAJ || rows == ROWS); }
+    static __device__ __forceinline__ bool inside(int rows, int kn) {
+        return kn >= BK && (KMAJ || rows == (HALF ? ROWS / 2 : ROWS));
+    }
     // All of a thread's chunks. (One branch for the tile: with one a chunk each
     // load was waited for before the next.)
-    static __device__ __forceinline__ void fetch(Chunk (&c)[PER], const T *g, int64_t ld, int t, int rows, int kn) {
+    static __device__ __forceinline__ void fetch(Chunk (&c)[PER], const T *g, int64_t ld, int t, int rows, int kn,
+                                                 int64_t pair = 0) {
         if (inside(rows, kn)) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) c[i] = load<true>(g, ld, i * NT + t, rows, kn);
+            for (int i = 0; i < PER; ++i) c[i] = load<true>(g, ld, i * NT + t, rows, kn, pair);
         } else {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) c[i] = load<false>(g, ld, i * NT + t, rows, kn);
+            for (int i = 0; i < PER; ++i) c[i] = load<false>(g, ld, i * NT + t, rows, kn, pair);
         }
     }
     // Where lane l's part of a fragment lies, but for the fragment's own
@@ -327,9 +344,16 @@ template <int FN>
 constexpr int gemm_write_bytes() {
     return 32 * (FN * 16 + 4) * 4;
 }
-template <typename T, int FM, int FN>
+template <typename T, int FM, int FN, int PAIR>
+__device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
+                                            const f32x4 (&acc)[FM][FN]);
+template <typename T, int FM, int FN, int PAIR = PAIR_NONE>
 __device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
                                            const f32x4 (&acc)[FM][FN]) {
+    if constexpr (PAIR != PAIR_NONE) {
+        gated_write<T, FM, FN, PAIR>(g, m0, n0, s, l, at, acc);
+        return;
+    }
     constexpr int E = 16 / sizeof(T), LD = FN * 16 + 4, LANES = FN * 16 / E, ROWS = 64 / LANES, STEPS = 32 / ROWS;
     static_assert(FM % 2 == 0 && LANES <= 64, "");
     float *own = reinterpret_cast<float *>(at);
@@ -375,25 +399,28 @@ __device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int
 }
 
 // WM x WN waves of 64 lanes, each (BM / WM) x (BN / WN) of the tile.
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_>
+// PAIR: a gated product's (ops_gated.h) rows of B (along n) or A (along m).
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_, int PAIR = PAIR_NONE>
 __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
-    typedef Tile<T, AK, BM, NT> TA;
-    typedef Tile<T, BK_, BN, NT> TB;
+    constexpr int CM = PAIR == PAIR_M ? BM / 2 : BM, CN = PAIR == PAIR_N ? BN / 2 : BN;  // results
+    typedef Tile<T, AK, BM, NT, PAIR == PAIR_M ? BM / WM / 2 : 0> TA;
+    typedef Tile<T, BK_, BN, NT, PAIR == PAIR_N ? BN / WN / 2 : 0> TB;
     constexpr int BK = TA::BK, ABYTES = BM * 128, STAGE = (BM + BN) * 128;
     int tm, tn, s;
     gemm_place(g, tm, tn, s);
-    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int64_t m0 = (int64_t)tm * CM, n0 = (int64_t)tn * CN;
     const int kbeg = s * g.kchunk, kend = min(g.k, kbeg + g.kchunk);
     const int t = threadIdx.x, l = t & 63, w = t >> 6, wm = w / WN * (BM / WM), wn = w % WN * (BN / WN);
-    const int rows_a = min((int64_t)BM, g.m - m0), rows_b = min((int64_t)BN, g.n - n0);
+    const int rows_a = min((int64_t)CM, g.m - m0), rows_b = min((int64_t)CN, g.n - n0);
     const T *ga = static_cast<const T *>(g.a) + (AK ? m0 * g.lda + kbeg : kbeg * g.lda + m0);
     const T *gb = static_cast<const T *>(g.b) + (BK_ ? n0 * g.ldb + kbeg : kbeg * g.ldb + n0);
     typename TA::Chunk ra[TA::PER];
     typename TB::Chunk rb[TB::PER];
+    const int64_t pair_a = PAIR == PAIR_M ? (AK ? g.m * g.lda : g.m) : 0, pair_b = PAIR == PAIR_N ? (BK_ ? g.n * g.ldb : g.n) : 0;
     auto fetch = [&](int k0) {
-        TA::fetch(ra, ga + (AK ? k0 : k0 * g.lda), g.lda, t, rows_a, kend - kbeg - k0);
-        TB::fetch(rb, gb + (BK_ ? k0 : k0 * g.ldb), g.ldb, t, rows_b, kend - kbeg - k0);
+        TA::fetch(ra, ga + (AK ? k0 : k0 * g.lda), g.lda, t, rows_a, kend - kbeg - k0, pair_a);
+        TB::fetch(rb, gb + (BK_ ? k0 : k0 * g.ldb), g.ldb, t, rows_b, kend - kbeg - k0, pair_b);
     };
     auto put = [&](char *at) {
 #pragma unroll
@@ -454,7 +481,7 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
             }
     }
     // behind the loop's last barrier: no wave reads the tiles any more
-    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, lds + w * gemm_write_bytes<FN>(), acc);
+    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, lds + w * gemm_write_bytes<FN>(), acc);
 }
 
 // The splits' sums added in a fixed order, then the epilogue: WAYS threads to
@@ -517,6 +544,7 @@ __device__ __forceinline__ void pack_lines(const OpsPackArgs &args) {
         if (at < a.dst_ld) store_n<T, E>(dst + at, v[j]);
     }
 }
+#ifndef OPS_GATED
 extern "C" __global__ __launch_bounds__(256) void mxo_pack_16(OpsPackArgs a) { pack_lines<f16>(a); }
 extern "C" __global__ __launch_bounds__(256) void mxo_pack_32(OpsPackArgs a) { pack_lines<float>(a); }
 
@@ -541,3 +569,4 @@ extern "C" __global__ __launch_bounds__(256) void mxo_pack_32(OpsPackArgs a) { p
 OPS_GEMM_TYPE(bf16, bf16)
 OPS_GEMM_TYPE(f16, f16)
 OPS_GEMM_TYPE(f32, float)
+#endif

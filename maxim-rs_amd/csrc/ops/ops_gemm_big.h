@@ -52,21 +52,22 @@ struct Stage {
     char *a, *b;
 };
 
-template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_, int ST>
+template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_, int ST, int PAIR = PAIR_NONE>
 __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&st)[ST]) {
     // the epilogue takes a quarter of the waves in each of four arrays
     static_assert((WM * WN + 3) / 4 * gemm_write_bytes<BN / WN / 16>() <= BM * 128 && BM == BN, "");
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
-    typedef Tile<T, AK, BM, NT> TA;
-    typedef Tile<T, BK_, BN, NT> TB;
+    constexpr int CM = PAIR == PAIR_M ? BM / 2 : BM, CN = PAIR == PAIR_N ? BN / 2 : BN;  // results
+    typedef Tile<T, AK, BM, NT, PAIR == PAIR_M ? BM / WM / 2 : 0> TA;
+    typedef Tile<T, BK_, BN, NT, PAIR == PAIR_N ? BN / WN / 2 : 0> TB;
     constexpr int BK = TA::BK;
     int tm, tn, s;
     gemm_place(g, tm, tn, s);
-    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int64_t m0 = (int64_t)tm * CM, n0 = (int64_t)tn * CN;
     const int kbeg = s * g.kchunk, kend = min(g.k, kbeg + g.kchunk);
     const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = w / WN * (BM / WM), wn = w % WN * (BN / WN);
-    const int rows_a = min((int64_t)BM, g.m - m0), rows_b = min((int64_t)BN, g.n - n0);
+    const int rows_a = min((int64_t)CM, g.m - m0), rows_b = min((int64_t)CN, g.n - n0);
     const T *ga = static_cast<const T *>(g.a) + (AK ? m0 * g.lda + kbeg : kbeg * g.lda + m0);
     const T *gb = static_cast<const T *>(g.b) + (BK_ ? n0 * g.ldb + kbeg : kbeg * g.ldb + n0);
     // A thread's chunks of a tile lie a fixed number of rows (along k: of k's)
@@ -81,20 +82,39 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     const uint32_t step_a = (AK ? NT / 8 : NT / TA::CPR) * lda, step_b = (BK_ ? NT / 8 : NT / TB::CPR) * ldb;
     uint32_t oa[OA], ob[OB];
     int ka, kb;  // along k: the chunks' first k, the same in all of them
+    // A gated product's chunks along k: a wave's lie in one half, which its
+    // buffer's base tells, and the line goes down by half the step. Along rows
+    // the half is the lane's, in its offset.
+    constexpr bool PA = PAIR == PAIR_M, PB = PAIR == PAIR_N;
+    const int64_t pair_a = PA ? (AK ? g.m * g.lda : g.m) * (int64_t)sizeof(T) : 0;
+    const int64_t pair_b = PB ? (BK_ ? g.n * g.ldb : g.n) * (int64_t)sizeof(T) : 0;
 #pragma unroll
     for (int i = OA - 1; i >= 0; --i) {
         int r;
         TA::where(i * NT + t, r, ka);
+        if constexpr (PA) {
+            const int at = TA::line(r) * (int)sizeof(T) + (TA::second(r) ? (int)pair_a : 0);
+            oa[i] = AK ? (t >> 3 & 7) * lda + ka * (int)sizeof(T) : TA::line(r) < rows_a ? ka * lda + at : kNowhere;
+            continue;
+        }
         oa[i] = AK || r < rows_a ? (AK ? r * lda + ka * (int)sizeof(T) : ka * lda + r * (int)sizeof(T)) : kNowhere;
     }
 #pragma unroll
     for (int i = OB - 1; i >= 0; --i) {
         int r;
         TB::where(i * NT + t, r, kb);
+        if constexpr (PB) {
+            const int at = TB::line(r) * (int)sizeof(T) + (TB::second(r) ? (int)pair_b : 0);
+            ob[i] = BK_ ? (t >> 3 & 7) * ldb + kb * (int)sizeof(T) : TB::line(r) < rows_b ? kb * ldb + at : kNowhere;
+            continue;
+        }
         ob[i] = BK_ || r < rows_b ? (BK_ ? r * ldb + kb * (int)sizeof(T) : kb * ldb + r * (int)sizeof(T)) : kNowhere;
     }
     const char *next_a = reinterpret_cast<const char *>(ga), *next_b = reinterpret_cast<const char *>(gb);
     int left = kend - kbeg;
+    auto half_buffer = [](const char *base, int64_t half, int size) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(base + half), 0, size, 0x00020000);
+    };
     // the next tile, in turn
     auto stage = [&](char *at, char *bt) {
         // (the compiler clamps in the vector unit; a buffer in vector registers
@@ -105,12 +125,30 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
         const __amdgpu_buffer_rsrc_t bufb =
             __builtin_amdgcn_make_buffer_rsrc((void *)next_b, 0, (BK_ ? rows_b : k) * ldb, 0x00020000);
         const uint32_t fa = !AK || ka < k ? oa[0] : kNowhere, fb = !BK_ || kb < k ? ob[0] : kNowhere;
+        if constexpr (PA && AK) {
 #pragma unroll
-        for (int i = 0; i < TA::PER; ++i)
-            lds_load16(bufa, at + (i * NT + w * 64) * 16, OA > 1 ? oa[OA > 1 ? i : 0] : fa + i * step_a);
+            for (int i = 0; i < TA::PER; ++i) {
+                const int r = i * (NT / 8) + w * 8;  // the wave's first row
+                lds_load16(half_buffer(next_a, TA::second(r) ? pair_a : 0, rows_a * lda), at + (i * NT + w * 64) * 16,
+                           fa + TA::line(r) * lda);
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < TB::PER; ++i)
-            lds_load16(bufb, bt + (i * NT + w * 64) * 16, OB > 1 ? ob[OB > 1 ? i : 0] : fb + i * step_b);
+            for (int i = 0; i < TA::PER; ++i)
+                lds_load16(bufa, at + (i * NT + w * 64) * 16, OA > 1 ? oa[OA > 1 ? i : 0] : fa + i * step_a);
+        }
+        if constexpr (PB && BK_) {
+#pragma unroll
+            for (int i = 0; i < TB::PER; ++i) {
+                const int r = i * (NT / 8) + w * 8;
+                lds_load16(half_buffer(next_b, TB::second(r) ? pair_b : 0, rows_b * ldb), bt + (i * NT + w * 64) * 16,
+                           fb + TB::line(r) * ldb);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TB::PER; ++i)
+                lds_load16(bufb, bt + (i * NT + w * 64) * 16, OB > 1 ? ob[OB > 1 ? i : 0] : fb + i * step_b);
+        }
         next_a += AK ? 128 : BK * lda;
         next_b += BK_ ? 128 : BK * ldb;
         left -= BK;
@@ -238,7 +276,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     }
     tiles_landed<0>();  // the last loads too, zeros: the tiles' LDS is free
     char *own = (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN>();
-    gemm_write<T, FM, FN>(g, m0 + wm, n0 + wn, s, l, own, acc);
+    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, own, acc);
 }
 
 #define OPS_STAGE(i, BM, BN)                              \
@@ -274,8 +312,10 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     OPS_DIRECT(4, name, T, 128, 128, 2, 2)    \
     OPS_DIRECT(4, name, T, 64, 64, 2, 2)
 
+#ifndef OPS_GATED
 OPS_DIRECT_TYPE(bf16, bf16)
 OPS_DIRECT_TYPE(f16, f16)
 OPS_DIRECT(2, f32, float, 128, 128, 2, 2)
 OPS_DIRECT(4, f32, float, 64, 64, 2, 2)
 OPS_DIRECT(2, f32, float, 64, 64, 2, 2)
+#endif

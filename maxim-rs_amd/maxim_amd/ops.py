@@ -75,6 +75,10 @@ def _lib():
             "mxh_dense_workspace": [M, M, M, B],
             "mxh_dense_backward": [I, V, M, M, M, M, I, F, M, M, N, V, U],
             "mxh_dense_backward_workspace": [M, M, M, I, M, M, N, B],
+            "mxh_gated": [I, V, M, M, N, I, F, M, M, V, U],
+            "mxh_gated_workspace": [M, M, M, B],
+            "mxh_gated_backward": [I, V, M, M, M, M, I, F, M, M, N, V, U],
+            "mxh_gated_backward_workspace": [M, M, M, M, M, N, B],
         }
         for name, args in sig.items():
             f = getattr(L, name)
@@ -177,6 +181,15 @@ def _new(x, X, n, planar):
         if by_rows != planar:
             t = t.movedim(-1, 0) if planar else t.movedim(0, -1)
     return t, Mat(t.data_ptr(), X.rows, n, 1 if by_rows else n, X.rows if by_rows else 1, X.dtype, 0)
+
+
+def _like_weight(w, W):
+    """An uninitialised result of a weight's shape, in its memory order."""
+    if W.col_stride == 1:
+        t = w.new_empty(w.shape)
+        return t, Mat(t.data_ptr(), W.rows, W.cols, W.cols, 1, W.dtype, 0)
+    t = w.new_empty((W.cols, W.rows)).t()
+    return t, Mat(t.data_ptr(), W.rows, W.cols, 1, W.rows, W.dtype, 0)
 
 
 def _workspace(n, x):
@@ -287,10 +300,7 @@ def dense_backward(dy, x, w, z=None, act=None, slope=0.0, planar=False, dx=True,
     if dx:
         gx, DX = _new(x, X, X.cols, planar)
     if dw:
-        # in w's own memory order
-        gw = w.new_empty(w.shape) if W.col_stride == 1 else w.new_empty((W.cols, W.rows)).t()
-        DW = (Mat(gw.data_ptr(), W.rows, W.cols, W.cols, 1, W.dtype, 0) if W.col_stride == 1 else
-              Mat(gw.data_ptr(), W.rows, W.cols, 1, W.rows, W.dtype, 0))
+        gw, DW = _like_weight(w, W)
     if db:
         gb = w.new_empty(W.rows, dtype=db_dtype)
         DB = _vec(gb, "db", d)
@@ -298,4 +308,47 @@ def dense_backward(dy, x, w, z=None, act=None, slope=0.0, planar=False, dx=True,
     _check(_L.mxh_dense_backward_workspace(DY, X, W, a, DX, DW, DB, size))
     ws = _workspace(size.value, x)
     _check(_L.mxh_dense_backward(d, _stream(d), DY, X, W, Z, a, slope, DX, DW, DB, _ptr(ws), size.value))
+    return gx, gw, gb
+
+
+def gated(x, w, bias=None, act="silu", slope=0.0, planar=False, save=False, out=None):
+    """mxh_gated: act(a) * c for (a | c) = x w^T + bias, w [2 n][k] with the
+    gate's n rows first, or with save (y, z), z = (a | c) for gated_backward."""
+    d = _device(x)
+    f = _act(act)
+    X = _mat(x, "x", d, planar)
+    W = _mat(w, "w", d, False)
+    B = None if bias is None else _vec(bias, "bias", d)
+    y, Y = _new(x, X, W.rows // 2, planar) if out is None else (out, _mat(out, "out", d, planar))
+    z, Z = _new(y, Y, W.rows, planar) if save else (None, None)
+    size = C.c_uint64()
+    _check(_L.mxh_gated_workspace(X, W, Y, size))
+    ws = _workspace(size.value, x)
+    _check(_L.mxh_gated(d, _stream(d), X, W, B, f, slope, Y, Z, _ptr(ws), size.value))
+    _written(out)
+    return (y, z) if save else y
+
+
+def gated_backward(dy, x, w, z, act="silu", slope=0.0, planar=False, dx=True, dw=True, db=True, db_dtype=None):
+    """mxh_gated_backward: (dx, dw, db) of gated(x, w, bias, act, slope), None
+    where one is off. db is of w's type or db_dtype (the bias's: w's or
+    float32)."""
+    d = _device(x)
+    f = _act(act)
+    X = _mat(x, "x", d, planar)
+    DY = _mat(dy, "dy", d, planar)
+    W = _mat(w, "w", d, False)
+    Z = _mat(z, "z", d, planar)
+    gx = gw = gb = DX = DW = DB = None
+    if dx:
+        gx, DX = _new(x, X, X.cols, planar)
+    if dw:
+        gw, DW = _like_weight(w, W)
+    if db:
+        gb = w.new_empty(W.rows, dtype=db_dtype)
+        DB = _vec(gb, "db", d)
+    size = C.c_uint64()
+    _check(_L.mxh_gated_backward_workspace(DY, X, W, DX, DW, DB, size))
+    ws = _workspace(size.value, x)
+    _check(_L.mxh_gated_backward(d, _stream(d), DY, X, W, Z, f, slope, DX, DW, DB, _ptr(ws), size.value))
     return gx, gw, gb
