@@ -1,6 +1,8 @@
 /*
  * maxim_block_ops.h - operators of a feed-forward block beside LayerNorm and
- * Dense (maxim_ops.h): the gated Dense, forward and backward.
+ * Dense (maxim_ops.h): the gated Dense, forward and backward; the gradients'
+ * global norm and clipping, between a backward pass and the optimizer; and
+ * Dense with weights in 4-bit blocks, for serving.
  *
  * Everything that maxim_ops.h says of operands, alignment, sizes, precision,
  * streams, captures, workspaces and errors holds here too; mxh_ops_ready loads
@@ -38,6 +40,68 @@ int mxh_gated_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
                        const mxh_vec *db, void *workspace, uint64_t workspace_bytes);
 int mxh_gated_backward_workspace(const mxh_mat *dy, const mxh_mat *x, const mxh_mat *w, const mxh_mat *dx,
                                  const mxh_mat *dw, const mxh_vec *db, uint64_t *bytes);
+
+/*
+ * The global norm of a list of gradients, N = sqrt(sum of all elements'
+ * squares), as one fp32 value on the device (0 of no elements). `grads` is
+ * host memory: `count` contiguous tensors of any types and sizes, zero among
+ * them; the call has read it when it returns. Squares and their sums are
+ * formed in 64 bits, so N is rounded once and infinite only past fp32's range,
+ * or with an infinity among the elements (NaN with a NaN).
+ */
+int mxh_grad_norm(int device, void *stream, const mxh_vec *grads, int64_t count, float *norm, void *workspace,
+                  uint64_t workspace_bytes);
+int mxh_grad_norm_workspace(const mxh_vec *grads, int64_t count, uint64_t *bytes);
+
+/*
+ * The same, and out[i] = grads[i] * (max_norm / N) where N > max_norm; else,
+ * and where N is not finite (a step that the caller skips), out[i] = grads[i].
+ * out NULL, or an out[i].data of grads[i].data: in place, with nothing written
+ * where nothing changes. Each out[i] has its gradient's size and type and lies
+ * apart from every other tensor. mxh_grad_norm_workspace gives the bytes.
+ */
+int mxh_grad_clip(int device, void *stream, const mxh_vec *grads, const mxh_vec *out, int64_t count, float max_norm,
+                  float *norm, void *workspace, uint64_t workspace_bytes);
+/* By a norm on the device that the caller has, as one added up over ranks. */
+int mxh_grad_clip_by(int device, void *stream, const mxh_vec *grads, const mxh_vec *out, int64_t count, float max_norm,
+                     const float *norm);
+
+/*
+ * A matrix [rows][cols] in blocks of 32 features with 4 bits an element (1
+ * sign, 2 exponent, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) and a scale of
+ * 8 bits, 2^(s - 127), 255 for NaN: 17 bytes for 32 elements.
+ *
+ * codes: a line of ceil(cols / 256) * 128 bytes a row, an element's code in the
+ * low half of its byte where its feature is even; scales: for 64 rows and 256
+ * features 512 bytes, that of row r and block b at [r / 64][b / 8][b % 4][r %
+ * 16][r / 16 % 4][b / 4 % 2]. Elements past the last feature are 0. Both are
+ * 16-byte aligned; mxh_mx4_size gives their bytes.
+ */
+typedef struct mxh_mx4 {
+    void *codes, *scales;
+    int64_t rows, cols;
+} mxh_mx4;
+int mxh_mx4_size(int64_t rows, int64_t cols, uint64_t *codes, uint64_t *scales);
+
+/*
+ * With m a block's largest magnitude: s - 127 = floor(log2 m) - 2, at least
+ * -127, and each element is x / 2^(s - 127) rounded to the nearest code, ties to
+ * even, 6 at most. A block with an infinity or a NaN is NaN. x of any type and
+ * either memory order; back, each value is rounded to y's type.
+ */
+int mxh_mx4_quantize(int device, void *stream, const mxh_mat *x, const mxh_mx4 *q);
+int mxh_mx4_dequantize(int device, void *stream, const mxh_mx4 *q, const mxh_mat *y);
+
+/*
+ * y = act(X W^T + bias) + residual with W = w [n][k] and X = x [rows][k] in the
+ * values of 4-bit blocks, x quantised in the call, the products on the matrix
+ * cores and summed in fp32. bias (of x's type or fp32) and residual may be
+ * NULL. residual and y have x's type and one memory order, x any. y may be the
+ * residual itself.
+ */
+int mxh_mx4_dense(int device, void *stream, const mxh_mat *x, const mxh_mx4 *w, const mxh_vec *bias, int act, float slope,
+                  const mxh_mat *residual, const mxh_mat *y, void *workspace, uint64_t workspace_bytes);
+int mxh_mx4_dense_workspace(const mxh_mat *x, const mxh_mx4 *w, const mxh_mat *y, uint64_t *bytes);
 
 #ifdef __cplusplus
 }

@@ -9,7 +9,7 @@
 #include <mutex>
 #include <vector>
 
-extern "C" const unsigned char mx_ops_hsaco[], mx_gated_hsaco[];
+extern "C" const unsigned char mx_ops_hsaco[], mx_gated_hsaco[], mx_grads_hsaco[], mx_mx4_hsaco[];
 
 namespace mxops {
 
@@ -20,7 +20,9 @@ struct Object {
     const char *what;
 };
 const Object kObjects[] = {{"mxo_", mx_ops_hsaco, "hipModuleLoadData (operators' gfx950 code object)"},
-                           {"mxg_", mx_gated_hsaco, "hipModuleLoadData (gated operators' gfx950 code object)"}};
+                           {"mxg_", mx_gated_hsaco, "hipModuleLoadData (gated operators' gfx950 code object)"},
+                           {"mxn_", mx_grads_hsaco, "hipModuleLoadData (gradient norm's gfx950 code object)"},
+                           {"mxq_", mx_mx4_hsaco, "hipModuleLoadData (4-bit operators' gfx950 code object)"}};
 constexpr int kNumObjects = sizeof(kObjects) / sizeof(kObjects[0]);
 
 struct Code {

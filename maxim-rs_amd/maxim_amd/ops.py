@@ -38,6 +38,11 @@ class Vec(C.Structure):
     _fields_ = [("data", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Mx4Mat(C.Structure):
+    """mxh_mx4"""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64)]
+
+
 _L = None
 _torch = None
 _forward_ad = None
@@ -66,6 +71,7 @@ def _lib():
         L = _hip_lib()
         V, I, F, U = C.c_void_p, C.c_int, C.c_float, C.c_uint64
         M, N, B = C.POINTER(Mat), C.POINTER(Vec), C.POINTER(C.c_uint64)
+        Q = C.POINTER(Mx4Mat)
         sig = {
             "mxh_ops_ready": [I],
             "mxh_layernorm": [I, V, M, N, N, F, M, V, V],
@@ -79,6 +85,15 @@ def _lib():
             "mxh_gated_workspace": [M, M, M, B],
             "mxh_gated_backward": [I, V, M, M, M, M, I, F, M, M, N, V, U],
             "mxh_gated_backward_workspace": [M, M, M, M, M, N, B],
+            "mxh_grad_norm": [I, V, N, C.c_int64, V, V, U],
+            "mxh_grad_norm_workspace": [N, C.c_int64, B],
+            "mxh_grad_clip": [I, V, N, N, C.c_int64, F, V, V, U],
+            "mxh_grad_clip_by": [I, V, N, N, C.c_int64, F, V],
+            "mxh_mx4_size": [C.c_int64, C.c_int64, B, B],
+            "mxh_mx4_quantize": [I, V, M, Q],
+            "mxh_mx4_dequantize": [I, V, Q, M],
+            "mxh_mx4_dense": [I, V, M, Q, N, I, F, M, M, V, U],
+            "mxh_mx4_dense_workspace": [M, Q, M, B],
         }
         for name, args in sig.items():
             f = getattr(L, name)
@@ -352,3 +367,165 @@ def gated_backward(dy, x, w, z, act="silu", slope=0.0, planar=False, dx=True, dw
     ws = _workspace(size.value, x)
     _check(_L.mxh_gated_backward(d, _stream(d), DY, X, W, Z, f, slope, DX, DW, DB, _ptr(ws), size.value))
     return gx, gw, gb
+
+
+def _filled(t, what):
+    """The tensor's elements lie side by side, in whatever order."""
+    if t.is_contiguous():
+        return
+    at = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != at:
+            raise P.MaximError("%s: its elements do not fill its storage (shape %s, strides %s)"
+                               % (what, tuple(t.shape), t.stride()))
+        at *= size
+
+
+def _list(tensors, what, device):
+    """Tensors as an array of vectors of their elements."""
+    a = (Vec * len(tensors))()
+    for i, t in enumerate(tensors):
+        name = "%s[%d]" % (what, i)
+        code = _tensor(t, name, device)
+        n = t.numel()
+        if n:
+            _filled(t, name)
+        v = a[i]
+        v.data, v.n, v.dtype = t.data_ptr(), n, code
+    return a
+
+
+def _grads(grads):
+    grads = list(grads)
+    if not grads:
+        raise P.MaximError("grads: no tensors")
+    _lib()
+    if not isinstance(grads[0], _torch.Tensor) or not grads[0].is_cuda:
+        raise P.MaximError("grads[0]: not a tensor on the card")
+    return grads, grads[0].get_device()
+
+
+def _norm_workspace(a, like):
+    size = C.c_uint64()
+    _check(_L.mxh_grad_norm_workspace(a, len(a), size))
+    return _workspace(size.value, like), size.value
+
+
+def grad_norm(grads):
+    """mxh_grad_norm: the 2-norm of all the tensors' elements together, an fp32
+    tensor of no dimensions on their device."""
+    grads, d = _grads(grads)
+    a = _list(grads, "grads", d)
+    norm = grads[0].new_empty((), dtype=_torch.float32)
+    ws, n = _norm_workspace(a, grads[0])
+    _check(_L.mxh_grad_norm(d, _stream(d), a, len(a), norm.data_ptr(), _ptr(ws), n))
+    return norm
+
+
+def clip_grads(grads, max_norm, norm=None, out=None):
+    """mxh_grad_clip: scales the tensors in place, or into the tensors of out, by
+    max_norm / N where their global norm N is larger than max_norm (and finite),
+    and returns N. With norm (an fp32 tensor of one element, such as one added
+    up over ranks) that is taken as N."""
+    grads, d = _grads(grads)
+    a = _list(grads, "grads", d)
+    b = None
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads):
+            raise P.MaximError("out: %d tensors for %d gradients" % (len(out), len(grads)))
+        for i, (g, o) in enumerate(zip(grads, out)):
+            if o is not g and (o.shape != g.shape or o.stride() != g.stride()):
+                raise P.MaximError("out[%d]: not its gradient's shape and strides" % i)
+        b = _list(out, "out", d)
+    if norm is None:
+        norm = grads[0].new_empty((), dtype=_torch.float32)
+        ws, n = _norm_workspace(a, grads[0])
+        _check(_L.mxh_grad_clip(d, _stream(d), a, b, len(a), max_norm, norm.data_ptr(), _ptr(ws), n))
+    else:
+        if _tensor(norm, "norm", d) != 0 or norm.numel() != 1:
+            raise P.MaximError("norm: not one fp32 value")
+        _check(_L.mxh_grad_clip_by(d, _stream(d), a, b, len(a), max_norm, norm.data_ptr()))
+    for t in grads if out is None else out:
+        _written(t)
+    return norm
+
+
+class Mx4:
+    """A tensor in 4-bit blocks along its features (mxh_mx4): `codes` and
+    `scales` (uint8, on the card), `shape` (positions, then features) and the
+    `dtype` of the tensor that it was made from."""
+
+    def __init__(self, codes, scales, shape, dtype):
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
+
+    def _mat(self):
+        rows = 1
+        for n in self.shape[:-1]:
+            rows *= n
+        return Mx4Mat(self.codes.data_ptr(), self.scales.data_ptr(), rows, self.shape[-1])
+
+    def plain(self):
+        """(codes, scales) as [rows][features / 2 bytes] and [rows][blocks]
+        tensors: the order in which others keep such blocks."""
+        m = self._mat()
+        tiles, groups, blocks = (m.cols + 255) // 256, (m.rows + 63) // 64, (m.cols + 31) // 32
+        s = self.scales.view(groups, tiles, 4, 16, 4, 2).permute(0, 4, 3, 1, 5, 2).reshape(groups * 64, tiles * 8)
+        return self.codes.view(m.rows, tiles * 128)[:, :(m.cols + 1) // 2], s[:m.rows, :blocks]
+
+
+def mx4_quantize(x, planar=False):
+    """mxh_mx4_quantize: x as an Mx4, in blocks along its features."""
+    d = _device(x)
+    X = _mat(x, "x", d, planar)
+    codes, scales = C.c_uint64(), C.c_uint64()
+    _check(_L.mxh_mx4_size(X.rows, X.cols, codes, scales))
+    shape = tuple(x.shape[1:]) + (x.shape[0],) if planar else tuple(x.shape)
+    q = Mx4(x.new_empty(codes.value, dtype=_torch.uint8), x.new_empty(scales.value, dtype=_torch.uint8), shape, x.dtype)
+    _check(_L.mxh_mx4_quantize(d, _stream(d), X, Mx4Mat(q.codes.data_ptr(), q.scales.data_ptr(), X.rows, X.cols)))
+    return q
+
+
+def _mx4(q, what, device):
+    if not isinstance(q, Mx4):
+        raise P.MaximError("%s: not an Mx4" % what)
+    for t in (q.codes, q.scales):
+        if not t.is_cuda or t.get_device() != device:
+            raise P.MaximError("%s: on another device than x" % what)
+    return q._mat()
+
+
+def mx4_dequantize(q, dtype=None, planar=False):
+    """mxh_mx4_dequantize: the values that an Mx4 stands for, as a tensor of
+    dtype (the original's if None)."""
+    _lib()
+    if not isinstance(q, Mx4):
+        raise P.MaximError("q: not an Mx4")
+    d = q.codes.get_device()
+    m = _mx4(q, "q", d)
+    dtype = dtype or q.dtype
+    y = q.codes.new_empty((q.shape[-1],) + q.shape[:-1] if planar else q.shape, dtype=dtype)
+    Y = (Mat(y.data_ptr(), m.rows, m.cols, 1, m.rows, 0, 0) if planar else
+         Mat(y.data_ptr(), m.rows, m.cols, m.cols, 1, 0, 0))
+    Y.dtype = _tensor(y, "y", d)
+    _check(_L.mxh_mx4_dequantize(d, _stream(d), m, Y))
+    return y
+
+
+def mx4_dense(x, w, bias=None, act=None, slope=0.0, residual=None, planar=False, out=None):
+    """mxh_mx4_dense: act(X W^T + bias) + residual with w an Mx4 of [n][k] and x
+    taken to 4-bit blocks in the call. out may be the residual."""
+    d = _device(x)
+    a = _act(act)
+    X = _mat(x, "x", d, planar)
+    W = _mx4(w, "w", d)
+    B = None if bias is None else _vec(bias, "bias", d)
+    R = None if residual is None else _mat(residual, "residual", d, planar)
+    like, Like = (x, X) if residual is None else (residual, R)
+    y, Y = _new(like, Like, W.rows, planar) if out is None else (out, _mat(out, "out", d, planar))
+    size = C.c_uint64()
+    _check(_L.mxh_mx4_dense_workspace(X, W, Y, size))
+    ws = _workspace(size.value, x)
+    _check(_L.mxh_mx4_dense(d, _stream(d), X, W, B, a, slope, R, Y, _ptr(ws), size.value))
+    _written(out)
+    return y
