@@ -56,6 +56,20 @@ __device__ __forceinline__ void store_upto(T *p, const Vec<T, N> &v, int64_t hav
         if (i < have) p[i] = v.v[i];
 }
 
+// The same for results, which nothing in this launch reads again: not kept in
+// L2, whose dirty lines are written back only when the kernel ends.
+template <typename T, int N>
+__device__ __forceinline__ void store_out(T *p, const Vec<T, N> &v, int64_t have) {
+    if (have >= N) {
+        if constexpr (sizeof(v) == 16)
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4 *>(p));
+        else
+            store_n<T, N>(p, v);
+        return;
+    }
+    store_upto<T, N>(p, v, have);
+}
+
 // E elements at p, of which the first `have` are the operand's and the others
 // anything, for the user to leave out (left out here, a load ahead of its use
 // would be waited for). WHOLE: all of them or none (the extent is a multiple of E). A lane

@@ -44,15 +44,15 @@ __device__ __forceinline__ void gated_finish(const OpsGemmArgs &g, int64_t m, in
         T *z = static_cast<T *>(g.z) + m * g.ldz + n;
 #pragma unroll
         for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(a[e]);
-        store_upto<T, E>(z, o, have);
+        store_out<T, E>(z, o, have);
 #pragma unroll
         for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(c[e]);
-        store_upto<T, E>(z + (PAIR == PAIR_N ? (int64_t)g.n : g.m * g.ldz), o, have);
+        store_out<T, E>(z + (PAIR == PAIR_N ? (int64_t)g.n : g.m * g.ldz), o, have);
     }
     act_fwd_n<E>(g.act, g.slope, a);
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(a[e] * c[e]);
-    store_upto<T, E>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
+    store_out<T, E>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
 }
 
 // Where split s's partial sums of row m, column n of a half lie: [splits][m][2 n]
@@ -81,24 +81,20 @@ __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, in
     const int lr = l / LANES, lc = l % LANES * E;
     const int64_t n = n0 + lc;
     float ba[E], bc[E];
-    if (g.splits == 1) gated_bias_cols<T, E>(g, n, ba, bc);
-#pragma unroll
-    for (int i = 0; i < FM / 2; ++i) {
-        const int64_t m = m0 + i * TALL + lr;
+    const bool whole = g.splits == 1;
+    if (whole) gated_bias_cols<T, E>(g, n, ba, bc);
+#pragma unroll 1
+    for (int h = 0; h < FM / 2; ++h) {
+        const int64_t m = m0 + h * TALL + lr;
         GatedBias<T> row[STEPS];
-        if (PAIR == PAIR_M && g.splits == 1) {
+        if (PAIR == PAIR_M && whole) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) row[k] = gated_bias_row<T>(g, m + k * ROWS);
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                *reinterpret_cast<f32x4 *>(own + (h * 16 + (l & 15)) * LD + j * 16 + (l >> 4) * 4) =
-                    acc[PAIR == PAIR_N ? 2 * i + h : i + h * (FM / 2)][j];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        for (int i = 0; i < FM / 2; ++i)
+            if (i == h) put_rows(own, l, acc, PAIR == PAIR_N ? 2 * i : i, PAIR == PAIR_N ? 2 * i + 1 : i + FM / 2);
+        wave_fence();
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
             float a[E], c[E];
@@ -108,7 +104,7 @@ __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, in
                 *reinterpret_cast<f32x4 *>(a + e) = *reinterpret_cast<const f32x4 *>(p + e);
                 *reinterpret_cast<f32x4 *>(c + e) = *reinterpret_cast<const f32x4 *>(p + OTHER + e);
             }
-            if (g.splits == 1) {
+            if (whole) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     a[e] += PAIR == PAIR_M ? row[k].a : ba[e];
@@ -121,9 +117,7 @@ __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, in
                 store_upto<float, E>(o + gated_part_half<PAIR>(g), __builtin_bit_cast(Vec<float, E>, c), g.n - n);
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_fence();
     }
 }
 

@@ -304,7 +304,7 @@ __device__ __forceinline__ void gemm_finish(const OpsGemmArgs &g, int64_t m, int
     if (g.z) {
 #pragma unroll
         for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(v[e]);
-        store_upto<T, E>(static_cast<T *>(g.z) + m * g.ldz + n, o, have);
+        store_out<T, E>(static_cast<T *>(g.z) + m * g.ldz + n, o, have);
     }
     act_fwd_n<E>(g.act, g.slope, v);
     if (g.res) {
@@ -313,7 +313,7 @@ __device__ __forceinline__ void gemm_finish(const OpsGemmArgs &g, int64_t m, int
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(v[e]);
-    store_upto<T, E>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
+    store_out<T, E>(static_cast<T *>(g.c) + m * g.ldc + n, o, have);
 }
 
 // Which tile and split a block takes. Consecutive blocks go to the 8 XCDs in
@@ -337,12 +337,33 @@ __device__ __forceinline__ void gemm_place(const OpsGemmArgs &g, int &tm, int &t
 // (`at`, gemm_write_bytes<FN>() of it), rows four floats longer than they are
 // so that 16 rows' writes fall into different banks; what comes back is 16
 // bytes of results a lane, whole lines of C a wave, with the bias of a lane's
-// columns held in registers and the residual on its way before the sums.
+// columns held in registers and the residual on its way before the sums. A loop
+// in the code too, and stores past the caches (store_out): unrolled, a 256 x 256
+// tile's epilogue was 75 KB of instructions that each wave fetches once, and
+// its results waited in L2 for the kernel's end: 4096 x 4096 bf16 results of
+// two steps of k (4-bit operands) took 22 us, so 14; 4096^3 in bf16 111, so 105.
 // (Written from the accumulators, with a bias load each, a 256 x 256 tile's
 // 32 quads a lane took 49 us.)
 template <int FN>
 constexpr int gemm_write_bytes() {
     return 32 * (FN * 16 + 4) * 4;
+}
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// Blocks `first` and `second` (rows of them) of the sums into the wave's 32
+// rows of LDS.
+template <int FM, int FN>
+__device__ __forceinline__ void put_rows(float *own, int l, const f32x4 (&acc)[FM][FN], int first, int second) {
+    constexpr int LD = FN * 16 + 4;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        float *p = own + (l & 15) * LD + j * 16 + (l >> 4) * 4;
+        *reinterpret_cast<f32x4 *>(p) = acc[first][j];
+        *reinterpret_cast<f32x4 *>(p + 16 * LD) = acc[second][j];
+    }
 }
 template <typename T, int FM, int FN, int PAIR>
 __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
@@ -359,42 +380,37 @@ __device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int
     float *own = reinterpret_cast<float *>(at);
     const int lr = l / LANES, lc = l % LANES * E;
     const int64_t n = n0 + lc;
+    const bool whole = g.splits == 1;
     float bias[E];
-    if (g.splits == 1) bias_fetch<T, E>(g, n, bias);
+    if (whole) bias_fetch<T, E>(g, n, bias);
+    constexpr int AT = STEPS < 4 ? STEPS : 4;  // steps at a time
+#pragma unroll 1
+    for (int u = 0; u < FM / 2 * STEPS; u += AT) {
+        const int64_t m = m0 + u * ROWS + lr;
+        Extra<T, E> x[AT];
+        if (whole && (g.res || g.bias_rows)) {
 #pragma unroll
-    for (int i = 0; i < FM; i += 2) {
-        const int64_t m = m0 + i * 16 + lr;
-        Extra<T, E> x[STEPS];
-        if (g.splits == 1 && (g.res || g.bias_rows)) {
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) extra_fetch<T, E>(g, m + k * ROWS, n, x[k]);
+            for (int k = 0; k < AT; ++k) extra_fetch<T, E>(g, m + k * ROWS, n, x[k]);
         }
+        if (AT == STEPS || u % STEPS == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int i = 0; i < FM / 2; ++i)
+                if (i == u / STEPS) put_rows(own, l, acc, 2 * i, 2 * i + 1);
+        }
+        wave_fence();
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
-                *reinterpret_cast<f32x4 *>(own + (h * 16 + (l & 15)) * LD + j * 16 + (l >> 4) * 4) = acc[i + h][j];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
+        for (int k = 0; k < AT; ++k) {
             float v[E];
-            const float *p = own + (k * ROWS + lr) * LD + lc;
+            const float *p = own + ((u % STEPS + k) * ROWS + lr) * LD + lc;
 #pragma unroll
             for (int e = 0; e < E; e += 4) *reinterpret_cast<f32x4 *>(v + e) = *reinterpret_cast<const f32x4 *>(p + e);
-            if (g.splits == 1) {
+            if (whole)
                 gemm_finish<T, E>(g, m + k * ROWS, n, v, bias, x[k]);
-            } else if (m + k * ROWS < g.m && n < g.n) {
-                Vec<float, E> o;
-#pragma unroll
-                for (int e = 0; e < E; ++e) o.v[e] = v[e];
-                store_upto<float, E>(g.part + ((int64_t)s * g.m + m + k * ROWS) * g.n + n, o, g.n - n);
-            }
+            else if (m + k * ROWS < g.m && n < g.n)
+                store_upto<float, E>(g.part + ((int64_t)s * g.m + m + k * ROWS) * g.n + n,
+                                     __builtin_bit_cast(Vec<float, E>, v), g.n - n);
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_fence();
     }
 }
 
