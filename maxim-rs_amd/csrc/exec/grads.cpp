@@ -56,36 +56,11 @@ static std::vector<GradsLaunch> cut(const mxh_vec *grads, const mxh_vec *out, in
     return launches;
 }
 
-static void launch(int dev, const char *name, int64_t grid, void *stream, void *args) {
+static void launch(int dev, const char *name, int64_t grid, unsigned block, void *stream, void *args) {
     void *params[] = {args};
-    check(hip().hipModuleLaunchKernel(function(dev, name), (unsigned)grid, 1, 1, 256, 1, 1, 0, (mxh::hipStream_t)stream,
+    check(hip().hipModuleLaunchKernel(function(dev, name), (unsigned)grid, 1, 1, block, 1, 1, 0, (mxh::hipStream_t)stream,
                                       params, nullptr),
           name);
-}
-
-static int64_t parts_of(const std::vector<GradsLaunch> &launches) {
-    int64_t n = 0;
-    for (const GradsLaunch &l : launches) n += l.grid;
-    return n;
-}
-// One block writes the norm itself.
-static uint64_t norm_bytes(const std::vector<GradsLaunch> &launches) {
-    const int64_t n = parts_of(launches);
-    return n <= 1 ? 0 : (uint64_t)n * 8;
-}
-
-static void run_norm(int device, void *stream, std::vector<GradsLaunch> &launches, float *norm, void *workspace) {
-    double *part = static_cast<double *>(workspace);
-    const int64_t parts = parts_of(launches);
-    for (GradsLaunch &l : launches) {
-        l.args.part = part;
-        l.args.norm = parts == 1 ? norm : nullptr;
-        launch(device, "mxn_squares", l.grid, stream, &l.args);
-        part += l.grid;
-    }
-    if (parts == 1) return;
-    GradsJoinArgs j{static_cast<double *>(workspace), norm, (int32_t)parts, 0};
-    launch(device, "mxn_norm", 1, stream, &j);
 }
 
 static void run_clip(int device, void *stream, std::vector<GradsLaunch> &launches, const float *norm, float max_norm) {
@@ -94,8 +69,47 @@ static void run_clip(int device, void *stream, std::vector<GradsLaunch> &launche
         GradsLaunch &l = launches[i];
         l.args.norm = const_cast<float *>(norm);
         l.args.max_norm = max_norm;
-        launch(device, "mxn_clip", l.grid, stream, &l.args);
+        launch(device, "mxn_clip", l.grid, 256, stream, &l.args);
     }
+}
+
+// The sum, and clipping, in one launch of one block.
+constexpr int64_t kFewChunks = 16;
+static bool few(const std::vector<GradsLaunch> &launches) {
+    return launches.empty() || (launches.size() == 1 && launches[0].grid <= kFewChunks);
+}
+static uint64_t norm_bytes(const std::vector<GradsLaunch> &launches) {
+    uint64_t n = 0;
+    if (!few(launches))
+        for (const GradsLaunch &l : launches) n += l.grid * 8;
+    return n;
+}
+
+// The norm, and where `clip` the results.
+static void run(int device, void *stream, std::vector<GradsLaunch> &launches, float *norm, void *workspace, bool clip,
+                float max_norm) {
+    if (launches.empty()) {  // no elements: the norm alone, 0
+        launches.emplace_back();
+        launches[0].args.count = 0;
+        launches[0].args.first[0] = 0;
+    }
+    if (few(launches)) {
+        GradsArgs &a = launches[0].args;
+        a.norm = norm;
+        a.clip = clip;
+        a.max_norm = max_norm;
+        launch(device, "mxn_small", 1, 1024, stream, &a);
+        return;
+    }
+    double *part = static_cast<double *>(workspace);
+    for (GradsLaunch &l : launches) {
+        l.args.part = part;
+        launch(device, "mxn_squares", l.grid, 256, stream, &l.args);
+        part += l.grid;
+    }
+    GradsJoinArgs j{static_cast<double *>(workspace), norm, (int32_t)(part - static_cast<double *>(workspace)), 0};
+    launch(device, "mxn_norm", 1, 256, stream, &j);
+    if (clip) run_clip(device, stream, launches, norm, max_norm);
 }
 
 static void check_norm(const float *norm) {
@@ -165,7 +179,7 @@ int mxh_grad_norm(int device, void *stream, const mxh_vec *grads, int64_t count,
         std::vector<GradsLaunch> launches = cut(grads, nullptr, count);
         check_workspace(workspace, workspace_bytes, norm_bytes(launches));
         OnDevice on(device);
-        run_norm(device, stream, launches, norm, workspace);
+        run(device, stream, launches, norm, workspace, false, 0.0f);
     });
 }
 
@@ -178,8 +192,7 @@ int mxh_grad_clip(int device, void *stream, const mxh_vec *grads, const mxh_vec 
         std::vector<GradsLaunch> launches = cut(grads, out, count);
         check_workspace(workspace, workspace_bytes, norm_bytes(launches));
         OnDevice on(device);
-        run_norm(device, stream, launches, norm, workspace);
-        run_clip(device, stream, launches, norm, max_norm);
+        run(device, stream, launches, norm, workspace, true, max_norm);
     });
 }
 

@@ -15,9 +15,9 @@ struct GradsArgs {
     uint32_t first[MXN_TENSORS + 1];
     int32_t count;
     double *part;        // a block's sum of squares each
-    float *norm;         // one block: written; clipping: read
+    float *norm;         // clipping: read; few chunks: written
     float max_norm;
-    int32_t pad;
+    int32_t clip;        // few chunks: not the norm alone
 };
 
 struct GradsJoinArgs {
