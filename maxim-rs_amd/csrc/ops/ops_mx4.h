@@ -39,12 +39,14 @@ __device__ __forceinline__ uint32_t mx4_codes(const float *v, float inverse) {
     u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, q[6], q[7], 1.0f, 3);
     return u;
 }
-__device__ __forceinline__ void mx4_values(uint32_t u, float scale, float *v) {
+// Eight codes' values, of which the first four have one scale and the others
+// another.
+__device__ __forceinline__ void mx4_values(uint32_t u, float scale, float scale2, float *v) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
 #define OPS_MX4_PAIR(i)                                                         \
     {                                                                           \
         const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(u, 1.0f, i);   \
-        v[2 * i] = p[0] * scale, v[2 * i + 1] = p[1] * scale;                   \
+        v[2 * i] = p[0] * (i < 2 ? scale : scale2), v[2 * i + 1] = p[1] * (i < 2 ? scale : scale2); \
     }
     OPS_MX4_PAIR(0) OPS_MX4_PAIR(1) OPS_MX4_PAIR(2) OPS_MX4_PAIR(3)
 #undef OPS_MX4_PAIR
@@ -52,24 +54,24 @@ __device__ __forceinline__ void mx4_values(uint32_t u, float scale, float *v) {
 // A scale's place in its group and tile: line r of 64, block b of 8.
 __device__ __forceinline__ int scale_at(int r, int b) { return (b & 3) * 128 + (r & 15) * 8 + (r >> 4) * 2 + (b >> 2); }
 
-// Rows with contiguous features: a block takes 64 rows by a tile, 32 lanes a
-// row with eight elements each, four lanes a block of 32.
+// Rows with contiguous features: a block takes 32 rows (half a group) by a
+// tile, 32 lanes a row with eight elements each, four lanes a block of 32.
 template <typename T>
 __device__ __forceinline__ void mx4_quantize_rows(const Mx4CodeArgs &a) {
-    __shared__ uint32_t sh[128];
+    __shared__ uint32_t sh[64];
     const int t = threadIdx.x, lane = t & 31, tile = blockIdx.x % a.tiles;
-    const int64_t group = blockIdx.x / a.tiles, r0 = group * 64;
+    const int64_t half = blockIdx.x / a.tiles, r0 = half * 32;
     const int64_t k = (int64_t)tile * 256 + lane * 8, have = a.cols - k;
-    if (t < 128) sh[t] = 0;  // scales of rows that are not there
+    if (t < 64) sh[t] = 0;  // scales of rows that are not there
     __syncthreads();
-    Vec<T, 8> x[8];
+    Vec<T, 8> x[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int64_t r = r0 + i * 8 + (t >> 5);
         x[i] = load_upto<T, 8>(static_cast<const T *>(a.x) + min(r, a.rows - 1) * a.rs + k, have);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int row = i * 8 + (t >> 5);
         float v[8];
         uint32_t top = 0;
@@ -83,10 +85,12 @@ __device__ __forceinline__ void mx4_quantize_rows(const Mx4CodeArgs &a) {
         const uint32_t s = mx4_scale(top), u = mx4_codes(v, mx4_inverse(s));
         if (r0 + row >= a.rows) continue;
         *reinterpret_cast<uint32_t *>(a.codes + ((r0 + row) * a.tiles + tile) * 128 + lane * 4) = u;
-        if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(sh)[scale_at(row, lane >> 2)] = (uint8_t)s;
+        // a half group's scales are every other dword of its group's
+        const int at = scale_at(row, lane >> 2);
+        if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(sh)[(at >> 3) * 4 + (at & 3)] = (uint8_t)s;
     }
     __syncthreads();
-    if (t < 128) reinterpret_cast<uint32_t *>(a.scales)[(group * a.tiles + tile) * 128 + t] = sh[t];
+    if (t < 64) reinterpret_cast<uint32_t *>(a.scales)[((half >> 1) * a.tiles + tile) * 128 + t * 2 + (half & 1)] = sh[t];
 }
 
 // Planar order: a block takes 64 positions by a tile, a lane one position of
@@ -130,20 +134,43 @@ template <typename T>
 __device__ __forceinline__ void mx4_dequantize_rows(const Mx4CodeArgs &a) {
     const int t = threadIdx.x, lane = t & 31, tile = blockIdx.x % a.tiles;
     const int64_t group = blockIdx.x / a.tiles, r0 = group * 64;
-    const int64_t k = (int64_t)tile * 256 + lane * 8, have = a.cols - k;
-    if (have <= 0) return;
     const uint8_t *scales = a.scales + (group * a.tiles + tile) * 512;
+    // fp32: a lane's eight elements are four of each half, so that a row's
+    // stores lie side by side
+    constexpr bool WIDE = sizeof(T) == 4;
+    uint32_t u[8];
+    uint8_t s[8], s2[8];
+    // (rows past the last are the last again)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int row = i * 8 + (t >> 5);
-        if (r0 + row >= a.rows) return;
-        float v[8];
-        mx4_values(*reinterpret_cast<const uint32_t *>(a.codes + ((r0 + row) * a.tiles + tile) * 128 + lane * 4),
-                   mx4_power(scales[scale_at(row, lane >> 2)]), v);
-        Vec<T, 8> o;
+        const int row = (int)min((int64_t)(i * 8 + (t >> 5)), a.rows - 1 - r0);
+        const uint8_t *line = a.codes + ((r0 + row) * a.tiles + tile) * 128;
+        if (WIDE) {
+            u[i] = *reinterpret_cast<const uint16_t *>(line + lane * 2) |
+                   (uint32_t) * reinterpret_cast<const uint16_t *>(line + 64 + lane * 2) << 16;
+            s[i] = scales[scale_at(row, lane >> 3)];
+            s2[i] = scales[scale_at(row, 4 + (lane >> 3))];
+        } else {
+            u[i] = *reinterpret_cast<const uint32_t *>(line + lane * 4);
+            s[i] = s2[i] = scales[scale_at(row, lane >> 2)];
+        }
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o.v[e] = from_f<T>(v[e]);
-        store_upto<T, 8>(static_cast<T *>(a.y) + (r0 + row) * a.rs + k, o, have);
+    for (int i = 0; i < 8; ++i) {
+        const int64_t r = r0 + i * 8 + (t >> 5);
+        if (r >= a.rows) return;
+        float v[8];
+        mx4_values(u[i], mx4_power(s[i]), mx4_power(s2[i]), v);
+        T *y = static_cast<T *>(a.y) + r * a.rs;
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int h = 0; h < 8 / E; ++h) {
+            const int64_t k = (int64_t)tile * 256 + h * 128 + lane * E;
+            Vec<T, E> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o.v[e] = from_f<T>(v[h * E + e]);
+            if (k < a.cols) store_out<T, E>(y + k, o, a.cols - k);
+        }
     }
 }
 template <typename T>
@@ -158,7 +185,7 @@ __device__ __forceinline__ void mx4_dequantize_planar(const Mx4CodeArgs &a) {
         T *p = static_cast<T *>(a.y) + r * a.rs + k * a.cs;
         float v[32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx4_values(u[i], scale, v + 8 * i);
+        for (int i = 0; i < 4; ++i) mx4_values(u[i], scale, scale, v + 8 * i);
 #pragma unroll
         for (int e = 0; e < 32; ++e)
             if (e < have) p[e * a.cs] = from_f<T>(v[e]);
