@@ -283,8 +283,9 @@ __device__ __forceinline__ void mx4_gemm(const Mx4GemmArgs &m, const Stage (&st)
     const int part = TT::lane_part(l);
     constexpr int HM = FM / 2;
     u32x4 fa[2][HM], fb[2][FN];
-    // a tile's scales: a dword has two fragments' bytes of both halves of k
-    uint32_t xa[FM / 2], xb[FN / 2];
+    // a tile's scales, and the next one's: a dword has two fragments' bytes of
+    // both halves of k
+    uint32_t xa[FM / 2], xb[FN / 2], ya[FM / 2], yb[FN / 2];
     auto take = [&](const LdsChar *at, int base, int kk) {
         return __builtin_bit_cast(u32x4, TT::frag(at, base, kk, part));
     };
@@ -301,9 +302,15 @@ __device__ __forceinline__ void mx4_gemm(const Mx4GemmArgs &m, const Stage (&st)
         const LdsChar *pa = (LdsChar *)scales + wm / 64 * 512 + (wm & 32) / 8 + l * 8;
         const LdsChar *pb = (LdsChar *)scales + GROUPS * 512 + wn / 64 * 512 + (wn & 32) / 8 + l * 8;
 #pragma unroll
-        for (int i = 0; i < FM / 2; ++i) xa[i] = *(SP)(pa + i / 2 * 512 + i % 2 * 4);
+        for (int i = 0; i < FM / 2; ++i) ya[i] = *(SP)(pa + i / 2 * 512 + i % 2 * 4);
 #pragma unroll
-        for (int j = 0; j < FN / 2; ++j) xb[j] = *(SP)(pb + j / 2 * 512 + j % 2 * 4);
+        for (int j = 0; j < FN / 2; ++j) yb[j] = *(SP)(pb + j / 2 * 512 + j % 2 * 4);
+    };
+    auto next_scales = [&] {
+#pragma unroll
+        for (int i = 0; i < FM / 2; ++i) xa[i] = ya[i];
+#pragma unroll
+        for (int j = 0; j < FN / 2; ++j) xb[j] = yb[j];
     };
     auto multiply = [&](int kk, int h) {
 #pragma unroll
@@ -314,8 +321,8 @@ __device__ __forceinline__ void mx4_gemm(const Mx4GemmArgs &m, const Stage (&st)
                 acc[f][j] = mx4_mma(j % 2 * 2 + kk, f % 2 * 2 + kk, fb[kk][j], fa[h][i], acc[f][j], xb[j / 2], xa[f / 2]);
             }
     };
-    // gemm_direct's four phases; the scales of the next tile are read when the
-    // last products of this one have taken theirs.
+    // gemm_direct's four phases; the next tile's scales are read as soon as it is
+    // there.
     auto tile = [&](const Stage &c, const Stage &n, char *csc, const char *nsc) {
         constexpr int MP = HM * FN;
         take_a(c, 0, 1);
@@ -329,13 +336,14 @@ __device__ __forceinline__ void mx4_gemm(const Mx4GemmArgs &m, const Stage (&st)
         multiply(1, 0);
         spread<HM, MP>();
         tiles_landed<AHEAD>();
+        take_scales(nsc);
         stage(c, csc);
         __builtin_amdgcn_sched_barrier(0);
         take_b(n, 0);
         take_a(n, 0, 0);
         multiply(1, 1);
         spread<HM + FN, MP>();
-        take_scales(nsc);
+        next_scales();
     };
 #pragma unroll
     for (int i = 0; i < ST; ++i) stage(st[i], sc[i]);
@@ -343,6 +351,7 @@ __device__ __forceinline__ void mx4_gemm(const Mx4GemmArgs &m, const Stage (&st)
     take_b(st[0], 0);
     take_a(st[0], 0, 0);
     take_scales(sc[0]);
+    next_scales();
     for (int kt = 0; kt < nk; kt += ST) {
 #pragma unroll
         for (int i = 0; i < ST; ++i) tile(st[i], st[(i + 1) % ST], sc[i], sc[(i + 1) % ST]);
