@@ -49,13 +49,14 @@ static void code_launch(Launches &launches, const char *way, const mxh_mat &x, b
                  cdiv(x.rows, at) * a.tiles, 1, 256, a);
 }
 
-// What a tile costs, as kTiles16 of ops.cpp has it: a step is 128 bytes of a
-// line, 256 elements.
+// What a tile costs in us, as kTiles16 of ops.cpp has it: a step is 128 bytes of
+// a line, 256 elements; `rest` with the launch that quantises x. Measured on
+// products of 16 to 4096 rows.
 struct Cost {
     int b, stages, fit;
     double one, all, rest;
 };
-static const Cost kTilesMx4[] = {{256, 2, 1, 1.6, 1.6, 10.0}, {128, 2, 2, 0.65, 0.93, 7.0}, {64, 4, 2, 0.25, 0.45, 4.0}};
+static const Cost kTilesMx4[] = {{256, 2, 1, 1.65, 1.65, 12.0}, {128, 2, 2, 1.0, 1.3, 8.0}, {64, 4, 2, 0.3, 0.45, 6.0}};
 
 struct Mx4Plan {
     bool few = false;  // the kernel of few rows
@@ -65,12 +66,15 @@ struct Mx4Plan {
     uint64_t bytes() const { return codes + scales + parts; }
 };
 
+// The tile and the cut of k that take the least time by those costs, or for up
+// to 16 rows the kernel that quantises x as it reads it: a block for 16 columns
+// and all of k, whose waves take an eighth of its tiles each, one after the
+// other. bf16, one row and 16: k = 4096 to 4096 columns 6.4 and 9.0 us, as tiles
+// of 64 9.2 and 9.5; k = 16384 to 1024 columns 15.9 and 22.7, tiles cut in eight
+// 10.4 and 11.0. 1024 x 4096 x 4096: 128 x 128 24 us, 64 x 64 26, 256 x 256 37;
+// 4096 x 256 x 4096: 20, 34 and 17.
 static Mx4Plan mx4_plan(const mxh_mat &x, int64_t n, bool by_cols) {
     Mx4Plan p;
-    if (by_cols && x.rows <= 16 && along_cols(x)) {
-        p.few = true;
-        return p;
-    }
     const int64_t steps = std::max<int64_t>(1, tiles_of(x.cols));
     double least = std::numeric_limits<double>::infinity();
     for (const Cost &t : kTilesMx4) {
@@ -81,10 +85,17 @@ static Mx4Plan mx4_plan(const mxh_mat &x, int64_t n, bool by_cols) {
             const int64_t total = tiles * splits, full = total / (256 * t.fit), left = cdiv(total % (256 * t.fit), 256);
             double us = full * (each * t.all + t.rest);
             if (left) us += each * std::max(t.one, t.all * left / t.fit) + t.rest;
-            if (splits > 1) us += 5.0 + (double)splits * x.rows * n * 8 / 5e6;
+            if (splits > 1) us += 3.0 + (double)splits * x.rows * n * 8 / 5e6;
             if (us >= least) continue;
             least = us;
             p.b = t.b, p.stages = t.stages, p.splits = splits, p.chunk = each;
+        }
+    }
+    if (by_cols && x.rows <= 16 && along_cols(x)) {
+        const double few = 3.3 + 0.065 * x.rows + (1.5 + 0.05 * x.rows) * cdiv(steps, 8) * std::max(1.0, cdiv(n, 16) / 256.0);
+        if (few <= least) {
+            p.few = true;
+            return p;
         }
     }
     p.codes = up(code_bytes(x.rows, x.cols));

@@ -378,32 +378,61 @@ __device__ __forceinline__ void mx4_skinny(const Mx4GemmArgs &m) {
     const uint8_t *sb = m.sb + n0 / 64 * tiles * 512 + q * 128 + r * 8 + (n0 / 16 & 3) * 2;
     const T *x = reinterpret_cast<const T *>(m.a) + (int64_t)min(r, g.m - 1) * g.lda;
     f32x4 acc = {0, 0, 0, 0};
-    for (int k = w * each; k < kend; ++k) {
-        u32x4 fb[2], fa[2];
+    // A tile's loads, two tiles ahead of its products (in fp32 one: x's two would
+    // not fit the registers).
+    constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
+    struct In {
+        u32x4 b[2];
+        uint32_t s;
+        Vec<T, 8> x[2][4];
+    };
+    auto fetch = [&](int k, In &in) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) in.b[h] = *reinterpret_cast<const u32x4 *>(b + (int64_t)k * 128 + h * 64);
+        in.s = *reinterpret_cast<const uint16_t *>(sb + (int64_t)k * 512);
+        const int64_t at = (int64_t)k * 256 + q * 32;
+        if ((int64_t)(k + 1) * 256 <= m.cols) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) in.x[h][i] = load_n<T, 8>(x + at + h * 128 + i * 8);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) in.x[h][i] = load_upto<T, 8>(x + at + h * 128 + i * 8, m.cols - at - h * 128 - i * 8);
+        }
+    };
+    auto use = [&](const In &in) {
+        u32x4 a[2];
         uint32_t sa[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) fb[h] = *reinterpret_cast<const u32x4 *>(b + (int64_t)k * 128 + h * 64);
-        const uint32_t s = *reinterpret_cast<const uint16_t *>(sb + (int64_t)k * 512);
-#pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int at = k * 256 + h * 128 + q * 32;
-            Vec<T, 8> v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = load_upto<T, 8>(x + at + i * 8, (int64_t)m.cols - at - i * 8);
             uint32_t top = 0;
             float f[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-                f[e] = to_f<T>(v[e / 8].v[e % 8]);
+                f[e] = to_f<T>(in.x[h][e / 8].v[e % 8]);
                 top = max(top, magnitude(f[e]));
             }
             sa[h] = mx4_scale(top);
             const float inverse = mx4_inverse(sa[h]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[h][i] = mx4_codes(f + 8 * i, inverse);
+            for (int i = 0; i < 4; ++i) a[h][i] = mx4_codes(f + 8 * i, inverse);
         }
-        acc = mx4_mma<0, 0>(fb[0], fa[0], acc, s, sa[0]);
-        acc = mx4_mma<1, 0>(fb[1], fa[1], acc, s, sa[1]);
+        acc = mx4_mma<0, 0>(in.b[0], a[0], acc, in.s, sa[0]);
+        acc = mx4_mma<1, 0>(in.b[1], a[1], acc, in.s, sa[1]);
+    };
+    In in[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (w * each + i < kend) fetch(w * each + i, in[i]);
+    for (int k = w * each; k < kend; k += AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k + i < kend) use(in[i]);
+            if (k + i + AHEAD < kend) fetch(k + i + AHEAD, in[i]);
+        }
     }
     sums[w][l] = acc;
     __syncthreads();

@@ -212,8 +212,8 @@ def _workspace(n, x):
 
 
 def _written(out):
-    """Tells autograd that a caller's tensor has new values (a result of the
-    call's own has no history)."""
+    """Tells autograd that a caller's tensor, or each of a list, has new values
+    (a result of the call's own has no history)."""
     if out is not None:
         _torch.autograd.graph.increment_version(out)
 
@@ -371,8 +371,6 @@ def gated_backward(dy, x, w, z, act="silu", slope=0.0, planar=False, dx=True, dw
 
 def _filled(t, what):
     """The tensor's elements lie side by side, in whatever order."""
-    if t.is_contiguous():
-        return
     at = 1
     for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
         if stride != at:
@@ -383,16 +381,17 @@ def _filled(t, what):
 
 def _list(tensors, what, device):
     """Tensors as an array of vectors of their elements."""
-    a = (Vec * len(tensors))()
-    for i, t in enumerate(tensors):
-        name = "%s[%d]" % (what, i)
-        code = _tensor(t, name, device)
-        n = t.numel()
-        if n:
-            _filled(t, name)
-        v = a[i]
-        v.data, v.n, v.dtype = t.data_ptr(), n, code
-    return a
+    a = []
+    try:
+        for t in tensors:
+            code = _tensor(t, what, device)
+            n = t.numel()
+            if n and not t.is_contiguous():
+                _filled(t, what)
+            a += (t.data_ptr(), n, code)  # a Vec's words, its type with the reserved half
+    except P.MaximError as e:
+        raise P.MaximError(str(e).replace(what, "%s[%d]" % (what, len(a) // 3), 1))
+    return (Vec * len(tensors)).from_buffer((C.c_int64 * len(a))(*a))
 
 
 def _grads(grads):
@@ -435,7 +434,8 @@ def clip_grads(grads, max_norm, norm=None, out=None):
         if len(out) != len(grads):
             raise P.MaximError("out: %d tensors for %d gradients" % (len(out), len(grads)))
         for i, (g, o) in enumerate(zip(grads, out)):
-            if o is not g and (o.shape != g.shape or o.stride() != g.stride()):
+            if o is not g and not (isinstance(o, _torch.Tensor) and isinstance(g, _torch.Tensor) and o.is_same_size(g) and
+                                   o.stride() == g.stride()):
                 raise P.MaximError("out[%d]: not its gradient's shape and strides" % i)
         b = _list(out, "out", d)
     if norm is None:
@@ -446,8 +446,7 @@ def clip_grads(grads, max_norm, norm=None, out=None):
         if _tensor(norm, "norm", d) != 0 or norm.numel() != 1:
             raise P.MaximError("norm: not one fp32 value")
         _check(_L.mxh_grad_clip_by(d, _stream(d), a, b, len(a), max_norm, norm.data_ptr()))
-    for t in grads if out is None else out:
-        _written(t)
+    _written(grads if out is None else out)
     return norm
 
 
@@ -456,22 +455,24 @@ class Mx4:
     `scales` (uint8, on the card), `shape` (positions, then features) and the
     `dtype` of the tensor that it was made from."""
 
-    def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
+    def __init__(self, data, code_bytes, rows, shape, dtype):
+        self._data, self._code_bytes, self._rows = data, code_bytes, rows
+        self.shape, self.dtype = shape, dtype
+
+    codes = property(lambda self: self._data[:self._code_bytes])
+    scales = property(lambda self: self._data[self._code_bytes:])
 
     def _mat(self):
-        rows = 1
-        for n in self.shape[:-1]:
-            rows *= n
-        return Mx4Mat(self.codes.data_ptr(), self.scales.data_ptr(), rows, self.shape[-1])
+        at = self._data.data_ptr()
+        return Mx4Mat(at, at + self._code_bytes, self._rows, self.shape[-1])
 
     def plain(self):
         """(codes, scales) as [rows][features / 2 bytes] and [rows][blocks]
         tensors: the order in which others keep such blocks."""
-        m = self._mat()
-        tiles, groups, blocks = (m.cols + 255) // 256, (m.rows + 63) // 64, (m.cols + 31) // 32
+        rows, cols = self._rows, self.shape[-1]
+        tiles, groups, blocks = (cols + 255) // 256, (rows + 63) // 64, (cols + 31) // 32
         s = self.scales.view(groups, tiles, 4, 16, 4, 2).permute(0, 4, 3, 1, 5, 2).reshape(groups * 64, tiles * 8)
-        return self.codes.view(m.rows, tiles * 128)[:, :(m.cols + 1) // 2], s[:m.rows, :blocks]
+        return self.codes.view(rows, tiles * 128)[:, :(cols + 1) // 2], s[:rows, :blocks]
 
 
 def mx4_quantize(x, planar=False):
@@ -481,17 +482,17 @@ def mx4_quantize(x, planar=False):
     codes, scales = C.c_uint64(), C.c_uint64()
     _check(_L.mxh_mx4_size(X.rows, X.cols, codes, scales))
     shape = tuple(x.shape[1:]) + (x.shape[0],) if planar else tuple(x.shape)
-    q = Mx4(x.new_empty(codes.value, dtype=_torch.uint8), x.new_empty(scales.value, dtype=_torch.uint8), shape, x.dtype)
-    _check(_L.mxh_mx4_quantize(d, _stream(d), X, Mx4Mat(q.codes.data_ptr(), q.scales.data_ptr(), X.rows, X.cols)))
+    # one allocation for both: codes are lines of 128 bytes
+    q = Mx4(x.new_empty(codes.value + scales.value, dtype=_torch.uint8), codes.value, X.rows, shape, x.dtype)
+    _check(_L.mxh_mx4_quantize(d, _stream(d), X, q._mat()))
     return q
 
 
 def _mx4(q, what, device):
     if not isinstance(q, Mx4):
         raise P.MaximError("%s: not an Mx4" % what)
-    for t in (q.codes, q.scales):
-        if not t.is_cuda or t.get_device() != device:
-            raise P.MaximError("%s: on another device than x" % what)
+    if q._data.get_device() != device:
+        raise P.MaximError("%s: on another device than x" % what)
     return q._mat()
 
 
@@ -501,10 +502,10 @@ def mx4_dequantize(q, dtype=None, planar=False):
     _lib()
     if not isinstance(q, Mx4):
         raise P.MaximError("q: not an Mx4")
-    d = q.codes.get_device()
-    m = _mx4(q, "q", d)
+    d = q._data.get_device()
+    m = q._mat()
     dtype = dtype or q.dtype
-    y = q.codes.new_empty((q.shape[-1],) + q.shape[:-1] if planar else q.shape, dtype=dtype)
+    y = q._data.new_empty((q.shape[-1],) + q.shape[:-1] if planar else q.shape, dtype=dtype)
     Y = (Mat(y.data_ptr(), m.rows, m.cols, 1, m.rows, 0, 0) if planar else
          Mat(y.data_ptr(), m.rows, m.cols, m.cols, 1, 0, 0))
     Y.dtype = _tensor(y, "y", d)
