@@ -312,7 +312,17 @@ Plan plan_of(const Product &p) {
     return plan_product(p.dtype, p.m, p.n, p.k, a, b, p.pair);
 }
 
-void product(Launches &launches, const Product &given, void *ws) {
+void join_splits(Launches &launches, const OpsGemmArgs &g, const std::string &of, const std::string &what) {
+    // few sums of many splits: eight threads to each
+    const bool deep = g.splits >= 16;
+    launches.add(of + (deep ? "join8_" : "join_") + what,
+                 std::min<int64_t>(4096, cdiv(g.m * cdiv(g.n, 4), deep ? 32 : 256)), 1, 256, g);
+}
+void join_product(Launches &launches, const OpsGemmArgs &g, int dtype) {
+    join_splits(launches, g, "mxo_", kTypeName[dtype]);
+}
+
+void product(Launches &launches, const Product &given, void *ws, OpsGemmArgs *later) {
     if (!given.m || !given.n) return;
     Product p = given;
     const bool ak = by_k(p.a), bk = by_k(p.b);
@@ -377,12 +387,8 @@ void product(Launches &launches, const Product &given, void *ws) {
     const std::string b = std::to_string(pl.tile);
     launches.add(of + "gemm_" + along + t + "_" + b + "x" + b + "_" + (ak ? "k" : "m") + (bk ? "k" : "m") + (pl.stages ? "_d" + std::to_string(pl.stages) : ""),
                  tm * tn * pl.splits, 1, pl.block, g);
-    if (pl.splits > 1) {
-        // few sums of many splits: eight threads to each
-        const bool deep = pl.splits >= 16;
-        launches.add(of + (deep ? "join8_" : "join_") + along + t,
-                     std::min<int64_t>(4096, cdiv(p.m * cdiv(p.n, 4), deep ? 32 : 256)), 1, 256, g);
-    }
+    if (pl.splits > 1 && later) *later = g;
+    else if (pl.splits > 1) join_splits(launches, g, of, along + t);
 }
 
 // An operand of a product as (own axis, summed axis): rows summed over or not.

@@ -59,7 +59,7 @@ class Launches {
     struct One {
         std::string name;
         unsigned gx, gy, block;
-        alignas(8) char args[192];
+        alignas(8) char args[200];
     };
     One at_[8];  // a Dense's backward pass: dz and its join, twice packing, product and join
     int n_ = 0;
@@ -278,8 +278,11 @@ struct Plan {
 
 // The tile, split and packing of a product, and its workspace.
 Plan plan_of(const Product &p);
-// Its launches, `ws` of the plan's bytes.
-void product(Launches &launches, const Product &p, void *ws);
+// Its launches, `ws` of the plan's bytes. `later`: where the sums are cut, not
+// the launch that joins them but its arguments (else splits stays 0).
+void product(Launches &launches, const Product &p, void *ws, OpsGemmArgs *later = nullptr);
+// The launch that joins a plain product's splits.
+void join_product(Launches &launches, const OpsGemmArgs &g, int dtype);
 // An operand of a product as (own axis, summed axis): rows summed over or not.
 Operand operand(const mxh_mat &m, bool sum_rows);
 

@@ -85,3 +85,13 @@ struct OpsJoinArgs {
     int32_t nparts, nout;
     int32_t dtype, pad;
 };
+
+// A gradient's two joins in one launch: a product's splits (`g`, to g.c; blocks
+// from 0) and the bias's partial sums (blocks from `first`).
+struct OpsGradJoinArgs {
+    OpsGemmArgs g;
+    const float *part;
+    void *out;
+    int32_t n, nparts;
+    int32_t first, dtype;
+};

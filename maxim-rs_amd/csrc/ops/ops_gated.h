@@ -219,16 +219,53 @@ __device__ __forceinline__ void gated_skinny(const OpsGemmArgs &g) {
 // and z. Stored rounded to the operands' type, as the products' matrix cores
 // take it (ops_rows.h has what that costs); the bias's sums take it before.
 //
+// act(z) and act'(z) as act_fwd and act_bwd have them, with what they share
+// formed once: an exponential and a reciprocal instead of two (the planar pass
+// of 64 bf16 features, silu, 71680 positions: 14.4 us, so 13.1).
+__device__ __forceinline__ void act_both(int act, float slope, float z, float &f, float &d) {
+    if (act == MXO_GELU) {
+        const float ax = fabsf(z), t = fminf(ax, 13.0f), p = phi_tail(ax);
+        f = fmaxf(z, 0.0f) - fminf(ax, 6.0f) * p;
+        d = (z >= 0.0f ? 1.0f - p : p) +
+            copysignf(t, z) * (0.3989422804014327f * __builtin_amdgcn_exp2f(t * t * -0.7213475204444817f));
+    } else if (act == MXO_SIGMOID) {
+        logistic(z, f, d);
+    } else if (act == MXO_SILU || act == MXO_GELU_TANH) {
+        const float c = fminf(fmaxf(z, -1e4f), 1e4f), q = kTanhB * c * c;
+        float s, e;
+        logistic(act == MXO_SILU ? c : kTanhA * c * (q + 1.0f), s, e);
+        f = fmaxf(z, -1e4f) * s;
+        d = __builtin_fmaf(act == MXO_SILU ? c : c * kTanhA * __builtin_fmaf(3.0f, q, 1.0f), e, s);
+    } else {
+        f = act_fwd(act, slope, z);
+        d = act_bwd(act, slope, z);
+        return;
+    }
+    f = z != z ? z : f;
+    d = z != z ? z : d;
+}
+
 // v: dy in, da out; u: a in, dc out.
 template <int E>
 __device__ __forceinline__ void gated_dz_n(int act, float slope, float *v, float *u, const float *c) {
-    float s[E], d[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) d[e] = v[e] * c[e], s[e] = u[e];
-    act_bwd_n<E>(act, slope, d, [&](int e) { return u[e]; });
-    act_fwd_n<E>(act, slope, s);
-#pragma unroll
-    for (int e = 0; e < E; ++e) u[e] = v[e] * s[e], v[e] = d[e];
+#define OPS_DZ(which)                                                  \
+    case which:                                                        \
+        _Pragma("unroll") for (int e = 0; e < E; ++e) {                \
+            float f, d;                                                \
+            act_both(which, slope, u[e], f, d);                        \
+            u[e] = v[e] * f, v[e] = v[e] * c[e] * d;                   \
+        }                                                              \
+        break;
+    switch (act) {
+        OPS_DZ(MXO_NONE)
+        OPS_DZ(MXO_GELU)
+        OPS_DZ(MXO_GELU_TANH)
+        OPS_DZ(MXO_SILU)
+        OPS_DZ(MXO_LRELU)
+        OPS_DZ(MXO_SIGMOID)
+        default: break;
+    }
+#undef OPS_DZ
 }
 
 // Rows with contiguous features: 64 x E features by a run of rows a block, a
@@ -322,6 +359,65 @@ __device__ __forceinline__ void gated_dz_planar(const OpsDzArgs &a) {
     }
 }
 
+// The joins of dw's splits and of the bias's partial sums. Few results and many
+// parts: 16 threads to four of dw's, 64 to a bias's, 16 parts in turn each at
+// most in flight, added in a fixed order. (128 x 64 results of 249 parts and 128
+// of 35, fp32: 12 us as two launches of their own, so 5.8.)
+template <typename T>
+__device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
+    __shared__ f32x4 sh[256];
+    const int t = threadIdx.x;
+    if ((int)blockIdx.x >= a.first) {
+        // four columns a block, 64 threads down the parts
+        float *s = reinterpret_cast<float *>(sh);
+        const int l = t & 3, w = t >> 2;
+        const int64_t c = ((int64_t)blockIdx.x - a.first) * 4 + l;
+        float v = 0.0f;
+        if (c < a.n) {
+#pragma unroll 4
+            for (int i = w; i < a.nparts; i += 64) v += a.part[(int64_t)i * a.n + c];
+        }
+        s[t] = v;
+#pragma unroll
+        for (int half = 32; half >= 1; half >>= 1) {
+            __syncthreads();
+            if (w < half) s[t] += s[t + half * 4];
+        }
+        if (w == 0 && c < a.n) {
+            if (a.dtype == MXO_F32) static_cast<float *>(a.out)[c] = s[t];
+            else if (a.dtype == MXO_F16) static_cast<f16 *>(a.out)[c] = from_f<f16>(s[t]);
+            else static_cast<bf16 *>(a.out)[c] = from_f<bf16>(s[t]);
+        }
+        return;
+    }
+    const OpsGemmArgs &g = a.g;
+    const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m, plane = (int64_t)g.m * g.n;
+    const int q = t & 15, way = t >> 4;
+    for (int64_t i0 = (int64_t)blockIdx.x * 16; i0 < total; i0 += (int64_t)a.first * 16) {
+        const int64_t i = i0 + q, m = i / quads, n = (i - m * quads) * 4;
+        f32x4 v = {0, 0, 0, 0};
+        if (i < total) {
+            const float *p = g.part + m * g.n + n;
+#pragma unroll 4
+            for (int s = way; s < g.splits; s += 16) {
+                const Vec<float, 4> o = load_upto<float, 4>(p + s * plane, g.n - n);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += o.v[e];
+            }
+        }
+        __syncthreads();
+        sh[t] = v;
+        __syncthreads();
+        if (way || i >= total) continue;
+#pragma unroll
+        for (int k = 1; k < 16; ++k) v += sh[k * 16 + q];
+        Vec<T, 4> o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.v[e] = from_f<T>(v[e]);
+        store_upto<T, 4>(static_cast<T *>(g.c) + m * g.ldc + n, o, g.n - n);
+    }
+}
+
 #define OPS_GATED1(name, T, B, WM, WN, axis, PAIR, tag, AK, BK)                                                  \
     extern "C" __global__ __launch_bounds__(64 * WM * WN) void mxg_gemm_##axis##_##name##_##B##x##B##_##tag(     \
         OpsGemmArgs g) {                                                                                         \
@@ -360,6 +456,7 @@ __device__ __forceinline__ void gated_dz_planar(const OpsDzArgs &a) {
     OPS_GATED_JOIN(name, T, n, PAIR_N)                                                                                   \
     OPS_GATED_JOIN(name, T, m, PAIR_M)                                                                                   \
     extern "C" __global__ __launch_bounds__(512) void mxg_skinny_##name(OpsGemmArgs g) { gated_skinny<T>(g); }           \
+    extern "C" __global__ __launch_bounds__(256) void mxg_grad_join_##name(OpsGradJoinArgs a) { grad_join<T>(a); }        \
     extern "C" __global__ __launch_bounds__(256) void mxg_dz_rows_##name(OpsDzArgs a) {                                  \
         __shared__ float sh[4][2][64 * 16 / sizeof(T)];                                                                  \
         if (a.cols % (16 / sizeof(T)) == 0) gated_dz_rows<T, true>(a, sh);                                               \

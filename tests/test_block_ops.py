@@ -471,7 +471,7 @@ def chosen(name):
                 out |= {"mxg_gemm_%s_%s_%sx%s_%s%s" % (a, t, b, b, o, "" if stages == "0" else "_d" + stages)
                         for a, o in (("n", "kk"), ("n", "km"), ("m", "km"), ("m", "mm"))}
             out |= {"mxg_%s_%s_%s" % (j, a, t) for j in ("join", "join8") for a in "nm"}
-            out |= {"mxg_skinny_" + t, "mxg_dz_rows_" + t, "mxg_dz_planar_" + t}
+            out |= {"mxg_skinny_" + t, "mxg_dz_rows_" + t, "mxg_dz_planar_" + t, "mxg_grad_join_" + t}
         elif name == "mx4":
             out |= {"mxq_gemm_%s_%sx%s_d%s" % (t, b, b, stages) for b, stages in tiles("mx4.cpp", "kTilesMx4")}
             out |= {"mxq_%s_%s_%s" % (w, o, t) for w in ("quantize", "dequantize") for o in ("rows", "planar")}
