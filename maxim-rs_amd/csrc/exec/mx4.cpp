@@ -43,8 +43,8 @@ static void code_launch(Launches &launches, const char *way, const mxh_mat &x, b
     // an axis of one element has no stride of its own
     a.rs = by_cols ? x.row_stride : 1, a.cs = by_cols ? 1 : x.col_stride;
     a.tiles = (int32_t)tiles_of(x.cols);
-    // rows are quantised by half groups of 32, all else goes by groups of 64
-    const int64_t at = by_cols && way[0] == 'q' ? 32 : 64;
+    // positions a block: rows are quantised by half groups, planes by 4 bytes a lane
+    const int64_t at = by_cols ? (way[0] == 'q' ? 32 : 64) : 64 * 4 / (int64_t)type_size(x.dtype);
     launches.add(std::string("mxq_") + way + (by_cols ? "_rows_" : "_planar_") + kTypeName[x.dtype],
                  cdiv(x.rows, at) * a.tiles, 1, 256, a);
 }

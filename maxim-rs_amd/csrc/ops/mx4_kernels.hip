@@ -25,10 +25,16 @@
     }
 #define OPS_MX4_TYPE(name, T)                                                                                        \
     extern "C" __global__ __launch_bounds__(256) void mxq_quantize_rows_##name(Mx4CodeArgs a) { mx4_quantize_rows<T>(a); }     \
-    extern "C" __global__ __launch_bounds__(256) void mxq_quantize_planar_##name(Mx4CodeArgs a) { mx4_quantize_planar<T>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void mxq_quantize_planar_##name(Mx4CodeArgs a) {                    \
+        __shared__ __align__(16) char codes[64 * 4 / sizeof(T) * 128];                                               \
+        __shared__ uint32_t scales[128 * 4 / sizeof(T)];                                                             \
+        mx4_quantize_planar<T>(a, codes, scales);                                                                    \
+    }                                                                                                                \
     extern "C" __global__ __launch_bounds__(256) void mxq_dequantize_rows_##name(Mx4CodeArgs a) { mx4_dequantize_rows<T>(a); } \
     extern "C" __global__ __launch_bounds__(256) void mxq_dequantize_planar_##name(Mx4CodeArgs a) {                  \
-        mx4_dequantize_planar<T>(a);                                                                                 \
+        __shared__ __align__(16) char codes[64 * 4 / sizeof(T) * 128];                                               \
+        __shared__ uint32_t scales[128 * 4 / sizeof(T)];                                                             \
+        mx4_dequantize_planar<T>(a, codes, scales);                                                                  \
     }                                                                                                                \
     extern "C" __global__ __launch_bounds__(512) void mxq_skinny_##name(Mx4GemmArgs m) { mx4_skinny<T>(m); }         \
     OPS_MX4_D2(name, T, 256, 2, 4)                                                                                   \

@@ -93,40 +93,59 @@ __device__ __forceinline__ void mx4_quantize_rows(const Mx4CodeArgs &a) {
     if (t < 64) reinterpret_cast<uint32_t *>(a.scales)[((half >> 1) * a.tiles + tile) * 128 + t * 2 + (half & 1)] = sh[t];
 }
 
-// Planar order: a block takes 64 positions by a tile, a lane one position of
-// two of its eight blocks.
+// Planar order: a block takes 64 positions (fp32) or 128 by a tile, a lane one
+// or two positions (4 bytes of a feature's plane) of two of the tile's eight
+// blocks. The codes go to memory through LDS, whole lines at a time.
 template <typename T>
-__device__ __forceinline__ void mx4_quantize_planar(const Mx4CodeArgs &a) {
-    __shared__ uint32_t sh[128];
+__device__ __forceinline__ void mx4_quantize_planar(const Mx4CodeArgs &a, char *codes, uint32_t *sh) {
+    constexpr int N = 4 / sizeof(T), ROWS = 64 * N;
     const int t = threadIdx.x, l = t & 63, w = t >> 6, tile = blockIdx.x % a.tiles;
-    const int64_t group = blockIdx.x / a.tiles, r0 = group * 64;
-    const int64_t r = min(r0 + l, a.rows - 1);
-    if (t < 128) sh[t] = 0;
-    __syncthreads();
+    const int64_t part = blockIdx.x / a.tiles, r0 = part * ROWS, r = r0 + l * N;
+    const int64_t have = a.rows - r;
     for (int b = w; b < 8; b += 4) {
-        const int64_t k = (int64_t)tile * 256 + b * 32, have = a.cols - k;
+        const int64_t k = (int64_t)tile * 256 + b * 32;
+        Vec<T, N> x[32];
         const T *p = static_cast<const T *>(a.x) + r * a.rs + k * a.cs;
-        T x[32];
-        float v[32];
-        uint32_t top = 0;
+        if (k + 32 <= a.cols && have >= N) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = e < have ? p[e * a.cs] : (T)0.0f;
+            for (int e = 0; e < 32; ++e) x[e] = load_n<T, N>(p + e * a.cs);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            v[e] = to_f<T>(x[e]);
-            top = max(top, magnitude(v[e]));
+            for (int e = 0; e < 32; ++e) x[e] = load_upto<T, N>(p + e * a.cs, k + e < a.cols ? have : 0);
         }
-        const uint32_t s = mx4_scale(top);
-        const float inverse = mx4_inverse(s);
-        u32x4 u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = mx4_codes(v + 8 * i, inverse);
-        if (r0 + l >= a.rows) continue;
-        *reinterpret_cast<u32x4 *>(a.codes + (r * a.tiles + tile) * 128 + b * 16) = u;
-        reinterpret_cast<uint8_t *>(sh)[scale_at(l, b)] = (uint8_t)s;
+        for (int i = 0; i < N; ++i) {
+            float v[32];
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                v[e] = to_f<T>(x[e].v[i]);
+                top = max(top, magnitude(v[e]));
+            }
+            const uint32_t s = mx4_scale(top);
+            const float inverse = mx4_inverse(s);
+            u32x4 u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = mx4_codes(v + 8 * j, inverse);
+            const int row = l * N + i;
+            *reinterpret_cast<u32x4 *>(codes + row * 128 + ((b ^ (l & 7)) << 4)) = u;
+            reinterpret_cast<uint8_t *>(sh)[(row >> 6) * 512 + scale_at(row & 63, b)] = (uint8_t)s;
+        }
     }
     __syncthreads();
-    if (t < 128) reinterpret_cast<uint32_t *>(a.scales)[(group * a.tiles + tile) * 128 + t] = sh[t];
+    // eight lanes a line
+#pragma unroll
+    for (int i = 0; i < ROWS / 32; ++i) {
+        const int row = i * 32 + (t >> 3), c = t & 7;
+        if (r0 + row < a.rows)
+            *reinterpret_cast<u32x4 *>(a.codes + ((r0 + row) * a.tiles + tile) * 128 + c * 16) =
+                *reinterpret_cast<const u32x4 *>(codes + row * 128 + ((c ^ (row / N & 7)) << 4));
+    }
+    // the groups that have rows
+    for (int i = t; i < 128 * N; i += 256) {
+        const int64_t group = part * N + i / 128;
+        if (group * 64 < a.rows) reinterpret_cast<uint32_t *>(a.scales)[(group * a.tiles + tile) * 128 + i % 128] = sh[i];
+    }
 }
 
 // And back, by the same blocks.
@@ -174,21 +193,43 @@ __device__ __forceinline__ void mx4_dequantize_rows(const Mx4CodeArgs &a) {
     }
 }
 template <typename T>
-__device__ __forceinline__ void mx4_dequantize_planar(const Mx4CodeArgs &a) {
+__device__ __forceinline__ void mx4_dequantize_planar(const Mx4CodeArgs &a, char *codes, uint32_t *sh) {
+    constexpr int N = 4 / sizeof(T), ROWS = 64 * N;
     const int t = threadIdx.x, l = t & 63, w = t >> 6, tile = blockIdx.x % a.tiles;
-    const int64_t group = blockIdx.x / a.tiles, r = group * 64 + l;
-    if (r >= a.rows) return;
+    const int64_t part = blockIdx.x / a.tiles, r0 = part * ROWS, r = r0 + l * N, have = a.rows - r;
+#pragma unroll
+    for (int i = 0; i < ROWS / 32; ++i) {
+        const int row = i * 32 + (t >> 3), c = t & 7;
+        const int64_t from = min(r0 + row, a.rows - 1);
+        *reinterpret_cast<u32x4 *>(codes + row * 128 + ((c ^ (row / N & 7)) << 4)) =
+            *reinterpret_cast<const u32x4 *>(a.codes + (from * a.tiles + tile) * 128 + c * 16);
+    }
+    for (int i = t; i < 128 * N; i += 256) {
+        const int64_t group = min(part * N + i / 128, (a.rows - 1) / 64);
+        sh[i] = reinterpret_cast<const uint32_t *>(a.scales)[(group * a.tiles + tile) * 128 + i % 128];
+    }
+    __syncthreads();
+    if (have <= 0) return;
     for (int b = w; b < 8; b += 4) {
-        const int64_t k = (int64_t)tile * 256 + b * 32, have = a.cols - k;
-        const u32x4 u = *reinterpret_cast<const u32x4 *>(a.codes + (r * a.tiles + tile) * 128 + b * 16);
-        const float scale = mx4_power(a.scales[(group * a.tiles + tile) * 512 + scale_at(l, b)]);
+        const int64_t k = (int64_t)tile * 256 + b * 32;
+        if (k >= a.cols) return;
+        float v[N][32];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = l * N + i;
+            const u32x4 u = *reinterpret_cast<const u32x4 *>(codes + row * 128 + ((b ^ (l & 7)) << 4));
+            const float scale = mx4_power(reinterpret_cast<const uint8_t *>(sh)[(row >> 6) * 512 + scale_at(row & 63, b)]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx4_values(u[j], scale, scale, v[i] + 8 * j);
+        }
         T *p = static_cast<T *>(a.y) + r * a.rs + k * a.cs;
-        float v[32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx4_values(u[i], scale, scale, v + 8 * i);
+        for (int e = 0; e < 32; ++e) {
+            Vec<T, N> o;
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-            if (e < have) p[e * a.cs] = from_f<T>(v[e]);
+            for (int i = 0; i < N; ++i) o.v[i] = from_f<T>(v[i][e]);
+            if (k + e < a.cols) store_upto<T, N>(p + e * a.cs, o, have);
+        }
     }
 }
 

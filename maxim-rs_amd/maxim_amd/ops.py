@@ -380,17 +380,23 @@ def _filled(t, what):
 
 
 def _list(tensors, what, device):
-    """Tensors as an array of vectors of their elements."""
+    """Tensors as an array of vectors of their elements. (Lists are long: the
+    ordinary tensor's checks are here, _tensor has the others' and the words.)"""
     a = []
+    plain = _forward_ad._current_level < 0
     try:
         for t in tensors:
-            code = _tensor(t, what, device)
+            code = _types.get(t.dtype)
+            if code is None or t.get_device() != device or t.requires_grad or not plain:
+                code = _tensor(t, what, device)
             n = t.numel()
-            if n and not t.is_contiguous():
+            if not t.is_contiguous() and n:
                 _filled(t, what)
             a += (t.data_ptr(), n, code)  # a Vec's words, its type with the reserved half
     except P.MaximError as e:
         raise P.MaximError(str(e).replace(what, "%s[%d]" % (what, len(a) // 3), 1))
+    except AttributeError:
+        raise P.MaximError("%s[%d]: not a tensor" % (what, len(a) // 3))
     return (Vec * len(tensors)).from_buffer((C.c_int64 * len(a))(*a))
 
 
@@ -433,11 +439,10 @@ def clip_grads(grads, max_norm, norm=None, out=None):
         out = list(out)
         if len(out) != len(grads):
             raise P.MaximError("out: %d tensors for %d gradients" % (len(out), len(grads)))
-        for i, (g, o) in enumerate(zip(grads, out)):
-            if o is not g and not (isinstance(o, _torch.Tensor) and isinstance(g, _torch.Tensor) and o.is_same_size(g) and
-                                   o.stride() == g.stride()):
-                raise P.MaximError("out[%d]: not its gradient's shape and strides" % i)
         b = _list(out, "out", d)
+        for i, (g, o) in enumerate(zip(grads, out)):
+            if not (g.is_same_size(o) and (g.is_contiguous() and o.is_contiguous() or g.stride() == o.stride())):
+                raise P.MaximError("out[%d]: not its gradient's shape and strides" % i)
     if norm is None:
         norm = grads[0].new_empty((), dtype=_torch.float32)
         ws, n = _norm_workspace(a, grads[0])

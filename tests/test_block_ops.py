@@ -400,7 +400,7 @@ def test_mx4_launches(card):
             l, = r["launches"]
             by_rows = m[4] == 1 and (m[3] != 1 or m[2] == 1 or m[1] == 1)
             assert l["tiles"] == -(-m[2] // 256)
-            each = 32 if "quantize_rows" in l["kernel"] and "dequantize" not in l["kernel"] else 64
+            each = 256 // SIZE[m[5]] if "planar" in l["kernel"] else 64 if "dequantize" in l["kernel"] else 32
             assert l["gx"] == -(-m[1] // each) * l["tiles"]
             assert ("_rows_" in l["kernel"]) == by_rows or m[1] == 1 or m[2] == 1
             continue
