@@ -7,6 +7,9 @@
 // its sums of a and of c lie in the same lanes, and neither z nor a second
 // product goes through memory unless z is kept. The weights are B where
 // features are contiguous in the results (PAIR_N), A in planar order (PAIR_M).
+// As a product of twice the columns: 8192 x 2048 to 2 x 4096 bf16 236 us, with z
+// (134 MB more) 250-263 (the product alone, of which all of z is stored, 221); 64
+// to 2 x 64 fp32 planes of 65536 with z, 67 MB, 18.6 us, 3.6 TB/s.
 #pragma once
 
 #include "ops_gemm_big.h"
@@ -163,7 +166,8 @@ __device__ __forceinline__ void gated_join(const OpsGemmArgs &g) {
 }
 
 // Up to 16 rows: ops_skinny.h's way, the block's 16 features of both halves at
-// once, each weight read once.
+// once, each weight read once (1 x 2048 to 2 x 8192 bf16, 67 MB: 15.1 us, 4.4
+// TB/s).
 template <typename T>
 __device__ __forceinline__ void gated_skinny(const OpsGemmArgs &g) {
     constexpr int E = 16 / sizeof(T), STEP = 4 * E, W = 8, AHEAD = 4;
@@ -217,7 +221,9 @@ __device__ __forceinline__ void gated_skinny(const OpsGemmArgs &g) {
 
 // dz = (dy c act'(a) | dy act(a)) and the bias's partial sums, one pass over dy
 // and z. Stored rounded to the operands' type, as the products' matrix cores
-// take it (ops_rows.h has what that costs); the bias's sums take it before.
+// take it (ops_rows.h has what that costs); the bias's sums take it before. Bound
+// by memory: 4096 x 2 x 2048 bf16, 84 MB, 15.5 us; 64 fp32 planes of 71680, 92 MB,
+// 16 us.
 //
 // act(z) and act'(z) as act_fwd and act_bwd have them, with what they share
 // formed once: an exponential and a reciprocal instead of two (the planar pass

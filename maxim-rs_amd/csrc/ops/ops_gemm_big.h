@@ -2,12 +2,15 @@
 // to LDS.
 //
 // Bound by the matrix cores where there are tiles enough, at the clock their
-// power leaves: bf16 8192^3 in 820-910 us (1.2-1.3 PFLOP/s; the library's
-// product 680-810), 4096^3 in 108-125 us (89-100). 8192 x 2048 x 8192 with 134
-// MB of results 262 us, with gelu 269, with the 134 MB of z as well 290: a
+// power leaves: bf16 8192^3 in 775-910 us (1.2-1.4 PFLOP/s; the library's
+// product 695-830), 4096^3 in 101-107 us (95-109). 8192 x 2048 x 8192 with 134
+// MB of results 221 us (194), with gelu 242, with the 134 MB of z as well 257: a
 // 256 x 256 tile takes 128 KiB of a CU's 160 KiB of LDS, so no second one fits
 // beside it and its results are written before its CU's next tile is begun. Two
-// smaller tiles a CU hide that, and lose more in products an LDS byte read.
+// smaller tiles a CU hide that, and lose more in products an LDS byte read. Four
+// waves with 128 x 128 sums each read LDS less (their sums in accumulation
+// registers) and take a step of k in 1.56 us instead of 1.41; lines brought to L2
+// tiles ahead, and wave priorities around the products, change nothing.
 #pragma once
 
 #include "ops_gemm.h"

@@ -1,5 +1,7 @@
-"""ctypes binding of the operators on device tensors (include/maxim_ops.h):
-LayerNorm and Dense, forward and backward, in fp32, fp16 or bf16.
+"""ctypes binding of the operators on device tensors (include/maxim_ops.h,
+include/maxim_block_ops.h): LayerNorm, Dense and gated Dense, forward and
+backward, in fp32, fp16 or bf16; the gradients' norm and clipping; 4-bit blocks
+and the Dense of them.
 
 Tensors are torch's, on the card; results and workspaces come from torch's
 allocator and the kernels go to torch's current stream of that device, so the
