@@ -7,8 +7,8 @@
 // its sums of a and of c lie in the same lanes, and neither z nor a second
 // product goes through memory unless z is kept. The weights are B where
 // features are contiguous in the results (PAIR_N), A in planar order (PAIR_M).
-// As a product of twice the columns: 8192 x 2048 to 2 x 4096 bf16 236 us, with z
-// (134 MB more) 250-263 (the product alone, of which all of z is stored, 221); 64
+// As a product of twice the columns: 8192 x 2048 to 2 x 4096 bf16 214 us, with z
+// (134 MB more) 221 (the product alone, of which all of z is stored, 217); 64
 // to 2 x 64 fp32 planes of 65536 with z, 67 MB, 18.6 us, 3.6 TB/s.
 #pragma once
 
@@ -76,7 +76,8 @@ template <typename T, int FM, int FN, int PAIR>
 __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
                                             const f32x4 (&acc)[FM][FN]) {
     constexpr int E = 16 / sizeof(T), LD = FN * 16 + 4;
-    constexpr int COLS = PAIR == PAIR_N ? FN * 8 : FN * 16, TALL = PAIR == PAIR_N ? 32 : 16;
+    constexpr bool ONE = PAIR == PAIR_N && FN > 4;  // a block of rows at a time, not two
+    constexpr int COLS = PAIR == PAIR_N ? FN * 8 : FN * 16, TALL = PAIR == PAIR_N && !ONE ? 32 : 16;
     constexpr int LANES = COLS / E, ROWS = 64 / LANES < TALL ? 64 / LANES : TALL, STEPS = TALL / ROWS;
     constexpr int OTHER = PAIR == PAIR_N ? COLS : 16 * LD;  // a value's sum from its gate's
     static_assert(FM % 2 == 0 && FN % 2 == 0 && LANES * ROWS == 64, "");
@@ -87,7 +88,7 @@ __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, in
     const bool whole = g.splits == 1;
     if (whole) gated_bias_cols<T, E>(g, n, ba, bc);
 #pragma unroll 1
-    for (int h = 0; h < FM / 2; ++h) {
+    for (int h = 0; h < (ONE ? FM : FM / 2); ++h) {
         const int64_t m = m0 + h * TALL + lr;
         GatedBias<T> row[STEPS];
         if (PAIR == PAIR_M && whole) {
@@ -95,8 +96,12 @@ __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, in
             for (int k = 0; k < STEPS; ++k) row[k] = gated_bias_row<T>(g, m + k * ROWS);
         }
 #pragma unroll
-        for (int i = 0; i < FM / 2; ++i)
-            if (i == h) put_rows(own, l, acc, PAIR == PAIR_N ? 2 * i : i, PAIR == PAIR_N ? 2 * i + 1 : i + FM / 2);
+        for (int i = 0; i < (ONE ? FM : FM / 2); ++i)
+            if (i == h) {
+                if (ONE) put_rows(own, l, acc, i, -1);
+                else put_rows(own, l, acc, PAIR == PAIR_N ? 2 * i : i, PAIR == PAIR_N ? 2 * i + 1 : i + FM / 2);
+                own_path(i);
+            }
         wave_fence();
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
@@ -449,11 +454,15 @@ __device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
         gemm_direct<T, B, B, WM, WN, AK, BK, 4, PAIR>(g, st);                                                    \
     }
 // x has the results' order: rows along k with w either way (PAIR_N), or planes
-#define OPS_GATED_ALL(KIND, name, T, B, WM, WN)                        \
+#define OPS_GATED_ROWS(KIND, name, T, B, WM, WN)                       \
     KIND(name, T, B, WM, WN, n, PAIR_N, kk, true, true)                \
-    KIND(name, T, B, WM, WN, n, PAIR_N, km, true, false)               \
+    KIND(name, T, B, WM, WN, n, PAIR_N, km, true, false)
+#define OPS_GATED_PLANES(KIND, name, T, B, WM, WN)                     \
     KIND(name, T, B, WM, WN, m, PAIR_M, km, true, false)               \
     KIND(name, T, B, WM, WN, m, PAIR_M, mm, false, false)
+#define OPS_GATED_ALL(KIND, name, T, B, WM, WN)                        \
+    OPS_GATED_ROWS(KIND, name, T, B, WM, WN)                           \
+    OPS_GATED_PLANES(KIND, name, T, B, WM, WN)
 #define OPS_GATED_JOIN(name, T, axis, PAIR)                                                                              \
     extern "C" __global__ __launch_bounds__(256) void mxg_join_##axis##_##name(OpsGemmArgs g) { gated_join<T, 1, PAIR>(g); } \
     extern "C" __global__ __launch_bounds__(256) void mxg_join8_##axis##_##name(OpsGemmArgs g) { gated_join<T, 8, PAIR>(g); }
@@ -473,8 +482,15 @@ __device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
 OPS_GATED_TYPE(bf16, bf16)
 OPS_GATED_TYPE(f16, f16)
 OPS_GATED_TYPE(f32, float)
-OPS_GATED_ALL(OPS_GATED_D2, bf16, bf16, 256, 2, 4)
-OPS_GATED_ALL(OPS_GATED_D2, f16, f16, 256, 2, 4)
+// 256 x 256: waves whose results are 64 wide, whole lines of y and z (with half
+// lines 8192 x 2048 to 2 x 4096 with z took 250 us, so 221); with w contiguous
+// along its rows they do not fit the registers
+OPS_GATED_D2(bf16, bf16, 256, 4, 2, n, PAIR_N, kk, true, true)
+OPS_GATED_D2(f16, f16, 256, 4, 2, n, PAIR_N, kk, true, true)
+OPS_GATED_D2(bf16, bf16, 256, 2, 4, n, PAIR_N, km, true, false)
+OPS_GATED_D2(f16, f16, 256, 2, 4, n, PAIR_N, km, true, false)
+OPS_GATED_PLANES(OPS_GATED_D2, bf16, bf16, 256, 2, 4)
+OPS_GATED_PLANES(OPS_GATED_D2, f16, f16, 256, 2, 4)
 OPS_GATED_ALL(OPS_GATED_D2, bf16, bf16, 128, 2, 2)
 OPS_GATED_ALL(OPS_GATED_D2, f16, f16, 128, 2, 2)
 OPS_GATED_ALL(OPS_GATED_D4, bf16, bf16, 128, 2, 2)

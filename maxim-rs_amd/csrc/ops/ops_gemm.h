@@ -344,17 +344,21 @@ __device__ __forceinline__ void gemm_place(const OpsGemmArgs &g, int &tm, int &t
 // two steps of k (4-bit operands) took 22 us, so 14; 4096^3 in bf16 111, so 105.
 // (Written from the accumulators, with a bias load each, a 256 x 256 tile's
 // 32 quads a lane took 49 us.)
-template <int FN>
+// (A gated product's eight blocks wide: 16 rows at a time.)
+template <int FN, int PAIR = PAIR_NONE>
 constexpr int gemm_write_bytes() {
-    return 32 * (FN * 16 + 4) * 4;
+    return (PAIR == PAIR_N && FN > 4 ? 16 : 32) * (FN * 16 + 4) * 4;
 }
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-// Blocks `first` and `second` (rows of them) of the sums into the wave's 32
-// rows of LDS.
+// Keeps branch i apart from the others (merged, they pick the sums that they
+// store from an array in scratch memory).
+__device__ __forceinline__ void own_path(int i) { asm volatile("; %0" ::"i"(i)); }
+// Blocks `first` and `second` (rows of them; -1: none) of the sums into the
+// wave's rows of LDS.
 template <int FM, int FN>
 __device__ __forceinline__ void put_rows(float *own, int l, const f32x4 (&acc)[FM][FN], int first, int second) {
     constexpr int LD = FN * 16 + 4;
@@ -362,7 +366,7 @@ __device__ __forceinline__ void put_rows(float *own, int l, const f32x4 (&acc)[F
     for (int j = 0; j < FN; ++j) {
         float *p = own + (l & 15) * LD + j * 16 + (l >> 4) * 4;
         *reinterpret_cast<f32x4 *>(p) = acc[first][j];
-        *reinterpret_cast<f32x4 *>(p + 16 * LD) = acc[second][j];
+        if (second >= 0) *reinterpret_cast<f32x4 *>(p + 16 * LD) = acc[second < 0 ? 0 : second][j];
     }
 }
 template <typename T, int FM, int FN, int PAIR>
@@ -395,7 +399,10 @@ __device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int
         if (AT == STEPS || u % STEPS == 0) {
 #pragma unroll
             for (int i = 0; i < FM / 2; ++i)
-                if (i == u / STEPS) put_rows(own, l, acc, 2 * i, 2 * i + 1);
+                if (i == u / STEPS) {
+                    put_rows(own, l, acc, 2 * i, 2 * i + 1);
+                    own_path(i);
+                }
         }
         wave_fence();
 #pragma unroll
@@ -497,7 +504,7 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
             }
     }
     // behind the loop's last barrier: no wave reads the tiles any more
-    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, lds + w * gemm_write_bytes<FN>(), acc);
+    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, lds + w * gemm_write_bytes<FN, PAIR>(), acc);
 }
 
 // The splits' sums added in a fixed order, then the epilogue: WAYS threads to

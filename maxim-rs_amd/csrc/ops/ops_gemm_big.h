@@ -58,7 +58,7 @@ struct Stage {
 template <typename T, int BM, int BN, int WM, int WN, bool AK, bool BK_, int ST, int PAIR = PAIR_NONE>
 __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&st)[ST]) {
     // the epilogue takes a quarter of the waves in each of four arrays
-    static_assert((WM * WN + 3) / 4 * gemm_write_bytes<BN / WN / 16>() <= BM * 128 && BM == BN, "");
+    static_assert((WM * WN + 3) / 4 * gemm_write_bytes<BN / WN / 16, PAIR>() <= BM * 128 && BM == BN, "");
     constexpr int NT = 64 * WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
     constexpr int CM = PAIR == PAIR_M ? BM / 2 : BM, CN = PAIR == PAIR_N ? BN / 2 : BN;  // results
     typedef Tile<T, AK, BM, NT, PAIR == PAIR_M ? BM / WM / 2 : 0> TA;
@@ -278,7 +278,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
         }
     }
     tiles_landed<0>();  // the last loads too, zeros: the tiles' LDS is free
-    char *own = (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN>();
+    char *own = (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN, PAIR>();
     gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, own, acc);
 }
 
