@@ -27,7 +27,7 @@ extern "C" {
  */
 int mxh_gated(int device, void *stream, const mxh_mat *x, const mxh_mat *w, const mxh_vec *bias, int act, float slope,
               const mxh_mat *y, const mxh_mat *z, void *workspace, uint64_t workspace_bytes);
-int mxh_gated_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, uint64_t *bytes);
+int mxh_gated_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, const mxh_mat *z, uint64_t *bytes);
 
 /*
  * Its gradients: with dz = (dy * c * act'(a) | dy * act(a)), dx = dz w, dw =
@@ -101,7 +101,8 @@ int mxh_mx4_dequantize(int device, void *stream, const mxh_mx4 *q, const mxh_mat
  */
 int mxh_mx4_dense(int device, void *stream, const mxh_mat *x, const mxh_mx4 *w, const mxh_vec *bias, int act, float slope,
                   const mxh_mat *residual, const mxh_mat *y, void *workspace, uint64_t workspace_bytes);
-int mxh_mx4_dense_workspace(const mxh_mat *x, const mxh_mx4 *w, const mxh_mat *y, uint64_t *bytes);
+int mxh_mx4_dense_workspace(const mxh_mat *x, const mxh_mx4 *w, const mxh_mat *residual, const mxh_mat *y,
+                            uint64_t *bytes);
 
 #ifdef __cplusplus
 }

@@ -35,6 +35,20 @@ static int64_t halves(const mxh_mat &w) {
     return w.rows / 2;
 }
 
+// The operands' sizes, types and strides, and the order that they have.
+static bool check_gated(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, const mxh_mat *z) {
+    const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &Y = need(y, "y");
+    check_first(X, "x");
+    check_mat(W, "w", X.dtype, W.rows, X.cols);
+    check_mat(Y, "y", X.dtype, X.rows, halves(W));
+    check_out(Y, "y");
+    if (z) {
+        check_mat(*z, "z", x->dtype, x->rows, w->rows);
+        check_out(*z, "z");
+    }
+    return common_order({x}, {y, z});
+}
+
 static mxh_mat like(const mxh_mat &m, int64_t cols) {
     mxh_mat r = m;
     r.cols = cols;
@@ -71,35 +85,22 @@ using namespace mxops;
 
 extern "C" {
 
-int mxh_gated_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, uint64_t *bytes) {
+int mxh_gated_workspace(const mxh_mat *x, const mxh_mat *w, const mxh_mat *y, const mxh_mat *z, uint64_t *bytes) {
     return guard([&] {
         if (!bytes) throw Error("bytes: missing");
-        check_first(need(x, "x"), "x");
-        check_mat(need(w, "w"), "w", x->dtype, w->rows, x->cols);
-        check_mat(need(y, "y"), "y", x->dtype, x->rows, halves(*w));
-        // operands of one row or column have both orders, and z may settle it
         *bytes = 0;
-        if (empty(*y)) return;
-        if (along_cols(*x) && out_by_cols(*y)) *bytes = plan_of(gated_product(*x, *w, *y, true)).bytes;
-        if (along_rows(*x) && out_by_rows(*y)) *bytes = std::max(*bytes, plan_of(gated_product(*x, *w, *y, false)).bytes);
+        const bool by_cols = check_gated(x, w, y, z);
+        if (!empty(*y)) *bytes = plan_of(gated_product(*x, *w, *y, by_cols)).bytes;
     });
 }
 
 int mxh_gated(int device, void *stream, const mxh_mat *x, const mxh_mat *w, const mxh_vec *bias, int act, float slope,
               const mxh_mat *y, const mxh_mat *z, void *workspace, uint64_t workspace_bytes) {
     return guard([&] {
-        const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &Y = need(y, "y");
-        check_first(X, "x");
-        check_mat(W, "w", X.dtype, W.rows, X.cols);
-        check_mat(Y, "y", X.dtype, X.rows, halves(W));
-        check_out(Y, "y");
+        const bool by_cols = check_gated(x, w, y, z);
+        const mxh_mat &X = *x, &W = *w, &Y = *y;
         check_act(act);
         if (bias) check_vec(*bias, "bias", W.rows, X.dtype);
-        if (z) {
-            check_mat(*z, "z", X.dtype, X.rows, W.rows);
-            check_out(*z, "z");
-        }
-        const bool by_cols = common_order({x}, {y, z});
         for (const mxh_mat *o : {y, z}) {
             if (!o) continue;
             refuse_overlap(*o, "an output", X, "x");
@@ -125,9 +126,10 @@ int mxh_gated_backward_workspace(const mxh_mat *dy, const mxh_mat *x, const mxh_
                                  const mxh_mat *dw, const mxh_vec *db, uint64_t *bytes) {
     return guard([&] {
         if (!bytes) throw Error("bytes: missing");
-        check_first(need(x, "x"), "x");
-        check_mat(need(w, "w"), "w", x->dtype, w->rows, x->cols);
-        check_mat(need(dy, "dy"), "dy", x->dtype, x->rows, halves(*w));
+        const mxh_mat &X = need(x, "x"), &W = need(w, "w"), &DY = need(dy, "dy");
+        check_first(X, "x");
+        check_mat(W, "w", X.dtype, W.rows, X.cols);
+        check_mat(DY, "dy", X.dtype, X.rows, halves(W));
         if (dx) check_mat(*dx, "dx", x->dtype, x->rows, x->cols);
         if (dw) check_mat(*dw, "dw", x->dtype, w->rows, w->cols);
         *bytes = std::max(gated_layout(*dy, true, *x, *w, dx, dw, db).total(),

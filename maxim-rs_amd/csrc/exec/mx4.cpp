@@ -104,6 +104,18 @@ static Mx4Plan mx4_plan(const mxh_mat &x, int64_t n, bool by_cols) {
     return p;
 }
 
+// The operands' sizes, types and strides, and the order that the results have.
+static bool check_dense(const mxh_mat *x, const mxh_mx4 *w, const mxh_mat *residual, const mxh_mat *y) {
+    const mxh_mat &X = need(x, "x"), &Y = need(y, "y");
+    check_first(X, "x");
+    if (!w) throw Error("w: missing");
+    check_mx4(w, "w", w->rows, X.cols);
+    check_mat(Y, "y", X.dtype, X.rows, w->rows);
+    check_out(Y, "y");
+    if (residual) check_mat(*residual, "residual", x->dtype, x->rows, w->rows);
+    return common_order({residual}, {y});
+}
+
 }  // namespace mxops
 
 using namespace mxops;
@@ -148,34 +160,23 @@ int mxh_mx4_dequantize(int device, void *stream, const mxh_mx4 *q, const mxh_mat
     });
 }
 
-int mxh_mx4_dense_workspace(const mxh_mat *x, const mxh_mx4 *w, const mxh_mat *y, uint64_t *bytes) {
+int mxh_mx4_dense_workspace(const mxh_mat *x, const mxh_mx4 *w, const mxh_mat *residual, const mxh_mat *y,
+                            uint64_t *bytes) {
     return guard([&] {
         if (!bytes) throw Error("bytes: missing");
-        check_first(need(x, "x"), "x");
-        if (!w) throw Error("w: missing");
-        check_mx4(w, "w", w->rows, x->cols);
-        check_mat(need(y, "y"), "y", x->dtype, x->rows, w->rows);
-        // a y of one row or column has both orders, and a residual may settle it
         *bytes = 0;
-        if (empty(*y)) return;
-        if (out_by_cols(*y)) *bytes = mx4_plan(*x, w->rows, true).bytes();
-        if (out_by_rows(*y)) *bytes = std::max(*bytes, mx4_plan(*x, w->rows, false).bytes());
+        const bool by_cols = check_dense(x, w, residual, y);
+        if (!empty(*y)) *bytes = mx4_plan(*x, w->rows, by_cols).bytes();
     });
 }
 
 int mxh_mx4_dense(int device, void *stream, const mxh_mat *x, const mxh_mx4 *w, const mxh_vec *bias, int act, float slope,
                   const mxh_mat *residual, const mxh_mat *y, void *workspace, uint64_t workspace_bytes) {
     return guard([&] {
-        const mxh_mat &X = need(x, "x"), &Y = need(y, "y");
-        check_first(X, "x");
-        if (!w) throw Error("w: missing");
-        check_mx4(w, "w", w->rows, X.cols);
-        check_mat(Y, "y", X.dtype, X.rows, w->rows);
-        check_out(Y, "y");
+        const bool by_cols = check_dense(x, w, residual, y);
+        const mxh_mat &X = *x, &Y = *y;
         check_act(act);
         if (bias) check_vec(*bias, "bias", w->rows, X.dtype);
-        if (residual) check_mat(*residual, "residual", X.dtype, X.rows, w->rows);
-        const bool by_cols = common_order({residual}, {y});
         refuse_overlap(Y, "y", X, "x");
         refuse_overlap(Y, "y", bytes_of(w->codes, code_bytes(w->rows, w->cols)), "w's codes");
         refuse_overlap(Y, "y", bytes_of(w->scales, scale_bytes(w->rows, w->cols)), "w's scales");

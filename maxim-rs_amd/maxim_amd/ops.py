@@ -84,7 +84,7 @@ def _lib():
             "mxh_dense_backward": [I, V, M, M, M, M, I, F, M, M, N, V, U],
             "mxh_dense_backward_workspace": [M, M, M, I, M, M, N, B],
             "mxh_gated": [I, V, M, M, N, I, F, M, M, V, U],
-            "mxh_gated_workspace": [M, M, M, B],
+            "mxh_gated_workspace": [M, M, M, M, B],
             "mxh_gated_backward": [I, V, M, M, M, M, I, F, M, M, N, V, U],
             "mxh_gated_backward_workspace": [M, M, M, M, M, N, B],
             "mxh_grad_norm": [I, V, N, C.c_int64, V, V, U],
@@ -95,7 +95,7 @@ def _lib():
             "mxh_mx4_quantize": [I, V, M, Q],
             "mxh_mx4_dequantize": [I, V, Q, M],
             "mxh_mx4_dense": [I, V, M, Q, N, I, F, M, M, V, U],
-            "mxh_mx4_dense_workspace": [M, Q, M, B],
+            "mxh_mx4_dense_workspace": [M, Q, M, M, B],
         }
         for name, args in sig.items():
             f = getattr(L, name)
@@ -339,7 +339,7 @@ def gated(x, w, bias=None, act="silu", slope=0.0, planar=False, save=False, out=
     y, Y = _new(x, X, W.rows // 2, planar) if out is None else (out, _mat(out, "out", d, planar))
     z, Z = _new(y, Y, W.rows, planar) if save else (None, None)
     size = C.c_uint64()
-    _check(_L.mxh_gated_workspace(X, W, Y, size))
+    _check(_L.mxh_gated_workspace(X, W, Y, Z, size))
     ws = _workspace(size.value, x)
     _check(_L.mxh_gated(d, _stream(d), X, W, B, f, slope, Y, Z, _ptr(ws), size.value))
     _written(out)
@@ -532,7 +532,7 @@ def mx4_dense(x, w, bias=None, act=None, slope=0.0, residual=None, planar=False,
     like, Like = (x, X) if residual is None else (residual, R)
     y, Y = _new(like, Like, W.rows, planar) if out is None else (out, _mat(out, "out", d, planar))
     size = C.c_uint64()
-    _check(_L.mxh_mx4_dense_workspace(X, W, Y, size))
+    _check(_L.mxh_mx4_dense_workspace(X, W, R, Y, size))
     ws = _workspace(size.value, x)
     _check(_L.mxh_mx4_dense(d, _stream(d), X, W, B, a, slope, R, Y, _ptr(ws), size.value))
     _written(out)

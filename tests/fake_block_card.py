@@ -65,8 +65,9 @@ def main():
             return {"rc": rc, "modules": fake.fake_modules()}
         if op == "gated":
             x, wt, y = m(c["x"]), m(c["w"]), m(c["y"])
-            rc = L.mxh_gated_workspace(x, wt, y, n)
-            rc = rc or L.mxh_gated(0, None, x, wt, w(g("bias")), g("act", 3), 0.2, y, m(g("z")), WORKSPACE, n.value)
+            z = m(g("z"))
+            rc = L.mxh_gated_workspace(x, wt, y, z, n)
+            rc = rc or L.mxh_gated(0, None, x, wt, w(g("bias")), g("act", 3), 0.2, y, z, WORKSPACE, n.value)
         elif op == "gated_backward":
             a = [m(c["dy"]), m(c["x"]), m(c["w"])]
             outs = [m(g("dx")), m(g("dw")), w(g("db"))]
@@ -86,8 +87,9 @@ def main():
             rc = L.mxh_mx4_dequantize(0, None, q(c["q"]), m(c["y"]))
         else:
             x, wt, y = m(c["x"]), q(c["w"]), m(c["y"])
-            rc = L.mxh_mx4_dense_workspace(x, wt, y, n)
-            rc = rc or L.mxh_mx4_dense(0, None, x, wt, w(g("bias")), g("act", 0), 0.2, m(g("residual")), y, WORKSPACE, n.value)
+            res = m(g("residual"))
+            rc = L.mxh_mx4_dense_workspace(x, wt, res, y, n)
+            rc = rc or L.mxh_mx4_dense(0, None, x, wt, w(g("bias")), g("act", 0), 0.2, res, y, WORKSPACE, n.value)
         return {"rc": rc, "error": P.last_error() if rc else "", "workspace": n.value,
                 "launches": json.loads(fake.fake_launches())}
 

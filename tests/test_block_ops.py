@@ -83,10 +83,13 @@ def test_gated_refusals():
     refused("not aligned", gated(mat(16, 32, 1), w, b, y))
     refused("device ordinal", O._lib().mxh_gated(64, None, x, w, b, 3, 0.0, y, z, None, 0))
     size = C.c_uint64()
-    refused("bytes: missing", O._lib().mxh_gated_workspace(x, w, y, None))
+    refused("bytes: missing", O._lib().mxh_gated_workspace(x, w, y, None, None))
+    refused("x: missing", O._lib().mxh_gated_workspace(None, w, y, None, size))
+    refused("w: missing", O._lib().mxh_gated_workspace(x, None, y, None, size))
+    refused("y: missing", O._lib().mxh_gated_workspace(x, w, None, None, size))
     # a long sum of few results is cut, which takes scratch
     x, w, y = mat(64, 65536), mat(16, 65536, 1 << 24), mat(64, 8, 1 << 26)
-    assert O._lib().mxh_gated_workspace(x, w, y, size) == 0 and size.value > 0
+    assert O._lib().mxh_gated_workspace(x, w, y, None, size) == 0 and size.value > 0
     refused("bytes of workspace", gated(x, w, None, y))
     refused("bytes of workspace, not", gated(x, w, None, y, ws=BASE + (1 << 36), n=size.value - 1))
     refused("16 bytes", gated(x, w, None, y, ws=BASE + (1 << 36) + 8, n=size.value))
@@ -115,6 +118,9 @@ def test_gated_backward_refusals():
     refused("dw overlaps dx", gated_backward(*a, dx, mat(48, 32, (4 << 20) + 64), db))
     refused("db overlaps dw", gated_backward(*a, dx, dw, vec(48, 5 << 20)))
     size = C.c_uint64()
+    for missing, ops in (("dy", (None, x, w)), ("x", (dy, None, w)), ("w", (dy, x, None))):
+        refused(missing + ": missing", O._lib().mxh_gated_backward_workspace(*ops, dx, dw, db, size))
+        refused(missing + ": missing", gated_backward(*ops, z, dx, dw, db))
     assert O._lib().mxh_gated_backward_workspace(dy, x, w, dx, dw, db, size) == 0 and size.value
     refused("bytes of workspace, not", gated_backward(*a, dx, dw, db, n=size.value - 1))
     refused("dx: [16][31]", O._lib().mxh_gated_backward_workspace(dy, x, w, mat(16, 31, 4 << 20), dw, db, size))
@@ -193,7 +199,12 @@ def test_mx4_refusals():
         return L.mxh_mx4_dense(0, None, x, w, b, act, 0.0, res, y, ws, n)
 
     w, y, b = mx4(24, 32), mat(16, 24, 2 << 20), vec(24)
+    for missing, ops in (("x", (None, w, None, y)), ("w", (x, None, None, y)), ("y", (x, w, None, None))):
+        refused(missing + ": missing", L.mxh_mx4_dense_workspace(*ops, s))
+    refused("bytes: missing", L.mxh_mx4_dense_workspace(x, w, None, y, None))
     refused("w: missing", dense(x, None, b, y))
+    refused("x: missing", dense(None, w, b, y))
+    refused("y: missing", dense(x, w, b, None))
     refused("w: [24][33]", dense(x, mx4(24, 33), b, y))
     refused("y: [16][25]", dense(x, w, b, mat(16, 25, 2 << 20)))
     refused("bias: 23", dense(x, w, vec(23), y))
@@ -206,7 +217,7 @@ def test_mx4_refusals():
     refused("y overlaps the residual", dense(x, w, b, y, res=mat(16, 24, (2 << 20) + 2)))
     size = C.c_uint64()
     x, y = mat(40, 32), mat(40, 24, 2 << 20)
-    assert L.mxh_mx4_dense_workspace(x, w, y, size) == 0 and size.value
+    assert L.mxh_mx4_dense_workspace(x, w, None, y, size) == 0 and size.value
     refused("bytes of workspace, not", dense(x, w, b, y, n=size.value - 1))
     refused("bytes of workspace", dense(x, w, b, y, ws=None))
 
@@ -310,6 +321,21 @@ def test_gated_launches(card, dtype):
         check_gated(c, r)
 
 
+def test_a_tokens_call_needs_no_workspace(card):
+    """One row of results lies in both orders: the one that the operands settle
+    counts."""
+    x, r = fmat(1, 4096, AT[0], True, 0, BF16), fmat(1, 4096, AT[5], True, 0, BF16)
+    calls = [gated_calls(1, 2048, 4096, BF16)[0],
+             {"op": "mx4_dense", "x": x, "w": [AT[2], AT[3], 4096, 4096], "y": fmat(1, 4096, AT[1], True, 0, BF16), "residual": r},
+             {"op": "mx4_dense", "x": x, "w": [AT[2], AT[3], 4096, 4096], "y": [AT[1], 1, 4096, 1, 1, BF16],
+              "residual": [AT[5], 1, 4096, 1, 3, BF16]}]
+    got = card(calls)
+    assert [g["rc"] for g in got] == [0, 0, 0]
+    assert [g["workspace"] for g in got[:2]] == [0, 0] and got[2]["workspace"] > 0
+    assert [l["kernel"][:10] for g in got for l in g["launches"]][:2] == ["mxg_skinny", "mxq_skinny"]
+    assert [l["m"] for l in got[2]["launches"] if "gemm" in l["kernel"]] == [4096]  # a residual of stride 3: planes of one position
+
+
 def test_gated_forms_of_single_rows_and_columns(card):
     """Axes of one element have any stride: the call's order holds, and only
     kernels that there are take part."""
@@ -410,8 +436,7 @@ def test_mx4_launches(card):
         assert len(l) == 1
         l = l[0]
         if "skinny" in l["kernel"]:
-            # (results of one row or column lie in both orders: the other's bytes too)
-            assert rows <= 16 and l["k"] == tiles and l["gx"] == -(-n // 16) and (r["workspace"] == 0 or rows == 1 or n == 1)
+            assert rows <= 16 and l["k"] == tiles and l["gx"] == -(-n // 16) and r["workspace"] == 0
             continue
         assert {l["m"], l["n"]} == {rows, n} and l["k"] == tiles
         if k:
