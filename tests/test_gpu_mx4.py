@@ -245,6 +245,25 @@ def test_mx4_dense_of_nothing_slices_and_places():
     assert torch.equal(O.mx4_dense(xt.t(), q).t(), O.mx4_dense(xt, q, planar=True))
 
 
+@pytest.mark.parametrize("planar", [False, True])
+def test_the_longest_lines(planar):
+    """As many features as a tile's offsets reach, and one block of 32 past
+    them refused: sums of a few powers of two, which are exact."""
+    k, at = (1 << 24) - 256, [0, 31, 32, (1 << 23) + 5, (1 << 24) - 300, (1 << 24) - 257]
+    w = torch.zeros(4, k, dtype=torch.bfloat16, device="cuda")
+    for j, c in enumerate(at):
+        w[j % 4, c] = 2.0 ** j
+    q = O.mx4_quantize(w)
+    for rows in (3, 20):
+        x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+        x[:, at] = torch.tensor([2.0 ** (i % 5) for i in range(rows)], dtype=torch.bfloat16, device="cuda")[:, None]
+        y = O.mx4_dense(x.t().contiguous() if planar else x, q, planar=planar)
+        want = x[:, :1].float() * torch.tensor([1.0 + 16, 2.0 + 32, 4.0, 8.0], device="cuda")
+        assert torch.equal((y.t() if planar else y).float(), want)
+    with pytest.raises(P.MaximError, match="out of range"):
+        O.mx4_quantize(torch.zeros(1, k + 32, dtype=torch.bfloat16, device="cuda"))
+
+
 def test_captured():
     x = torch.randn(100, 512, device="cuda").bfloat16()
     q = O.mx4_quantize(torch.randn(300, 512, device="cuda"))
