@@ -171,7 +171,8 @@ int mxh_gated_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         Launches launches;
         char *ws = static_cast<char *>(workspace);
         const std::string t = kTypeName[X.dtype];
-        OpsDzArgs a{};
+        OpsGatedDzArgs dz{};
+        OpsDzArgs &a = dz.d;
         a.dy = DY.data;
         a.z = Z.data;
         a.rows = DY.rows;
@@ -179,17 +180,20 @@ int mxh_gated_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         a.dyrs = DY.row_stride, a.dycs = DY.col_stride;
         a.zrs = Z.row_stride, a.zcs = Z.col_stride;
         if (l.dz_bytes) l.dz.data = a.dz = ws, a.drs = l.dz.row_stride, a.dcs = l.dz.col_stride;
-        if (db) a.part = reinterpret_cast<float *>(ws + l.dz_bytes);
+        // one part, with rows: its sums are db itself
+        const bool whole = db && l.parts == 1 && DY.rows;
+        if (whole) dz.db = db->data, dz.db_type = db->dtype;
+        else if (db) a.part = reinterpret_cast<float *>(ws + l.dz_bytes);
         a.nparts = (int32_t)gated_parts(DY, by_cols);
         a.act = act;
         a.slope = slope;
-        if ((a.dz || a.part) && !empty(DY))
+        if ((a.dz || a.part || dz.db) && !empty(DY))
             launches.add((by_cols ? "mxg_dz_rows_" : "mxg_dz_planar_") + t,
-                         by_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, a);
+                         by_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, dz);
         void *pw = ws + l.dz_bytes + l.part_bytes;
         if (dx && !empty(*dx)) product(launches, product_dx(l, W, *dx), pw);
         OpsGradJoinArgs j{};
-        if (dw && !empty(*dw)) product(launches, product_dw(l, X, *dw), pw, db ? &j.g : nullptr);
+        if (dw && !empty(*dw)) product(launches, product_dw(l, X, *dw), pw, db && !whole ? &j.g : nullptr);
         const int64_t parts = DY.rows ? l.parts : 0, quads = j.g.m * cdiv(j.g.n, 4);
         // dw's splits and the bias's parts in one launch, where dw is small
         if (j.g.splits > 1 && quads <= 65536) {
@@ -202,7 +206,7 @@ int mxh_gated_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
             launches.add("mxg_grad_join_" + t, j.first + cdiv(W.rows, 4), 1, 256, j);
         } else {
             if (j.g.splits > 1) join_product(launches, j.g, X.dtype);
-            if (db) join(launches, a.part, parts, W.rows, db->data, nullptr, db->dtype);
+            if (db && !whole) join(launches, a.part, parts, W.rows, db->data, nullptr, db->dtype);
         }
         launches.run(device, stream);
     });

@@ -95,3 +95,11 @@ struct OpsGradJoinArgs {
     int32_t n, nparts;
     int32_t first, dtype;
 };
+
+// The gated Dense's dz pass: z and dz have twice dy's features, cols the half's.
+// A single part needs no joining: its sums are the bias's gradient.
+struct OpsGatedDzArgs {
+    OpsDzArgs d;
+    void *db;  // null: the sums go to d.part
+    int32_t db_type, pad;
+};

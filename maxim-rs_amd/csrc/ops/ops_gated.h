@@ -279,10 +279,22 @@ __device__ __forceinline__ void gated_dz_n(int act, float slope, float *v, float
 #undef OPS_DZ
 }
 
+__device__ __forceinline__ void store_sum(void *out, int dtype, int64_t i, float v) {
+    if (dtype == MXO_F32) static_cast<float *>(out)[i] = v;
+    else if (dtype == MXO_F16) static_cast<f16 *>(out)[i] = from_f<f16>(v);
+    else static_cast<bf16 *>(out)[i] = from_f<bf16>(v);
+}
+// A part's sum of feature i of 2 cols.
+__device__ __forceinline__ void keep_sum(const OpsGatedDzArgs &g, int64_t part, int64_t i, float v) {
+    if (g.db) store_sum(g.db, g.db_type, i, v);
+    else g.d.part[2 * part * g.d.cols + i] = v;
+}
+
 // Rows with contiguous features: 64 x E features by a run of rows a block, a
 // wave a row at a time.
 template <typename T, bool WHOLE>
-__device__ __forceinline__ void gated_dz_rows(const OpsDzArgs &a, float (*sh)[2][64 * 16 / sizeof(T)]) {
+__device__ __forceinline__ void gated_dz_rows(const OpsGatedDzArgs &g, float (*sh)[2][64 * 16 / sizeof(T)]) {
+    const OpsDzArgs &a = g.d;
     constexpr int E = 16 / sizeof(T);
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + l) * E, p = blockIdx.y, have = a.cols - c;
@@ -320,7 +332,7 @@ __device__ __forceinline__ void gated_dz_rows(const OpsDzArgs &a, float (*sh)[2]
                     for (int64_t k = 2 * a.cols - c; k < a.drs - c; ++k) dz[k] = (T)0.0f;
             }
         }
-    if (!a.part) return;
+    if (!a.part && !g.db) return;
 #pragma unroll
     for (int e = 0; e < E; ++e) sh[w][0][l * E + e] = sa[e], sh[w][1][l * E + e] = sc[e];
     __syncthreads();
@@ -328,12 +340,13 @@ __device__ __forceinline__ void gated_dz_rows(const OpsDzArgs &a, float (*sh)[2]
         const int h = k >= 64 * E, i = k - h * 64 * E;
         const int64_t col = (int64_t)blockIdx.x * 64 * E + i;
         if (col < a.cols)
-            a.part[(2 * p + h) * a.cols + col] = (sh[0][h][i] + sh[1][h][i]) + (sh[2][h][i] + sh[3][h][i]);
+            keep_sum(g, p, h * a.cols + col, (sh[0][h][i] + sh[1][h][i]) + (sh[2][h][i] + sh[3][h][i]));
     }
 }
 // Planar order: one feature by a run of positions a block.
 template <typename T>
-__device__ __forceinline__ void gated_dz_planar(const OpsDzArgs &a) {
+__device__ __forceinline__ void gated_dz_planar(const OpsGatedDzArgs &g) {
+    const OpsDzArgs &a = g.d;
     constexpr int E = 16 / sizeof(T);
     __shared__ float sh[2][4];
     const int64_t c = blockIdx.x, p = blockIdx.y;
@@ -360,13 +373,13 @@ __device__ __forceinline__ void gated_dz_planar(const OpsDzArgs &a) {
             store_n<T, E>(dz + a.cols * a.dcs + r, oc);
         }
     }
-    if (!a.part) return;
+    if (!a.part && !g.db) return;
     sa = wave_sum(sa), sc = wave_sum(sc);
     if ((threadIdx.x & 63) == 0) sh[0][threadIdx.x >> 6] = sa, sh[1][threadIdx.x >> 6] = sc;
     __syncthreads();
     if (threadIdx.x < 2) {
         const float *s = sh[threadIdx.x];
-        a.part[(2 * p + threadIdx.x) * a.cols + c] = (s[0] + s[1]) + (s[2] + s[3]);
+        keep_sum(g, p, threadIdx.x * a.cols + c, (s[0] + s[1]) + (s[2] + s[3]));
     }
 }
 
@@ -394,11 +407,7 @@ __device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
             __syncthreads();
             if (w < half) s[t] += s[t + half * 4];
         }
-        if (w == 0 && c < a.n) {
-            if (a.dtype == MXO_F32) static_cast<float *>(a.out)[c] = s[t];
-            else if (a.dtype == MXO_F16) static_cast<f16 *>(a.out)[c] = from_f<f16>(s[t]);
-            else static_cast<bf16 *>(a.out)[c] = from_f<bf16>(s[t]);
-        }
+        if (w == 0 && c < a.n) store_sum(a.out, a.dtype, c, s[t]);
         return;
     }
     const OpsGemmArgs &g = a.g;
@@ -472,12 +481,12 @@ __device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
     OPS_GATED_JOIN(name, T, m, PAIR_M)                                                                                   \
     extern "C" __global__ __launch_bounds__(512) void mxg_skinny_##name(OpsGemmArgs g) { gated_skinny<T>(g); }           \
     extern "C" __global__ __launch_bounds__(256) void mxg_grad_join_##name(OpsGradJoinArgs a) { grad_join<T>(a); }        \
-    extern "C" __global__ __launch_bounds__(256) void mxg_dz_rows_##name(OpsDzArgs a) {                                  \
+    extern "C" __global__ __launch_bounds__(256) void mxg_dz_rows_##name(OpsGatedDzArgs a) {                                  \
         __shared__ float sh[4][2][64 * 16 / sizeof(T)];                                                                  \
-        if (a.cols % (16 / sizeof(T)) == 0) gated_dz_rows<T, true>(a, sh);                                               \
+        if (a.d.cols % (16 / sizeof(T)) == 0) gated_dz_rows<T, true>(a, sh);                                               \
         else gated_dz_rows<T, false>(a, sh);                                                                             \
     }                                                                                                                    \
-    extern "C" __global__ __launch_bounds__(256) void mxg_dz_planar_##name(OpsDzArgs a) { gated_dz_planar<T>(a); }
+    extern "C" __global__ __launch_bounds__(256) void mxg_dz_planar_##name(OpsGatedDzArgs a) { gated_dz_planar<T>(a); }
 
 OPS_GATED_TYPE(bf16, bf16)
 OPS_GATED_TYPE(f16, f16)

@@ -58,8 +58,10 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned gx, unsigned gy, unsi
         std::memcpy(&a, params[0], sizeof(a));
         product(a);
     } else if (begins("mxg_dz")) {
-        OpsDzArgs a;
-        std::memcpy(&a, params[0], sizeof(a));
+        OpsGatedDzArgs g;
+        std::memcpy(&g, params[0], sizeof(g));
+        const OpsDzArgs &a = g.d;
+        put("db", (intptr_t)g.db);
         put("dz", (intptr_t)a.dz), put("part", (intptr_t)a.part), put("nparts", a.nparts), put("drs", a.drs), put("dcs", a.dcs);
     } else if (begins("mxq_gemm") || begins("mxq_skinny")) {
         Mx4GemmArgs a;

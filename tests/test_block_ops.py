@@ -276,7 +276,9 @@ def check_gated(c, r):
             line, lines = (l["drs"], rows) if "rows" in l["kernel"] else (l["dcs"], 2 * n)
             assert l["dz"] == F.WORKSPACE and l["dz"] + line * lines * size <= end
             assert line * size % 16 == 0 and line >= (2 * n if "rows" in l["kernel"] else rows)
-            assert l["part"] + l["nparts"] * 2 * n * 4 <= end
+            # a single part is the bias's gradient itself
+            assert (l["db"] != 0) == (l["nparts"] == 1) == (l["part"] == 0)
+            assert l["part"] + l["nparts"] * 2 * n * 4 <= end or l["db"] == c["db"][0]
         f = re.match(r"mx([og])_gemm_(?:([nm])_)?(bf16|f16|f32)_(\d+)x\d+_([km])([km])(_d\d)?$", l["kernel"])
         if not f:
             continue
