@@ -56,13 +56,14 @@ __device__ __forceinline__ void store_upto(T *p, const Vec<T, N> &v, int64_t hav
         if (i < have) p[i] = v.v[i];
 }
 
+typedef uint32_t u32x4_at_any __attribute__((ext_vector_type(4), aligned(2)));
 // The same for results, which nothing in this launch reads again: not kept in
 // L2, whose dirty lines are written back only when the kernel ends.
 template <typename T, int N>
 __device__ __forceinline__ void store_out(T *p, const Vec<T, N> &v, int64_t have) {
     if (have >= N) {
         if constexpr (sizeof(v) == 16)
-            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4 *>(p));
+            __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4_at_any *>(p));
         else
             store_n<T, N>(p, v);
         return;
