@@ -74,8 +74,8 @@ int mxh_grad_clip_by(int device, void *stream, const mxh_vec *grads, const mxh_v
  * codes: a line of ceil(cols / 256) * 128 bytes a row, an element's code in the
  * low half of its byte where its feature is even; scales: for 64 rows and 256
  * features 512 bytes, that of row r and block b at [r / 64][b / 8][b % 4][r %
- * 16][r / 16 % 4][b / 4 % 2]. Elements past the last feature are 0. Both are
- * 16-byte aligned; mxh_mx4_size gives their bytes.
+ * 16][r / 16 % 4][b / 4 % 2]. Elements past the last feature and scales past
+ * the last row are 0. Both are 16-byte aligned; mxh_mx4_size gives their bytes.
  */
 typedef struct mxh_mx4 {
     void *codes, *scales;

@@ -92,7 +92,11 @@ __device__ __forceinline__ void mx4_quantize_rows(const Mx4CodeArgs &a) {
         if ((lane & 3) == 0) reinterpret_cast<uint8_t *>(sh)[(at >> 3) * 4 + (at & 3)] = (uint8_t)s;
     }
     __syncthreads();
-    if (t < 64) reinterpret_cast<uint32_t *>(a.scales)[((half >> 1) * a.tiles + tile) * 128 + t * 2 + (half & 1)] = sh[t];
+    if (t < 64) {
+        uint32_t *scales = reinterpret_cast<uint32_t *>(a.scales) + ((half >> 1) * a.tiles + tile) * 128 + t * 2;
+        scales[half & 1] = sh[t];
+        if (!(half & 1) && r0 + 32 >= a.rows) scales[1] = 0;  // a half group that no block has
+    }
 }
 
 // Planar order: a block takes 64 positions (fp32) or 128 by a tile, a lane one

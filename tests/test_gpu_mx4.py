@@ -90,6 +90,24 @@ def test_quantize_and_back(rows, k, dt, planar):
         check_quantize(x, v, planar)
 
 
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 63, 64, 97])
+@pytest.mark.parametrize("k", [40, 256, 300])
+def test_all_bytes_are_written(rows, k):
+    # both orders fill the whole storage, and alike: zeros for the rows and
+    # features that are not there
+    x, _ = make(31, rows, k, torch.bfloat16)
+    stored = []
+    for t, planar in ((x, False), (x.t().contiguous(), True)):
+        q = O.mx4_quantize(t, planar=planar)
+        q._data.fill_(0xff)
+        O._check(O._L.mxh_mx4_quantize(0, O._stream(0), O._mat(t, "x", 0, planar), q._mat()))
+        stored.append(q._data.cpu())
+    assert torch.equal(stored[0], stored[1])
+    tiles = (k + 255) // 256
+    scales = stored[0][q._code_bytes:].view(-1, tiles, 4, 16, 4, 2).permute(0, 4, 3, 1, 5, 2).reshape(-1, tiles * 8)
+    assert not scales[rows:].any() and not scales[:, (k + 31) // 32:].any()
+
+
 def test_every_16_bit_value():
     """Each finite bf16 and fp16 value beside a 6 of every one of some scales,
     so that elements fall on and between all codes, and alone."""
