@@ -65,6 +65,17 @@ static int64_t gated_parts(const mxh_mat &dy, bool by_cols) {
     return std::min<int64_t>(65535, cdiv(dy.rows, turn * std::max<int64_t>(1, dy.rows / (turn * want))));
 }
 
+// The dz pass's blocks across the features.
+static int64_t gated_across(const mxh_mat &dy, bool by_cols) {
+    return by_cols ? cdiv(dy.cols, 64 * 16 / (int64_t)type_size(dy.dtype)) : dy.cols;
+}
+// So many blocks' largest magnitudes each block reads for itself (16 KiB, from
+// L2); more of them one block reads for all.
+constexpr int64_t kFewTops = 4096;
+// Blocks that form dz again, which mostly leave at once (4096 x 2 x 2048 out of
+// range: 256 and 512 take 4 us more, 2048 nothing less).
+constexpr int64_t kBlocksAgain = 1024;
+
 static BwdLayout gated_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x, const mxh_mat &w, const mxh_mat *dx,
                               const mxh_mat *dw, const mxh_vec *db) {
     BwdLayout l;
@@ -74,6 +85,9 @@ static BwdLayout gated_layout(const mxh_mat &dy, bool by_cols, const mxh_mat &x,
         l.parts = gated_parts(dy, by_cols);
         l.part_bytes = up((uint64_t)l.parts * 2 * dy.cols * 4);
     }
+    // fp16: a magnitude a block, the largest, and what the products take back
+    if (l.dz_bytes && dy.dtype == MXH_F16)
+        l.top_bytes = up((uint64_t)(gated_across(dy, by_cols) * gated_parts(dy, by_cols) + 2) * 4);
     if (dx && !empty(*dx)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dx(l, w, *dx)).bytes);
     if (dw && !empty(*dw)) l.product_bytes = std::max(l.product_bytes, plan_of(product_dw(l, x, *dw)).bytes);
     return l;
@@ -187,13 +201,32 @@ int mxh_gated_backward(int device, void *stream, const mxh_mat *dy, const mxh_ma
         a.nparts = (int32_t)gated_parts(DY, by_cols);
         a.act = act;
         a.slope = slope;
-        if ((a.dz || a.part || dz.db) && !empty(DY))
-            launches.add((by_cols ? "mxg_dz_rows_" : "mxg_dz_planar_") + t,
-                         by_cols ? cdiv(DY.cols, 64 * 16 / (int64_t)type_size(DY.dtype)) : DY.cols, a.nparts, 256, dz);
-        void *pw = ws + l.dz_bytes + l.part_bytes;
-        if (dx && !empty(*dx)) product(launches, product_dx(l, W, *dx), pw);
+        const float *back = nullptr;
+        if ((a.dz || a.part || dz.db) && !empty(DY)) {
+            const std::string name = (by_cols ? "mxg_dz_rows_" : "mxg_dz_planar_") + t;
+            const int64_t across = gated_across(DY, by_cols), blocks = across * a.nparts;
+            if (l.top_bytes) dz.top = reinterpret_cast<float *>(ws + l.dz_bytes + l.part_bytes);
+            launches.add(name, across, a.nparts, 256, dz);
+            if (l.top_bytes) {
+                dz.ntop = (int32_t)blocks;
+                back = dz.back = dz.top + blocks + 1;
+                if (blocks > kFewTops) {
+                    dz.pass = MXO_DZ_TOPS;
+                    launches.add(name, 1, 1, 256, dz);
+                    dz.top += blocks, dz.ntop = 1;
+                }
+                dz.pass = MXO_DZ_SCALED;
+                launches.add(name, across, std::max<int64_t>(1, std::min<int64_t>(a.nparts, kBlocksAgain / across)), 256, dz);
+            }
+        }
+        void *pw = ws + l.dz_bytes + l.part_bytes + l.top_bytes;
+        auto gradient = [&](Product p, OpsGemmArgs *later) {
+            p.back = back;
+            product(launches, p, pw, later);
+        };
+        if (dx && !empty(*dx)) gradient(product_dx(l, W, *dx), nullptr);
         OpsGradJoinArgs j{};
-        if (dw && !empty(*dw)) product(launches, product_dw(l, X, *dw), pw, db && !whole ? &j.g : nullptr);
+        if (dw && !empty(*dw)) gradient(product_dw(l, X, *dw), db && !whole ? &j.g : nullptr);
         const int64_t parts = DY.rows ? l.parts : 0, quads = j.g.m * cdiv(j.g.n, 4);
         // dw's splits and the bias's parts in one launch, where dw is small
         if (j.g.splits > 1 && quads <= 65536) {

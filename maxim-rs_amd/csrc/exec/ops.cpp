@@ -355,6 +355,7 @@ void product(Launches &launches, const Product &given, void *ws, OpsGemmArgs *la
     g.b = p.b.data;
     g.c = p.c;
     g.z = p.z;
+    g.back = p.back;
     g.res = p.res;
     g.part = reinterpret_cast<float *>(at);
     g.lda = ak ? p.a.own : p.a.sum;

@@ -61,7 +61,10 @@ class Launches {
         unsigned gx, gy, block;
         alignas(8) char args[200];
     };
-    One at_[8];  // a Dense's backward pass: dz and its join, twice packing, product and join
+    // a gated Dense's backward pass: dz in up to three launches and its join, twice
+    // packing, product and join
+    static constexpr int kMost = 10;
+    One at_[kMost];
     int n_ = 0;
 
 public:
@@ -77,7 +80,7 @@ public:
     }
     void run(int dev, void *stream) {
         OnDevice on(dev);
-        mxh::hipFunction_t f[8];
+        mxh::hipFunction_t f[kMost];
         for (int i = 0; i < n_; ++i) f[i] = function(dev, at_[i].name);
         for (int i = 0; i < n_; ++i) {
             One &o = at_[i];
@@ -260,6 +263,7 @@ struct Product {
     int64_t ldr = 0;
     void *z = nullptr;
     int64_t ldz = 0;
+    const float *back = nullptr;  // fp16: what the sums are multiplied by
     int act = MXH_NONE;
     float slope = 0.0f;
 };
@@ -294,8 +298,8 @@ void join(Launches &launches, const float *part, int64_t nparts, int64_t n, void
 struct BwdLayout {
     mxh_mat dz{};
     int64_t parts = 0;
-    uint64_t dz_bytes = 0, part_bytes = 0, product_bytes = 0;
-    uint64_t total() const { return dz_bytes + part_bytes + product_bytes; }
+    uint64_t dz_bytes = 0, part_bytes = 0, top_bytes = 0, product_bytes = 0;
+    uint64_t total() const { return dz_bytes + part_bytes + top_bytes + product_bytes; }
 };
 Product product_dx(const BwdLayout &l, const mxh_mat &w, const mxh_mat &dx);
 Product product_dw(const BwdLayout &l, const mxh_mat &x, const mxh_mat &dw);

@@ -19,6 +19,7 @@ struct OpsGemmArgs {
     const void *a, *b, *bias, *res;
     void *c, *z;
     float *part;  // [splits][m][n] partial sums when splits > 1
+    const float *back;  // fp16: sums are times *back (null: as they are)
     int64_t lda, ldb, ldc, ldr, ldz;
     int32_t m, n, k;
     int32_t splits, kchunk;  // split s covers k in [s kchunk, (s + 1) kchunk)
@@ -97,9 +98,15 @@ struct OpsGradJoinArgs {
 };
 
 // The gated Dense's dz pass: z and dz have twice dy's features, cols the half's.
-// A single part needs no joining: its sums are the bias's gradient.
+// A single part needs no joining: its sums are the bias's gradient. fp16: each
+// block's largest finite |dz| goes to `top`, where the launch that follows finds
+// the scale that dz needs.
+enum { MXO_DZ = 0, MXO_DZ_SCALED, MXO_DZ_TOPS };
 struct OpsGatedDzArgs {
     OpsDzArgs d;
-    void *db;  // null: the sums go to d.part
-    int32_t db_type, pad;
+    void *db;     // null: the sums go to d.part
+    float *top;   // [ntop], and one more for all of them; null: none are kept
+    float *back;  // what the products take dz's scale back by
+    int32_t db_type, pass;
+    int32_t ntop, pad;
 };

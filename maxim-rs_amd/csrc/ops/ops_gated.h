@@ -290,6 +290,71 @@ __device__ __forceinline__ void keep_sum(const OpsGatedDzArgs &g, int64_t part, 
     else g.d.part[2 * part * g.d.cols + i] = v;
 }
 
+// dz in fp16. A product of three values leaves fp16's range where the gradients
+// it leads to do not: past 65504 it would be infinite, and below 2^-14 it loses
+// bits. So the pass keeps each block's largest finite |dz| (`top`), and a second
+// launch of it, from the largest of all: 1 to 65520, or nothing: dz is right as it
+// is, and the blocks leave; else they form dz again, times the power of two that
+// takes the largest into [2^14, 2^15), which the products' sums are divided by.
+// An element is off by half a step of its own, or by 2^-25 as it is and 2^-39 of
+// the largest where it was scaled. (One scale for all: a row's own would do for dx, whose sums stay in a row, but not for dw.
+// Scaling always would take a pass over dy and z before this one.) A backward pass
+// of 4096 x 1024 to 2 x 2048 takes 99 us without any of this, 105 with dz in range
+// (the magnitudes 1, the launch that leaves 3 to 4) and 113 with dz out of it; 64 to
+// 2 x 64 planes of 71680 30, 34 and 44.
+template <typename T>
+constexpr bool kScaled = __is_same(T, f16);
+// The largest of 256 threads' values, in all of them.
+__device__ __forceinline__ float block_top(float v) {
+    __shared__ float at[4];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
+    if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(at[0], at[1]), fmaxf(at[2], at[3]));
+}
+// The larger of `top` and the finite magnitudes of v and u (NaN drops out of a
+// maximum by itself).
+template <int E>
+__device__ __forceinline__ float top_of(float top, const float *v, const float *u) {
+    float m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(fmaxf(m, fabsf(v[e])), fabsf(u[e]));
+    if (m == __builtin_inff()) {
+        m = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float a = fabsf(v[e]), b = fabsf(u[e]);
+            m = fmaxf(fmaxf(m, a < __builtin_inff() ? a : 0.0f), b < __builtin_inff() ? b : 0.0f);
+        }
+    }
+    return fmaxf(top, m);
+}
+__device__ __forceinline__ void keep_top(const OpsGatedDzArgs &g, float v) {
+    if (!g.top) return;
+    v = block_top(v);
+    if (threadIdx.x == 0) g.top[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = v;
+}
+// What this launch's dz is multiplied by; 0: there is nothing to do. Many blocks'
+// magnitudes are brought to one by a launch of their own (MXO_DZ_TOPS), not by
+// every block.
+__device__ __forceinline__ float dz_scale(const OpsGatedDzArgs &g) {
+    if (g.pass == MXO_DZ) return 1.0f;
+    float v = 0.0f;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < g.ntop; i += 256) v = fmaxf(v, g.top[i]);
+    v = block_top(v);
+    if (g.pass == MXO_DZ_TOPS) {
+        if (threadIdx.x == 0) g.top[g.ntop] = v;
+        return 0.0f;
+    }
+    const bool fits = v == 0.0f || (v >= 1.0f && v < 65520.0f);
+    // (it multiplies dy, exactly, and 2^60 at most keeps what follows finite)
+    const int e = fits ? 0 : min(14 + 127 - (int)(__builtin_bit_cast(uint32_t, v) >> 23), 60);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *g.back = __builtin_bit_cast(float, (127 - e) << 23);
+    return fits ? 0.0f : __builtin_bit_cast(float, (127 + e) << 23);
+}
+
 // Rows with contiguous features: 64 x E features by a run of rows a block, a
 // wave a row at a time.
 template <typename T, bool WHOLE>
@@ -298,7 +363,12 @@ __device__ __forceinline__ void gated_dz_rows(const OpsGatedDzArgs &g, float (*s
     constexpr int E = 16 / sizeof(T);
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t c = ((int64_t)blockIdx.x * 64 + l) * E, p = blockIdx.y, have = a.cols - c;
-    const int64_t chunk = (a.rows + a.nparts - 1) / a.nparts, end = min(a.rows, (p + 1) * chunk);
+    // (the second launch's blocks take longer runs)
+    const int nparts = kScaled<T> ? (int)gridDim.y : a.nparts;
+    const int64_t chunk = (a.rows + nparts - 1) / nparts, end = min(a.rows, (p + 1) * chunk);
+    float scale = 1.0f, top = 0.0f;
+    if constexpr (kScaled<T>)
+        if ((scale = dz_scale(g)) == 0.0f) return;
     float sa[E], sc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sa[e] = sc[e] = 0.0f;
@@ -314,7 +384,12 @@ __device__ __forceinline__ void gated_dz_rows(const OpsGatedDzArgs &g, float (*s
             Vec<T, E> o;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = elem<T>(vd, e), u[e] = elem<T>(vz, e), m[e] = elem<T>(vc, e);
+            if constexpr (kScaled<T>) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] *= scale;
+            }
             gated_dz_n<E>(a.act, a.slope, v, u, m);
+            if constexpr (kScaled<T>) top = top_of<E>(top, v, u);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 // features past the last are not there to be summed or stored
@@ -332,6 +407,10 @@ __device__ __forceinline__ void gated_dz_rows(const OpsGatedDzArgs &g, float (*s
                     for (int64_t k = 2 * a.cols - c; k < a.drs - c; ++k) dz[k] = (T)0.0f;
             }
         }
+    if constexpr (kScaled<T>) {
+        if (g.pass != MXO_DZ) return;  // the sums are there
+        keep_top(g, top);
+    }
     if (!a.part && !g.db) return;
 #pragma unroll
     for (int e = 0; e < E; ++e) sh[w][0][l * E + e] = sa[e], sh[w][1][l * E + e] = sc[e];
@@ -350,10 +429,13 @@ __device__ __forceinline__ void gated_dz_planar(const OpsGatedDzArgs &g) {
     constexpr int E = 16 / sizeof(T);
     __shared__ float sh[2][4];
     const int64_t c = blockIdx.x, p = blockIdx.y;
-    const int64_t chunk = ((a.rows + a.nparts - 1) / a.nparts + E - 1) / E * E, end = min(a.rows, (p + 1) * chunk);
+    const int nparts = kScaled<T> ? (int)gridDim.y : a.nparts;
+    const int64_t chunk = ((a.rows + nparts - 1) / nparts + E - 1) / E * E, end = min(a.rows, (p + 1) * chunk);
     const T *dy = static_cast<const T *>(a.dy) + c * a.dycs, *z = static_cast<const T *>(a.z) + c * a.zcs;
     T *dz = static_cast<T *>(a.dz) + c * a.dcs;
-    float sa = 0.0f, sc = 0.0f;
+    float sa = 0.0f, sc = 0.0f, scale = 1.0f, top = 0.0f;
+    if constexpr (kScaled<T>)
+        if ((scale = dz_scale(g)) == 0.0f) return;
     for (int64_t r = p * chunk + threadIdx.x * E; r < end; r += 256 * E) {
         const Vec<T, E> vd = load_upto<T, E>(dy + r, end - r), vz = load_upto<T, E>(z + r, end - r);
         const Vec<T, E> vc = load_upto<T, E>(z + a.cols * a.zcs + r, end - r);
@@ -361,7 +443,13 @@ __device__ __forceinline__ void gated_dz_planar(const OpsGatedDzArgs &g) {
         Vec<T, E> oa, oc;
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = to_f<T>(vd.v[e]), u[e] = to_f<T>(vz.v[e]), m[e] = to_f<T>(vc.v[e]);
+        if constexpr (kScaled<T>) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] *= scale;
+        }
         gated_dz_n<E>(a.act, a.slope, v, u, m);
+        // (past the end dy is 0, and so is dz)
+        if constexpr (kScaled<T>) top = top_of<E>(top, v, u);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             if (r + e < end) sa += v[e], sc += u[e];
@@ -372,6 +460,10 @@ __device__ __forceinline__ void gated_dz_planar(const OpsGatedDzArgs &g) {
             store_n<T, E>(dz + r, oa);
             store_n<T, E>(dz + a.cols * a.dcs + r, oc);
         }
+    }
+    if constexpr (kScaled<T>) {
+        if (g.pass != MXO_DZ) return;
+        keep_top(g, top);
     }
     if (!a.part && !g.db) return;
     sa = wave_sum(sa), sc = wave_sum(sc);
@@ -413,6 +505,7 @@ __device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
     const OpsGemmArgs &g = a.g;
     const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m, plane = (int64_t)g.m * g.n;
     const int q = t & 15, way = t >> 4;
+    const float back = back_of<T>(g);
     for (int64_t i0 = (int64_t)blockIdx.x * 16; i0 < total; i0 += (int64_t)a.first * 16) {
         const int64_t i = i0 + q, m = i / quads, n = (i - m * quads) * 4;
         f32x4 v = {0, 0, 0, 0};
@@ -431,9 +524,11 @@ __device__ __forceinline__ void grad_join(const OpsGradJoinArgs &a) {
         if (way || i >= total) continue;
 #pragma unroll
         for (int k = 1; k < 16; ++k) v += sh[k * 16 + q];
+        float r[4] = {v[0], v[1], v[2], v[3]};
+        scale_back<T, 4>(r, back);
         Vec<T, 4> o;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o.v[e] = from_f<T>(v[e]);
+        for (int e = 0; e < 4; ++e) o.v[e] = from_f<T>(r[e]);
         store_upto<T, 4>(static_cast<T *>(g.c) + m * g.ldc + n, o, g.n - n);
     }
 }

@@ -289,13 +289,29 @@ __device__ __forceinline__ void bias_fetch(const OpsGemmArgs &g, int64_t n, floa
 #pragma unroll
     for (int e = 0; e < E; ++e) bias[e] = g.bias && !g.bias_rows && n + e < g.n ? param<T>(g.bias, n + e, g.bias_f32) : 0.0f;
 }
+// What the sums are multiplied by, of an operand that was scaled to fp16's range
+// (ops_gated.h): read at a kernel's start (read where the results are stored, a
+// 256 x 256 tile's product took 3 us more).
+template <typename T>
+__device__ __forceinline__ float back_of(const OpsGemmArgs &g) {
+    if constexpr (__is_same(T, f16)) return g.back ? *g.back : 1.0f;
+    return 1.0f;
+}
+template <typename T, int E>
+__device__ __forceinline__ void scale_back(float *v, float back) {
+    if constexpr (__is_same(T, f16)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= back;
+    }
+}
 // Bias, z, activation and residual for E consecutive n of row m, rounding once
 // to T at each store. The sum and all of this are fp32.
 template <typename T, int E>
 __device__ __forceinline__ void gemm_finish(const OpsGemmArgs &g, int64_t m, int64_t n, float *v, const float *bias,
-                                            const Extra<T, E> &x) {
+                                            const Extra<T, E> &x, float back = 1.0f) {
     if (m >= g.m || n >= g.n) return;
     const int64_t have = g.n - n;
+    scale_back<T, E>(v, back);
     if (g.bias) {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] += g.bias_rows ? x.bias_row : bias[e];
@@ -374,7 +390,7 @@ __device__ __forceinline__ void gated_write(const OpsGemmArgs &g, int64_t m0, in
                                             const f32x4 (&acc)[FM][FN]);
 template <typename T, int FM, int FN, int PAIR = PAIR_NONE>
 __device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int64_t n0, int s, int l, char *at,
-                                           const f32x4 (&acc)[FM][FN]) {
+                                           const f32x4 (&acc)[FM][FN], float back = 1.0f) {
     if constexpr (PAIR != PAIR_NONE) {
         gated_write<T, FM, FN, PAIR>(g, m0, n0, s, l, at, acc);
         return;
@@ -412,7 +428,7 @@ __device__ __forceinline__ void gemm_write(const OpsGemmArgs &g, int64_t m0, int
 #pragma unroll
             for (int e = 0; e < E; e += 4) *reinterpret_cast<f32x4 *>(v + e) = *reinterpret_cast<const f32x4 *>(p + e);
             if (whole)
-                gemm_finish<T, E>(g, m + k * ROWS, n, v, bias, x[k]);
+                gemm_finish<T, E>(g, m + k * ROWS, n, v, bias, x[k], back);
             else if (m + k * ROWS < g.m && n < g.n)
                 store_upto<float, E>(g.part + ((int64_t)s * g.m + m + k * ROWS) * g.n + n,
                                      __builtin_bit_cast(Vec<float, E>, v), g.n - n);
@@ -432,6 +448,7 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
     constexpr int BK = TA::BK, ABYTES = BM * 128, STAGE = (BM + BN) * 128;
     int tm, tn, s;
     gemm_place(g, tm, tn, s);
+    const float back = back_of<T>(g);
     const int64_t m0 = (int64_t)tm * CM, n0 = (int64_t)tn * CN;
     const int kbeg = s * g.kchunk, kend = min(g.k, kbeg + g.kchunk);
     const int t = threadIdx.x, l = t & 63, w = t >> 6, wm = w / WN * (BM / WM), wn = w % WN * (BN / WN);
@@ -504,7 +521,7 @@ __device__ __forceinline__ void gemm_tile(const OpsGemmArgs &g, char *lds) {
             }
     }
     // behind the loop's last barrier: no wave reads the tiles any more
-    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, lds + w * gemm_write_bytes<FN, PAIR>(), acc);
+    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, lds + w * gemm_write_bytes<FN, PAIR>(), acc, back);
 }
 
 // The splits' sums added in a fixed order, then the epilogue: WAYS threads to
@@ -515,6 +532,7 @@ __device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
     __shared__ f32x4 sh[WAYS > 1 ? 256 : 1];
     const int64_t quads = ((int64_t)g.n + 3) / 4, total = quads * g.m, plane = (int64_t)g.m * g.n;
     const int q = threadIdx.x % Q, way = threadIdx.x / Q;
+    const float back = back_of<T>(g);
     for (int64_t i0 = (int64_t)blockIdx.x * Q; i0 < total; i0 += (int64_t)gridDim.x * Q) {
         const int64_t i = i0 + q, m = i / quads, n = (i - m * quads) * 4;
         f32x4 v = {0, 0, 0, 0};
@@ -540,7 +558,7 @@ __device__ __forceinline__ void gemm_join(const OpsGemmArgs &g) {
         Extra<T, 4> x;
         bias_fetch<T, 4>(g, n, bias);
         extra_fetch<T, 4>(g, m, n, x);
-        gemm_finish<T, 4>(g, m, n, r, bias, x);
+        gemm_finish<T, 4>(g, m, n, r, bias, x, back);
     }
 }
 

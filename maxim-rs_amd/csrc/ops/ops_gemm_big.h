@@ -66,6 +66,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     constexpr int BK = TA::BK;
     int tm, tn, s;
     gemm_place(g, tm, tn, s);
+    const float back = back_of<T>(g);
     const int64_t m0 = (int64_t)tm * CM, n0 = (int64_t)tn * CN;
     const int kbeg = s * g.kchunk, kend = min(g.k, kbeg + g.kchunk);
     const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -279,7 +280,7 @@ __device__ __forceinline__ void gemm_direct(const OpsGemmArgs &g, const Stage (&
     }
     tiles_landed<0>();  // the last loads too, zeros: the tiles' LDS is free
     char *own = (w & 1 ? w & 2 ? st[1].b : st[1].a : w & 2 ? st[0].b : st[0].a) + (w >> 2) * gemm_write_bytes<FN, PAIR>();
-    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, own, acc);
+    gemm_write<T, FM, FN, PAIR>(g, m0 + wm * CM / BM, n0 + wn * CN / BN, s, l, own, acc, back);
 }
 
 #define OPS_STAGE(i, BM, BN)                              \

@@ -19,6 +19,7 @@ __device__ __forceinline__ void gemm_skinny(const OpsGemmArgs &g) {
     constexpr int E = 16 / sizeof(T), STEP = 4 * E, W = 8, AHEAD = 8;
     typedef typename Mma<T>::Frag Frag;
     __shared__ f32x4 sums[W][64];
+    const float back = back_of<T>(g);
     const int t = threadIdx.x, l = t & 63, w = t >> 6, r = l & 15, q = l >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16;
     // this wave's k's, whole steps; past them nothing is loaded
@@ -59,7 +60,7 @@ __device__ __forceinline__ void gemm_skinny(const OpsGemmArgs &g) {
     Extra<T, 4> x;
     bias_fetch<T, 4>(g, n, bias);
     extra_fetch<T, 4>(g, m, n, x);
-    gemm_finish<T, 4>(g, m, n, out, bias, x);
+    gemm_finish<T, 4>(g, m, n, out, bias, x, back);
 }
 
 #define OPS_SKINNY(name, T) \
