@@ -185,15 +185,21 @@ def _act(act):
     return ACTS[act]
 
 
-def _new(x, X, n, planar):
+def _either(X):
+    """Whether a matrix lies in both orders: both strides 1, or one position."""
+    return X.rows <= 1 or X.row_stride == X.col_stride == 1
+
+
+def _new(x, X, n, planar, other=None):
     """An uninitialised result of x's positions with n features, in x's memory
-    order (X: x as a matrix): the tensor, and it as a matrix."""
+    order (X: x as a matrix), or where x lies in both the other matrix's: the
+    tensor, and it as a matrix."""
     if n == X.cols and x.is_contiguous():
         t, by_rows = _torch.empty_like(x), planar
     else:
         rest = tuple(x.shape[1:] if planar else x.shape[:-1])
-        # both strides 1, or a single position: the call's own order
-        by_rows = planar if X.rows <= 1 or X.row_stride == X.col_stride == 1 else X.row_stride == 1
+        order = other if other is not None and _either(X) else X
+        by_rows = planar if _either(order) else order.row_stride == 1  # the call's own order if both lie in both
         t = x.new_empty((n,) + rest if by_rows else rest + (n,))
         if by_rows != planar:
             t = t.movedim(-1, 0) if planar else t.movedim(0, -1)
@@ -337,7 +343,7 @@ def gated(x, w, bias=None, act="silu", slope=0.0, planar=False, save=False, out=
     W = _mat(w, "w", d, False)
     B = None if bias is None else _vec(bias, "bias", d)
     y, Y = _new(x, X, W.rows // 2, planar) if out is None else (out, _mat(out, "out", d, planar))
-    z, Z = _new(y, Y, W.rows, planar) if save else (None, None)
+    z, Z = _new(y, Y, W.rows, planar, X) if save else (None, None)  # a y of one feature has both orders
     size = C.c_uint64()
     _check(_L.mxh_gated_workspace(X, W, Y, Z, size))
     ws = _workspace(size.value, x)
