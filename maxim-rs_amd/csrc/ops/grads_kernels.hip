@@ -100,13 +100,32 @@ extern "C" __global__ __launch_bounds__(256) void mxn_norm(GradsJoinArgs a) {
     if (threadIdx.x == 0) *a.norm = (float)__builtin_sqrt(s);
 }
 
+// What gradients are multiplied by: a norm that is not finite, or not past the
+// bound, leaves them as they are. A quotient below fp32's normal range has too few
+// bits of its own, and a gradient near the range's other end brings its product
+// back: there it is 64 bits wide.
+struct Factor {
+    float f;
+    double wide;  // not 0: instead of f
+};
+__device__ __forceinline__ Factor factor(float norm, float most) {
+    if (!(norm > most && norm < __builtin_inff())) return {1.0f, 0.0};
+    const float f = most / norm;
+    return {f, f < 0x1p-126f ? (double)most / norm : 0.0};
+}
+
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const T *p, T *q, int64_t have, float f, int t) {
+__device__ __forceinline__ void chunk_scale(const T *p, T *q, int64_t have, const Factor &f, int t) {
     constexpr int E = 16 / sizeof(T);
     auto scale = [&](Vec<T, E> &v) {
-        if (f == 1.0f) return;  // the same bits, NaN's too
+        if (f.f == 1.0f) return;  // the same bits, NaN's too
+        if (f.wide != 0.0) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v.v[e] = from_f<T>(to_f<T>(v.v[e]) * f);
+            for (int e = 0; e < E; ++e) v.v[e] = from_f<T>((float)(to_f<T>(v.v[e]) * f.wide));
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) v.v[e] = from_f<T>(to_f<T>(v.v[e]) * f.f);
     };
     if (have >= MXN_CHUNK / (int)sizeof(T)) {
         Vec<T, E> v[4];
@@ -126,10 +145,10 @@ __device__ __forceinline__ void chunk_scale(const T *p, T *q, int64_t have, floa
     }
 }
 
-__device__ __forceinline__ void scale_chunk(const GradsArgs &a, const Chunk &c, float f, int t) {
+__device__ __forceinline__ void scale_chunk(const GradsArgs &a, const Chunk &c, const Factor &f, int t) {
     const void *p = a.src[c.tensor];
     void *q = a.dst[c.tensor];
-    if (f == 1.0f && p == q) return;
+    if (f.f == 1.0f && p == q) return;
     if (c.type == MXO_F32)
         chunk_scale<float>(static_cast<const float *>(p) + c.at, static_cast<float *>(q) + c.at, c.have, f, t);
     else if (c.type == MXO_F16)
@@ -137,15 +156,11 @@ __device__ __forceinline__ void scale_chunk(const GradsArgs &a, const Chunk &c, 
     else
         chunk_scale<bf16>(static_cast<const bf16 *>(p) + c.at, static_cast<bf16 *>(q) + c.at, c.have, f, t);
 }
-// A norm that is not finite, or not past the bound: as they are.
-__device__ __forceinline__ float factor(float norm, float most) {
-    return norm > most && norm < __builtin_inff() ? most / norm : 1.0f;
-}
 
 extern "C" __global__ __launch_bounds__(256) void mxn_clip(GradsArgs a) {
     const int l = threadIdx.x & 63;
     const uint32_t lo = first_of(a, l), hi = first_of(a, l + 64), chunks = a.first[a.count];
-    const float f = factor(*a.norm, a.max_norm);
+    const Factor f = factor(*a.norm, a.max_norm);
     for (uint32_t b = blockIdx.x; b < chunks; b += gridDim.x) scale_chunk(a, chunk_at(a, lo, hi, chunks - 1 - b), f, threadIdx.x);
 }
 
@@ -167,6 +182,6 @@ extern "C" __global__ __launch_bounds__(1024) void mxn_small(GradsArgs a) {
     const float norm = (float)__builtin_sqrt(s);
     if (threadIdx.x == 0) *a.norm = norm;
     if (!a.clip) return;
-    const float f = factor(norm, a.max_norm);
+    const Factor f = factor(norm, a.max_norm);
     for (uint32_t c = g; c < chunks; c += 4) scale_chunk(a, chunk_at(a, lo, hi, c), f, t);
 }
