@@ -7,9 +7,10 @@
 // its sums of a and of c lie in the same lanes, and neither z nor a second
 // product goes through memory unless z is kept. The weights are B where
 // features are contiguous in the results (PAIR_N), A in planar order (PAIR_M).
-// As a product of twice the columns: 8192 x 2048 to 2 x 4096 bf16 214 us, with z
-// (134 MB more) 221 (the product alone, of which all of z is stored, 217); 64
-// to 2 x 64 fp32 planes of 65536 with z, 67 MB, 18.6 us, 3.6 TB/s.
+// As a product of twice the columns: 8192 x 2048 to 2 x 4096 bf16 225 us a call,
+// with z (134 MB more) 229 to 242 by the card's clock (the product alone, of
+// which all of z is stored, 222 to 227); 64 to 2 x 64 fp32 planes of 65536 with z,
+// 67 MB, 18.4 us, 3.6 TB/s.
 #pragma once
 
 #include "ops_gemm_big.h"
@@ -587,7 +588,7 @@ OPS_GATED_TYPE(bf16, bf16)
 OPS_GATED_TYPE(f16, f16)
 OPS_GATED_TYPE(f32, float)
 // 256 x 256: waves whose results are 64 wide, whole lines of y and z (with half
-// lines 8192 x 2048 to 2 x 4096 with z took 250 us, so 221); with w contiguous
+// lines 8192 x 2048 to 2 x 4096 with z took 256 us, so 231); with w contiguous
 // along its rows they do not fit the registers
 OPS_GATED_D2(bf16, bf16, 256, 4, 2, n, PAIR_N, kk, true, true)
 OPS_GATED_D2(f16, f16, 256, 4, 2, n, PAIR_N, kk, true, true)

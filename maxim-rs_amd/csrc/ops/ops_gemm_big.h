@@ -4,7 +4,7 @@
 // Bound by the matrix cores where there are tiles enough, at the clock their
 // power leaves: bf16 8192^3 in 775-910 us (1.2-1.4 PFLOP/s; the library's
 // product 695-830), 4096^3 in 101-107 us (95-109). 8192 x 2048 x 8192 with 134
-// MB of results 221 us (194), with gelu 242, with the 134 MB of z as well 257: a
+// MB of results 221-227 us (194), with gelu 242-251, with the 134 MB of z as well 257-267: a
 // 256 x 256 tile takes 128 KiB of a CU's 160 KiB of LDS, so no second one fits
 // beside it and its results are written before its CU's next tile is begun. Two
 // smaller tiles a CU hide that, and lose more in products an LDS byte read. Four
