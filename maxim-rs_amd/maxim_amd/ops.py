@@ -355,7 +355,8 @@ def gated(x, w, bias=None, act="silu", slope=0.0, planar=False, save=False, out=
 def gated_backward(dy, x, w, z, act="silu", slope=0.0, planar=False, dx=True, dw=True, db=True, db_dtype=None):
     """mxh_gated_backward: (dx, dw, db) of gated(x, w, bias, act, slope), None
     where one is off. db is of w's type or db_dtype (the bias's: w's or
-    float32)."""
+    float32). In 16 bits the products take dz rounded to x's type, in fp16 scaled
+    into its range."""
     d = _device(x)
     f = _act(act)
     X = _mat(x, "x", d, planar)
